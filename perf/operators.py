@@ -316,10 +316,12 @@ def _pool_of(cache, case, layers):
     base, stride = cache.pool_address()
     blocks = cache.max_blocks
 
-    class Memory:
+    class Memory:  # the tensor holds it, and so the cache, for as long as the blocks are looked at
         __cuda_array_interface__ = {"shape": (blocks * stride,), "typestr": "|u1", "data": (base, False), "version": 2}
 
-    raw = torch.as_tensor(Memory(), device=DEVICE)
+    memory = Memory()
+    memory.owner = cache
+    raw = torch.as_tensor(memory, device=DEVICE)
     b, kvh, d = case["block"], case["kv_heads"], case["dim"]
     if not case["q8"]:
         return raw.view(torch.float32).as_strided((blocks, layers, 2, b, kvh * d),
