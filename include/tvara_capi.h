@@ -61,6 +61,8 @@ typedef struct tvara_kv_cache tvara_kv_cache;
 typedef struct tvara_attn_plan tvara_attn_plan;
 typedef struct tvara_prefill_plan tvara_prefill_plan;
 typedef struct tvara_radix tvara_radix;
+typedef struct tvara_tree_plan tvara_tree_plan;
+typedef struct tvara_slot_plan tvara_slot_plan;
 
 /* BlockHandle (kv.hpp:35) */
 typedef struct {
@@ -262,6 +264,18 @@ TVARA_API int tvara_kv_append_batch(tvara_kv_cache* cache, const uint64_t* seque
 /* `count` consecutive appends to one sequence (a prompt's K/V) */
 TVARA_API int tvara_kv_append_tokens(tvara_kv_cache* cache, uint64_t sequence, const float* keys,
                                      const float* values, size_t count, int device_ptrs, size_t* applied);
+/* Room for tokens[i] more tokens at the end of sequences[i]: the block work of
+ * as many appends (zeroed new blocks, copy-on-write of a shared tail) with no
+ * rows written; they are written through a slot plan (below), or truncated
+ * again.  A reserved slot that nothing wrote reads as zeros, or as what a
+ * truncated token left there.  All or nothing: a failure leaves every sequence at
+ * its entry length.  No counterpart in the reference. */
+TVARA_API int tvara_kv_reserve(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, const size_t* tokens);
+/* The pool's device address and the bytes from one block to the next, for
+ * kernels of the caller's own that read blocks through block tables.  Q8_0
+ * blocks hold, per layer and kind, each KV head's int8 rows and then its fp16
+ * scales (rows of head_dim / 32), a head starting on 16 bytes. */
+TVARA_API int tvara_kv_pool_address(tvara_kv_cache* cache, void** base, size_t* stride);
 /* PagedCache::read (kv.hpp:110-113): kv_width floats of one position */
 TVARA_API int tvara_kv_read(tvara_kv_cache* cache, uint64_t sequence, size_t layer, size_t position, int value,
                             float* out);
@@ -364,6 +378,95 @@ TVARA_API int tvara_prefill_plan_launch(tvara_prefill_plan* plan, size_t layer, 
 /* Synchronise the plan's last launch and report a non-finite score. */
 TVARA_API int tvara_prefill_plan_check(tvara_prefill_plan* plan);
 TVARA_API void tvara_prefill_plan_destroy(tvara_prefill_plan* plan);
+
+/* ------------------------------------------- speculative decoding with trees
+ *
+ * A tree of drafted tokens hangs on the end of a sequence: node j of tree i has a
+ * parent among the nodes before it, or -1 where it follows the cached text.
+ * Nodes are packed, one tree after the other, and so are their rows.  Their K/V
+ * are rows of the caller's, outside the cache, until a part of them is accepted:
+ *
+ *   tvara_kv_reserve            room for the longest path of every tree
+ *   tvara_tree_plan_create, tvara_slot_plan_create
+ *   tvara_tree_plan_launch      attention, every layer
+ *   tvara_tree_plan_accept      the confirmed path of every tree, from the logits
+ *   tvara_slot_plan_build       the slots of the accepted tokens
+ *   tvara_slot_plan_write       their K/V rows, all layers
+ *   tvara_kv_truncate_batch     to what was accepted, once the host has read it
+ *
+ * with no wait for the GPU before the last.  The reference speculates through its
+ * Python layer (python/tvara/speculative.py, speculative_tree.py) one
+ * tvara_sequence_decode_batch at a time. */
+
+/* The listed trees, resident: sequences[i] (which may be listed again) is seen up
+ * to visible[i] tokens (NULL: all of it) and has nodes[i] nodes (0 to 1,024),
+ * parents [sum nodes] with -1 <= parents[j] < j within its tree.  precision
+ * TVARA_ATTN_F32, or TVARA_ATTN_F32X3 as tvara_attn_prefill has it where the
+ * layout has such tiles (head_dim 64 or 128, blocks of a power of two from 16
+ * tokens) and f32 elsewhere; bf16 is refused.  Launching fails with TVARA_INVALID
+ * once the cache has changed. */
+TVARA_API tvara_tree_plan* tvara_tree_plan_create(tvara_kv_cache* cache, const uint64_t* sequences, size_t count,
+                                                  size_t heads, size_t context, const size_t* visible,
+                                                  const size_t* nodes, const int32_t* parents, int precision);
+/* Attention of every node over its sequence's cached tokens, the nodes above it
+ * and itself: q and out f32 [sum nodes][heads * head_dim], keys and values rows
+ * of kv_width floats row_stride floats apart (0: kv_width; a multiple of 4),
+ * device pointers, asynchronous on `stream` (NULL: the cache's).  What a node
+ * does not see never reaches its row, whatever it holds.  Launches of one plan run
+ * in stream order: they share its partial results. */
+TVARA_API int tvara_tree_plan_launch(tvara_tree_plan* plan, size_t layer, const float* q, const float* keys,
+                                     const float* values, size_t row_stride, float* out, void* stream);
+/* Greedy acceptance: e = first[i]; while a child of the current node (a root at
+ * the start) has token e, the lowest such child joins the path and e becomes the
+ * largest of its logits' index (the lowest on ties); next[i] = e.  tokens [sum
+ * nodes], logits f32 [sum nodes] rows of vocab, logits_stride floats apart (0:
+ * vocab); path [count][path_stride] receives the accepted nodes as packed rows and
+ * -1 behind them, accepted [count] how many.  A NaN logit is never the largest.
+ * It, or a path longer than path_stride (which ends there), is reported by
+ * tvara_tree_plan_check.  Device pointers, asynchronous; needs no cache data, so the plan may be stale. */
+TVARA_API int tvara_tree_plan_accept(tvara_tree_plan* plan, const uint32_t* tokens, const uint32_t* first,
+                                     const float* logits, size_t vocab, size_t logits_stride, int32_t* path,
+                                     size_t path_stride, int32_t* accepted, uint32_t* next, void* stream);
+/* Synchronise the plan's last launch and report a non-finite score, or what
+ * acceptance found. */
+TVARA_API int tvara_tree_plan_check(tvara_tree_plan* plan);
+TVARA_API void tvara_tree_plan_destroy(tvara_tree_plan* plan);
+/* A plan, one launch and its check in one synchronous call: host pointers, or
+ * device pointers where device_ptrs is nonzero; keys and values [sum nodes][kv_width]. */
+TVARA_API int tvara_attn_tree(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, size_t layer, size_t heads,
+                              size_t context, const size_t* visible, const size_t* nodes, const int32_t* parents,
+                              const float* q, const float* keys, const float* values, float* out, int precision,
+                              int device_ptrs);
+
+/* The block ids of the listed sequences, resident (at most 65,535); calls fail
+ * with TVARA_INVALID once the cache's tables have changed. */
+TVARA_API tvara_slot_plan* tvara_slot_plan_create(tvara_kv_cache* cache, const uint64_t* sequences, size_t count);
+/* From device lengths, asynchronously: counts[i] tokens of sequence i from
+ * position starts[i] on have
+ *   offsets [count + 1]    the sums of the counts before each sequence
+ *   positions [capacity]   starts[i] + j
+ *   slots [capacity]       block id * tokens_per_block + position in the block
+ * at offsets[i] + j, or at i * stride + j for a stride above 0 (capacity at least
+ * count * stride); entries without a token are -1.  tables [count][width] are the
+ * block ids, -1 behind a sequence's own.  Any output may be NULL.  Slots are
+ * for writing: a position outside the sequence's blocks, or in a block that
+ * another sequence or a prefix node shares, has slot -1; that, a negative count,
+ * or tokens beyond the capacity (which are left out) are reported by
+ * tvara_slot_plan_check. */
+TVARA_API int tvara_slot_plan_build(tvara_slot_plan* plan, const int32_t* starts, const int32_t* counts, size_t stride,
+                                    size_t capacity, int32_t* offsets, int32_t* positions, int64_t* slots,
+                                    int32_t* tables, size_t width, void* stream);
+/* K/V rows of every layer into slots, f32 as they are or encoded as appends
+ * encode them: entry t (of n) takes row rows[t] (NULL: row t) of row_count rows to
+ * slots[t]; an entry with slot -1 is skipped.  Element (row, layer, column) lies at
+ * row * row_stride + layer * layer_stride + column floats.  A slot outside the pool
+ * or a row outside the rows is skipped and reported by tvara_slot_plan_check.  Two entries of one slot
+ * leave either's bytes.  Device pointers, asynchronous. */
+TVARA_API int tvara_slot_plan_write(tvara_slot_plan* plan, const int64_t* slots, const int32_t* rows, size_t n,
+                                    const float* keys, const float* values, size_t row_count, size_t row_stride,
+                                    size_t layer_stride, void* stream);
+TVARA_API int tvara_slot_plan_check(tvara_slot_plan* plan);
+TVARA_API void tvara_slot_plan_destroy(tvara_slot_plan* plan);
 
 /* ----------------------------------------------------------------- timing */
 

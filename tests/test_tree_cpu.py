@@ -1,0 +1,33 @@
+"""Entry points of speculative decoding with trees refuse closed handles (no
+device calls: CPU only)."""
+
+import numpy as np
+import pytest
+
+from tvara_amd import _capi, attention
+
+
+def test_closed_handles_are_refused():
+    lib = _capi.lib()
+    n = np.zeros(1, np.uint64)
+    for rc in (lib.tvara_kv_reserve(None, None, 0, None), lib.tvara_kv_pool_address(None, None, None),
+               lib.tvara_tree_plan_launch(None, 0, None, None, None, 0, None, None),
+               lib.tvara_tree_plan_accept(None, None, None, None, 1, 0, None, 0, None, None, None),
+               lib.tvara_tree_plan_check(None),
+               lib.tvara_attn_tree(None, None, 0, 0, 1, 1, None, None, None, None, None, None, None, 0, 0),
+               lib.tvara_slot_plan_build(None, None, None, 0, 0, None, None, None, None, 0, None),
+               lib.tvara_slot_plan_write(None, None, None, 0, None, None, 0, 0, 0, None),
+               lib.tvara_slot_plan_check(None)):
+        assert rc == _capi.INVALID
+    assert not lib.tvara_tree_plan_create(None, None, 0, 1, 1, None, None, None, 0)
+    assert lib.tvara_last_status() == _capi.INVALID
+    assert not lib.tvara_slot_plan_create(None, None, 0)
+    lib.tvara_tree_plan_destroy(None)
+    lib.tvara_slot_plan_destroy(None)
+    assert n[0] == 0
+
+
+def test_trees_of_unequal_lists_are_refused():
+    for nodes, parents in (([1], [-1, 0]), ([1, 2], [-1, -1]), ([], [])):
+        with pytest.raises(_capi.InvalidArgument):
+            attention._trees([1, 2], nodes, parents, None)

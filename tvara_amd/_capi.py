@@ -107,6 +107,21 @@ SIGNATURES = {
     "tvara_prefill_plan_launch": (C.c_int, [_vp, _sz, _vp, _vp, _vp]),
     "tvara_prefill_plan_check": (C.c_int, [_vp]),
     "tvara_prefill_plan_destroy": (None, [_vp]),
+    "tvara_kv_reserve": (C.c_int, [_vp, C.POINTER(_u64), _sz, C.POINTER(_sz)]),
+    "tvara_kv_pool_address": (C.c_int, [_vp, C.POINTER(_vp), C.POINTER(_sz)]),
+    "tvara_tree_plan_create": (_vp, [_vp, C.POINTER(_u64), _sz, _sz, _sz, C.POINTER(_sz), C.POINTER(_sz),
+                                     C.POINTER(C.c_int32), C.c_int]),
+    "tvara_tree_plan_launch": (C.c_int, [_vp, _sz, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "tvara_tree_plan_accept": (C.c_int, [_vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp]),
+    "tvara_tree_plan_check": (C.c_int, [_vp]),
+    "tvara_tree_plan_destroy": (None, [_vp]),
+    "tvara_attn_tree": (C.c_int, [_vp, C.POINTER(_u64), _sz, _sz, _sz, _sz, C.POINTER(_sz), C.POINTER(_sz),
+                                  C.POINTER(C.c_int32), _fp, _fp, _fp, _fp, C.c_int, C.c_int]),
+    "tvara_slot_plan_create": (_vp, [_vp, C.POINTER(_u64), _sz]),
+    "tvara_slot_plan_build": (C.c_int, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "tvara_slot_plan_write": (C.c_int, [_vp, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp]),
+    "tvara_slot_plan_check": (C.c_int, [_vp]),
+    "tvara_slot_plan_destroy": (None, [_vp]),
     "tvara_profile_enable": (C.c_int, [C.c_int]),
     "tvara_profile_read": (C.c_int, [C.c_char_p, C.POINTER(C.c_double), C.POINTER(_sz)]),
     "tvara_profile_reset": (C.c_int, []),

@@ -5,7 +5,9 @@
 * ``fused_prompt_attention`` / ``prefill_batch`` -- attention.hpp:85-89, a
   causal chunk over cached positions, in f32 (reference semantics) or on bf16
   MFMA tiles;
-* ``DecodePlan`` -- resident block tables for repeated device launches.
+* ``DecodePlan`` -- resident block tables for repeated device launches;
+* ``TreePlan`` / ``tree_batch`` -- trees of drafted tokens over cached
+  sequences: their attention and their greedy acceptance.
 """
 
 from __future__ import annotations
@@ -158,6 +160,75 @@ class PrefillPlan:
     def close(self):
         if getattr(self, "h", None):
             self.lib.tvara_prefill_plan_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        self.close()
+
+
+def _trees(seqs, nodes, parents, visible):
+    seqs = np.ascontiguousarray(seqs, dtype=np.uint64).reshape(-1)
+    nodes = np.ascontiguousarray(nodes, dtype=np.uintp).reshape(-1)
+    parents = np.ascontiguousarray(parents, dtype=np.int32).reshape(-1)
+    if nodes.size != seqs.size or int(nodes.sum()) != parents.size:
+        raise InvalidArgument("sequences, nodes and parents differ in length")
+    if visible is not None:
+        visible = np.ascontiguousarray(np.broadcast_to(np.asarray(visible, dtype=np.uintp), seqs.shape))
+    vp = visible.ctypes.data_as(C.POINTER(_sz)) if visible is not None else None
+    keep = (seqs, nodes, parents, visible)
+    return keep, (seqs.ctypes.data_as(C.POINTER(C.c_uint64)), nodes.ctypes.data_as(C.POINTER(_sz)),
+                  parents.ctypes.data_as(C.POINTER(C.c_int32)), vp)
+
+
+def tree_batch(cache, q, seqs, nodes, parents, keys, values, layer, heads, context, visible=None, precision="f32"):
+    """Attention of trees of drafted tokens (tvara_attn_tree): tree i hangs on
+    seqs[i] and has nodes[i] of the packed nodes, parents (-1: a root) within
+    its tree; q [nodes, heads * head_dim], keys and values [nodes, kv_width]."""
+    if precision not in _PRECISION:
+        raise InvalidArgument("unknown attention precision")
+    (seqs, nodes, parents, visible), (sp, np_, pp, vp) = _trees(seqs, nodes, parents, visible)
+    rows, hidden = parents.size, heads * cache.head_dim
+    q = _f32(q).reshape(rows, hidden)
+    k, v = _f32(keys).reshape(rows, cache.kv_width), _f32(values).reshape(rows, cache.kv_width)
+    out = np.empty((max(rows, 1), hidden), np.float32)
+    _capi.check(cache.lib.tvara_attn_tree(cache.h, sp, seqs.size, layer, heads, context, vp, np_, pp, _ptr(q), _ptr(k),
+                                          _ptr(v), _ptr(out), _PRECISION[precision], 0))
+    return out[:rows]
+
+
+class TreePlan:
+    """Resident trees of drafted tokens over cached sequences (tvara_tree_plan_*)."""
+
+    def __init__(self, cache, seqs, nodes, parents, heads, context, visible=None, precision="f32"):
+        if precision not in _PRECISION:
+            raise InvalidArgument("unknown attention precision")
+        self.cache = cache
+        self.lib = cache.lib
+        (seqs, nodes, parents, visible), (sp, np_, pp, vp) = _trees(seqs, nodes, parents, visible)
+        self.rows = parents.size
+        self.h = self.lib.tvara_tree_plan_create(cache.h, sp, seqs.size, heads, context, vp, np_, pp,
+                                                 _PRECISION[precision])
+        if not self.h:
+            _capi.raise_last()
+
+    def launch(self, layer, q_ptr, keys_ptr, values_ptr, out_ptr, row_stride=0, stream=None):
+        """Asynchronous attention over device pointers (ints); K/V rows are
+        row_stride floats apart (0: kv_width)."""
+        _capi.check(self.lib.tvara_tree_plan_launch(self.h, layer, q_ptr, keys_ptr, values_ptr, row_stride, out_ptr,
+                                                    stream))
+
+    def accept(self, tokens_ptr, first_ptr, logits_ptr, vocab, path_ptr, path_stride, accepted_ptr, next_ptr,
+               logits_stride=0, stream=None):
+        """Asynchronous greedy acceptance over device pointers (ints)."""
+        _capi.check(self.lib.tvara_tree_plan_accept(self.h, tokens_ptr, first_ptr, logits_ptr, vocab, logits_stride,
+                                                    path_ptr, path_stride, accepted_ptr, next_ptr, stream))
+
+    def check(self):
+        _capi.check(self.lib.tvara_tree_plan_check(self.h))
+
+    def close(self):
+        if getattr(self, "h", None):
+            self.lib.tvara_tree_plan_destroy(self.h)
             self.h = None
 
     def __del__(self):

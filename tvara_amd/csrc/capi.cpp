@@ -18,6 +18,7 @@
 #include "host_copy.hpp"
 #include "kv_cache.hpp"
 #include "model.hpp"
+#include "tree.hpp"
 
 using tvara_amd::AttnPlan;
 using tvara_amd::DeviceCache;
@@ -58,6 +59,14 @@ struct tvara_model {
 
 struct tvara_prefill_plan {
     tvara_amd::PrefillPlan plan;
+};
+
+struct tvara_tree_plan {
+    tvara_amd::TreePlan plan;
+};
+
+struct tvara_slot_plan {
+    tvara_amd::SlotPlan plan;
 };
 
 namespace tvara_amd {
@@ -360,6 +369,162 @@ int tvara_prefill_plan_check(tvara_prefill_plan* plan) {
 }
 
 void tvara_prefill_plan_destroy(tvara_prefill_plan* plan) { delete plan; }
+
+// ------------------------------------------------- trees of drafted tokens
+
+int tvara_kv_reserve(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, const size_t* tokens) {
+    return guard([&] { live(cache).reserve(sequences, count, tokens); });
+}
+
+int tvara_kv_pool_address(tvara_kv_cache* cache, void** base, size_t* stride) {
+    return guard([&] {
+        auto& c = live(cache);
+        c.flush();  // blocks that were handed out read as zeros
+        if (base) *base = c.pool();
+        if (stride) *stride = c.layout().stride;
+    });
+}
+
+tvara_tree_plan* tvara_tree_plan_create(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, size_t heads,
+                                        size_t context, const size_t* visible, const size_t* nodes,
+                                        const int32_t* parents, int precision) {
+    tvara_tree_plan* out = nullptr;
+    guard([&] {
+        auto& c = live(cache);
+        tvara_amd::check_attention_config(c, heads, context);
+        auto p = std::make_unique<tvara_tree_plan>();
+        p->plan.build(&c, sequences, count, heads, context, visible, nodes, parents, precision);
+        out = p.release();
+    });
+    return out;
+}
+
+int tvara_tree_plan_launch(tvara_tree_plan* plan, size_t layer, const float* q, const float* keys, const float* values,
+                           size_t row_stride, float* out, void* stream) {
+    return guard([&] {
+        if (!plan) throw std::invalid_argument("null tree plan");
+        if (plan->plan.rows && (!q || !keys || !values || !out)) throw std::invalid_argument("invalid fused attention shape");
+        if (!aligned16(q) || !aligned16(keys) || !aligned16(values) || !aligned16(out) || row_stride % 4)
+            throw std::invalid_argument("device buffers must be 16-byte aligned");
+        if (layer > static_cast<size_t>(std::numeric_limits<int>::max()))
+            throw std::invalid_argument("invalid fused attention shape");
+        hipStream_t s = stream ? static_cast<hipStream_t>(stream) : plan->plan.cache->stream();
+        plan->plan.launch(static_cast<int>(layer), q, keys, values, row_stride, out, s);
+    });
+}
+
+int tvara_tree_plan_accept(tvara_tree_plan* plan, const uint32_t* tokens, const uint32_t* first, const float* logits,
+                           size_t vocab, size_t logits_stride, int32_t* path, size_t path_stride, int32_t* accepted,
+                           uint32_t* next, void* stream) {
+    return guard([&] {
+        if (!plan) throw std::invalid_argument("null tree plan");
+        if (!first || !accepted || !next || (path_stride && !path) || (plan->plan.rows && (!tokens || !logits)))
+            throw std::invalid_argument("null acceptance buffers");
+        if (!aligned16(tokens) || !aligned16(first) || !aligned16(logits) || !aligned16(path) || !aligned16(accepted) ||
+            !aligned16(next))
+            throw std::invalid_argument("device buffers must be 16-byte aligned");
+        hipStream_t s = stream ? static_cast<hipStream_t>(stream) : plan->plan.cache->stream();
+        plan->plan.accept(tokens, first, logits, vocab, logits_stride, path, path_stride, accepted, next, s);
+    });
+}
+
+int tvara_tree_plan_check(tvara_tree_plan* plan) {
+    return guard([&] {
+        if (!plan) throw std::invalid_argument("null tree plan");
+        plan->plan.check();
+    });
+}
+
+void tvara_tree_plan_destroy(tvara_tree_plan* plan) { delete plan; }
+
+int tvara_attn_tree(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, size_t layer, size_t heads,
+                    size_t context, const size_t* visible, const size_t* nodes, const int32_t* parents, const float* q,
+                    const float* keys, const float* values, float* out, int precision, int device_ptrs) {
+    return guard([&] {
+        auto& c = live(cache);
+        tvara_amd::check_attention_config(c, heads, context);
+        if (!count) return;
+        if (layer >= c.geometry().layers) throw std::invalid_argument("invalid fused attention shape");
+        tvara_amd::TreePlan plan;
+        plan.build(&c, sequences, count, heads, context, visible, nodes, parents, precision);
+        if (!plan.rows) return;
+        if (!q || !keys || !values || !out) throw std::invalid_argument("invalid fused attention shape");
+        hipStream_t s = c.stream();
+        if (device_ptrs) {
+            if (!aligned16(q) || !aligned16(keys) || !aligned16(values) || !aligned16(out))
+                throw std::invalid_argument("device buffers must be 16-byte aligned");
+            plan.launch(static_cast<int>(layer), q, keys, values, 0, out, s);
+            plan.check();
+            return;
+        }
+        // q | keys | values in one copy in, each on 16 bytes; the output comes back through pinned memory
+        const size_t nq = plan.rows * heads * c.geometry().head_dim, nk = plan.rows * c.geometry().kv_width();
+        const size_t k_at = (nq + 3) / 4 * 4, v_at = k_at + (nk + 3) / 4 * 4, o_at = v_at + (nk + 3) / 4 * 4;
+        tvara_amd::HostCopier& copier = tvara_amd::HostCopier::shared();
+        std::lock_guard<std::mutex> hold(copier.lock());
+        auto* in = static_cast<float*>(cache->io_in.acquire(o_at * sizeof(float)));
+        auto stage = [&](float* to, const float* from, size_t n) {
+            copier.parallel_copy(reinterpret_cast<char*>(to), reinterpret_cast<const char*>(from), n * sizeof(float));
+        };
+        stage(in, q, nq);
+        stage(in + k_at, keys, nk);
+        stage(in + v_at, values, nk);
+        auto* d = static_cast<float*>(cache->io.ensure((o_at + nq) * sizeof(float)));
+        TVARA_HIP(hipMemcpyAsync(d, in, o_at * sizeof(float), hipMemcpyHostToDevice, s));
+        cache->io_in.release(s);
+        plan.launch(static_cast<int>(layer), d, d + k_at, d + v_at, 0, d + o_at, s);
+        auto* back = static_cast<float*>(cache->io_out.acquire(nq * sizeof(float)));
+        TVARA_HIP(hipMemcpyAsync(back, d + o_at, nq * sizeof(float), hipMemcpyDeviceToHost, s));
+        plan.check();
+        stage(out, back, nq);
+    });
+}
+
+tvara_slot_plan* tvara_slot_plan_create(tvara_kv_cache* cache, const uint64_t* sequences, size_t count) {
+    tvara_slot_plan* out = nullptr;
+    guard([&] {
+        auto& c = live(cache);
+        auto p = std::make_unique<tvara_slot_plan>();
+        p->plan.build(&c, sequences, count);
+        out = p.release();
+    });
+    return out;
+}
+
+int tvara_slot_plan_build(tvara_slot_plan* plan, const int32_t* starts, const int32_t* counts, size_t stride,
+                          size_t capacity, int32_t* offsets, int32_t* positions, int64_t* slots, int32_t* tables,
+                          size_t width, void* stream) {
+    return guard([&] {
+        if (!plan) throw std::invalid_argument("null slot plan");
+        if (!starts || !counts) throw std::invalid_argument("null slot map lengths");
+        if (!aligned16(starts) || !aligned16(counts) || !aligned16(offsets) || !aligned16(positions) ||
+            !aligned16(slots) || !aligned16(tables))
+            throw std::invalid_argument("device buffers must be 16-byte aligned");
+        hipStream_t s = stream ? static_cast<hipStream_t>(stream) : plan->plan.cache->stream();
+        plan->plan.map(starts, counts, stride, capacity, offsets, positions, slots, tables, width, s);
+    });
+}
+
+int tvara_slot_plan_write(tvara_slot_plan* plan, const int64_t* slots, const int32_t* rows, size_t n, const float* keys,
+                          const float* values, size_t row_count, size_t row_stride, size_t layer_stride, void* stream) {
+    return guard([&] {
+        if (!plan) throw std::invalid_argument("null slot plan");
+        if (n && (!slots || !keys || !values)) throw std::invalid_argument("null KV write buffers");
+        if (!aligned16(slots) || !aligned16(rows) || !aligned16(keys) || !aligned16(values))
+            throw std::invalid_argument("device buffers must be 16-byte aligned");
+        hipStream_t s = stream ? static_cast<hipStream_t>(stream) : plan->plan.cache->stream();
+        plan->plan.write(slots, rows, n, keys, values, row_count, row_stride, layer_stride, s);
+    });
+}
+
+int tvara_slot_plan_check(tvara_slot_plan* plan) {
+    return guard([&] {
+        if (!plan) throw std::invalid_argument("null slot plan");
+        plan->plan.check();
+    });
+}
+
+void tvara_slot_plan_destroy(tvara_slot_plan* plan) { delete plan; }
 
 // ------------------------------------------------------- model-level exports
 // c_api.cpp:35-78: return conventions (nullptr / 0 / -1), messages and the

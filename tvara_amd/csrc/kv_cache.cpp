@@ -65,6 +65,7 @@ DeviceCache::DeviceCache(const Geometry& g, int format) : meta_(g), format_(form
     if (lay_.stride > kMax / geo.max_blocks) throw std::invalid_argument("KV capacity overflow");
     int dev = 0;
     TVARA_HIP(hipGetDevice(&dev));
+    device_ = dev;
     TVARA_HIP(hipDeviceGetAttribute(&cus_, hipDeviceAttributeMultiprocessorCount, dev));
     if (hipDeviceGetAttribute(&xcds_, hipDeviceAttributeNumberOfXccs, dev) != hipSuccess || xcds_ < 1) xcds_ = 1;
     TVARA_HIP(hipMalloc(&pool_, lay_.stride * geo.max_blocks));
@@ -84,6 +85,12 @@ DeviceCache::~DeviceCache() {
 size_t DeviceCache::canonical_block_bytes() const {
     const size_t elements = geometry().elements_per_block();
     return format_ == kF32 ? elements * sizeof(float) : elements / 32 * 34;
+}
+
+void DeviceCache::check_device() const {
+    int dev = 0;
+    TVARA_HIP(hipGetDevice(&dev));
+    if (dev != device_) throw std::invalid_argument("the KV cache is on another device");
 }
 
 void DeviceCache::synchronize() { TVARA_HIP(hipStreamSynchronize(stream_)); }
@@ -225,6 +232,25 @@ const RowOp* DeviceCache::reserve_tokens(uint64_t seq, size_t count) {
     if (w.applied) run_block_init(w.init);
     if (w.failure) std::rethrow_exception(w.failure);
     return upload(*this, kRowOps, w.rows.data(), w.rows.size());
+}
+
+void DeviceCache::reserve(const uint64_t* seqs, size_t n, const size_t* tokens) {
+    if (n && (!seqs || !tokens)) throw std::invalid_argument("invalid KV reservation");
+    std::vector<uint64_t> list;
+    std::vector<size_t> lengths(n);
+    const Geometry& g = geometry();
+    for (size_t i = 0; i < n; ++i) {
+        lengths[i] = sequence(seqs[i]).length;
+        // (more than the pool holds: refused before a list of that size is made)
+        if (tokens[i] > g.max_blocks * g.tokens_per_block) throw CacheExhausted();
+        list.insert(list.end(), tokens[i], seqs[i]);
+    }
+    AppendWork w = meta_.plan_appends(list.data(), list.size());
+    if (w.applied) run_block_init(w.init);
+    if (w.failure) {
+        for (size_t i = 0; i < n; ++i) meta_.truncate(seqs[i], lengths[i]);
+        std::rethrow_exception(w.failure);
+    }
 }
 
 void DeviceCache::write_layer_rows(const RowOp* ops, size_t n, int layer, const float* keys, const float* values) {

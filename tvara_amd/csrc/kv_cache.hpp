@@ -32,6 +32,8 @@ public:
     const std::shared_ptr<PlanPool>& plan_pool() const { return plans_; }
     uint64_t epoch() const { return meta_.epoch(); }
     int compute_units() const { return cus_; }
+    // throws where another device than the cache's is the current one
+    void check_device() const;
     int xcds() const { return xcds_; }  // XCDs (L2 domains) the workgroups are dealt over
     void synchronize();
 
@@ -74,6 +76,11 @@ public:
     // appends that took effect still runs, then the error is rethrown and the
     // caller truncates.
     const RowOp* reserve_tokens(uint64_t seq, size_t count);
+    // Room for tokens[i] more tokens at the end of sequences[i], in order: the
+    // ledger's appends and their block work, with no rows written (new blocks
+    // are zeros, slots of a block that was there keep what they held).  All or
+    // nothing: a failure leaves every sequence at its entry length.
+    void reserve(const uint64_t* seqs, size_t n, const size_t* tokens);
     // layer `layer`'s K and V rows ([n][kv_width] floats, row i for the
     // token of ops[i]) into their slots
     void write_layer_rows(const RowOp* ops, size_t n, int layer, const float* keys, const float* values);
@@ -110,7 +117,7 @@ private:
     BlockLayout lay_{};
     char* pool_ = nullptr;
     hipStream_t stream_ = nullptr;
-    int cus_ = 256, xcds_ = 1;
+    int cus_ = 256, xcds_ = 1, device_ = 0;
     hipEvent_t ordered_[2] = {nullptr, nullptr};
     std::shared_ptr<PlanPool> plans_ = std::make_shared<PlanPool>();
     DeviceBuffer scratch_[6];

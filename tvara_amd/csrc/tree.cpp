@@ -1,0 +1,327 @@
+// Plans of speculative decoding with token trees (tree.hpp): what the host
+// checks and lays out; the kernels are in tree.hip, tree_accept.hip and slots.hip.
+#include "tree.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <limits>
+#include <map>
+
+namespace tvara_amd {
+
+namespace {
+constexpr size_t kIntMax = static_cast<size_t>(std::numeric_limits<int32_t>::max());
+
+size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+}  // namespace
+
+// ------------------------------------------------------------ the region
+
+PlanRegion::~PlanRegion() {
+    if (buf_ && home_ && null_stream_) home_->give(std::move(buf_));
+}
+
+void PlanRegion::place(DeviceCache& c, std::vector<Section>& sections) {
+    size_t total = 0, copied = 0;
+    for (Section& s : sections) {
+        s.at = total;
+        total = round_up(total + std::max<size_t>(s.bytes, 1), 256);
+        if (s.data) copied = total;
+    }
+    hipStream_t s = c.stream();
+    null_stream_ = s == nullptr;
+    home_ = c.plan_pool();
+    buf_ = s ? std::make_unique<PlanPool::Set>() : home_->take(total);
+    try {
+        buf_->region.ensure(total);
+    } catch (const std::runtime_error&) {  // no memory, unless closed plans hold some
+        (void)hipGetLastError();
+        home_->clear();
+        buf_->region.ensure(total);
+    }
+    if (copied) {
+        char* host = static_cast<char*>(buf_->staging.acquire(copied));
+        std::memset(host, 0, copied);
+        for (const Section& x : sections)
+            if (x.data && x.bytes) std::memcpy(host + x.at, x.data, x.bytes);
+        TVARA_HIP(hipMemcpyAsync(device(), host, copied, hipMemcpyHostToDevice, s));
+        buf_->staging.release(s);
+    }
+    auto* f = static_cast<volatile int*>(buf_->flag.acquire(kFlags * sizeof(int)));
+    for (int i = 0; i < kFlags; ++i) f[i] = 0;
+    last_ = s;
+}
+
+void PlanRegion::launched(hipStream_t s) {
+    null_stream_ &= s == nullptr;
+    last_ = s;
+}
+
+int PlanRegion::check() {
+    TVARA_HIP(hipStreamSynchronize(last_));
+    auto* f = static_cast<volatile int*>(buf_->flag.ptr);
+    int set = 0;
+    for (int i = 0; i < kFlags; ++i) {
+        if (f[i]) set |= 1 << i;
+        f[i] = 0;
+    }
+    return set;
+}
+
+// -------------------------------------------------------------- the trees
+
+void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t h, size_t context,
+                     const size_t* visible, const size_t* nodes, const int32_t* parents, int prec) {
+    cache = c;
+    const Geometry& g = c->geometry();
+    c->check_device();
+    if (!n || !sequences || !nodes) throw std::invalid_argument("empty tree plan");
+    if (prec != 0 && prec != 2) throw std::invalid_argument("tree attention is f32 or f32x3");
+    heads = static_cast<int>(h);
+    group = static_cast<int>(h / g.kv_heads);
+    precision = prec;
+    count = n;
+    rows = 0;
+    size_t most = 0;
+    for (size_t i = 0; i < n; ++i) {
+        if (nodes[i] > kMaxTreeNodes) throw std::invalid_argument("a token tree has at most 1,024 nodes");
+        rows += nodes[i];
+        most = std::max(most, nodes[i]);
+        if (rows > kIntMax / h) throw std::invalid_argument("attention batch too large");
+    }
+    if (rows && !parents) throw std::invalid_argument("invalid token tree");
+    words = static_cast<int>(std::max<size_t>(1, (most + 31) / 32));
+
+    std::vector<int4> trees(n);
+    std::vector<uint32_t> mask(rows * words, 0);
+    std::vector<int32_t> tab;
+    std::map<uint64_t, int32_t> offset;
+    std::vector<size_t> depth(most);
+    size_t row0 = 0;
+    for (size_t i = 0; i < n; ++i) {
+        const Table& t = c->sequence(sequences[i]);
+        const size_t seen = visible ? std::min(visible[i], t.length) : t.length;
+        if (seen > kIntMax - kMaxTreeNodes) throw std::invalid_argument("sequence too long for the device kernels");
+        if (seen > context) throw std::invalid_argument("invalid fused attention shape");
+        for (size_t j = 0; j < nodes[i]; ++j) {
+            const int32_t p = parents[row0 + j];
+            if (p < -1 || p >= static_cast<int32_t>(j)) throw std::invalid_argument("invalid token tree");
+            uint32_t* m = &mask[(row0 + j) * words];
+            if (p >= 0) std::copy_n(&mask[(row0 + p) * words], words, m);
+            m[j / 32] |= 1u << (j % 32);
+            depth[j] = p < 0 ? 1 : depth[p] + 1;
+            if (depth[j] > context - seen) throw std::invalid_argument("token tree exceeds the context");
+        }
+        if (!offset.count(sequences[i])) {
+            offset[sequences[i]] = static_cast<int32_t>(tab.size());
+            for (const Handle& b : t.blocks) tab.push_back(static_cast<int32_t>(b.id));
+            if (tab.size() > kIntMax) throw std::invalid_argument("attention batch too large");
+        }
+        trees[i] = make_int4(offset[sequences[i]], static_cast<int>(seen), static_cast<int>(nodes[i]), static_cast<int>(row0));
+        row0 += nodes[i];
+    }
+    epoch = c->epoch();
+
+    // Runs of cached tokens, so that a long context fills the chip: about four
+    // waves a SIMD, 64 tokens or more each; the last run takes the tree's own.
+    std::vector<int4> work;
+    std::vector<int2> runs(rows);
+    size_t total = 0;
+    for (const int4& t : trees) total += static_cast<size_t>(t.y) * t.z;
+    const size_t target = static_cast<size_t>(c->compute_units()) * 16 / std::max<size_t>(1, h);
+    const size_t split = std::min(round_up(std::max<size_t>(total / std::max<size_t>(1, target), 64), 64), kIntMax / 2);
+    split_tokens = static_cast<int>(split);
+    slots = 0;
+    for (size_t i = 0; i < n; ++i) {
+        const int4& t = trees[i];
+        const int parts = static_cast<int>(std::max<size_t>(1, (static_cast<size_t>(t.y) + split - 1) / split));
+        for (int j = 0; j < t.z; ++j) {
+            runs[t.w + j] = make_int2(static_cast<int>(slots), parts);
+            if (parts > 1) slots += parts;
+            for (int p = 0; p < parts; ++p) work.push_back(make_int4(static_cast<int>(i), j, p, parts));
+        }
+        if (slots > kIntMax / h || work.size() > kIntMax) throw std::invalid_argument("attention batch too large");
+    }
+    items = static_cast<int>(work.size());
+
+    std::vector<PlanRegion::Section> s = {
+        {tab.data(), tab.size() * sizeof(int32_t)},   {trees.data(), n * sizeof(int4)},
+        {mask.data(), mask.size() * sizeof(uint32_t)}, {work.data(), work.size() * sizeof(int4)},
+        {runs.data(), runs.size() * sizeof(int2)},     {parents, rows * sizeof(int32_t)},
+        {nullptr, slots * h * g.head_dim * sizeof(float)}, {nullptr, slots * h * 2 * sizeof(float)},
+        {nullptr, std::max(rows, kAcceptParts) * sizeof(uint64_t)},
+    };
+    region.place(*c, s);
+    size_t* at[] = {&tables_at, &trees_at, &mask_at, &work_at, &runs_at, &parents_at, &acc_at, &ml_at, &best_at};
+    for (size_t i = 0; i < s.size(); ++i) *at[i] = s[i].at;
+}
+
+void TreePlan::launch(int layer, const float* q, const float* keys, const float* values, size_t row_stride, float* out,
+                      hipStream_t s) {
+    if (cache->epoch() != epoch) throw std::invalid_argument("tree plan is stale: the cache changed");
+    const Geometry& g = cache->geometry();
+    if (layer < 0 || static_cast<size_t>(layer) >= g.layers) throw std::invalid_argument("invalid fused attention shape");
+    if (!row_stride) row_stride = g.kv_width();
+    if (row_stride < g.kv_width()) throw std::invalid_argument("token rows overlap");
+    if (!rows) return;
+    cache->check_device();
+    cache->flush();
+    cache->enter(s);
+    char* d = region.device();
+    TreeArgs a{};
+    a.pool = cache->pool();
+    a.lay = cache->layout();
+    a.layer = layer;
+    a.heads = heads;
+    a.group = group;
+    a.tables = reinterpret_cast<const int32_t*>(d + tables_at);
+    a.trees = reinterpret_cast<const int4*>(d + trees_at);
+    a.mask = reinterpret_cast<const uint32_t*>(d + mask_at);
+    a.words = words;
+    a.work = reinterpret_cast<const int4*>(d + work_at);
+    a.split_tokens = split_tokens;
+    a.runs = reinterpret_cast<const int2*>(d + runs_at);
+    a.rows = static_cast<int>(rows);
+    a.q = q;
+    a.keys = keys;
+    a.values = values;
+    a.row_stride = row_stride;
+    a.out = out;
+    a.part_acc = reinterpret_cast<float*>(d + acc_at);
+    a.part_ml = reinterpret_cast<float*>(d + ml_at);
+    a.qscale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(g.head_dim)));
+    a.err = region.flags();
+    launch_tree_rows(a, items, s);
+    if (slots) launch_tree_merge(a, s);
+    cache->leave(s);
+    region.launched(s);
+}
+
+void TreePlan::accept(const uint32_t* tokens, const uint32_t* first, const float* logits, size_t vocab,
+                      size_t logits_stride, int32_t* path, size_t path_stride, int32_t* accepted, uint32_t* next,
+                      hipStream_t s) {
+    if (!vocab || vocab > kIntMax) throw std::invalid_argument("invalid vocabulary");
+    if (!logits_stride) logits_stride = vocab;
+    if (logits_stride < vocab) throw std::invalid_argument("logit rows overlap");
+    cache->check_device();
+    AcceptArgs a{};
+    char* d = region.device();
+    a.trees = reinterpret_cast<const int4*>(d + trees_at);
+    a.parents = reinterpret_cast<const int32_t*>(d + parents_at);
+    a.count = static_cast<int>(count);
+    a.rows = static_cast<int>(rows);
+    a.tokens = tokens;
+    a.first = first;
+    a.logits = logits;
+    a.vocab = vocab;
+    a.logits_stride = logits_stride;
+    a.splits = tree_accept_splits(rows, vocab);
+    a.best = reinterpret_cast<uint64_t*>(d + best_at);
+    a.path = path;
+    a.path_stride = path_stride;
+    a.accepted = accepted;
+    a.next = next;
+    a.err = region.flags() + 1;
+    cache->enter(s);  // (the plan's upload)
+    launch_tree_accept(a, s);
+    cache->leave(s);
+    region.launched(s);
+}
+
+void TreePlan::check() {
+    const int set = region.check();
+    if (set & 1) throw std::invalid_argument("invalid online attention input");
+    if (set & 2) throw std::invalid_argument("invalid logits or path of a token tree");
+}
+
+// -------------------------------------------------------------- the slots
+
+void SlotPlan::build(DeviceCache* c, const uint64_t* sequences, size_t n) {
+    cache = c;
+    c->check_device();
+    if (!n || !sequences) throw std::invalid_argument("empty slot plan");
+    if (n > 65535) throw std::invalid_argument("a slot plan has at most 65,535 sequences");
+    count = n;
+    std::vector<int32_t> ids;
+    std::vector<int2> seqs(n);
+    for (size_t i = 0; i < n; ++i) {
+        const Table& t = c->sequence(sequences[i]);
+        if (ids.size() + t.blocks.size() > kIntMax) throw std::invalid_argument("slot plan too large");
+        seqs[i] = make_int2(static_cast<int>(ids.size()), static_cast<int>(t.blocks.size()));
+        // a block that others hold too is not this sequence's to write
+        for (const Handle& b : t.blocks) {
+            const uint32_t shared = c->references(b) > 1 ? 0x80000000u : 0u;
+            ids.push_back(static_cast<int32_t>(static_cast<uint32_t>(b.id) | shared));
+        }
+    }
+    epoch = c->epoch();
+    std::vector<PlanRegion::Section> s = {{ids.data(), ids.size() * sizeof(int32_t)}, {seqs.data(), n * sizeof(int2)}};
+    region.place(*c, s);
+    seqs_at = s[1].at;
+}
+
+void SlotPlan::map(const int32_t* starts, const int32_t* counts, size_t stride, size_t capacity, int32_t* offsets,
+                   int32_t* positions, int64_t* slots, int32_t* tables, size_t width, hipStream_t s) {
+    if (cache->epoch() != epoch) throw std::invalid_argument("slot plan is stale: the cache changed");
+    if (capacity > kIntMax || stride > kIntMax || width > kIntMax || (tables && width > kIntMax / count))
+        throw std::invalid_argument("slot map too large");
+    if (stride && capacity < stride * count) throw std::invalid_argument("slot map smaller than its sequences");
+    cache->check_device();
+    cache->enter(s);
+    SlotArgs a{};
+    a.ids = reinterpret_cast<const int32_t*>(region.device());
+    a.seqs = reinterpret_cast<const int2*>(region.device() + seqs_at);
+    a.count = static_cast<int>(count);
+    a.tpb = cache->layout().tpb;
+    a.starts = starts;
+    a.counts = counts;
+    a.stride = stride;
+    a.capacity = capacity;
+    a.offsets = offsets;
+    a.positions = positions;
+    a.slots = slots;
+    a.tables = tables;
+    a.width = width;
+    a.err = region.flags();
+    launch_slot_map(a, s);
+    cache->leave(s);
+    region.launched(s);
+}
+
+void SlotPlan::write(const int64_t* slots, const int32_t* rows, size_t n, const float* keys, const float* values,
+                     size_t row_count, size_t row_stride, size_t layer_stride, hipStream_t s) {
+    if (cache->epoch() != epoch) throw std::invalid_argument("slot plan is stale: the cache changed");
+    const Geometry& g = cache->geometry();
+    if (n > kIntMax || row_count > kIntMax) throw std::invalid_argument("KV write too large");
+    if (row_stride < g.kv_width() || (g.layers > 1 && layer_stride < g.kv_width()))
+        throw std::invalid_argument("token rows overlap");
+    if (!n) return;
+    cache->check_device();
+    cache->flush();
+    cache->enter(s);
+    WriteArgs a{};
+    a.pool = cache->pool();
+    a.lay = cache->layout();
+    a.slot_count = static_cast<int64_t>(g.max_blocks * g.tokens_per_block);
+    a.slots = slots;
+    a.rows = rows;
+    a.n = n;
+    a.row_count = row_count;
+    a.keys = keys;
+    a.values = values;
+    a.row_stride = row_stride;
+    a.layer_stride = layer_stride;
+    a.err = region.flags() + 1;
+    launch_slot_write(a, s);
+    cache->leave(s);
+    region.launched(s);
+}
+
+void SlotPlan::check() {
+    const int set = region.check();
+    if (set & 1) throw std::invalid_argument("slot map outside the sequences' own blocks");
+    if (set & 2) throw std::invalid_argument("KV write outside the pool or the rows");
+}
+
+}  // namespace tvara_amd

@@ -1,0 +1,151 @@
+// Attention of token trees over the paged cache: row r of a tree attends to
+// the sequence's cached tokens, the nodes above it and itself,
+//   o = sum_k p_k v_k,  p = softmax_k(q . k / sqrt(d)),
+// with the nodes' K/V in rows of their own, outside the cache (they join it only
+// when they are accepted).
+#include "common.hpp"
+#include "device_util.hpp"
+#include "q8.hpp"
+#include "tree.hpp"
+
+namespace tvara_amd {
+namespace {
+
+constexpr int kMaxDim = 512;
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// element `column` of a cached K (kind 0) or V row
+__device__ __forceinline__ float cached_element(const TreeArgs& a, int block, int kind, int slot, int column) {
+    const char* base = a.pool + static_cast<size_t>(block) * a.lay.stride;
+    const size_t sec = static_cast<size_t>(a.layer) * 2 + kind;
+    if (a.lay.format == kF32)
+        return reinterpret_cast<const float*>(base)[(sec * a.lay.tpb + slot) * a.lay.kv_width + column];
+    const char* s = base + sec * a.lay.section;
+    const int8_t q = reinterpret_cast<const int8_t*>(s)[q8_byte_offset(a.lay, slot, column)];
+    return half_bits_to_float(*reinterpret_cast<const uint16_t*>(s + q8_scale_offset(a.lay, slot, column / 32))) *
+           static_cast<float>(q);
+}
+
+// Any head_dim and block size, f32 arithmetic: a wave per (run of a node's
+// cached tokens, query head); lanes are keys for the scores and columns for the
+// output.  A work item is x: tree, y: node, z: run, w: runs; the last run takes
+// the tree's nodes.
+__global__ __launch_bounds__(64) void tree_rows_kernel(const TreeArgs a) {
+    __shared__ float qs[kMaxDim];
+    const int lane = threadIdx.x, h = blockIdx.y, kh = h / a.group;
+    const int D = a.lay.head_dim, tpb = a.lay.tpb;
+    const int4 it = a.work[blockIdx.x], tree = a.trees[it.x];
+    const size_t row = static_cast<size_t>(tree.w) + it.y;
+    const int k0 = it.z * a.split_tokens, k1 = it.z + 1 == it.w ? tree.y : k0 + a.split_tokens;
+    const int cached = k1 - k0, keys = cached + (it.z + 1 == it.w ? it.y + 1 : 0);
+    const int32_t* tab = a.tables + tree.x;
+    const uint32_t* mask = a.mask + row * a.words;
+    const float* qr = a.q + (row * a.heads + h) * D;
+    for (int d = lane; d < D; d += 64) qs[d] = qr[d] * a.qscale;
+    __syncthreads();
+    auto node_row = [&](const float* rows, int node) {
+        return rows + (static_cast<size_t>(tree.w) + node) * a.row_stride + static_cast<size_t>(kh) * D;
+    };
+    auto seen = [&](int j) {
+        if (j >= keys) return false;
+        const int node = j - cached;
+        return node < 0 || (mask[node >> 5] >> (node & 31) & 1);
+    };
+    float m = -INFINITY, l = 0.f, acc[kMaxDim / 64];
+#pragma unroll
+    for (int i = 0; i < kMaxDim / 64; ++i) acc[i] = 0.f;
+    bool bad = false;
+    for (int base = 0; base < keys; base += 64) {
+        const int j = base + lane;
+        const bool ok = seen(j);
+        float s = -INFINITY;
+        if (ok) {
+            s = 0.f;
+            if (j < cached) {
+                const int p = k0 + j, block = tab[p / tpb], slot = p % tpb;
+                for (int d = 0; d < D; ++d) s = fmaf(qs[d], cached_element(a, block, 0, slot, kh * D + d), s);
+            } else {
+                const float* k = node_row(a.keys, j - cached);
+                for (int d = 0; d < D; ++d) s = fmaf(qs[d], k[d], s);
+            }
+            bad |= !__builtin_isfinite(s);
+        }
+        float mx = s;
+        for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+        const float mnew = fmaxf(m, mx);
+        if (mnew == -INFINITY) continue;  // no key seen yet
+        const float alpha = fast_exp2(m - mnew), pj = ok ? fast_exp2(s - mnew) : 0.f;
+        float ps = pj;
+        for (int o = 32; o >= 1; o >>= 1) ps += __shfl_xor(ps, o);
+        l = l * alpha + ps;
+        m = mnew;
+#pragma unroll
+        for (int i = 0; i < kMaxDim / 64; ++i) acc[i] *= alpha;
+        uint64_t left = __ballot(ok);  // values of keys that are not seen are not read
+        while (left) {
+            const int jj = __builtin_ctzll(left);
+            left &= left - 1;
+            const float w = __shfl(pj, jj);
+            const int p = k0 + base + jj;
+            const float* v = base + jj < cached ? nullptr : node_row(a.values, base + jj - cached);
+            const int block = v ? 0 : tab[p / tpb], slot = p % tpb;
+#pragma unroll
+            for (int i = 0; i < kMaxDim / 64; ++i) {
+                const int d = i * 64 + lane;
+                if (d < D) acc[i] = fmaf(w, v ? v[d] : cached_element(a, block, 1, slot, kh * D + d), acc[i]);
+            }
+        }
+    }
+    if (__any(bad) && lane == 0) *a.err = 1;
+    const bool whole = it.w == 1;
+    const size_t at = whole ? row * a.heads + h : (static_cast<size_t>(a.runs[row].x) + it.z) * a.heads + h;
+    float* o = (whole ? a.out : a.part_acc) + at * D;
+    const float inv = whole ? l : 1.f;
+#pragma unroll
+    for (int i = 0; i < kMaxDim / 64; ++i) {
+        const int d = i * 64 + lane;
+        if (d < D) o[d] = acc[i] / inv;
+    }
+    if (!whole && lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(m, l);
+}
+
+// A row's runs combined in order: a thread per two columns.
+__global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
+    const int D = a.lay.head_dim, half = D / 2;
+    const size_t t = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x, at = t / half;
+    if (at >= static_cast<size_t>(a.rows) * a.heads) return;
+    const int2 runs = a.runs[at / a.heads];
+    if (runs.y == 1) return;
+    const int c = 2 * static_cast<int>(t % half), h = static_cast<int>(at % a.heads);
+    float m = -INFINITY, l = 0.f;
+    float2 sum = make_float2(0.f, 0.f);
+    for (int r = 0; r < runs.y; ++r) {
+        const size_t p = (static_cast<size_t>(runs.x) + r) * a.heads + h;
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
+        if (ml.x == -INFINITY) continue;
+        const float2 x = *reinterpret_cast<const float2*>(a.part_acc + p * D + c);
+        const float mn = fmaxf(m, ml.x), wm = fast_exp2(m - mn), wr = fast_exp2(ml.x - mn);
+        l = l * wm + ml.y * wr;
+        sum.x = sum.x * wm + x.x * wr;
+        sum.y = sum.y * wm + x.y * wr;
+        m = mn;
+    }
+    *reinterpret_cast<float2*>(a.out + at * D + c) = make_float2(sum.x / l, sum.y / l);
+}
+
+}  // namespace
+
+void launch_tree_rows(const TreeArgs& a, int items, hipStream_t s) {
+    if (a.lay.head_dim > kMaxDim) throw std::invalid_argument("head_dim above 512 is not supported");
+    launch("tree_attention", tree_rows_kernel, dim3(items, a.heads), dim3(64), 0, s, a);
+    TVARA_HIP(hipGetLastError());
+}
+
+void launch_tree_merge(const TreeArgs& a, hipStream_t s) {
+    const size_t threads = static_cast<size_t>(a.rows) * a.heads * (a.lay.head_dim / 2);
+    launch("tree_attention_merge", tree_merge_kernel, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, s, a);
+    TVARA_HIP(hipGetLastError());
+}
+
+}  // namespace tvara_amd

@@ -256,6 +256,20 @@ class PagedCache:
         self._check(rc)
         return applied.value
 
+    def reserve(self, seqs, tokens):
+        """Room for tokens[i] more tokens at the end of seqs[i], with no rows
+        written (SlotPlan.write does); all or nothing."""
+        seqs = np.ascontiguousarray(seqs, dtype=np.uint64).reshape(-1)
+        tokens = np.ascontiguousarray(np.broadcast_to(np.asarray(tokens, dtype=np.uintp), seqs.shape))
+        self._check(self.lib.tvara_kv_reserve(self.h, seqs.ctypes.data_as(_u64p), seqs.size,
+                                              tokens.ctypes.data_as(C.POINTER(C.c_size_t))))
+
+    def pool_address(self):
+        """(device address of block 0, bytes from one block to the next)"""
+        base, stride = C.c_void_p(), C.c_size_t()
+        self._check(self.lib.tvara_kv_pool_address(self.h, C.byref(base), C.byref(stride)))
+        return base.value, stride.value
+
     def read(self, seq, layer, position, value=False):
         out = np.empty(self.kv_width, np.float32)
         self._check(self.lib.tvara_kv_read(self.h, seq, layer, position, int(value), _ptr(out)))
@@ -335,3 +349,42 @@ class PagedCache:
         from .attention import fused_prompt_attention
 
         return fused_prompt_attention(queries, self, seq, layer, start, count, heads, context, precision)
+
+
+class SlotPlan:
+    """Resident block ids of listed sequences (tvara_slot_plan_*): slot maps and
+    block tables from device lengths, and K/V writes through them.  Pointers
+    are device addresses (ints); launches are asynchronous."""
+
+    def __init__(self, cache, seqs):
+        self.cache = cache
+        self.lib = cache.lib
+        seqs = np.ascontiguousarray(seqs, dtype=np.uint64).reshape(-1)
+        self.h = self.lib.tvara_slot_plan_create(cache.h, seqs.ctypes.data_as(_u64p), seqs.size)
+        if not self.h:
+            _capi.raise_last(self.lib)
+
+    def build(self, starts_ptr, counts_ptr, stride, capacity, offsets_ptr=None, positions_ptr=None, slots_ptr=None,
+              tables_ptr=None, width=0, stream=None):
+        """Offsets [n + 1], positions and slots [capacity] of counts[i] (int32)
+        tokens from position starts[i] on, packed (stride 0) or stride entries a
+        sequence, -1 where there is none; tables [n, width] of block ids."""
+        _capi.check(self.lib.tvara_slot_plan_build(self.h, starts_ptr, counts_ptr, stride, capacity, offsets_ptr,
+                                                   positions_ptr, slots_ptr, tables_ptr, width, stream), self.lib)
+
+    def write(self, slots_ptr, rows_ptr, n, keys_ptr, values_ptr, row_count, row_stride, layer_stride, stream=None):
+        """K/V rows of every layer into slots (int64; -1: skipped), entry t from
+        row rows[t] (int32; None: row t) of row_count."""
+        _capi.check(self.lib.tvara_slot_plan_write(self.h, slots_ptr, rows_ptr, n, keys_ptr, values_ptr, row_count,
+                                                   row_stride, layer_stride, stream), self.lib)
+
+    def check(self):
+        _capi.check(self.lib.tvara_slot_plan_check(self.h), self.lib)
+
+    def close(self):
+        if getattr(self, "h", None):
+            self.lib.tvara_slot_plan_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        self.close()
