@@ -123,27 +123,16 @@ void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t
     }
     epoch = c->epoch();
 
-    // Runs of cached tokens, so that a long context fills the chip: about four
-    // waves a SIMD, 64 tokens or more each; the last run takes the tree's own.
     std::vector<int4> work;
     std::vector<int2> runs(rows);
-    size_t total = 0;
-    for (const int4& t : trees) total += static_cast<size_t>(t.y) * t.z;
-    const size_t target = static_cast<size_t>(c->compute_units()) * 16 / std::max<size_t>(1, h);
-    const size_t split = std::min(round_up(std::max<size_t>(total / std::max<size_t>(1, target), 64), 64), kIntMax / 2);
-    split_tokens = static_cast<int>(split);
     slots = 0;
-    for (size_t i = 0; i < n; ++i) {
-        const int4& t = trees[i];
-        const int parts = static_cast<int>(std::max<size_t>(1, (static_cast<size_t>(t.y) + split - 1) / split));
-        for (int j = 0; j < t.z; ++j) {
-            runs[t.w + j] = make_int2(static_cast<int>(slots), parts);
-            if (parts > 1) slots += parts;
-            for (int p = 0; p < parts; ++p) work.push_back(make_int4(static_cast<int>(i), j, p, parts));
-        }
-        if (slots > kIntMax / h || work.size() > kIntMax) throw std::invalid_argument("attention batch too large");
-    }
-    items = static_cast<int>(work.size());
+    tile_rows = tree_tiles_supported(c->layout()) ? tree_tile_rows(most * group) : 0;
+    if (tile_rows)
+        tile_work(trees, work, runs);
+    else
+        row_work(trees, work, runs);
+    if (slots > kIntMax / h || work.size() > kIntMax) throw std::invalid_argument("attention batch too large");
+    items = static_cast<int>(tile_rows ? work.size() / 2 : work.size());
 
     std::vector<PlanRegion::Section> s = {
         {tab.data(), tab.size() * sizeof(int32_t)},   {trees.data(), n * sizeof(int4)},
@@ -155,6 +144,67 @@ void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t
     region.place(*c, s);
     size_t* at[] = {&tables_at, &trees_at, &mask_at, &work_at, &runs_at, &parents_at, &acc_at, &ml_at, &best_at};
     for (size_t i = 0; i < s.size(); ++i) *at[i] = s[i].at;
+}
+
+// Runs of cached tokens, so that a long context fills the chip: about four waves
+// a SIMD, 64 tokens or more each; the last run takes the tree's own.
+void TreePlan::row_work(const std::vector<int4>& trees, std::vector<int4>& work, std::vector<int2>& runs) {
+    size_t total = 0;
+    for (const int4& t : trees) total += static_cast<size_t>(t.y) * t.z;
+    const size_t target = std::max<size_t>(1, static_cast<size_t>(cache->compute_units()) * 16 / heads);
+    const size_t split = std::min(round_up(std::max<size_t>(total / target, 64), 64), kIntMax / 2);
+    split_tokens = static_cast<int>(split);
+    for (size_t i = 0; i < trees.size(); ++i) {
+        const int4& t = trees[i];
+        const int parts = static_cast<int>(std::max<size_t>(1, (static_cast<size_t>(t.y) + split - 1) / split));
+        for (int j = 0; j < t.z; ++j) {
+            runs[t.w + j] = make_int2(static_cast<int>(slots), parts);
+            if (parts > 1) slots += parts;
+            for (int p = 0; p < parts; ++p) work.push_back(make_int4(static_cast<int>(i), j, p, parts));
+        }
+    }
+}
+
+// Runs of steps of the tiles, as many as give every CU a workgroup.
+void TreePlan::tile_work(const std::vector<int4>& trees, std::vector<int4>& work, std::vector<int2>& runs) {
+    const int kv_heads = cache->layout().kv_heads;
+    auto cached_steps = [](const int4& t) { return (t.y + kTreeStep - 1) / kTreeStep; };
+    // steps over the tree's own nodes of the row block from row r0
+    auto own_steps = [&](const int4& t, int r0) {
+        return (std::min(t.z * group, r0 + tile_rows) - 1) / group / kTreeStep + 1;
+    };
+    size_t total = 0;
+    for (const int4& t : trees)
+        for (int r0 = 0; r0 < t.z * group; r0 += tile_rows)
+            total += static_cast<size_t>(kv_heads) * (cached_steps(t) + own_steps(t, r0));
+    const size_t units = cache->compute_units();
+    const size_t per = std::max<size_t>(4, (total + units - 1) / units);
+    struct Item {
+        int4 where;
+        int step, end;
+    };
+    std::vector<Item> list;
+    for (size_t i = 0; i < trees.size(); ++i) {
+        const int4& t = trees[i];
+        if (!t.z) continue;
+        const int steps = cached_steps(t) + own_steps(t, (t.z * group - 1) / tile_rows * tile_rows);
+        const int parts = static_cast<int>((steps + per - 1) / per), len = (steps + parts - 1) / parts;
+        for (int j = 0; j < t.z; ++j) {
+            runs[t.w + j] = make_int2(static_cast<int>(slots), parts);
+            if (parts > 1) slots += parts;
+        }
+        for (int p = 0; p < parts; ++p)
+            for (int h = 0; h < kv_heads; ++h)
+                for (int r0 = 0; r0 < t.z * group; r0 += tile_rows) {
+                    const int all = cached_steps(t) + own_steps(t, r0);
+                    list.push_back({make_int4(static_cast<int>(i), h, r0, p), std::min(p * len, all), std::min((p + 1) * len, all)});
+                }
+    }
+    std::stable_sort(list.begin(), list.end(), [](const Item& x, const Item& y) { return x.end - x.step > y.end - y.step; });
+    for (const Item& x : list) {
+        work.push_back(x.where);
+        work.push_back(make_int4(x.step, x.end, 0, 0));
+    }
 }
 
 void TreePlan::launch(int layer, const float* q, const float* keys, const float* values, size_t row_stride, float* out,
@@ -192,7 +242,10 @@ void TreePlan::launch(int layer, const float* q, const float* keys, const float*
     a.part_ml = reinterpret_cast<float*>(d + ml_at);
     a.qscale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(g.head_dim)));
     a.err = region.flags();
-    launch_tree_rows(a, items, s);
+    if (tile_rows)
+        launch_tree_tiles(a, tile_rows, items, precision == 2, s);
+    else
+        launch_tree_rows(a, items, s);
     if (slots) launch_tree_merge(a, s);
     cache->leave(s);
     region.launched(s);

@@ -90,6 +90,12 @@ struct WriteArgs {
 // tree.hip
 void launch_tree_rows(const TreeArgs& a, int items, hipStream_t s);
 void launch_tree_merge(const TreeArgs& a, hipStream_t s);
+// tree_tiles.hip: head_dim 64 and 128; a workgroup takes up to tree_tile_rows(rows
+// of the largest tree and KV head) rows, and work has two entries a workgroup
+bool tree_tiles_supported(const BlockLayout& lay);
+int tree_tile_rows(size_t most);
+constexpr int kTreeStep = 32;  // keys of a step
+void launch_tree_tiles(const TreeArgs& a, int rows, int workgroups, bool x3, hipStream_t s);
 // tree_accept.hip: rows * splits is at most the larger of rows and kAcceptParts
 constexpr size_t kAcceptParts = 2048;
 int tree_accept_splits(size_t rows, size_t vocab);
@@ -137,6 +143,7 @@ struct TreePlan {
     DeviceCache* cache = nullptr;
     uint64_t epoch = 0;
     int heads = 0, group = 0, precision = 0, words = 1, items = 0, split_tokens = 0;
+    int tile_rows = 0;  // rows of a workgroup of the tiles (0: the row kernel)
     size_t count = 0, rows = 0, slots = 0;
     PlanRegion region;
     size_t tables_at = 0, trees_at = 0, mask_at = 0, work_at = 0, runs_at = 0, parents_at = 0, acc_at = 0, ml_at = 0,
@@ -144,6 +151,9 @@ struct TreePlan {
 
     void build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t heads, size_t context,
                const size_t* visible, const size_t* nodes, const int32_t* parents, int precision);
+    // the workgroups of the kernel, and each node row's first partial and runs
+    void row_work(const std::vector<int4>& trees, std::vector<int4>& work, std::vector<int2>& runs);
+    void tile_work(const std::vector<int4>& trees, std::vector<int4>& work, std::vector<int2>& runs);
     void launch(int layer, const float* q, const float* keys, const float* values, size_t row_stride, float* out,
                 hipStream_t s);
     void accept(const uint32_t* tokens, const uint32_t* first, const float* logits, size_t vocab, size_t logits_stride,

@@ -1,0 +1,550 @@
+// Attention of token trees on the matrix cores, for head_dim 64 and 128 over f32
+// or Q8_0 blocks of a power of two from 16 tokens.
+//
+// A row is a (node, query head) pair; the rows of one (tree, KV head) share its
+// keys.  A wave takes 16 * NT rows and walks keys 32 at a time ("a step"), all of
+// its operands in registers: no LDS and no barrier until its keys are done.
+//  S^T = K Q^T: the lane (g, r) = (l / 16, l % 16) loads four columns at a time of
+//    key r, which are the operands as they come, since the numbering of a
+//    contraction's terms is free as long as Q has the same.
+//  O^T = V^T P^T: lane (g, r) loads four columns of the keys 4g + i of each 16,
+//    so it holds V^T's operand for four output tiles (tile j: column j of every
+//    lane's four) and its own scores are P^T's.
+// Steps are dealt in turn to WK of the workgroup's four waves (WR row blocks
+// times WK), whose results meet in LDS.  A long context is cut into runs, a
+// workgroup each, that leave partials for a merge.  After the cached steps come
+// those over the tree's own nodes, with a mask word a row.
+//
+// f32: v_mfma_f32_16x16x4_f32.  f32x3 (kX3): 16x16x32 on split operands, hi * hi +
+// hi * lo + lo * hi: keys and queries as fp16 parts, values and probabilities as
+// bf16 parts, as the prompt chunks' tiles have it.  Softmax in log2 units with a
+// running maximum that moves only where a step exceeds it by 2^8.
+#include <algorithm>
+
+#include "common.hpp"
+#include "device_util.hpp"
+#include "q8.hpp"
+#include "tree.hpp"
+
+namespace tvara_amd {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kThreshold = 8.0f;
+constexpr int kStep = 32, kWaves = 4;
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ float finite_or_zero(float x) { return __builtin_isfinite(x) ? x : 0.f; }
+
+// x = hi + lo in 16-bit parts, each rounded to nearest: 22 bits as fp16 (a value
+// beyond its range gives NaN), 16 as bf16
+template <class T2>
+__device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned& lo) {
+    const f32x2 v = {x, y};
+    const T2 h = __builtin_convertvector(v, T2);
+    const T2 l = __builtin_convertvector(v - __builtin_convertvector(h, f32x2), T2);
+    hi = __builtin_bit_cast(unsigned, h);
+    lo = __builtin_bit_cast(unsigned, l);
+}
+
+template <int D, int NT, int WR, bool kQ8, bool kX3>
+__global__ __launch_bounds__(64 * kWaves, 1) void tree_tile_kernel(const TreeArgs a) {
+    constexpr int WK = kWaves / WR, C = D / 16, KC = D / 32, H = D / 64;
+    __shared__ f32x4 sums[kWaves][4][NT][64];
+    __shared__ float2 stats[kWaves][16 * NT];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, r16 = lane & 15, wk = wave % WK;
+    // x: tree, y: KV head, z: first row, w: run; then x: first step, y: its end
+    const int4 it = a.work[2 * blockIdx.x], st = a.work[2 * blockIdx.x + 1];
+    const int4 tree = a.trees[it.x];
+    const int cached = tree.y, nodes = tree.z, kh = it.y, G = a.group, kvw = a.lay.kv_width;
+    const int row0 = it.z + (wave / WK) * 16 * NT;
+
+    // this lane's row of each row tile
+    int node[NT], head[NT];
+    bool live[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = row0 + 16 * nt + r16;
+        node[nt] = r / G;
+        head[nt] = kh * G + r - node[nt] * G;
+        live[nt] = node[nt] < nodes;
+    }
+    // column of element 0 of a lane's c-th four of a key, and of the h-th four of
+    // a value (r: the loading lane's r16, or an output row of the tiles)
+    auto kcol = [&](int c) { return kQ8 ? 64 * (c / 4) + 16 * g + 4 * (c % 4) : 16 * c + 4 * g; };
+    auto vcol = [](int h, int r) { return kQ8 ? (D / 16) * r + 4 * h : 64 * h + 4 * r; };
+
+    f32x4 qf[kX3 ? 1 : NT][kX3 ? 1 : C];
+    u32x4 qh[kX3 ? NT : 1][kX3 ? KC : 1], ql[kX3 ? NT : 1][kX3 ? KC : 1];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const float* qp = a.q + (static_cast<size_t>(tree.w + node[nt]) * a.heads + head[nt]) * D;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            if (live[nt]) x = *reinterpret_cast<const f32x4*>(qp + kcol(c));
+            x *= a.qscale;
+            if constexpr (kX3) {
+                unsigned h0, h1, l0, l1;
+                split2<f16x2>(x[0], x[1], h0, l0);
+                split2<f16x2>(x[2], x[3], h1, l1);
+                qh[nt][c / 2][2 * (c % 2)] = h0;
+                qh[nt][c / 2][2 * (c % 2) + 1] = h1;
+                ql[nt][c / 2][2 * (c % 2)] = l0;
+                ql[nt][c / 2][2 * (c % 2) + 1] = l1;
+            } else {
+                qf[nt][c] = x;
+            }
+        }
+    }
+
+    f32x4 acc[4 * H][NT];  // tile (h, j) at 4h + j
+    float m[NT], l[NT], nonfinite = 0.f;  // nonfinite: NaN once a score is not finite
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        m[nt] = -INFINITY;
+        l[nt] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < 4 * H; ++dt) acc[dt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    f32x4 s[2][NT];  // scores, then probabilities, of keys 16mt + 4g + i
+    auto scores = [&](const f32x4 (&k)[2][C]) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[mt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (kX3) {
+#pragma unroll
+                for (int kc = 0; kc < KC; ++kc) {
+                    u32x4 hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const f32x4 x = k[mt][2 * kc + e / 2];
+                        unsigned h1, l1;
+                        split2<f16x2>(x[2 * (e % 2)], x[2 * (e % 2) + 1], h1, l1);
+                        hi[e] = h1;
+                        lo[e] = l1;
+                    }
+                    const f16x8 kh8 = __builtin_bit_cast(f16x8, hi), kl8 = __builtin_bit_cast(f16x8, lo);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const f16x8 q8 = __builtin_bit_cast(f16x8, qh[nt][kc]);
+                        s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl8, q8, s[mt][nt], 0, 0, 0);
+                        s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh8, __builtin_bit_cast(f16x8, ql[nt][kc]),
+                                                                           s[mt][nt], 0, 0, 0);
+                        s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh8, q8, s[mt][nt], 0, 0, 0);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[mt][c][i], qf[nt][c][i], s[mt][nt], 0, 0, 0);
+            }
+        }
+    };
+    // seen(mt, i, nt): whether the row sees the key
+    auto softmax = [&](auto masked, auto&& seen) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float x = s[mt][nt][i];
+                    if constexpr (decltype(masked)::value) {
+                        const bool on = seen(mt, i, nt);
+                        nonfinite = fmaf(on ? x : 0.f, 0.f, nonfinite);
+                        x = on ? x : -INFINITY;
+                        s[mt][nt][i] = x;
+                    } else {
+                        nonfinite = fmaf(x, 0.f, nonfinite);
+                    }
+                    mx = fmaxf(mx, x);
+                }
+            if (__any(mx > m[nt] + kThreshold)) {
+                const float mn = fmaxf(m[nt], cross_row_max(mx));
+                const float alpha = m[nt] == -INFINITY ? 0.f : fast_exp2(m[nt] - mn);
+                m[nt] = mn;
+                l[nt] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < 4 * H; ++dt) acc[dt][nt] *= alpha;
+            }
+            const float base = m[nt] == -INFINITY ? 0.f : m[nt];  // (no key seen yet: probabilities 0)
+            float sum = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = fast_exp2(s[mt][nt][i] - base);
+                    s[mt][nt][i] = p;
+                    sum += p;
+                }
+            l[nt] += sum;
+        }
+    };
+    auto output = [&](const f32x4 (&v)[2][4][H]) {
+        if constexpr (kX3) {
+            u32x4 ph[NT], pl[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    unsigned h1, l1;
+                    split2<bf16x2>(s[e / 2][nt][2 * (e % 2)], s[e / 2][nt][2 * (e % 2) + 1], h1, l1);
+                    ph[nt][e] = h1;
+                    pl[nt][e] = l1;
+                }
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    u32x4 hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        unsigned h1, l1;
+                        split2<bf16x2>(v[e / 2][2 * (e % 2)][h][j], v[e / 2][2 * (e % 2) + 1][h][j], h1, l1);
+                        hi[e] = h1;
+                        lo[e] = l1;
+                    }
+                    const bf16x8 vh = __builtin_bit_cast(bf16x8, hi), vl = __builtin_bit_cast(bf16x8, lo);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        f32x4& o = acc[4 * h + j][nt];
+                        const bf16x8 p8 = __builtin_bit_cast(bf16x8, ph[nt]);
+                        o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vl, p8, o, 0, 0, 0);
+                        o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh, __builtin_bit_cast(bf16x8, pl[nt]), o, 0, 0, 0);
+                        o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh, p8, o, 0, 0, 0);
+                    }
+                }
+        } else {
+            // a step's part is a chain of eight from zero, added to the rest: as
+            // short as a long context's sums need it
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    f32x4 part[NT];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) part[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+                                part[nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[mt][i][h][j], s[mt][nt][i], part[nt], 0, 0, 0);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) acc[4 * h + j][nt] += part[nt];
+                }
+        }
+    };
+
+    // ---- cached steps: this wave's are step0 + wk, + WK, ...
+    const int csteps = (cached + kStep - 1) / kStep, end = min(st.y, csteps);
+    const int tpb = a.lay.tpb, tsh = __builtin_ctz(static_cast<unsigned>(tpb));
+    const int32_t* tab = a.tables + tree.x;
+    const size_t kbytes = kQ8 ? static_cast<size_t>(a.layer) * 2 * a.lay.section + static_cast<size_t>(kh) * a.lay.head_bytes
+                              : (static_cast<size_t>(a.layer) * 2 * tpb * kvw + static_cast<size_t>(kh) * D) * sizeof(float);
+    const size_t vsec = kQ8 ? a.lay.section : static_cast<size_t>(tpb) * kvw * sizeof(float);
+    const int rowb = kQ8 ? D : kvw * static_cast<int>(sizeof(float));  // from one slot to the next
+    const unsigned koff = static_cast<unsigned>(r16 * rowb + kcol(0) * (kQ8 ? 1 : 4));
+    const unsigned voff = static_cast<unsigned>(4 * g * rowb + vcol(0, r16) * (kQ8 ? 1 : 4));
+    int step = st.x + wk;
+    if (step < end) {
+        const int last = (cached - 1) >> 4;  // 16 keys a table lookup; past the end the last again
+        // lane 2i + mt: the block of the wave's i-th step from here
+        auto lookup = [&](int from) { return tab[min(2 * (from + (lane >> 1) * WK) + (lane & 1), last) << 4 >> tsh]; };
+        int ids = lookup(step), more = lookup(step + 32 * WK), at = 0;
+        auto block = [&](int mt, int stp) {
+            const int id = __builtin_amdgcn_readlane(ids, 2 * at + mt);
+            const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
+            return a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes + static_cast<size_t>(slot) * rowb;
+        };
+        f32x4 k[2][C], v[2][4][H];
+        auto load_k = [&](int stp) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+                const char* b = block(mt, stp);
+                if constexpr (kQ8) {
+                    const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
+                    const char* sc = b + static_cast<size_t>(tpb - slot) * D + static_cast<size_t>(slot) * (D / 32) * 2;
+#pragma unroll
+                    for (int u = 0; u < H; ++u) {
+                        const u32x4 w = *reinterpret_cast<const u32x4*>(b + koff + 64 * u);
+                        const float d = half_bits_to_float(
+                            *reinterpret_cast<const uint16_t*>(sc + (r16 * (D / 32) + 2 * u + (g >> 1)) * 2));
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const unsigned b4 = w[c];
+                            k[mt][4 * u + c] = f32x4{sbyte_to_float<0>(b4) * d, sbyte_to_float<1>(b4) * d,
+                                                     sbyte_to_float<2>(b4) * d, sbyte_to_float<3>(b4) * d};
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < C; ++c) k[mt][c] = *reinterpret_cast<const f32x4*>(b + koff + 64 * c);
+                }
+            }
+        };
+        auto load_v = [&](int stp) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+                const char* b = block(mt, stp) + vsec;
+                if constexpr (kQ8) {
+                    const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
+                    const char* sc = b + static_cast<size_t>(tpb - slot) * D + static_cast<size_t>(slot) * (D / 32) * 2;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float d = half_bits_to_float(*reinterpret_cast<const uint16_t*>(
+                            sc + ((4 * g + i) * (D / 32) + (D / 16) * r16 / 32) * 2));
+#pragma unroll
+                        for (int h = 0; h < H; ++h) {
+                            const unsigned b4 = *reinterpret_cast<const unsigned*>(b + voff + i * D + 4 * h);
+                            v[mt][i][h] = f32x4{sbyte_to_float<0>(b4) * d, sbyte_to_float<1>(b4) * d,
+                                                sbyte_to_float<2>(b4) * d, sbyte_to_float<3>(b4) * d};
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int h = 0; h < H; ++h)
+                            v[mt][i][h] = *reinterpret_cast<const f32x4*>(b + static_cast<size_t>(i) * rowb + voff + 256 * h);
+                }
+            }
+        };
+        load_k(step);
+        load_v(step);
+        for (; step < end; step += WK) {
+            const int next = step + WK;
+            scores(k);
+            // the loads of the next step go out as soon as a register is free (past
+            // the end the last step's again: its blocks are there)
+            if (++at == 32) {
+                at = 0;
+                ids = more;
+                more = lookup(next + 32 * WK);
+            }
+            load_k(next);
+            if (kStep * step + kStep <= cached) {
+                softmax(std::false_type{}, [](int, int, int) { return true; });
+            } else {  // the last keys: what lies behind them is not seen, and its values are zeros
+                softmax(std::true_type{}, [&](int mt, int i, int) { return kStep * step + 16 * mt + 4 * g + i < cached; });
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (kStep * step + 16 * mt + 4 * g + i >= cached)
+#pragma unroll
+                            for (int h = 0; h < H; ++h) v[mt][i][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+            output(v);
+            load_v(next);
+        }
+    }
+
+    // ---- the tree's own nodes
+    for (; step < st.y; step += WK) {
+        const int n0 = kStep * (step - csteps);
+        const float* kb = a.keys + static_cast<size_t>(tree.w) * a.row_stride + static_cast<size_t>(kh) * D;
+        const float* vb = a.values + static_cast<size_t>(tree.w) * a.row_stride + static_cast<size_t>(kh) * D;
+        f32x4 k[2][C], v[2][4][H];
+        uint32_t mask[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            mask[nt] = live[nt] ? a.mask[static_cast<size_t>(tree.w + node[nt]) * a.words + (step - csteps)] : 0u;
+        float odd = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+            const float* kr = kb + static_cast<size_t>(min(n0 + 16 * mt + r16, nodes - 1)) * a.row_stride;
+#pragma unroll
+            for (int c = 0; c < C; ++c) k[mt][c] = *reinterpret_cast<const f32x4*>(kr + kcol(c));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float* vr = vb + static_cast<size_t>(min(n0 + 16 * mt + 4 * g + i, nodes - 1)) * a.row_stride;
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    v[mt][i][h] = *reinterpret_cast<const f32x4*>(vr + vcol(h, r16));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) odd = fmaf(v[mt][i][h][j], 0.f, odd);
+                }
+            }
+        }
+        scores(k);
+        softmax(std::true_type{}, [&](int mt, int i, int nt) { return (mask[nt] >> (16 * mt + 4 * g + i) & 1u) != 0; });
+        const bool plain = !__any(odd != 0.f);  // (0, or NaN where a value is not finite)
+        if (!plain) {
+            // Zero times such a value would reach rows that do not see it: it is
+            // zero in the product, and added below to the rows that do.
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[mt][i][h][j] = finite_or_zero(v[mt][i][h][j]);
+        }
+        output(v);
+        if (plain) continue;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll 1
+            for (int e = 0; e < 16; ++e) {
+                const int key = n0 + 16 * mt + e, i = e & 3;
+                if (key >= nodes) break;
+                const float* vr = vb + static_cast<size_t>(key) * a.row_stride;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float own = i == 0 ? s[mt][nt][0] : i == 1 ? s[mt][nt][1] : i == 2 ? s[mt][nt][2] : s[mt][nt][3];
+                    const float p = __shfl(own, r16 + 16 * (e >> 2));
+                    const bool on = (mask[nt] >> (16 * mt + e) & 1u) != 0;
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+#pragma unroll
+                        for (int o = 0; o < 4; ++o) {
+                            const f32x4 x = *reinterpret_cast<const f32x4*>(vr + vcol(h, 4 * g + o));
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (on && !__builtin_isfinite(x[j])) acc[4 * h + j][nt][o] = fmaf(p, x[j], acc[4 * h + j][nt][o]);
+                        }
+                }
+            }
+    }
+    if (__any(nonfinite != 0.f) && lane == 0) *a.err = 1;
+
+    // ---- the waves that shared these rows' keys, together
+    float total[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) total[nt] = cross_row_sum(l[nt]);
+    if constexpr (WK > 1) {
+        if (g == 0)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) stats[wave][16 * nt + r16] = make_float2(m[nt], total[nt]);
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) top = fmaxf(top, stats[wave - wk + w][16 * nt + r16].x);
+            const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) {
+                const float2 x = stats[wave - wk + w][16 * nt + r16];
+                sum = fmaf(fast_exp2(x.x - base), x.y, sum);
+            }
+            const float scale = fast_exp2(m[nt] - base);
+#pragma unroll
+            for (int dt = 0; dt < 4 * H; ++dt) acc[dt][nt] *= scale;
+            m[nt] = top;
+            total[nt] = sum;
+        }
+    }
+    // four columns of output row 4g + i of the tiles, of a row tile's row r16
+    bool bad = false;
+    auto store = [&](int h, int i, int nt, f32x4 x) {
+        if (!live[nt]) return;
+        const size_t row = static_cast<size_t>(tree.w) + node[nt];
+        const int2 runs = a.runs[row];
+        if (runs.y == 1) {
+            x /= total[nt];
+            if constexpr (kX3)
+                bad |= !(__builtin_isfinite(x[0]) && __builtin_isfinite(x[1]) && __builtin_isfinite(x[2]) && __builtin_isfinite(x[3]));
+            *reinterpret_cast<f32x4*>(a.out + (row * a.heads + head[nt]) * D + vcol(h, 4 * g + i)) = x;
+        } else {
+            const size_t p = (static_cast<size_t>(runs.x) + it.w) * a.heads + head[nt];
+            *reinterpret_cast<f32x4*>(a.part_acc + p * D + vcol(h, 4 * g + i)) = x;
+            if (h == 0 && i == 0 && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m[nt], total[nt]);
+        }
+    };
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        if constexpr (WK > 1) {
+            if (h) __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    sums[wave][i][nt][lane] =
+                        f32x4{acc[4 * h][nt][i], acc[4 * h + 1][nt][i], acc[4 * h + 2][nt][i], acc[4 * h + 3][nt][i]};
+            __syncthreads();
+#pragma unroll
+            for (int ii = 0; ii < 4 / WK; ++ii) {
+                const int i = wk * (4 / WK) + ii;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    f32x4 x = sums[wave - wk][i][nt][lane];
+#pragma unroll
+                    for (int w = 1; w < WK; ++w) x += sums[wave - wk + w][i][nt][lane];
+                    store(h, i, nt, x);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    store(h, i, nt, f32x4{acc[4 * h][nt][i], acc[4 * h + 1][nt][i], acc[4 * h + 2][nt][i], acc[4 * h + 3][nt][i]});
+        }
+    }
+    if (bad) *a.err = 1;
+}
+
+template <int D, bool kQ8, bool kX3>
+void launch_shape(const TreeArgs& a, int rows, int workgroups, hipStream_t s) {
+    auto go = [&](auto kernel) {
+        launch("tree_attention_tiles", kernel, dim3(workgroups), dim3(64 * kWaves), 0, s, a);
+    };
+    switch (rows) {
+        case 16: return go(tree_tile_kernel<D, 1, 1, kQ8, kX3>);
+        case 32: return go(tree_tile_kernel<D, 2, 1, kQ8, kX3>);
+        case 64: return go(tree_tile_kernel<D, 2, 2, kQ8, kX3>);
+        default: return go(tree_tile_kernel<D, 2, 4, kQ8, kX3>);
+    }
+}
+
+}  // namespace
+
+bool tree_tiles_supported(const BlockLayout& lay) {
+    return (lay.head_dim == 64 || lay.head_dim == 128) && lay.tpb >= 16 && (lay.tpb & (lay.tpb - 1)) == 0 &&
+           lay.stride <= static_cast<size_t>(1) << 31;
+}
+
+int tree_tile_rows(size_t most) {
+    int rows = 16;
+    while (rows < 128 && static_cast<size_t>(rows) < most) rows *= 2;
+    return rows;
+}
+
+void launch_tree_tiles(const TreeArgs& a, int rows, int workgroups, bool x3, hipStream_t s) {
+    const bool q8 = a.lay.format == kQ8;
+    if (a.lay.head_dim == 128) {
+        if (x3)
+            q8 ? launch_shape<128, true, true>(a, rows, workgroups, s) : launch_shape<128, false, true>(a, rows, workgroups, s);
+        else
+            q8 ? launch_shape<128, true, false>(a, rows, workgroups, s) : launch_shape<128, false, false>(a, rows, workgroups, s);
+    } else {
+        if (x3)
+            q8 ? launch_shape<64, true, true>(a, rows, workgroups, s) : launch_shape<64, false, true>(a, rows, workgroups, s);
+        else
+            q8 ? launch_shape<64, true, false>(a, rows, workgroups, s) : launch_shape<64, false, false>(a, rows, workgroups, s);
+    }
+    TVARA_HIP(hipGetLastError());
+}
+
+}  // namespace tvara_amd
