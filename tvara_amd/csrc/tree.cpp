@@ -126,7 +126,7 @@ void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t
     std::vector<int4> work;
     std::vector<int2> runs(rows);
     slots = 0;
-    tile_rows = tree_tiles_supported(c->layout()) ? tree_tile_rows(most * group) : 0;
+    tile_rows = tree_tiles_supported(c->layout()) ? tree_tile_rows(most * group, precision == 2) : 0;
     if (tile_rows)
         tile_work(trees, work, runs);
     else
@@ -177,7 +177,8 @@ void TreePlan::tile_work(const std::vector<int4>& trees, std::vector<int4>& work
     for (const int4& t : trees)
         for (int r0 = 0; r0 < t.z * group; r0 += tile_rows)
             total += static_cast<size_t>(kv_heads) * (cached_steps(t) + own_steps(t, r0));
-    const size_t units = cache->compute_units();
+    // two workgroups a CU share it where they are the shared kernel's
+    const size_t units = static_cast<size_t>(cache->compute_units()) * (tile_rows > 32 ? 2 : 1);
     const size_t per = std::max<size_t>(4, (total + units - 1) / units);
     struct Item {
         int4 where;

@@ -93,7 +93,7 @@ void launch_tree_merge(const TreeArgs& a, hipStream_t s);
 // tree_tiles.hip: head_dim 64 and 128; a workgroup takes up to tree_tile_rows(rows
 // of the largest tree and KV head) rows, and work has two entries a workgroup
 bool tree_tiles_supported(const BlockLayout& lay);
-int tree_tile_rows(size_t most);
+int tree_tile_rows(size_t most, bool x3);
 constexpr int kTreeStep = 32;  // keys of a step
 void launch_tree_tiles(const TreeArgs& a, int rows, int workgroups, bool x3, hipStream_t s);
 // tree_accept.hip: rows * splits is at most the larger of rows and kAcceptParts

@@ -39,6 +39,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kThreshold = 8.0f;
 constexpr int kStep = 32, kWaves = 4;
+constexpr int kBufferWord3 = 0x00020000;  // gfx9 buffer descriptor, dword 3
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -505,17 +506,416 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_tile_kernel(const TreeArg
     if (bad) *a.err = 1;
 }
 
+// Many rows of a (tree, KV head), f32x3: four waves of 32 rows each share every
+// key.  A wave in turn is given 16 keys, or the values of 32, of a step to come: it
+// loads them an iteration ahead into registers, splits them once for all the rows
+// and leaves the parts in LDS in the order in which the products' lanes read them
+// (lane l its own 16 bytes: no conflicts), in the other of two buffers; one barrier
+// an iteration of S steps.  Loads go through descriptors that end with the last
+// key, so that what lies behind it reads as zeros.
+template <int D, bool kQ8>
+__global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeArgs a) {
+    constexpr int NT = 2, C = D / 16, KC = D / 32, H = D / 64;
+    constexpr int S = 128 / D;        // steps an iteration: eight float4 a thread
+    constexpr int KW = kWaves / 2;    // waves that take keys; the others take values
+    constexpr int TK = 128 / D;       // key tiles of 16 a wave takes
+    __shared__ u32x4 klds[2][S][2 * KC * 2][64];
+    __shared__ u32x4 vlds[2][S][4 * H * 2][64];
+    __shared__ int odds[2][S][H];     // the tree's own values: some are not finite
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, r16 = lane & 15;
+    const int4 it = a.work[2 * blockIdx.x], st = a.work[2 * blockIdx.x + 1];
+    const int4 tree = a.trees[it.x];
+    const int cached = tree.y, nodes = tree.z, kh = it.y, G = a.group, kvw = a.lay.kv_width;
+    const int row0 = it.z + wave * 16 * NT;
+    const bool active = row0 < nodes * G;  // (a wave without rows still stages)
+    auto node_of = [&](int nt) { return (row0 + 16 * nt + r16) / G; };
+
+    // the lane's c-th four columns of a key: as the staging lane holds them
+    auto kcol = [&](int c) { return kQ8 ? 64 * (c / 4) + 16 * g + 4 * (c % 4) : 16 * c + 4 * g; };
+    u32x4 qh[NT][KC], ql[NT][KC];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int node = node_of(nt), head = kh * G + row0 + 16 * nt + r16 - node * G;
+        const float* qp = a.q + (static_cast<size_t>(tree.w + node) * a.heads + head) * D;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            if (node < nodes) x = *reinterpret_cast<const f32x4*>(qp + kcol(c));
+            x *= a.qscale;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                unsigned hi, lo;
+                split2<f16x2>(x[2 * e], x[2 * e + 1], hi, lo);
+                qh[nt][c / 2][2 * (c % 2) + e] = hi;
+                ql[nt][c / 2][2 * (c % 2) + e] = lo;
+            }
+        }
+    }
+    f32x4 acc[4 * H][NT];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        m[nt] = -INFINITY;
+        l[nt] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < 4 * H; ++dt) acc[dt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // ---- staging.  Wave w < KW: TK key tiles of 16 from mt0 on, of step kstep of the
+    // iteration; else: the value half vh of its step.
+    const bool takes_keys = wave < KW;
+    const int mt0 = wave * TK % 2, vh = (wave - KW) % H;
+    const int sub = takes_keys ? wave * TK / 2 : (wave - KW) / H;  // its step of the iteration
+    const int csteps = (cached + kStep - 1) / kStep;
+    const int tpb = a.lay.tpb, tsh = __builtin_ctz(static_cast<unsigned>(tpb));
+    const int32_t* tab = a.tables + tree.x;
+    const size_t section = kQ8 ? a.lay.section : static_cast<size_t>(tpb) * kvw * sizeof(float);
+    const size_t kbytes = (static_cast<size_t>(a.layer) * 2 + (takes_keys ? 0 : 1)) * section +
+                          (kQ8 ? static_cast<size_t>(kh) * a.lay.head_bytes : static_cast<size_t>(kh) * D * sizeof(float));
+    const int rowb = kQ8 ? D : kvw * static_cast<int>(sizeof(float));
+    const int last = max(cached - 1, 0) >> 4;  // the last 16 cached keys
+    const char* own = reinterpret_cast<const char*>((takes_keys ? a.keys : a.values) +
+                                                    static_cast<size_t>(tree.w) * a.row_stride + static_cast<size_t>(kh) * D);
+    const int ownb = static_cast<int>(a.row_stride * sizeof(float));
+    f32x4 raw[8];                     // eight float4
+    u32x4 rawq[kQ8 ? 2 : 1];          // Q8_0: their bytes and scales
+    unsigned rawd[kQ8 ? 8 : 1];
+    // lane 2i + mt: the block of key tile mt of this wave's step in the i-th iteration from here
+    auto lookup = [&](int step) {
+        return cached ? tab[min(2 * min(step + (lane >> 1) * S, csteps) + (lane & 1), last) << 4 >> tsh] : 0;
+    };
+    int ids = lookup(st.x + sub), more = lookup(st.x + 32 * S + sub), at = 0;
+    // 16 keys: their rows up to the last key, `range` bytes a row from the start
+    auto tile16 = [&](int step, int mt, int range, int& pitch) {
+        const char* base;
+        int left;
+        if (kQ8 || step < csteps) {
+            const int t = min(2 * step + mt, last);
+            const int id = __builtin_amdgcn_readlane(ids, 2 * at + mt);
+            base = a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes + static_cast<size_t>((t << 4) & (tpb - 1)) * rowb;
+            left = cached - 16 * (2 * step + mt);
+            pitch = rowb;
+        } else {
+            const int n = kStep * (step - csteps) + 16 * mt;
+            base = own + static_cast<size_t>(n) * ownb;
+            left = nodes - n;
+            pitch = ownb;
+        }
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, left > 0 ? (min(left, 16) - 1) * pitch + range : 0,
+                                                 kBufferWord3);
+    };
+    auto load_rows = [&](int step) {
+        int pitch;
+        const __amdgpu_buffer_rsrc_t t0 = tile16(step, takes_keys && D == 128 ? mt0 : 0, D * 4, pitch);
+        const __amdgpu_buffer_rsrc_t t1 = takes_keys && D == 128 ? t0 : tile16(step, 1, D * 4, pitch);
+        const int far = takes_keys && D == 128 ? 256 : 0, by = takes_keys ? 64 : pitch;
+        const int off = takes_keys ? r16 * pitch + 16 * g : 4 * g * pitch + 256 * vh + 16 * r16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            raw[i] = __builtin_amdgcn_raw_buffer_load_b128(t0, off, i * by, 0);
+            raw[4 + i] = __builtin_amdgcn_raw_buffer_load_b128(t1, off, i * by + far, 0);
+        }
+    };
+    auto load = [&](int step) {
+        if constexpr (!kQ8) {
+            load_rows(step);
+        } else {
+            int pitch;
+            const __amdgpu_buffer_rsrc_t t0 = tile16(step, 0, D, pitch), t1 = tile16(step, 1, D, pitch);
+            // a key tile's scales, from the block's scale plane on
+            auto scales = [&](int mt) {
+                const int t = min(2 * step + mt, last), slot = (t << 4) & (tpb - 1), left = cached - 16 * (2 * step + mt);
+                const int id = __builtin_amdgcn_readlane(ids, 2 * at + mt);
+                const char* base = a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes + static_cast<size_t>(tpb) * D +
+                                   static_cast<size_t>(slot) * (D / 32) * 2;
+                return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, max(min(left, 16), 0) * (D / 32) * 2, kBufferWord3);
+            };
+            const __amdgpu_buffer_rsrc_t s0 = scales(0), s1 = scales(1);
+            if (takes_keys) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {  // D = 128: halves of the columns; 64: the two key tiles
+                    const bool second = D == 128 ? mt0 : u;
+                    const int cu = D == 128 ? u : 0;
+                    rawq[u] = __builtin_amdgcn_raw_buffer_load_b128(second ? t1 : t0, r16 * D + 16 * g, 64 * cu, 0);
+                    rawd[u] = __builtin_amdgcn_raw_buffer_load_b16(second ? s1 : s0, (r16 * (D / 32) + (g >> 1)) * 2, 4 * cu, 0);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    rawq[i / 4][i % 4] = __builtin_amdgcn_raw_buffer_load_b32(i < 4 ? t0 : t1, 4 * g * D + 64 * vh + 4 * r16, i % 4 * D, 0);
+                    rawd[i] = __builtin_amdgcn_raw_buffer_load_b16(i < 4 ? s0 : s1, (4 * g * (D / 32) + 2 * vh + (r16 >> 3)) * 2,
+                                                                   i % 4 * (D / 32) * 2, 0);
+                }
+            }
+        }
+        if (++at == 32) {
+            at = 0;
+            ids = more;
+            more = lookup(step + 33 * S);
+        }
+    };
+    auto stage = [&](int buf, int step, const f32x4 (&x)[8]) {
+        if (takes_keys) {
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {  // an operand: two float4
+                u32x4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    unsigned h1, l1;
+                    split2<f16x2>(x[2 * p + e / 2][2 * (e % 2)], x[2 * p + e / 2][2 * (e % 2) + 1], h1, l1);
+                    hi[e] = h1;
+                    lo[e] = l1;
+                }
+                const int o = D == 128 ? mt0 * KC + p : p;  // [mt][kc]
+                klds[buf][sub][2 * o][lane] = hi;
+                klds[buf][sub][2 * o + 1][lane] = lo;
+            }
+        } else {
+            f32x4 y[8];
+            float odd = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = x[i];
+            if (step >= csteps) {
+                // Zero times a value that is not finite would reach rows that do not
+                // see it: it is zero in the product, and added to the rows that do.
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        odd = fmaf(y[i][j], 0.f, odd);
+                        y[i][j] = finite_or_zero(y[i][j]);
+                    }
+                const bool any = __any(odd != 0.f);
+                if (lane == 0) odds[buf][sub][vh] = any;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u32x4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    unsigned h1, l1;
+                    split2<bf16x2>(y[2 * e][j], y[2 * e + 1][j], h1, l1);
+                    hi[e] = h1;
+                    lo[e] = l1;
+                }
+                vlds[buf][sub][2 * (4 * vh + j)][lane] = hi;
+                vlds[buf][sub][2 * (4 * vh + j) + 1][lane] = lo;
+            }
+        }
+    };
+    auto put = [&](int buf, int step) {
+        if constexpr (kQ8) {
+            f32x4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned w = rawq[i / 4][i % 4];
+                const float d = half_bits_to_float(static_cast<uint16_t>(takes_keys ? rawd[i / 4] : rawd[i]));
+                x[i] = f32x4{sbyte_to_float<0>(w) * d, sbyte_to_float<1>(w) * d, sbyte_to_float<2>(w) * d, sbyte_to_float<3>(w) * d};
+            }
+            stage(buf, step, x);
+        } else {
+            stage(buf, step, raw);
+        }
+    };
+
+    auto compute = [&](int buf, int t, int step) {
+        f32x4 s[2][NT];  // scores, then probabilities, of keys 16mt + 4g + i
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) {
+                const f16x8 kh8 = __builtin_bit_cast(f16x8, klds[buf][t][2 * (mt * KC + kc)][lane]);
+                const f16x8 kl8 = __builtin_bit_cast(f16x8, klds[buf][t][2 * (mt * KC + kc) + 1][lane]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl8, __builtin_bit_cast(f16x8, qh[nt][kc]),
+                                                                       kc ? s[mt][nt] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh8, __builtin_bit_cast(f16x8, ql[nt][kc]), s[mt][nt], 0, 0, 0);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh8, __builtin_bit_cast(f16x8, qh[nt][kc]), s[mt][nt], 0, 0, 0);
+            }
+        // what a row does not see: keys behind the last cached one, other branches' nodes
+        const bool tail = step >= csteps;
+        if (tail || kStep * step + kStep > cached) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int node = node_of(nt);
+                uint32_t mask = tail ? 0u : (1u << (cached - kStep * step)) - 1;
+                if (tail && node < nodes) mask = a.mask[static_cast<size_t>(tree.w + node) * a.words + (step - csteps)];
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!(mask >> (16 * mt + 4 * g + i) & 1u)) s[mt][nt][i] = -INFINITY;
+            }
+        }
+        // (a score that is not finite is NaN here, and so is its row's sum: an input
+        // beyond fp16 is infinite in one part and its opposite in the other)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[mt][nt][i]);
+            if (__any(mx > m[nt] + kThreshold)) {
+                const float mn = fmaxf(m[nt], cross_row_max(mx));
+                const float alpha = m[nt] == -INFINITY ? 0.f : fast_exp2(m[nt] - mn);
+                m[nt] = mn;
+                l[nt] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < 4 * H; ++dt) acc[dt][nt] *= alpha;
+            }
+            const float base = m[nt] == -INFINITY ? 0.f : m[nt];  // (no key seen yet: probabilities 0)
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = fast_exp2(s[mt][nt][i] - base);
+                    s[mt][nt][i] = p;
+                    l[nt] += p;
+                }
+        }
+        bool odd = false;
+        if (tail)
+#pragma unroll
+            for (int h = 0; h < H; ++h) odd |= odds[buf][t][h] != 0;
+        if (odd) {
+            const int n0 = kStep * (step - csteps);
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll 1
+                for (int e = 0; e < 16; ++e) {
+                    const int key = n0 + 16 * mt + e, i = e & 3;
+                    if (key >= nodes) break;
+                    const float* vr = a.values + static_cast<size_t>(tree.w + key) * a.row_stride + static_cast<size_t>(kh) * D;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const int node = node_of(nt);
+                        const float mine = i == 0 ? s[mt][nt][0] : i == 1 ? s[mt][nt][1] : i == 2 ? s[mt][nt][2] : s[mt][nt][3];
+                        const float p = __shfl(mine, r16 + 16 * (e >> 2));
+                        const bool on = node < nodes &&
+                                        (a.mask[static_cast<size_t>(tree.w + node) * a.words + (step - csteps)] >> (16 * mt + e) & 1u);
+#pragma unroll
+                        for (int h = 0; h < H; ++h)
+#pragma unroll
+                            for (int o = 0; o < 4; ++o) {
+                                const f32x4 y = *reinterpret_cast<const f32x4*>(vr + 64 * h + 4 * (4 * g + o));
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+                                    if (on && !__builtin_isfinite(y[j])) acc[4 * h + j][nt][o] = fmaf(p, y[j], acc[4 * h + j][nt][o]);
+                            }
+                    }
+                }
+        }
+        u32x4 ph[NT], pl[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                unsigned h1, l1;
+                split2<bf16x2>(s[e / 2][nt][2 * (e % 2)], s[e / 2][nt][2 * (e % 2) + 1], h1, l1);
+                ph[nt][e] = h1;
+                pl[nt][e] = l1;
+            }
+#pragma unroll
+        for (int dt = 0; dt < 4 * H; ++dt) {
+            const bf16x8 vh8 = __builtin_bit_cast(bf16x8, vlds[buf][t][2 * dt][lane]);
+            const bf16x8 vl8 = __builtin_bit_cast(bf16x8, vlds[buf][t][2 * dt + 1][lane]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                acc[dt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vl8, __builtin_bit_cast(bf16x8, ph[nt]), acc[dt][nt], 0, 0, 0);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                acc[dt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh8, __builtin_bit_cast(bf16x8, pl[nt]), acc[dt][nt], 0, 0, 0);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                acc[dt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh8, __builtin_bit_cast(bf16x8, ph[nt]), acc[dt][nt], 0, 0, 0);
+        }
+    };
+
+    // Q8_0 blocks: the tree's own f32 rows are not in the pipeline of the cached ones
+    const int end = kQ8 ? min(st.y, csteps) : st.y;
+    if (st.x < end) {
+        load(st.x + sub);
+        put(0, st.x + sub);
+        load(st.x + S + sub);
+        __syncthreads();
+        int buf = 0;
+        for (int step = st.x; step < end; step += S, buf ^= 1) {
+            put(buf ^ 1, step + S + sub);
+            load(step + 2 * S + sub);
+            if (active)
+#pragma unroll 1
+                for (int t = 0; t < S && step + t < end; ++t) compute(buf, t, step + t);
+            __syncthreads();
+        }
+    }
+    if constexpr (kQ8) {
+#pragma unroll 1
+        for (int step = max(st.x, csteps); step < st.y; ++step) {
+            if (sub == 0) {
+                const int n0 = kStep * (step - csteps);
+                f32x4 x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int key = n0 + (takes_keys ? 16 * (D == 128 ? mt0 : i / 4) + r16 : 16 * (i / 4) + 4 * g + i % 4);
+                    const int col = takes_keys ? kcol(D == 128 ? i : i % 4) : 64 * vh + 4 * r16;
+                    x[i] = *reinterpret_cast<const f32x4*>(own + static_cast<size_t>(min(key, nodes - 1)) * ownb + 4 * col);
+                }
+                stage(0, step, x);
+            }
+            __syncthreads();
+            if (active) compute(0, 0, step);
+            __syncthreads();
+        }
+    }
+
+    bool bad = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const float total = cross_row_sum(l[nt]);
+        const int node = node_of(nt), head = kh * G + row0 + 16 * nt + r16 - node * G;
+        if (node >= nodes) continue;
+        const size_t row = static_cast<size_t>(tree.w) + node;
+        const int2 runs = a.runs[row];
+        const bool whole = runs.y == 1;
+        const size_t to = whole ? row * a.heads + head : (static_cast<size_t>(runs.x) + it.w) * a.heads + head;
+        float* o = (whole ? a.out : a.part_acc) + to * D + 16 * g;
+        const float inv = whole ? total : 1.f;
+        if (!whole && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * to) = make_float2(m[nt], total);
+        bad |= !__builtin_isfinite(total);
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 x = f32x4{acc[4 * h][nt][i], acc[4 * h + 1][nt][i], acc[4 * h + 2][nt][i], acc[4 * h + 3][nt][i]} / inv;
+                bad |= !(__builtin_isfinite(x[0]) && __builtin_isfinite(x[1]) && __builtin_isfinite(x[2]) && __builtin_isfinite(x[3]));
+                *reinterpret_cast<f32x4*>(o + 64 * h + 4 * i) = x;
+            }
+    }
+    if (bad) *a.err = 1;
+}
+
 template <int D, bool kQ8, bool kX3>
 void launch_shape(const TreeArgs& a, int rows, int workgroups, hipStream_t s) {
     auto go = [&](auto kernel) {
         launch("tree_attention_tiles", kernel, dim3(workgroups), dim3(64 * kWaves), 0, s, a);
     };
-    switch (rows) {
-        case 16: return go(tree_tile_kernel<D, 1, 1, kQ8, kX3>);
-        case 32: return go(tree_tile_kernel<D, 2, 1, kQ8, kX3>);
-        case 64: return go(tree_tile_kernel<D, 2, 2, kQ8, kX3>);
-        default: return go(tree_tile_kernel<D, 2, 4, kQ8, kX3>);
+    if constexpr (kX3) {
+        if (rows > 32) {
+            go(tree_shared_kernel<D, kQ8>);
+            return;
+        }
     }
+    if (rows == 16)
+        go(tree_tile_kernel<D, 1, 1, kQ8, kX3>);
+    else
+        go(tree_tile_kernel<D, 2, 1, kQ8, kX3>);
 }
 
 }  // namespace
@@ -525,10 +925,10 @@ bool tree_tiles_supported(const BlockLayout& lay) {
            lay.stride <= static_cast<size_t>(1) << 31;
 }
 
-int tree_tile_rows(size_t most) {
-    int rows = 16;
-    while (rows < 128 && static_cast<size_t>(rows) < most) rows *= 2;
-    return rows;
+int tree_tile_rows(size_t most, bool x3) {
+    if (most <= 16) return 16;
+    if (most <= 32 || !x3) return 32;
+    return 128;
 }
 
 void launch_tree_tiles(const TreeArgs& a, int rows, int workgroups, bool x3, hipStream_t s) {
