@@ -177,8 +177,8 @@ void TreePlan::tile_work(const std::vector<int4>& trees, std::vector<int4>& work
     for (const int4& t : trees)
         for (int r0 = 0; r0 < t.z * group; r0 += tile_rows)
             total += static_cast<size_t>(kv_heads) * (cached_steps(t) + own_steps(t, r0));
-    // two workgroups a CU share it where they are the shared kernel's
-    const size_t units = static_cast<size_t>(cache->compute_units()) * (tile_rows > 32 ? 2 : 1);
+    // (two workgroups of 128 rows share a CU)
+    const size_t units = static_cast<size_t>(cache->compute_units()) * (tile_rows == 128 ? 2 : 1);
     const size_t per = std::max<size_t>(4, (total + units - 1) / units);
     struct Item {
         int4 where;

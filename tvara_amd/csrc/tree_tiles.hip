@@ -15,9 +15,8 @@
 // workgroup each, that leave partials for a merge.  After the cached steps come
 // those over the tree's own nodes, with a mask word a row.
 //
-// f32: v_mfma_f32_16x16x4_f32.  f32x3 (kX3): 16x16x32 on split operands, hi * hi +
-// hi * lo + lo * hi: keys and queries as fp16 parts, values and probabilities as
-// bf16 parts, as the prompt chunks' tiles have it.  Softmax in log2 units with a
+// f32: v_mfma_f32_16x16x4_f32.  f32x3 (kX3): 16x16x32 on operands in two fp16
+// parts, hi * hi + hi * lo + lo * hi.  Softmax in log2 units with a
 // running maximum that moves only where a step exceeds it by 2^8.
 #include <algorithm>
 
@@ -31,8 +30,6 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -45,15 +42,41 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 
 __device__ __forceinline__ float finite_or_zero(float x) { return __builtin_isfinite(x) ? x : 0.f; }
 
-// x = hi + lo in 16-bit parts, each rounded to nearest: 22 bits as fp16 (a value
-// beyond its range gives NaN), 16 as bf16
-template <class T2>
+// Where 64 runs of bytes start and how far they go, one a lane.
+struct Spans {
+    unsigned lo, hi;
+    int range;
+    __device__ __forceinline__ void set(const char* base, int bytes) {
+        const uint64_t b = reinterpret_cast<uint64_t>(base);
+        lo = static_cast<unsigned>(b);
+        hi = static_cast<unsigned>(b >> 32);
+        range = bytes;
+    }
+    // lane i's as a buffer descriptor, in scalar registers
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor(int i) const {
+        const uint64_t b = static_cast<uint64_t>(static_cast<unsigned>(__builtin_amdgcn_readlane(hi, i))) << 32 |
+                           static_cast<unsigned>(__builtin_amdgcn_readlane(lo, i));
+        return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(b), 0, __builtin_amdgcn_readlane(range, i), kBufferWord3);
+    }
+};
+
+// Ends a rare branch that loads: where it joins the common path nothing of it is in
+// flight, so that no wait for it is put there, which would wait for the loads
+// ahead too (they return in order).
+__device__ __forceinline__ void wait_for_loads() { __builtin_amdgcn_s_waitcnt(0); }
+
+// Two values as hi + lo in fp16, each rounded to nearest (22 bits; beyond fp16's
+// range one is infinite and the other its opposite).  `one` is 1, hidden from the
+// compiler, so that x - hi stays a mixed-precision fma: four instructions a pair
+// where converting hi back takes six.
 __device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned& lo) {
+    float one = 1.f;
+    asm("" : "+s"(one));
     const f32x2 v = {x, y};
-    const T2 h = __builtin_convertvector(v, T2);
-    const T2 l = __builtin_convertvector(v - __builtin_convertvector(h, f32x2), T2);
+    const f16x2 h = __builtin_convertvector(v, f16x2);
+    const f32x2 rest = {fmaf(-static_cast<float>(h[0]), one, x), fmaf(-static_cast<float>(h[1]), one, y)};
     hi = __builtin_bit_cast(unsigned, h);
-    lo = __builtin_bit_cast(unsigned, l);
+    lo = __builtin_bit_cast(unsigned, __builtin_convertvector(rest, f16x2));
 }
 
 template <int D, int NT, int WR, bool kQ8, bool kX3>
@@ -96,8 +119,8 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_tile_kernel(const TreeArg
             x *= a.qscale;
             if constexpr (kX3) {
                 unsigned h0, h1, l0, l1;
-                split2<f16x2>(x[0], x[1], h0, l0);
-                split2<f16x2>(x[2], x[3], h1, l1);
+                split2(x[0], x[1], h0, l0);
+                split2(x[2], x[3], h1, l1);
                 qh[nt][c / 2][2 * (c % 2)] = h0;
                 qh[nt][c / 2][2 * (c % 2) + 1] = h1;
                 ql[nt][c / 2][2 * (c % 2)] = l0;
@@ -132,7 +155,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_tile_kernel(const TreeArg
                     for (int e = 0; e < 4; ++e) {
                         const f32x4 x = k[mt][2 * kc + e / 2];
                         unsigned h1, l1;
-                        split2<f16x2>(x[2 * (e % 2)], x[2 * (e % 2) + 1], h1, l1);
+                        split2(x[2 * (e % 2)], x[2 * (e % 2) + 1], h1, l1);
                         hi[e] = h1;
                         lo[e] = l1;
                     }
@@ -206,7 +229,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_tile_kernel(const TreeArg
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     unsigned h1, l1;
-                    split2<bf16x2>(s[e / 2][nt][2 * (e % 2)], s[e / 2][nt][2 * (e % 2) + 1], h1, l1);
+                    split2(s[e / 2][nt][2 * (e % 2)], s[e / 2][nt][2 * (e % 2) + 1], h1, l1);
                     ph[nt][e] = h1;
                     pl[nt][e] = l1;
                 }
@@ -218,18 +241,18 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_tile_kernel(const TreeArg
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         unsigned h1, l1;
-                        split2<bf16x2>(v[e / 2][2 * (e % 2)][h][j], v[e / 2][2 * (e % 2) + 1][h][j], h1, l1);
+                        split2(v[e / 2][2 * (e % 2)][h][j], v[e / 2][2 * (e % 2) + 1][h][j], h1, l1);
                         hi[e] = h1;
                         lo[e] = l1;
                     }
-                    const bf16x8 vh = __builtin_bit_cast(bf16x8, hi), vl = __builtin_bit_cast(bf16x8, lo);
+                    const f16x8 vh = __builtin_bit_cast(f16x8, hi), vl = __builtin_bit_cast(f16x8, lo);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         f32x4& o = acc[4 * h + j][nt];
-                        const bf16x8 p8 = __builtin_bit_cast(bf16x8, ph[nt]);
-                        o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vl, p8, o, 0, 0, 0);
-                        o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh, __builtin_bit_cast(bf16x8, pl[nt]), o, 0, 0, 0);
-                        o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh, p8, o, 0, 0, 0);
+                        const f16x8 p8 = __builtin_bit_cast(f16x8, ph[nt]);
+                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, p8, o, 0, 0, 0);
+                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(f16x8, pl[nt]), o, 0, 0, 0);
+                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, p8, o, 0, 0, 0);
                     }
                 }
         } else {
@@ -506,7 +529,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_tile_kernel(const TreeArg
     if (bad) *a.err = 1;
 }
 
-// Many rows of a (tree, KV head), f32x3: four waves of 32 rows each share every
+// Many rows of a (tree, KV head), f32x3: four waves of up to 32 rows each share every
 // key.  A wave in turn is given 16 keys, or the values of 32, of a step to come: it
 // loads them an iteration ahead into registers, splits them once for all the rows
 // and leaves the parts in LDS in the order in which the products' lanes read them
@@ -516,27 +539,29 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_tile_kernel(const TreeArg
 template <int D, bool kQ8>
 __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeArgs a) {
     constexpr int NT = 2, C = D / 16, KC = D / 32, H = D / 64;
-    constexpr int S = 128 / D;        // steps an iteration: eight float4 a thread
-    constexpr int KW = kWaves / 2;    // waves that take keys; the others take values
-    constexpr int TK = 128 / D;       // key tiles of 16 a wave takes
-    __shared__ u32x4 klds[2][S][2 * KC * 2][64];
-    __shared__ u32x4 vlds[2][S][4 * H * 2][64];
-    __shared__ int odds[2][S][H];     // the tree's own values: some are not finite
+    constexpr int S = 128 / D;       // steps an iteration: eight float4 a thread
+    constexpr int KW = kWaves / 2;   // waves that take keys; the others take values
+    constexpr int TK = 128 / D;      // key tiles of 16 a wave takes
+    constexpr int VO = 4 * KC, OPS = VO + 8 * H;  // operands of a step: hi, lo of [mt][kc] keys, then of the value tiles
+    __shared__ u32x4 parts[2][S][OPS][64];
+    __shared__ int odds[2][S][H];    // the tree's own values: some are not finite
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, r16 = lane & 15;
     const int4 it = a.work[2 * blockIdx.x], st = a.work[2 * blockIdx.x + 1];
     const int4 tree = a.trees[it.x];
     const int cached = tree.y, nodes = tree.z, kh = it.y, G = a.group, kvw = a.lay.kv_width;
-    const int row0 = it.z + wave * 16 * NT;
-    const bool active = row0 < nodes * G;  // (a wave without rows still stages)
-    auto node_of = [&](int nt) { return (row0 + 16 * nt + r16) / G; };
+    // 16 rows a tile, dealt to the waves in turn; a wave without any still stages
+    const int row0 = it.z + wave * 16, left_rows = nodes * G - row0;
+    const int tiles = left_rows > 16 * kWaves ? 2 : left_rows > 0 ? 1 : 0;
+    auto row_of = [&](int nt) { return row0 + 16 * kWaves * nt + r16; };
+    auto node_of = [&](int nt) { return row_of(nt) / G; };
 
     // the lane's c-th four columns of a key: as the staging lane holds them
     auto kcol = [&](int c) { return kQ8 ? 64 * (c / 4) + 16 * g + 4 * (c % 4) : 16 * c + 4 * g; };
     u32x4 qh[NT][KC], ql[NT][KC];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int node = node_of(nt), head = kh * G + row0 + 16 * nt + r16 - node * G;
+        const int node = node_of(nt), head = kh * G + row_of(nt) - node * G;
         const float* qp = a.q + (static_cast<size_t>(tree.w + node) * a.heads + head) * D;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -546,7 +571,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 unsigned hi, lo;
-                split2<f16x2>(x[2 * e], x[2 * e + 1], hi, lo);
+                split2(x[2 * e], x[2 * e + 1], hi, lo);
                 qh[nt][c / 2][2 * (c % 2) + e] = hi;
                 ql[nt][c / 2][2 * (c % 2) + e] = lo;
             }
@@ -562,11 +587,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
         for (int dt = 0; dt < 4 * H; ++dt) acc[dt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // ---- staging.  Wave w < KW: TK key tiles of 16 from mt0 on, of step kstep of the
-    // iteration; else: the value half vh of its step.
+    // ---- staging: TK key tiles of 16 from mt0 on, or the value half vh, of step
+    // `sub` of the iteration
     const bool takes_keys = wave < KW;
     const int mt0 = wave * TK % 2, vh = (wave - KW) % H;
-    const int sub = takes_keys ? wave * TK / 2 : (wave - KW) / H;  // its step of the iteration
+    const int sub = takes_keys ? wave * TK / 2 : (wave - KW) / H;
     const int csteps = (cached + kStep - 1) / kStep;
     const int tpb = a.lay.tpb, tsh = __builtin_ctz(static_cast<unsigned>(tpb));
     const int32_t* tab = a.tables + tree.x;
@@ -581,81 +606,65 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
     f32x4 raw[8];                     // eight float4
     u32x4 rawq[kQ8 ? 2 : 1];          // Q8_0: their bytes and scales
     unsigned rawd[kQ8 ? 8 : 1];
-    // lane 2i + mt: the block of key tile mt of this wave's step in the i-th iteration from here
-    auto lookup = [&](int step) {
+    // Lane 2i + mt has key tile mt (16 keys) of this wave's step in the i-th
+    // iteration from here: its block, and where its rows start and how many bytes
+    // there are to the end of the last key, zero behind it.
+    auto lookup = [&](int step) __attribute__((always_inline)) {
         return cached ? tab[min(2 * min(step + (lane >> 1) * S, csteps) + (lane & 1), last) << 4 >> tsh] : 0;
     };
-    int ids = lookup(st.x + sub), more = lookup(st.x + 32 * S + sub), at = 0;
-    // 16 keys: their rows up to the last key, `range` bytes a row from the start
-    auto tile16 = [&](int step, int mt, int range, int& pitch) {
-        const char* base;
-        int left;
-        if (kQ8 || step < csteps) {
-            const int t = min(2 * step + mt, last);
-            const int id = __builtin_amdgcn_readlane(ids, 2 * at + mt);
-            base = a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes + static_cast<size_t>((t << 4) & (tpb - 1)) * rowb;
-            left = cached - 16 * (2 * step + mt);
-            pitch = rowb;
-        } else {
-            const int n = kStep * (step - csteps) + 16 * mt;
-            base = own + static_cast<size_t>(n) * ownb;
-            left = nodes - n;
-            pitch = ownb;
-        }
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, left > 0 ? (min(left, 16) - 1) * pitch + range : 0,
-                                                 kBufferWord3);
+    Spans rows16, scales16;
+    auto spans = [&](int step, int id) __attribute__((always_inline)) {
+        const int mine = step + (lane >> 1) * S, key = 16 * (2 * mine + (lane & 1)), n = key - kStep * csteps;
+        const char* block = a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes;
+        const int slot = key & (tpb - 1), left = min(cached - key, 16), own_left = min(nodes - n, 16);
+        if (kQ8 || mine < csteps)
+            rows16.set(block + static_cast<size_t>(slot) * rowb, left > 0 ? (left - 1) * rowb + (kQ8 ? D : 4 * D) : 0);
+        else
+            rows16.set(own + static_cast<size_t>(n) * ownb, own_left > 0 ? (own_left - 1) * ownb + 4 * D : 0);
+        if constexpr (kQ8)
+            scales16.set(block + static_cast<size_t>(tpb) * D + static_cast<size_t>(slot) * (D / 32) * 2, max(left, 0) * (D / 32) * 2);
     };
-    auto load_rows = [&](int step) {
-        int pitch;
-        const __amdgpu_buffer_rsrc_t t0 = tile16(step, takes_keys && D == 128 ? mt0 : 0, D * 4, pitch);
-        const __amdgpu_buffer_rsrc_t t1 = takes_keys && D == 128 ? t0 : tile16(step, 1, D * 4, pitch);
-        const int far = takes_keys && D == 128 ? 256 : 0, by = takes_keys ? 64 : pitch;
-        const int off = takes_keys ? r16 * pitch + 16 * g : 4 * g * pitch + 256 * vh + 16 * r16;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            raw[i] = __builtin_amdgcn_raw_buffer_load_b128(t0, off, i * by, 0);
-            raw[4 + i] = __builtin_amdgcn_raw_buffer_load_b128(t1, off, i * by + far, 0);
-        }
-    };
-    auto load = [&](int step) {
+    int more = lookup(st.x + 32 * S + sub), at = 0;
+    spans(st.x + sub, lookup(st.x + sub));
+    auto load = [&](int step) __attribute__((always_inline)) {
+        // the key tiles of a thread's first and second half of the loads
+        const int ia = 2 * at + (takes_keys && D == 128 ? mt0 : 0), ib = 2 * at + (takes_keys && D == 128 ? mt0 : 1);
+        const __amdgpu_buffer_rsrc_t t0 = rows16.descriptor(ia), t1 = rows16.descriptor(ib);
         if constexpr (!kQ8) {
-            load_rows(step);
-        } else {
-            int pitch;
-            const __amdgpu_buffer_rsrc_t t0 = tile16(step, 0, D, pitch), t1 = tile16(step, 1, D, pitch);
-            // a key tile's scales, from the block's scale plane on
-            auto scales = [&](int mt) {
-                const int t = min(2 * step + mt, last), slot = (t << 4) & (tpb - 1), left = cached - 16 * (2 * step + mt);
-                const int id = __builtin_amdgcn_readlane(ids, 2 * at + mt);
-                const char* base = a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes + static_cast<size_t>(tpb) * D +
-                                   static_cast<size_t>(slot) * (D / 32) * 2;
-                return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, max(min(left, 16), 0) * (D / 32) * 2, kBufferWord3);
-            };
-            const __amdgpu_buffer_rsrc_t s0 = scales(0), s1 = scales(1);
-            if (takes_keys) {
+            const int pitch = step < csteps ? rowb : ownb;
+            const int far = takes_keys && D == 128 ? 256 : 0, by = takes_keys ? 64 : pitch;
+            const int off = takes_keys ? r16 * pitch + 16 * g : 4 * g * pitch + 256 * vh + 16 * r16;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {  // D = 128: halves of the columns; 64: the two key tiles
-                    const bool second = D == 128 ? mt0 : u;
-                    const int cu = D == 128 ? u : 0;
-                    rawq[u] = __builtin_amdgcn_raw_buffer_load_b128(second ? t1 : t0, r16 * D + 16 * g, 64 * cu, 0);
-                    rawd[u] = __builtin_amdgcn_raw_buffer_load_b16(second ? s1 : s0, (r16 * (D / 32) + (g >> 1)) * 2, 4 * cu, 0);
-                }
+            for (int i = 0; i < 4; ++i) {
+                raw[i] = __builtin_amdgcn_raw_buffer_load_b128(t0, off, i * by, 0);
+                raw[4 + i] = __builtin_amdgcn_raw_buffer_load_b128(t1, off, i * by + far, 0);
+            }
+        } else {
+            const __amdgpu_buffer_rsrc_t s0 = scales16.descriptor(ia), s1 = scales16.descriptor(ib);
+            const int off = takes_keys ? r16 * D + 16 * g : 4 * g * D + 64 * vh + 4 * r16;
+            const int soff = takes_keys ? (r16 * (D / 32) + (g >> 1)) * 2 : (4 * g * (D / 32) + 2 * vh + (r16 >> 3)) * 2;
+            if (takes_keys) {
+                const int far = D == 128 ? 1 : 0;
+                rawq[0] = __builtin_amdgcn_raw_buffer_load_b128(t0, off, 0, 0);
+                rawq[1] = __builtin_amdgcn_raw_buffer_load_b128(t1, off, 64 * far, 0);
+                rawd[0] = __builtin_amdgcn_raw_buffer_load_b16(s0, soff, 0, 0);
+                rawd[1] = __builtin_amdgcn_raw_buffer_load_b16(s1, soff, 4 * far, 0);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    rawq[i / 4][i % 4] = __builtin_amdgcn_raw_buffer_load_b32(i < 4 ? t0 : t1, 4 * g * D + 64 * vh + 4 * r16, i % 4 * D, 0);
-                    rawd[i] = __builtin_amdgcn_raw_buffer_load_b16(i < 4 ? s0 : s1, (4 * g * (D / 32) + 2 * vh + (r16 >> 3)) * 2,
-                                                                   i % 4 * (D / 32) * 2, 0);
+                    rawq[i / 4][i % 4] = __builtin_amdgcn_raw_buffer_load_b32(i < 4 ? t0 : t1, off, i % 4 * D, 0);
+                    rawd[i] = __builtin_amdgcn_raw_buffer_load_b16(i < 4 ? s0 : s1, soff, i % 4 * (D / 32) * 2, 0);
                 }
             }
         }
         if (++at == 32) {
             at = 0;
-            ids = more;
+            spans(step + S, more);
             more = lookup(step + 33 * S);
+            wait_for_loads();
         }
     };
-    auto stage = [&](int buf, int step, const f32x4 (&x)[8]) {
+    auto stage = [&](int buf, int step, const f32x4 (&x)[8]) __attribute__((always_inline)) {
         if (takes_keys) {
 #pragma unroll
             for (int p = 0; p < 4; ++p) {  // an operand: two float4
@@ -663,48 +672,47 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     unsigned h1, l1;
-                    split2<f16x2>(x[2 * p + e / 2][2 * (e % 2)], x[2 * p + e / 2][2 * (e % 2) + 1], h1, l1);
+                    split2(x[2 * p + e / 2][2 * (e % 2)], x[2 * p + e / 2][2 * (e % 2) + 1], h1, l1);
                     hi[e] = h1;
                     lo[e] = l1;
                 }
                 const int o = D == 128 ? mt0 * KC + p : p;  // [mt][kc]
-                klds[buf][sub][2 * o][lane] = hi;
-                klds[buf][sub][2 * o + 1][lane] = lo;
+                parts[buf][sub][2 * o][lane] = hi;
+                parts[buf][sub][2 * o + 1][lane] = lo;
             }
         } else {
-            f32x4 y[8];
+            const bool tail = step >= csteps;
             float odd = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = x[i];
-            if (step >= csteps) {
-                // Zero times a value that is not finite would reach rows that do not
-                // see it: it is zero in the product, and added to the rows that do.
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        odd = fmaf(y[i][j], 0.f, odd);
-                        y[i][j] = finite_or_zero(y[i][j]);
-                    }
-                const bool any = __any(odd != 0.f);
-                if (lane == 0) odds[buf][sub][vh] = any;
-            }
-#pragma unroll
             for (int j = 0; j < 4; ++j) {
+                f32x4 y[2] = {{x[0][j], x[1][j], x[2][j], x[3][j]}, {x[4][j], x[5][j], x[6][j], x[7][j]}};
+                if (tail) {
+                    // Zero times a value that is not finite would reach rows that do not
+                    // see it: it is zero in the product, and added to the rows that do.
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        odd = fmaf(y[e / 4][e % 4], 0.f, odd);
+                        y[e / 4][e % 4] = finite_or_zero(y[e / 4][e % 4]);
+                    }
+                }
                 u32x4 hi, lo;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     unsigned h1, l1;
-                    split2<bf16x2>(y[2 * e][j], y[2 * e + 1][j], h1, l1);
+                    split2(y[e / 2][2 * (e % 2)], y[e / 2][2 * (e % 2) + 1], h1, l1);
                     hi[e] = h1;
                     lo[e] = l1;
                 }
-                vlds[buf][sub][2 * (4 * vh + j)][lane] = hi;
-                vlds[buf][sub][2 * (4 * vh + j) + 1][lane] = lo;
+                parts[buf][sub][VO + 2 * (4 * vh + j)][lane] = hi;
+                parts[buf][sub][VO + 2 * (4 * vh + j) + 1][lane] = lo;
+            }
+            if (tail) {
+                const bool any = __any(odd != 0.f);
+                if (lane == 0) odds[buf][sub][vh] = any;
             }
         }
     };
-    auto put = [&](int buf, int step) {
+    auto put = [&](int buf, int step) __attribute__((always_inline)) {
         if constexpr (kQ8) {
             f32x4 x[8];
 #pragma unroll
@@ -719,25 +727,40 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
         }
     };
 
-    auto compute = [&](int buf, int t, int step) {
-        f32x4 s[2][NT];  // scores, then probabilities, of keys 16mt + 4g + i
+    f32x4 s[2][NT];  // scores, then probabilities, of keys 16mt + 4g + i
+    auto operands = [&](int buf, int t) __attribute__((always_inline)) {
+        unsigned at16 = static_cast<unsigned>((buf * S + t) * OPS * 64 + lane);
+        asm("" : "+v"(at16));  // one address, the operands at constant offsets from it
+        return &parts[0][0][0][0] + at16;
+    };
+    // (operands are read from LDS one ahead of their products)
+    auto scores = [&](int buf, int t) __attribute__((always_inline)) {
+        const u32x4* op = operands(buf, t);
+        u32x4 hi = op[0], lo = op[64];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-            for (int kc = 0; kc < KC; ++kc) {
-                const f16x8 kh8 = __builtin_bit_cast(f16x8, klds[buf][t][2 * (mt * KC + kc)][lane]);
-                const f16x8 kl8 = __builtin_bit_cast(f16x8, klds[buf][t][2 * (mt * KC + kc) + 1][lane]);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl8, __builtin_bit_cast(f16x8, qh[nt][kc]),
-                                                                       kc ? s[mt][nt] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh8, __builtin_bit_cast(f16x8, ql[nt][kc]), s[mt][nt], 0, 0, 0);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh8, __builtin_bit_cast(f16x8, qh[nt][kc]), s[mt][nt], 0, 0, 0);
+        for (int o = 0; o < 2 * KC; ++o) {
+            const int mt = o / KC, kc = o % KC;
+            const f16x8 kh8 = __builtin_bit_cast(f16x8, hi), kl8 = __builtin_bit_cast(f16x8, lo);
+            if (o + 1 < 2 * KC) {
+                hi = op[64 * (2 * o + 2)];
+                lo = op[64 * (2 * o + 3)];
             }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl8, __builtin_bit_cast(f16x8, qh[nt][kc]),
+                                                                   kc ? s[mt][nt] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh8, __builtin_bit_cast(f16x8, ql[nt][kc]), s[mt][nt], 0, 0, 0);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh8, __builtin_bit_cast(f16x8, qh[nt][kc]), s[mt][nt], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    u32x4 ph[NT], pl[NT];
+    auto softmax = [&](int buf, int t, int step) __attribute__((always_inline)) {
         // what a row does not see: keys behind the last cached one, other branches' nodes
         const bool tail = step >= csteps;
         if (tail || kStep * step + kStep > cached) {
@@ -752,6 +775,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
                     for (int i = 0; i < 4; ++i)
                         if (!(mask >> (16 * mt + 4 * g + i) & 1u)) s[mt][nt][i] = -INFINITY;
             }
+            wait_for_loads();
         }
         // (a score that is not finite is NaN here, and so is its row's sum: an input
         // beyond fp16 is infinite in one part and its opposite in the other)
@@ -787,19 +811,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
         if (odd) {
             const int n0 = kStep * (step - csteps);
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
-#pragma unroll 1
-                for (int e = 0; e < 16; ++e) {
-                    const int key = n0 + 16 * mt + e, i = e & 3;
-                    if (key >= nodes) break;
-                    const float* vr = a.values + static_cast<size_t>(tree.w + key) * a.row_stride + static_cast<size_t>(kh) * D;
+            for (int nt = 0; nt < NT; ++nt) {
+                const int node = node_of(nt);
+                const uint32_t mask = node < nodes ? a.mask[static_cast<size_t>(tree.w + node) * a.words + (step - csteps)] : 0u;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const int node = node_of(nt);
+                for (int mt = 0; mt < 2; ++mt)
+#pragma unroll 1
+                    for (int e = 0; e < 16; ++e) {
+                        const int key = n0 + 16 * mt + e, i = e & 3;
+                        if (key >= nodes) break;
+                        const float* vr = a.values + static_cast<size_t>(tree.w + key) * a.row_stride + static_cast<size_t>(kh) * D;
                         const float mine = i == 0 ? s[mt][nt][0] : i == 1 ? s[mt][nt][1] : i == 2 ? s[mt][nt][2] : s[mt][nt][3];
                         const float p = __shfl(mine, r16 + 16 * (e >> 2));
-                        const bool on = node < nodes &&
-                                        (a.mask[static_cast<size_t>(tree.w + node) * a.words + (step - csteps)] >> (16 * mt + e) & 1u);
+                        const bool on = (mask >> (16 * mt + e) & 1u) != 0;
 #pragma unroll
                         for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -810,31 +834,40 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
                                     if (on && !__builtin_isfinite(y[j])) acc[4 * h + j][nt][o] = fmaf(p, y[j], acc[4 * h + j][nt][o]);
                             }
                     }
-                }
+            }
+            wait_for_loads();
         }
-        u32x4 ph[NT], pl[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 unsigned h1, l1;
-                split2<bf16x2>(s[e / 2][nt][2 * (e % 2)], s[e / 2][nt][2 * (e % 2) + 1], h1, l1);
+                split2(s[e / 2][nt][2 * (e % 2)], s[e / 2][nt][2 * (e % 2) + 1], h1, l1);
                 ph[nt][e] = h1;
                 pl[nt][e] = l1;
             }
+    };
+    auto output = [&](int buf, int t) __attribute__((always_inline)) {
+        const u32x4* op = operands(buf, t) + 64 * VO;
+        u32x4 hi = op[0], lo = op[64];
 #pragma unroll
         for (int dt = 0; dt < 4 * H; ++dt) {
-            const bf16x8 vh8 = __builtin_bit_cast(bf16x8, vlds[buf][t][2 * dt][lane]);
-            const bf16x8 vl8 = __builtin_bit_cast(bf16x8, vlds[buf][t][2 * dt + 1][lane]);
+            const f16x8 vh8 = __builtin_bit_cast(f16x8, hi), vl8 = __builtin_bit_cast(f16x8, lo);
+            if (dt + 1 < 4 * H) {
+                hi = op[64 * (2 * dt + 2)];
+                lo = op[64 * (2 * dt + 3)];
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-                acc[dt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vl8, __builtin_bit_cast(bf16x8, ph[nt]), acc[dt][nt], 0, 0, 0);
+                acc[dt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl8, __builtin_bit_cast(f16x8, ph[nt]), acc[dt][nt], 0, 0, 0);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-                acc[dt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh8, __builtin_bit_cast(bf16x8, pl[nt]), acc[dt][nt], 0, 0, 0);
+                acc[dt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh8, __builtin_bit_cast(f16x8, pl[nt]), acc[dt][nt], 0, 0, 0);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-                acc[dt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh8, __builtin_bit_cast(bf16x8, ph[nt]), acc[dt][nt], 0, 0, 0);
+                acc[dt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh8, __builtin_bit_cast(f16x8, ph[nt]), acc[dt][nt], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
@@ -849,46 +882,56 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
         for (int step = st.x; step < end; step += S, buf ^= 1) {
             put(buf ^ 1, step + S + sub);
             load(step + 2 * S + sub);
-            if (active)
+            if (tiles)
 #pragma unroll 1
-                for (int t = 0; t < S && step + t < end; ++t) compute(buf, t, step + t);
+                for (int t = 0; t < S && step + t < end; ++t) {
+                    scores(buf, t);
+                    softmax(buf, t, step + t);
+                    output(buf, t);
+                }
             __syncthreads();
         }
     }
     if constexpr (kQ8) {
 #pragma unroll 1
-        for (int step = max(st.x, csteps); step < st.y; ++step) {
-            if (sub == 0) {
-                const int n0 = kStep * (step - csteps);
-                f32x4 x[8];
+        for (int step = max(st.x, csteps); step < st.y; step += S) {
+            const int n0 = kStep * (step + sub - csteps);
+            f32x4 x[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int key = n0 + (takes_keys ? 16 * (D == 128 ? mt0 : i / 4) + r16 : 16 * (i / 4) + 4 * g + i % 4);
-                    const int col = takes_keys ? kcol(D == 128 ? i : i % 4) : 64 * vh + 4 * r16;
-                    x[i] = *reinterpret_cast<const f32x4*>(own + static_cast<size_t>(min(key, nodes - 1)) * ownb + 4 * col);
-                }
-                stage(0, step, x);
+            for (int i = 0; i < 8; ++i) {
+                const int key = n0 + (takes_keys ? 16 * (D == 128 ? mt0 : i / 4) + r16 : 16 * (i / 4) + 4 * g + i % 4);
+                const int col = takes_keys ? kcol(D == 128 ? i : i % 4) : 64 * vh + 4 * r16;
+                x[i] = *reinterpret_cast<const f32x4*>(own + static_cast<size_t>(min(key, nodes - 1)) * ownb + 4 * col);
             }
+            stage(0, step + sub, x);
             __syncthreads();
-            if (active) compute(0, 0, step);
+            if (tiles)
+#pragma unroll 1
+                for (int t = 0; t < S && step + t < st.y; ++t) {
+                    scores(0, t);
+                    softmax(0, t, step + t);
+                    output(0, t);
+                }
             __syncthreads();
         }
     }
 
+    float total[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) total[nt] = cross_row_sum(l[nt]);
     bool bad = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const float total = cross_row_sum(l[nt]);
-        const int node = node_of(nt), head = kh * G + row0 + 16 * nt + r16 - node * G;
+        const int node = node_of(nt), head = kh * G + row_of(nt) - node * G;
         if (node >= nodes) continue;
         const size_t row = static_cast<size_t>(tree.w) + node;
         const int2 runs = a.runs[row];
         const bool whole = runs.y == 1;
         const size_t to = whole ? row * a.heads + head : (static_cast<size_t>(runs.x) + it.w) * a.heads + head;
         float* o = (whole ? a.out : a.part_acc) + to * D + 16 * g;
-        const float inv = whole ? total : 1.f;
-        if (!whole && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * to) = make_float2(m[nt], total);
-        bad |= !__builtin_isfinite(total);
+        const float inv = whole ? total[nt] : 1.f;
+        if (!whole && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * to) = make_float2(m[nt], total[nt]);
+        bad |= !__builtin_isfinite(total[nt]);
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
