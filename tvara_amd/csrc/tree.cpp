@@ -132,17 +132,27 @@ void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t
     else
         row_work(trees, work, runs);
     if (slots > kIntMax / h || work.size() > kIntMax) throw std::invalid_argument("attention batch too large");
-    items = static_cast<int>(tile_rows ? work.size() / 2 : work.size());
+    items = static_cast<int>(tile_rows ? work.size() / 3 : work.size());
+
+    // acceptance's: each row's tree, and counters that start at zero
+    std::vector<int32_t> tree_of(rows), zeros(std::max(n, blocks), 0);
+    every_tree_has_nodes = true;
+    for (size_t i = 0; i < n; ++i) {
+        std::fill_n(tree_of.begin() + trees[i].w, trees[i].z, static_cast<int32_t>(i));
+        every_tree_has_nodes &= trees[i].z > 0;
+    }
 
     std::vector<PlanRegion::Section> s = {
         {tab.data(), tab.size() * sizeof(int32_t)},   {trees.data(), n * sizeof(int4)},
         {mask.data(), mask.size() * sizeof(uint32_t)}, {work.data(), work.size() * sizeof(int4)},
         {runs.data(), runs.size() * sizeof(int2)},     {parents, rows * sizeof(int32_t)},
+        {tree_of.data(), rows * sizeof(int32_t)},      {zeros.data(), n * sizeof(int)},
+        {zeros.data(), blocks * sizeof(int)},
         {nullptr, slots * h * g.head_dim * sizeof(float)}, {nullptr, slots * h * 2 * sizeof(float)},
-        {nullptr, std::max(rows, kAcceptParts) * sizeof(uint64_t)},
+        {nullptr, (rows + kAcceptParts) * sizeof(uint64_t)},
     };
     region.place(*c, s);
-    size_t* at[] = {&tables_at, &trees_at, &mask_at, &work_at, &runs_at, &parents_at, &acc_at, &ml_at, &best_at};
+    size_t* at[] = {&tables_at, &trees_at, &mask_at, &work_at, &runs_at, &parents_at, &tree_of_at, &done_at, &block_done_at, &acc_at, &ml_at, &best_at};
     for (size_t i = 0; i < s.size(); ++i) *at[i] = s[i].at;
 }
 
@@ -165,9 +175,12 @@ void TreePlan::row_work(const std::vector<int4>& trees, std::vector<int4>& work,
     }
 }
 
-// Runs of steps of the tiles, as many as give every CU a workgroup.
+// Runs of steps of the tiles, as many as give every CU its workgroups.  Ids go to the
+// XCDs round-robin: the row blocks of one run, which read the same keys, go to one
+// XCD, whose L2 then has them, and the XCDs' lists are filled by the fewest steps so
+// far, each ordered from the longest run to the shortest.
 void TreePlan::tile_work(const std::vector<int4>& trees, std::vector<int4>& work, std::vector<int2>& runs) {
-    const int kv_heads = cache->layout().kv_heads;
+    const int kv_heads = cache->layout().kv_heads, xcds = std::max(1, cache->xcds());
     auto cached_steps = [](const int4& t) { return (t.y + kTreeStep - 1) / kTreeStep; };
     // steps over the tree's own nodes of the row block from row r0
     auto own_steps = [&](const int4& t, int r0) {
@@ -177,35 +190,46 @@ void TreePlan::tile_work(const std::vector<int4>& trees, std::vector<int4>& work
     for (const int4& t : trees)
         for (int r0 = 0; r0 < t.z * group; r0 += tile_rows)
             total += static_cast<size_t>(kv_heads) * (cached_steps(t) + own_steps(t, r0));
-    // (two workgroups of 128 rows share a CU)
-    const size_t units = static_cast<size_t>(cache->compute_units()) * (tile_rows == 128 ? 2 : 1);
+    const size_t units = static_cast<size_t>(cache->compute_units()) * tree_tile_units(cache->layout(), tile_rows, precision == 2);
     const size_t per = std::max<size_t>(4, (total + units - 1) / units);
-    struct Item {
-        int4 where;
-        int step, end;
+    struct Group {  // the row blocks of a run
+        int tree, head, run, runs, slot, block, step, end;
     };
-    std::vector<Item> list;
+    std::vector<Group> groups;
+    blocks = 0;
     for (size_t i = 0; i < trees.size(); ++i) {
         const int4& t = trees[i];
         if (!t.z) continue;
-        const int steps = cached_steps(t) + own_steps(t, (t.z * group - 1) / tile_rows * tile_rows);
+        const int row_blocks = (t.z * group - 1) / tile_rows + 1;
+        const int steps = cached_steps(t) + own_steps(t, (row_blocks - 1) * tile_rows);
         const int parts = static_cast<int>((steps + per - 1) / per), len = (steps + parts - 1) / parts;
-        for (int j = 0; j < t.z; ++j) {
-            runs[t.w + j] = make_int2(static_cast<int>(slots), parts);
-            if (parts > 1) slots += parts;
-        }
         for (int p = 0; p < parts; ++p)
             for (int h = 0; h < kv_heads; ++h)
-                for (int r0 = 0; r0 < t.z * group; r0 += tile_rows) {
-                    const int all = cached_steps(t) + own_steps(t, r0);
-                    list.push_back({make_int4(static_cast<int>(i), h, r0, p), std::min(p * len, all), std::min((p + 1) * len, all)});
-                }
+                groups.push_back({static_cast<int>(i), h, p, parts, static_cast<int>(slots),
+                                  static_cast<int>(blocks) + h * row_blocks, p * len, std::min((p + 1) * len, steps)});
+        blocks += static_cast<size_t>(kv_heads) * row_blocks;
+        for (int j = 0; j < t.z; ++j) runs[t.w + j] = make_int2(static_cast<int>(slots + static_cast<size_t>(j) * parts), parts);
+        if (parts > 1) slots += static_cast<size_t>(t.z) * parts;
+        if (slots > kIntMax / heads || blocks > kIntMax) throw std::invalid_argument("attention batch too large");
     }
-    std::stable_sort(list.begin(), list.end(), [](const Item& x, const Item& y) { return x.end - x.step > y.end - y.step; });
-    for (const Item& x : list) {
-        work.push_back(x.where);
-        work.push_back(make_int4(x.step, x.end, 0, 0));
+    std::stable_sort(groups.begin(), groups.end(), [](const Group& x, const Group& y) { return x.end - x.step > y.end - y.step; });
+    std::vector<std::vector<int4>> lists(xcds);
+    std::vector<size_t> load(xcds, 0);
+    for (const Group& x : groups) {
+        const int4& t = trees[x.tree];
+        const size_t to = std::min_element(load.begin(), load.end()) - load.begin();
+        for (int r0 = 0, b = 0; r0 < t.z * group; r0 += tile_rows, ++b) {
+            const int all = cached_steps(t) + own_steps(t, r0);
+            const int step = std::min(x.step, all), end = std::min(x.end, all);
+            lists[to].insert(lists[to].end(), {t, make_int4(x.head, r0, step, end), make_int4(x.run, x.runs, x.slot, x.block + b)});
+            load[to] += end - step + 1;
+        }
     }
+    size_t longest = 0;
+    for (const auto& l : lists) longest = std::max(longest, l.size());
+    work.assign(longest * xcds, make_int4(0, 0, 0, 0));  // (padding has no nodes)
+    for (int x = 0; x < xcds; ++x)
+        for (size_t k = 0; k < lists[x].size(); ++k) work[3 * (k / 3 * xcds + x) + k % 3] = lists[x][k];
 }
 
 void TreePlan::launch(int layer, const float* q, const float* keys, const float* values, size_t row_stride, float* out,
@@ -242,12 +266,16 @@ void TreePlan::launch(int layer, const float* q, const float* keys, const float*
     a.part_acc = reinterpret_cast<float*>(d + acc_at);
     a.part_ml = reinterpret_cast<float*>(d + ml_at);
     a.qscale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(g.head_dim)));
+    // few workgroups merge their runs themselves, which saves the second launch
+    const bool alone = tile_rows && items <= kTreeMergeMax;
+    a.done = alone ? reinterpret_cast<int*>(d + block_done_at) : nullptr;
+    a.check = tile_rows && precision == 2;
     a.err = region.flags();
     if (tile_rows)
         launch_tree_tiles(a, tile_rows, items, precision == 2, s);
     else
         launch_tree_rows(a, items, s);
-    if (slots) launch_tree_merge(a, s);
+    if (slots && !alone) launch_tree_merge(a, s);
     cache->leave(s);
     region.launched(s);
 }
@@ -270,7 +298,10 @@ void TreePlan::accept(const uint32_t* tokens, const uint32_t* first, const float
     a.logits = logits;
     a.vocab = vocab;
     a.logits_stride = logits_stride;
-    a.splits = tree_accept_splits(rows, vocab);
+    a.done = reinterpret_cast<int*>(d + done_at);
+    a.tree_of = reinterpret_cast<const int32_t*>(d + tree_of_at);
+    a.every_tree_has_nodes = every_tree_has_nodes;
+    tree_accept_parts(a);
     a.best = reinterpret_cast<uint64_t*>(d + best_at);
     a.path = path;
     a.path_stride = path_stride;
@@ -350,6 +381,8 @@ void SlotPlan::write(const int64_t* slots, const int32_t* rows, size_t n, const 
     if (n > kIntMax || row_count > kIntMax) throw std::invalid_argument("KV write too large");
     if (row_stride < g.kv_width() || (g.layers > 1 && layer_stride < g.kv_width()))
         throw std::invalid_argument("token rows overlap");
+    if (cache->format() == kQ8 && (row_stride % 4 || (g.layers > 1 && layer_stride % 4)))
+        throw std::invalid_argument("device buffers must be 16-byte aligned");
     if (!n) return;
     cache->check_device();
     cache->flush();

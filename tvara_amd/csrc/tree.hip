@@ -131,7 +131,9 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
         sum.y = sum.y * wm + x.y * wr;
         m = mn;
     }
-    *reinterpret_cast<float2*>(a.out + at * D + c) = make_float2(sum.x / l, sum.y / l);
+    const float2 o = make_float2(sum.x / l, sum.y / l);
+    if (a.check && !(__builtin_isfinite(o.x) && __builtin_isfinite(o.y))) *a.err = 1;
+    *reinterpret_cast<float2*>(a.out + at * D + c) = o;
 }
 
 }  // namespace

@@ -36,6 +36,8 @@ struct TreeArgs {
     float* out;            // [node rows][heads][head_dim]
     float* part_acc;       // [partials][heads][head_dim]
     float* part_ml;        // [partials][heads][2]: maximum (log2 units), normaliser
+    int* done;             // per row block: runs done in this launch, zero between launches (null: launch_tree_merge)
+    bool check;            // a merged result that is not finite sets *err
     float qscale;          // log2(e) / sqrt(head_dim)
     int* err;
 };
@@ -50,7 +52,11 @@ struct AcceptArgs {
     const float* logits;     // [node rows], logits_stride apart
     size_t vocab, logits_stride;
     int splits;              // parts of a row's vocabulary
+    size_t part;             // logits of a part
     uint64_t* best;          // [node rows][splits]
+    int* done;               // [trees]: parts done in this launch, zero between launches (null: a launch of its own walks)
+    const int32_t* tree_of;  // [node rows]
+    bool every_tree_has_nodes;
     int32_t* path;           // [trees][path_stride]: accepted node rows, -1 behind
     size_t path_stride;
     int32_t* accepted;       // [trees]
@@ -91,14 +97,18 @@ struct WriteArgs {
 void launch_tree_rows(const TreeArgs& a, int items, hipStream_t s);
 void launch_tree_merge(const TreeArgs& a, hipStream_t s);
 // tree_tiles.hip: head_dim 64 and 128; a workgroup takes up to tree_tile_rows(rows
-// of the largest tree and KV head) rows, and work has two entries a workgroup
+// of the largest tree and KV head) rows, and work has three entries a workgroup: the tree (as trees); KV head, first
+// row, first step, end; run, runs, the tree's first partial, its row block
 bool tree_tiles_supported(const BlockLayout& lay);
 int tree_tile_rows(size_t most, bool x3);
+int tree_tile_units(const BlockLayout& lay, int rows, bool x3);  // workgroups that share a CU
 constexpr int kTreeStep = 32;  // keys of a step
+constexpr int kTreeMergeMax = 128;  // workgroups of the largest launch that merges its runs itself
 void launch_tree_tiles(const TreeArgs& a, int rows, int workgroups, bool x3, hipStream_t s);
-// tree_accept.hip: rows * splits is at most the larger of rows and kAcceptParts
-constexpr size_t kAcceptParts = 2048;
-int tree_accept_splits(size_t rows, size_t vocab);
+// tree_accept.hip: chooses part, splits and whether done stays; rows * splits is at
+// most rows + kAcceptParts
+constexpr size_t kAcceptParts = 4096;
+void tree_accept_parts(AcceptArgs& a);
 void launch_tree_accept(const AcceptArgs& a, hipStream_t s);
 // slots.hip
 void launch_slot_map(const SlotArgs& a, hipStream_t s);
@@ -144,10 +154,11 @@ struct TreePlan {
     uint64_t epoch = 0;
     int heads = 0, group = 0, precision = 0, words = 1, items = 0, split_tokens = 0;
     int tile_rows = 0;  // rows of a workgroup of the tiles (0: the row kernel)
-    size_t count = 0, rows = 0, slots = 0;
+    size_t count = 0, rows = 0, slots = 0, blocks = 0;
     PlanRegion region;
     size_t tables_at = 0, trees_at = 0, mask_at = 0, work_at = 0, runs_at = 0, parents_at = 0, acc_at = 0, ml_at = 0,
-           best_at = 0;
+           best_at = 0, done_at = 0, block_done_at = 0, tree_of_at = 0;
+    bool every_tree_has_nodes = true;
 
     void build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t heads, size_t context,
                const size_t* visible, const size_t* nodes, const int32_t* parents, int precision);

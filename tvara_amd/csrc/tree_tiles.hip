@@ -10,8 +10,7 @@
 //  O^T = V^T P^T: lane (g, r) loads four columns of the keys 4g + i of each 16,
 //    so it holds V^T's operand for four output tiles (tile j: column j of every
 //    lane's four) and its own scores are P^T's.
-// Steps are dealt in turn to WK of the workgroup's four waves (WR row blocks
-// times WK), whose results meet in LDS.  A long context is cut into runs, a
+// Steps are dealt in turn to the workgroup's four waves, whose results meet in LDS.  A long context is cut into runs, a
 // workgroup each, that leave partials for a merge.  After the cached steps come
 // those over the tree's own nodes, with a mask word a row.
 //
@@ -79,18 +78,106 @@ __device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned&
     lo = __builtin_bit_cast(unsigned, __builtin_convertvector(rest, f16x2));
 }
 
-template <int D, int NT, int WR, bool kQ8, bool kX3>
-__global__ __launch_bounds__(64 * kWaves, 1) void tree_tile_kernel(const TreeArgs a) {
-    constexpr int WK = kWaves / WR, C = D / 16, KC = D / 32, H = D / 64;
+__device__ __forceinline__ bool all_finite(f32x4 x) {
+    return __builtin_isfinite(x[0]) && __builtin_isfinite(x[1]) && __builtin_isfinite(x[2]) && __builtin_isfinite(x[3]);
+}
+
+// A workgroup's work: a tree (TreeArgs::trees), the KV head and first row of a row
+// block, and a run of its steps; the partials of the tree's node j are slot + j *
+// runs on, and `block` counts the row block's finished runs.
+struct Item {
+    int4 tree;
+    int head, row0, step, end, run, runs, slot, block;
+};
+__device__ __forceinline__ Item item_of(const TreeArgs& a) {
+    const int4 t = a.work[3 * blockIdx.x], x = a.work[3 * blockIdx.x + 1], y = a.work[3 * blockIdx.x + 2];
+    return {t, x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+}
+
+// partials of a launch that merges them itself go past the XCD's L2
+__device__ __forceinline__ void put_partial(const TreeArgs& a, float* to, f32x4 x) {
+    if (!a.done) {
+        *reinterpret_cast<f32x4*>(to) = x;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) __hip_atomic_store(to + i, x[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void put_partial(const TreeArgs& a, float* to, float2 x) {
+    if (!a.done) {
+        *reinterpret_cast<float2*>(to) = x;
+        return;
+    }
+    __hip_atomic_store(to, x.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(to + 1, x.y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The last workgroup of a row block's runs combines them in order, as
+// tree_merge_kernel does.  Every wave waits for its partials' stores before the
+// count; release and acquire at device scope order them against the last one's
+// reads.  Releases write an XCD's L2 back, one after the other, so only launches of
+// few workgroups come here (TreePlan::launch).
+template <int D>
+__device__ void merge_rows(const TreeArgs& a, const Item& it, int rows, bool check) {
+    __shared__ int last;
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int* done = a.done + it.block;
+        const int before = __hip_atomic_fetch_add(done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        last = before == it.runs - 1;
+        if (last) __hip_atomic_store(done, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last) return;
+    auto ld = [](const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    const int live = min(rows, it.tree.z * a.group - it.row0);
+    for (int e = threadIdx.x; e < live * (D / 4); e += 64 * kWaves) {
+        const int r = it.row0 + e / (D / 4), c = 4 * (e % (D / 4)), node = r / a.group, head = it.head * a.group + r - node * a.group;
+        const size_t first = (static_cast<size_t>(it.slot) + static_cast<size_t>(node) * it.runs) * a.heads + head;
+        float m = -INFINITY, l = 0.f;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        constexpr int U = 4;  // runs requested together
+        for (int r0 = 0; r0 < it.runs; r0 += U) {
+            float rm[U], rl[U];
+            f32x4 x[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                const size_t p = first + static_cast<size_t>(min(r0 + k, it.runs - 1)) * a.heads;
+                const float* pa = a.part_acc + p * D + c;
+                rm[k] = ld(a.part_ml + 2 * p);
+                rl[k] = ld(a.part_ml + 2 * p + 1);
+                x[k] = f32x4{ld(pa), ld(pa + 1), ld(pa + 2), ld(pa + 3)};
+            }
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                if (r0 + k >= it.runs || rm[k] == -INFINITY) continue;
+                const float mn = fmaxf(m, rm[k]), wm = fast_exp2(m - mn), wr = fast_exp2(rm[k] - mn);
+                l = l * wm + rl[k] * wr;
+                sum = sum * wm + x[k] * wr;
+                m = mn;
+            }
+        }
+        sum /= l;
+        if (check && !all_finite(sum)) *a.err = 1;
+        *reinterpret_cast<f32x4*>(a.out + ((static_cast<size_t>(it.tree.w) + node) * a.heads + head) * D + c) = sum;
+    }
+}
+
+template <int D, int NT, bool kQ8, bool kX3>
+__global__ __launch_bounds__(64 * kWaves, NT * D * (kX3 ? 2 : 1) <= 128 ? 2 : 1) void tree_tile_kernel(const TreeArgs a) {
+    constexpr int WK = kWaves, C = D / 16, KC = D / 32, H = D / 64;
     __shared__ f32x4 sums[kWaves][4][NT][64];
     __shared__ float2 stats[kWaves][16 * NT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g = lane >> 4, r16 = lane & 15, wk = wave % WK;
-    // x: tree, y: KV head, z: first row, w: run; then x: first step, y: its end
-    const int4 it = a.work[2 * blockIdx.x], st = a.work[2 * blockIdx.x + 1];
-    const int4 tree = a.trees[it.x];
-    const int cached = tree.y, nodes = tree.z, kh = it.y, G = a.group, kvw = a.lay.kv_width;
-    const int row0 = it.z + (wave / WK) * 16 * NT;
+    const int g = lane >> 4, r16 = lane & 15, wk = wave;
+    const Item it = item_of(a);
+    if (!it.tree.z) return;  // the list's padding
+    const int4 tree = it.tree;
+    const int cached = tree.y, nodes = tree.z, kh = it.head, G = a.group, kvw = a.lay.kv_width;
+    const int row0 = it.row0;
 
     // this lane's row of each row tile
     int node[NT], head[NT];
@@ -279,7 +366,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_tile_kernel(const TreeArg
     };
 
     // ---- cached steps: this wave's are step0 + wk, + WK, ...
-    const int csteps = (cached + kStep - 1) / kStep, end = min(st.y, csteps);
+    const int csteps = (cached + kStep - 1) / kStep, end = min(it.end, csteps);
     const int tpb = a.lay.tpb, tsh = __builtin_ctz(static_cast<unsigned>(tpb));
     const int32_t* tab = a.tables + tree.x;
     const size_t kbytes = kQ8 ? static_cast<size_t>(a.layer) * 2 * a.lay.section + static_cast<size_t>(kh) * a.lay.head_bytes
@@ -288,7 +375,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_tile_kernel(const TreeArg
     const int rowb = kQ8 ? D : kvw * static_cast<int>(sizeof(float));  // from one slot to the next
     const unsigned koff = static_cast<unsigned>(r16 * rowb + kcol(0) * (kQ8 ? 1 : 4));
     const unsigned voff = static_cast<unsigned>(4 * g * rowb + vcol(0, r16) * (kQ8 ? 1 : 4));
-    int step = st.x + wk;
+    int step = it.step + wk;
     if (step < end) {
         const int last = (cached - 1) >> 4;  // 16 keys a table lookup; past the end the last again
         // lane 2i + mt: the block of the wave's i-th step from here
@@ -383,7 +470,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_tile_kernel(const TreeArg
     }
 
     // ---- the tree's own nodes
-    for (; step < st.y; step += WK) {
+    for (; step < it.end; step += WK) {
         const int n0 = kStep * (step - csteps);
         const float* kb = a.keys + static_cast<size_t>(tree.w) * a.row_stride + static_cast<size_t>(kh) * D;
         const float* vb = a.values + static_cast<size_t>(tree.w) * a.row_stride + static_cast<size_t>(kh) * D;
@@ -456,77 +543,59 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_tile_kernel(const TreeArg
     float total[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) total[nt] = cross_row_sum(l[nt]);
-    if constexpr (WK > 1) {
-        if (g == 0)
+    if (g == 0)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) stats[wave][16 * nt + r16] = make_float2(m[nt], total[nt]);
-        __syncthreads();
+        for (int nt = 0; nt < NT; ++nt) stats[wave][16 * nt + r16] = make_float2(m[nt], total[nt]);
+    __syncthreads();
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            float top = -INFINITY, sum = 0.f;
+    for (int nt = 0; nt < NT; ++nt) {
+        float top = -INFINITY, sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < WK; ++w) top = fmaxf(top, stats[wave - wk + w][16 * nt + r16].x);
-            const float base = top == -INFINITY ? 0.f : top;
+        for (int w = 0; w < WK; ++w) top = fmaxf(top, stats[w][16 * nt + r16].x);
+        const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-            for (int w = 0; w < WK; ++w) {
-                const float2 x = stats[wave - wk + w][16 * nt + r16];
-                sum = fmaf(fast_exp2(x.x - base), x.y, sum);
-            }
-            const float scale = fast_exp2(m[nt] - base);
-#pragma unroll
-            for (int dt = 0; dt < 4 * H; ++dt) acc[dt][nt] *= scale;
-            m[nt] = top;
-            total[nt] = sum;
+        for (int w = 0; w < WK; ++w) {
+            const float2 x = stats[w][16 * nt + r16];
+            sum = fmaf(fast_exp2(x.x - base), x.y, sum);
         }
+        const float scale = fast_exp2(m[nt] - base);
+#pragma unroll
+        for (int dt = 0; dt < 4 * H; ++dt) acc[dt][nt] *= scale;
+        m[nt] = top;
+        total[nt] = sum;
     }
     // four columns of output row 4g + i of the tiles, of a row tile's row r16
     bool bad = false;
-    auto store = [&](int h, int i, int nt, f32x4 x) {
-        if (!live[nt]) return;
-        const size_t row = static_cast<size_t>(tree.w) + node[nt];
-        const int2 runs = a.runs[row];
-        if (runs.y == 1) {
-            x /= total[nt];
-            if constexpr (kX3)
-                bad |= !(__builtin_isfinite(x[0]) && __builtin_isfinite(x[1]) && __builtin_isfinite(x[2]) && __builtin_isfinite(x[3]));
-            *reinterpret_cast<f32x4*>(a.out + (row * a.heads + head[nt]) * D + vcol(h, 4 * g + i)) = x;
-        } else {
-            const size_t p = (static_cast<size_t>(runs.x) + it.w) * a.heads + head[nt];
-            *reinterpret_cast<f32x4*>(a.part_acc + p * D + vcol(h, 4 * g + i)) = x;
-            if (h == 0 && i == 0 && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m[nt], total[nt]);
-        }
-    };
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-        if constexpr (WK > 1) {
-            if (h) __syncthreads();
+        if (h) __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    sums[wave][i][nt][lane] =
-                        f32x4{acc[4 * h][nt][i], acc[4 * h + 1][nt][i], acc[4 * h + 2][nt][i], acc[4 * h + 3][nt][i]};
-            __syncthreads();
+            for (int nt = 0; nt < NT; ++nt)
+                sums[wave][i][nt][lane] =
+                    f32x4{acc[4 * h][nt][i], acc[4 * h + 1][nt][i], acc[4 * h + 2][nt][i], acc[4 * h + 3][nt][i]};
+        __syncthreads();
 #pragma unroll
-            for (int ii = 0; ii < 4 / WK; ++ii) {
-                const int i = wk * (4 / WK) + ii;
+        for (int nt = 0; nt < NT; ++nt) {
+            f32x4 x = sums[0][wave][nt][lane];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    f32x4 x = sums[wave - wk][i][nt][lane];
-#pragma unroll
-                    for (int w = 1; w < WK; ++w) x += sums[wave - wk + w][i][nt][lane];
-                    store(h, i, nt, x);
-                }
+            for (int w = 1; w < WK; ++w) x += sums[w][wave][nt][lane];
+            if (!live[nt]) continue;
+            const size_t row = static_cast<size_t>(tree.w) + node[nt];
+            if (it.runs == 1) {
+                x /= total[nt];
+                bad |= kX3 && !all_finite(x);
+                *reinterpret_cast<f32x4*>(a.out + (row * a.heads + head[nt]) * D + vcol(h, 4 * g + wave)) = x;
+            } else {
+                const size_t p = (static_cast<size_t>(it.slot) + static_cast<size_t>(node[nt]) * it.runs + it.run) * a.heads + head[nt];
+                put_partial(a, a.part_acc + p * D + vcol(h, 4 * g + wave), x);
+                if (h == 0 && wave == 0 && g == 0) put_partial(a, a.part_ml + 2 * p, make_float2(m[nt], total[nt]));
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    store(h, i, nt, f32x4{acc[4 * h][nt][i], acc[4 * h + 1][nt][i], acc[4 * h + 2][nt][i], acc[4 * h + 3][nt][i]});
         }
     }
     if (bad) *a.err = 1;
+    if (it.runs > 1 && a.done) merge_rows<D>(a, it, 16 * NT, kX3);
 }
 
 // Many rows of a (tree, KV head), f32x3: four waves of up to 32 rows each share every
@@ -547,11 +616,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
     __shared__ int odds[2][S][H];    // the tree's own values: some are not finite
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, r16 = lane & 15;
-    const int4 it = a.work[2 * blockIdx.x], st = a.work[2 * blockIdx.x + 1];
-    const int4 tree = a.trees[it.x];
-    const int cached = tree.y, nodes = tree.z, kh = it.y, G = a.group, kvw = a.lay.kv_width;
+    const Item it = item_of(a);
+    if (!it.tree.z) return;  // the list's padding
+    const int4 tree = it.tree;
+    const int cached = tree.y, nodes = tree.z, kh = it.head, G = a.group, kvw = a.lay.kv_width;
     // 16 rows a tile, dealt to the waves in turn; a wave without any still stages
-    const int row0 = it.z + wave * 16, left_rows = nodes * G - row0;
+    const int row0 = it.row0 + wave * 16, left_rows = nodes * G - row0;
     const int tiles = left_rows > 16 * kWaves ? 2 : left_rows > 0 ? 1 : 0;
     auto row_of = [&](int nt) { return row0 + 16 * kWaves * nt + r16; };
     auto node_of = [&](int nt) { return row_of(nt) / G; };
@@ -624,8 +694,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
         if constexpr (kQ8)
             scales16.set(block + static_cast<size_t>(tpb) * D + static_cast<size_t>(slot) * (D / 32) * 2, max(left, 0) * (D / 32) * 2);
     };
-    int more = lookup(st.x + 32 * S + sub), at = 0;
-    spans(st.x + sub, lookup(st.x + sub));
+    int more = lookup(it.step + 32 * S + sub), at = 0;
+    spans(it.step + sub, lookup(it.step + sub));
     auto load = [&](int step) __attribute__((always_inline)) {
         // the key tiles of a thread's first and second half of the loads
         const int ia = 2 * at + (takes_keys && D == 128 ? mt0 : 0), ib = 2 * at + (takes_keys && D == 128 ? mt0 : 1);
@@ -872,14 +942,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
     };
 
     // Q8_0 blocks: the tree's own f32 rows are not in the pipeline of the cached ones
-    const int end = kQ8 ? min(st.y, csteps) : st.y;
-    if (st.x < end) {
-        load(st.x + sub);
-        put(0, st.x + sub);
-        load(st.x + S + sub);
+    const int end = kQ8 ? min(it.end, csteps) : it.end;
+    if (it.step < end) {
+        load(it.step + sub);
+        put(0, it.step + sub);
+        load(it.step + S + sub);
         __syncthreads();
         int buf = 0;
-        for (int step = st.x; step < end; step += S, buf ^= 1) {
+        for (int step = it.step; step < end; step += S, buf ^= 1) {
             put(buf ^ 1, step + S + sub);
             load(step + 2 * S + sub);
             if (tiles)
@@ -894,7 +964,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
     }
     if constexpr (kQ8) {
 #pragma unroll 1
-        for (int step = max(st.x, csteps); step < st.y; step += S) {
+        for (int step = max(it.step, csteps); step < it.end; step += S) {
             const int n0 = kStep * (step + sub - csteps);
             f32x4 x[8];
 #pragma unroll
@@ -907,7 +977,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
             __syncthreads();
             if (tiles)
 #pragma unroll 1
-                for (int t = 0; t < S && step + t < st.y; ++t) {
+                for (int t = 0; t < S && step + t < it.end; ++t) {
                     scores(0, t);
                     softmax(0, t, step + t);
                     output(0, t);
@@ -924,24 +994,27 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
     for (int nt = 0; nt < NT; ++nt) {
         const int node = node_of(nt), head = kh * G + row_of(nt) - node * G;
         if (node >= nodes) continue;
-        const size_t row = static_cast<size_t>(tree.w) + node;
-        const int2 runs = a.runs[row];
-        const bool whole = runs.y == 1;
-        const size_t to = whole ? row * a.heads + head : (static_cast<size_t>(runs.x) + it.w) * a.heads + head;
+        const bool whole = it.runs == 1;
+        const size_t to = (whole ? static_cast<size_t>(tree.w) + node
+                                 : static_cast<size_t>(it.slot) + static_cast<size_t>(node) * it.runs + it.run) * a.heads + head;
         float* o = (whole ? a.out : a.part_acc) + to * D + 16 * g;
         const float inv = whole ? total[nt] : 1.f;
-        if (!whole && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * to) = make_float2(m[nt], total[nt]);
+        if (!whole && g == 0) put_partial(a, a.part_ml + 2 * to, make_float2(m[nt], total[nt]));
         bad |= !__builtin_isfinite(total[nt]);
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const f32x4 x = f32x4{acc[4 * h][nt][i], acc[4 * h + 1][nt][i], acc[4 * h + 2][nt][i], acc[4 * h + 3][nt][i]} / inv;
-                bad |= !(__builtin_isfinite(x[0]) && __builtin_isfinite(x[1]) && __builtin_isfinite(x[2]) && __builtin_isfinite(x[3]));
-                *reinterpret_cast<f32x4*>(o + 64 * h + 4 * i) = x;
+                bad |= !all_finite(x);
+                if (whole)
+                    *reinterpret_cast<f32x4*>(o + 64 * h + 4 * i) = x;
+                else
+                    put_partial(a, o + 64 * h + 4 * i, x);
             }
     }
     if (bad) *a.err = 1;
+    if (it.runs > 1 && a.done) merge_rows<D>(a, it, 128, true);
 }
 
 template <int D, bool kQ8, bool kX3>
@@ -956,9 +1029,9 @@ void launch_shape(const TreeArgs& a, int rows, int workgroups, hipStream_t s) {
         }
     }
     if (rows == 16)
-        go(tree_tile_kernel<D, 1, 1, kQ8, kX3>);
+        go(tree_tile_kernel<D, 1, kQ8, kX3>);
     else
-        go(tree_tile_kernel<D, 2, 1, kQ8, kX3>);
+        go(tree_tile_kernel<D, 2, kQ8, kX3>);
 }
 
 }  // namespace
@@ -972,6 +1045,10 @@ int tree_tile_rows(size_t most, bool x3) {
     if (most <= 16) return 16;
     if (most <= 32 || !x3) return 32;
     return 128;
+}
+
+int tree_tile_units(const BlockLayout& lay, int rows, bool x3) {
+    return rows > 32 || lay.head_dim / 16 * rows * (x3 ? 2 : 1) <= 128 ? 2 : 1;
 }
 
 void launch_tree_tiles(const TreeArgs& a, int rows, int workgroups, bool x3, hipStream_t s) {
