@@ -126,16 +126,16 @@ void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t
     std::vector<int4> work;
     std::vector<int2> runs(rows);
     slots = 0;
-    tile_rows = tree_tiles_supported(c->layout()) ? tree_tile_rows(most * group, precision == 2) : 0;
-    if (tile_rows)
+    tiles = tree_tiles_supported(c->layout()) ? tree_tile_shape(c->layout(), most * group, precision == 2) : TreeTileShape{};
+    if (tiles.rows)
         tile_work(trees, work, runs);
     else
         row_work(trees, work, runs);
     if (slots > kIntMax / h || work.size() > kIntMax) throw std::invalid_argument("attention batch too large");
-    items = static_cast<int>(tile_rows ? work.size() / 3 : work.size());
+    items = static_cast<int>(tiles.rows ? work.size() / 3 : work.size());
 
     // acceptance's: each row's tree, and counters that start at zero
-    std::vector<int32_t> tree_of(rows), zeros(std::max(n, blocks), 0);
+    std::vector<int32_t> tree_of(rows), zeros(n, 0);
     every_tree_has_nodes = true;
     for (size_t i = 0; i < n; ++i) {
         std::fill_n(tree_of.begin() + trees[i].w, trees[i].z, static_cast<int32_t>(i));
@@ -147,12 +147,11 @@ void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t
         {mask.data(), mask.size() * sizeof(uint32_t)}, {work.data(), work.size() * sizeof(int4)},
         {runs.data(), runs.size() * sizeof(int2)},     {parents, rows * sizeof(int32_t)},
         {tree_of.data(), rows * sizeof(int32_t)},      {zeros.data(), n * sizeof(int)},
-        {zeros.data(), blocks * sizeof(int)},
         {nullptr, slots * h * g.head_dim * sizeof(float)}, {nullptr, slots * h * 2 * sizeof(float)},
         {nullptr, (rows + kAcceptParts) * sizeof(uint64_t)},
     };
     region.place(*c, s);
-    size_t* at[] = {&tables_at, &trees_at, &mask_at, &work_at, &runs_at, &parents_at, &tree_of_at, &done_at, &block_done_at, &acc_at, &ml_at, &best_at};
+    size_t* at[] = {&tables_at, &trees_at, &mask_at, &work_at, &runs_at, &parents_at, &tree_of_at, &done_at, &acc_at, &ml_at, &best_at};
     for (size_t i = 0; i < s.size(); ++i) *at[i] = s[i].at;
 }
 
@@ -184,33 +183,44 @@ void TreePlan::tile_work(const std::vector<int4>& trees, std::vector<int4>& work
     auto cached_steps = [](const int4& t) { return (t.y + kTreeStep - 1) / kTreeStep; };
     // steps over the tree's own nodes of the row block from row r0
     auto own_steps = [&](const int4& t, int r0) {
-        return (std::min(t.z * group, r0 + tile_rows) - 1) / group / kTreeStep + 1;
+        return (std::min(t.z * group, r0 + tiles.rows) - 1) / group / kTreeStep + 1;
+    };
+    auto steps_of = [&](const int4& t) {  // of its last row block, which has the most
+        return cached_steps(t) + own_steps(t, (t.z * group - 1) / tiles.rows * tiles.rows);
     };
     size_t total = 0;
     for (const int4& t : trees)
-        for (int r0 = 0; r0 < t.z * group; r0 += tile_rows)
+        for (int r0 = 0; r0 < t.z * group; r0 += tiles.rows)
             total += static_cast<size_t>(kv_heads) * (cached_steps(t) + own_steps(t, r0));
-    const size_t units = static_cast<size_t>(cache->compute_units()) * tree_tile_units(cache->layout(), tile_rows, precision == 2);
-    const size_t per = std::max<size_t>(4, (total + units - 1) / units);
+    // Steps of a run: an even share, or up to twice that if the chip then holds all
+    // workgroups at once: a second round for a few of them costs more.
+    const size_t units = static_cast<size_t>(cache->compute_units()) * tiles.units;
+    const size_t even = std::max<size_t>(tiles.least, (total + units - 1) / units);
+    size_t per = even;
+    for (size_t p = even; p <= 2 * even; p += (even + 15) / 16) {
+        size_t workgroups = 0;
+        for (const int4& t : trees)
+            if (t.z) workgroups += ((steps_of(t) + p - 1) / p) * ((t.z * group - 1) / tiles.rows + 1) * kv_heads;
+        if (workgroups <= units) {
+            per = p;
+            break;
+        }
+    }
     struct Group {  // the row blocks of a run
-        int tree, head, run, runs, slot, block, step, end;
+        int tree, head, run, runs, slot, step, end;
     };
     std::vector<Group> groups;
-    blocks = 0;
     for (size_t i = 0; i < trees.size(); ++i) {
         const int4& t = trees[i];
         if (!t.z) continue;
-        const int row_blocks = (t.z * group - 1) / tile_rows + 1;
-        const int steps = cached_steps(t) + own_steps(t, (row_blocks - 1) * tile_rows);
+        const int steps = steps_of(t);
         const int parts = static_cast<int>((steps + per - 1) / per), len = (steps + parts - 1) / parts;
         for (int p = 0; p < parts; ++p)
             for (int h = 0; h < kv_heads; ++h)
-                groups.push_back({static_cast<int>(i), h, p, parts, static_cast<int>(slots),
-                                  static_cast<int>(blocks) + h * row_blocks, p * len, std::min((p + 1) * len, steps)});
-        blocks += static_cast<size_t>(kv_heads) * row_blocks;
+                groups.push_back({static_cast<int>(i), h, p, parts, static_cast<int>(slots), p * len, std::min((p + 1) * len, steps)});
         for (int j = 0; j < t.z; ++j) runs[t.w + j] = make_int2(static_cast<int>(slots + static_cast<size_t>(j) * parts), parts);
         if (parts > 1) slots += static_cast<size_t>(t.z) * parts;
-        if (slots > kIntMax / heads || blocks > kIntMax) throw std::invalid_argument("attention batch too large");
+        if (slots > kIntMax / heads) throw std::invalid_argument("attention batch too large");
     }
     std::stable_sort(groups.begin(), groups.end(), [](const Group& x, const Group& y) { return x.end - x.step > y.end - y.step; });
     std::vector<std::vector<int4>> lists(xcds);
@@ -218,10 +228,10 @@ void TreePlan::tile_work(const std::vector<int4>& trees, std::vector<int4>& work
     for (const Group& x : groups) {
         const int4& t = trees[x.tree];
         const size_t to = std::min_element(load.begin(), load.end()) - load.begin();
-        for (int r0 = 0, b = 0; r0 < t.z * group; r0 += tile_rows, ++b) {
+        for (int r0 = 0; r0 < t.z * group; r0 += tiles.rows) {
             const int all = cached_steps(t) + own_steps(t, r0);
             const int step = std::min(x.step, all), end = std::min(x.end, all);
-            lists[to].insert(lists[to].end(), {t, make_int4(x.head, r0, step, end), make_int4(x.run, x.runs, x.slot, x.block + b)});
+            lists[to].insert(lists[to].end(), {t, make_int4(x.head, r0, step, end), make_int4(x.run, x.runs, x.slot, 0)});
             load[to] += end - step + 1;
         }
     }
@@ -266,16 +276,13 @@ void TreePlan::launch(int layer, const float* q, const float* keys, const float*
     a.part_acc = reinterpret_cast<float*>(d + acc_at);
     a.part_ml = reinterpret_cast<float*>(d + ml_at);
     a.qscale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(g.head_dim)));
-    // few workgroups merge their runs themselves, which saves the second launch
-    const bool alone = tile_rows && items <= kTreeMergeMax;
-    a.done = alone ? reinterpret_cast<int*>(d + block_done_at) : nullptr;
-    a.check = tile_rows && precision == 2;
+    a.check = tiles.rows && precision == 2;
     a.err = region.flags();
-    if (tile_rows)
-        launch_tree_tiles(a, tile_rows, items, precision == 2, s);
+    if (tiles.rows)
+        launch_tree_tiles(a, tiles.rows, items, precision == 2, s);
     else
         launch_tree_rows(a, items, s);
-    if (slots && !alone) launch_tree_merge(a, s);
+    if (slots) launch_tree_merge(a, s);
     cache->leave(s);
     region.launched(s);
 }

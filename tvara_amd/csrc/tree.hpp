@@ -36,7 +36,6 @@ struct TreeArgs {
     float* out;            // [node rows][heads][head_dim]
     float* part_acc;       // [partials][heads][head_dim]
     float* part_ml;        // [partials][heads][2]: maximum (log2 units), normaliser
-    int* done;             // per row block: runs done in this launch, zero between launches (null: launch_tree_merge)
     bool check;            // a merged result that is not finite sets *err
     float qscale;          // log2(e) / sqrt(head_dim)
     int* err;
@@ -96,14 +95,17 @@ struct WriteArgs {
 // tree.hip
 void launch_tree_rows(const TreeArgs& a, int items, hipStream_t s);
 void launch_tree_merge(const TreeArgs& a, hipStream_t s);
-// tree_tiles.hip: head_dim 64 and 128; a workgroup takes up to tree_tile_rows(rows
-// of the largest tree and KV head) rows, and work has three entries a workgroup: the tree (as trees); KV head, first
-// row, first step, end; run, runs, the tree's first partial, its row block
+// tree_tiles.hip: head_dim 64 and 128.  Work has three entries a workgroup: the tree
+// (as trees); KV head, first row, first step, end; run, runs, the tree's first partial.
 bool tree_tiles_supported(const BlockLayout& lay);
-int tree_tile_rows(size_t most, bool x3);
-int tree_tile_units(const BlockLayout& lay, int rows, bool x3);  // workgroups that share a CU
 constexpr int kTreeStep = 32;  // keys of a step
-constexpr int kTreeMergeMax = 128;  // workgroups of the largest launch that merges its runs itself
+struct TreeTileShape {
+    int rows;   // of a workgroup
+    int units;  // workgroups that share a CU
+    int least;  // steps of a run
+};
+// for trees of up to `most` rows a KV head
+TreeTileShape tree_tile_shape(const BlockLayout& lay, size_t most, bool x3);
 void launch_tree_tiles(const TreeArgs& a, int rows, int workgroups, bool x3, hipStream_t s);
 // tree_accept.hip: chooses part, splits and whether done stays; rows * splits is at
 // most rows + kAcceptParts
@@ -153,11 +155,11 @@ struct TreePlan {
     DeviceCache* cache = nullptr;
     uint64_t epoch = 0;
     int heads = 0, group = 0, precision = 0, words = 1, items = 0, split_tokens = 0;
-    int tile_rows = 0;  // rows of a workgroup of the tiles (0: the row kernel)
-    size_t count = 0, rows = 0, slots = 0, blocks = 0;
+    TreeTileShape tiles{};  // rows 0: the row kernel
+    size_t count = 0, rows = 0, slots = 0;
     PlanRegion region;
     size_t tables_at = 0, trees_at = 0, mask_at = 0, work_at = 0, runs_at = 0, parents_at = 0, acc_at = 0, ml_at = 0,
-           best_at = 0, done_at = 0, block_done_at = 0, tree_of_at = 0;
+           best_at = 0, done_at = 0, tree_of_at = 0;
     bool every_tree_has_nodes = true;
 
     void build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t heads, size_t context,

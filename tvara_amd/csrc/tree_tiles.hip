@@ -10,9 +10,9 @@
 //  O^T = V^T P^T: lane (g, r) loads four columns of the keys 4g + i of each 16,
 //    so it holds V^T's operand for four output tiles (tile j: column j of every
 //    lane's four) and its own scores are P^T's.
-// Steps are dealt in turn to the workgroup's four waves, whose results meet in LDS.  A long context is cut into runs, a
-// workgroup each, that leave partials for a merge.  After the cached steps come
-// those over the tree's own nodes, with a mask word a row.
+// Steps are dealt in turn to the workgroup's waves, whose results meet in LDS.  A
+// long context is cut into runs, a workgroup each, that leave partials for a merge.
+// After the cached steps come those over the tree's own nodes, with a mask word a row.
 //
 // f32: v_mfma_f32_16x16x4_f32.  f32x3 (kX3): 16x16x32 on operands in two fp16
 // parts, hi * hi + hi * lo + lo * hi.  Softmax in log2 units with a
@@ -84,93 +84,21 @@ __device__ __forceinline__ bool all_finite(f32x4 x) {
 
 // A workgroup's work: a tree (TreeArgs::trees), the KV head and first row of a row
 // block, and a run of its steps; the partials of the tree's node j are slot + j *
-// runs on, and `block` counts the row block's finished runs.
+// runs on.
 struct Item {
     int4 tree;
-    int head, row0, step, end, run, runs, slot, block;
+    int head, row0, step, end, run, runs, slot;
 };
 __device__ __forceinline__ Item item_of(const TreeArgs& a) {
     const int4 t = a.work[3 * blockIdx.x], x = a.work[3 * blockIdx.x + 1], y = a.work[3 * blockIdx.x + 2];
-    return {t, x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-}
-
-// partials of a launch that merges them itself go past the XCD's L2
-__device__ __forceinline__ void put_partial(const TreeArgs& a, float* to, f32x4 x) {
-    if (!a.done) {
-        *reinterpret_cast<f32x4*>(to) = x;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) __hip_atomic_store(to + i, x[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void put_partial(const TreeArgs& a, float* to, float2 x) {
-    if (!a.done) {
-        *reinterpret_cast<float2*>(to) = x;
-        return;
-    }
-    __hip_atomic_store(to, x.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(to + 1, x.y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-// The last workgroup of a row block's runs combines them in order, as
-// tree_merge_kernel does.  Every wave waits for its partials' stores before the
-// count; release and acquire at device scope order them against the last one's
-// reads.  Releases write an XCD's L2 back, one after the other, so only launches of
-// few workgroups come here (TreePlan::launch).
-template <int D>
-__device__ void merge_rows(const TreeArgs& a, const Item& it, int rows, bool check) {
-    __shared__ int last;
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_s_waitcnt(0);
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int* done = a.done + it.block;
-        const int before = __hip_atomic_fetch_add(done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-        last = before == it.runs - 1;
-        if (last) __hip_atomic_store(done, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (!last) return;
-    auto ld = [](const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-    const int live = min(rows, it.tree.z * a.group - it.row0);
-    for (int e = threadIdx.x; e < live * (D / 4); e += 64 * kWaves) {
-        const int r = it.row0 + e / (D / 4), c = 4 * (e % (D / 4)), node = r / a.group, head = it.head * a.group + r - node * a.group;
-        const size_t first = (static_cast<size_t>(it.slot) + static_cast<size_t>(node) * it.runs) * a.heads + head;
-        float m = -INFINITY, l = 0.f;
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        constexpr int U = 4;  // runs requested together
-        for (int r0 = 0; r0 < it.runs; r0 += U) {
-            float rm[U], rl[U];
-            f32x4 x[U];
-#pragma unroll
-            for (int k = 0; k < U; ++k) {
-                const size_t p = first + static_cast<size_t>(min(r0 + k, it.runs - 1)) * a.heads;
-                const float* pa = a.part_acc + p * D + c;
-                rm[k] = ld(a.part_ml + 2 * p);
-                rl[k] = ld(a.part_ml + 2 * p + 1);
-                x[k] = f32x4{ld(pa), ld(pa + 1), ld(pa + 2), ld(pa + 3)};
-            }
-#pragma unroll
-            for (int k = 0; k < U; ++k) {
-                if (r0 + k >= it.runs || rm[k] == -INFINITY) continue;
-                const float mn = fmaxf(m, rm[k]), wm = fast_exp2(m - mn), wr = fast_exp2(rm[k] - mn);
-                l = l * wm + rl[k] * wr;
-                sum = sum * wm + x[k] * wr;
-                m = mn;
-            }
-        }
-        sum /= l;
-        if (check && !all_finite(sum)) *a.err = 1;
-        *reinterpret_cast<f32x4*>(a.out + ((static_cast<size_t>(it.tree.w) + node) * a.heads + head) * D + c) = sum;
-    }
+    return {t, x.x, x.y, x.z, x.w, y.x, y.y, y.z};
 }
 
 template <int D, int NT, bool kQ8, bool kX3>
-__global__ __launch_bounds__(64 * kWaves, NT * D * (kX3 ? 2 : 1) <= 128 ? 2 : 1) void tree_tile_kernel(const TreeArgs a) {
+__global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel(const TreeArgs a) {
     constexpr int WK = kWaves, C = D / 16, KC = D / 32, H = D / 64;
-    __shared__ f32x4 sums[kWaves][4][NT][64];
-    __shared__ float2 stats[kWaves][16 * NT];
+    __shared__ f32x4 sums[WK][4][NT][64];
+    __shared__ float2 stats[WK][16 * NT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, r16 = lane & 15, wk = wave;
     const Item it = item_of(a);
@@ -578,24 +506,24 @@ __global__ __launch_bounds__(64 * kWaves, NT * D * (kX3 ? 2 : 1) <= 128 ? 2 : 1)
         __syncthreads();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            f32x4 x = sums[0][wave][nt][lane];
+            const int i = wave;
+            f32x4 x = sums[0][i][nt][lane];
 #pragma unroll
-            for (int w = 1; w < WK; ++w) x += sums[w][wave][nt][lane];
+            for (int w = 1; w < WK; ++w) x += sums[w][i][nt][lane];
             if (!live[nt]) continue;
             const size_t row = static_cast<size_t>(tree.w) + node[nt];
             if (it.runs == 1) {
                 x /= total[nt];
                 bad |= kX3 && !all_finite(x);
-                *reinterpret_cast<f32x4*>(a.out + (row * a.heads + head[nt]) * D + vcol(h, 4 * g + wave)) = x;
+                *reinterpret_cast<f32x4*>(a.out + (row * a.heads + head[nt]) * D + vcol(h, 4 * g + i)) = x;
             } else {
                 const size_t p = (static_cast<size_t>(it.slot) + static_cast<size_t>(node[nt]) * it.runs + it.run) * a.heads + head[nt];
-                put_partial(a, a.part_acc + p * D + vcol(h, 4 * g + wave), x);
-                if (h == 0 && wave == 0 && g == 0) put_partial(a, a.part_ml + 2 * p, make_float2(m[nt], total[nt]));
+                *reinterpret_cast<f32x4*>(a.part_acc + p * D + vcol(h, 4 * g + i)) = x;
+                if (h == 0 && i == 0 && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m[nt], total[nt]);
             }
         }
     }
     if (bad) *a.err = 1;
-    if (it.runs > 1 && a.done) merge_rows<D>(a, it, 16 * NT, kX3);
 }
 
 // Many rows of a (tree, KV head), f32x3: four waves of up to 32 rows each share every
@@ -999,7 +927,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
                                  : static_cast<size_t>(it.slot) + static_cast<size_t>(node) * it.runs + it.run) * a.heads + head;
         float* o = (whole ? a.out : a.part_acc) + to * D + 16 * g;
         const float inv = whole ? total[nt] : 1.f;
-        if (!whole && g == 0) put_partial(a, a.part_ml + 2 * to, make_float2(m[nt], total[nt]));
+        if (!whole && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * to) = make_float2(m[nt], total[nt]);
         bad |= !__builtin_isfinite(total[nt]);
 #pragma unroll
         for (int h = 0; h < H; ++h)
@@ -1007,31 +935,23 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
             for (int i = 0; i < 4; ++i) {
                 const f32x4 x = f32x4{acc[4 * h][nt][i], acc[4 * h + 1][nt][i], acc[4 * h + 2][nt][i], acc[4 * h + 3][nt][i]} / inv;
                 bad |= !all_finite(x);
-                if (whole)
-                    *reinterpret_cast<f32x4*>(o + 64 * h + 4 * i) = x;
-                else
-                    put_partial(a, o + 64 * h + 4 * i, x);
+                *reinterpret_cast<f32x4*>(o + 64 * h + 4 * i) = x;
             }
     }
     if (bad) *a.err = 1;
-    if (it.runs > 1 && a.done) merge_rows<D>(a, it, 128, true);
 }
 
 template <int D, bool kQ8, bool kX3>
 void launch_shape(const TreeArgs& a, int rows, int workgroups, hipStream_t s) {
-    auto go = [&](auto kernel) {
-        launch("tree_attention_tiles", kernel, dim3(workgroups), dim3(64 * kWaves), 0, s, a);
-    };
-    if constexpr (kX3) {
-        if (rows > 32) {
-            go(tree_shared_kernel<D, kQ8>);
-            return;
-        }
-    }
+    auto go = [&](auto kernel) { launch("tree_attention_tiles", kernel, dim3(workgroups), dim3(64 * kWaves), 0, s, a); };
     if (rows == 16)
         go(tree_tile_kernel<D, 1, kQ8, kX3>);
-    else
+    else if constexpr (kX3)
+        rows == 32 ? go(tree_tile_kernel<D, 2, kQ8, kX3>) : go(tree_shared_kernel<D, kQ8>);
+    else if constexpr (D == 128)
         go(tree_tile_kernel<D, 2, kQ8, kX3>);
+    else
+        throw std::logic_error("no f32 tree kernel for these rows");
 }
 
 }  // namespace
@@ -1041,14 +961,26 @@ bool tree_tiles_supported(const BlockLayout& lay) {
            lay.stride <= static_cast<size_t>(1) << 31;
 }
 
-int tree_tile_rows(size_t most, bool x3) {
-    if (most <= 16) return 16;
-    if (most <= 32 || !x3) return 32;
-    return 128;
-}
-
-int tree_tile_units(const BlockLayout& lay, int rows, bool x3) {
-    return rows > 32 || lay.head_dim / 16 * rows * (x3 ? 2 : 1) <= 128 ? 2 : 1;
+// 16 contexts of 2048 tokens, 32 query and 8 KV heads, microseconds with each block:
+//   f32x3, head_dim 128:  16 rows  16: 52.6  32: 55.0;  40 rows  32: 62.9  128: 63.9
+//                         64 rows  32: 65.6  128: 73.7;  96 rows  32: 115.8  128: 80.8
+//   f32x3, head_dim 64:   64 rows  32: 44.8  128: 48.5;  96 rows  32: 60.0  128: 51.2
+//   f32, head_dim 64:     16 rows  16: 36.3  32: 41.3;   64 rows  16: 64.4  32: 64.5
+//     (24 to 96 rows, ragged: 16: 56.1  32: 57.2;  one context of 512: 16: 11.2  32: 12.8)
+//   f32, head_dim 128:    32 rows  16: 63.7  32: 63.4;   64 rows  16: 115.2  32: 99.0
+// Two workgroups share a CU where 256 registers hold a wave, or LDS a workgroup's keys.
+// A run has at least a step a wave, and no more where there are CUs: a wave's second
+// step waits for memory again (one context of 512 tokens in runs of 4 steps: 12.7,
+// of 8: 14.0, of 12: 15.3, each with its merge).
+TreeTileShape tree_tile_shape(const BlockLayout& lay, size_t most, bool x3) {
+    TreeTileShape t{};
+    if (x3)
+        t.rows = most <= 16 ? 16 : most <= 64 ? 32 : 128;
+    else
+        t.rows = most <= 16 || lay.head_dim == 64 ? 16 : 32;
+    t.units = t.rows == 128 || lay.head_dim == 64 ? 2 : 1;
+    t.least = kWaves;
+    return t;
 }
 
 void launch_tree_tiles(const TreeArgs& a, int rows, int workgroups, bool x3, hipStream_t s) {
