@@ -128,6 +128,26 @@ TVARA_API int tvara_sequence_truncate(tvara_model* model, uint64_t sequence, siz
 TVARA_API int tvara_sequences_decode(tvara_model* model, const uint64_t* sequences, const uint32_t* tokens,
                                      size_t count, float* logits, size_t logits_count);
 
+/* One step of speculative decoding for `count` distinct sequences: every node of
+ * every tree of drafted tokens passes through the model at once, and the nodes that
+ * greedy decoding would have taken are appended.  Tree i has nodes[i] (up to 1,024)
+ * of the packed tokens; parents[] numbers them within their tree, a parent before
+ * its children, -1 for a child of the sequence's end.  first[i] is the token that
+ * the sequence's own last logits chose (of the prompt, or next[i] of the call
+ * before).  From there: the lowest child with the expected token is accepted, and its
+ * logits' maximum (the lowest index on ties) is the token expected next.
+ *   accepted[i]  how many nodes were taken; their K/V are appended
+ *   path         as long as tokens, tree i's part at its first node: the accepted
+ *                nodes, numbered within the tree, -1 behind
+ *   next[i]      the token expected after them
+ * The logits are those of tvara_sequences_decode token by token (f32 attention);
+ * they stay on the GPU.  The pool needs blocks for the accepted nodes only.  All or
+ * nothing: on failure no sequence changes.  Returns 0 / -1.  No counterpart in the
+ * reference ABI. */
+TVARA_API int tvara_sequences_verify_trees(tvara_model* model, const uint64_t* sequences, size_t count,
+                                           const size_t* nodes, const int32_t* parents, const uint32_t* tokens,
+                                           const uint32_t* first, int32_t* path, size_t* accepted, uint32_t* next);
+
 /* The model's KV cache as a tvara_kv_cache handle owned by the model (the
  * in-process PagedModelExecutor::cache(), paged_model.hpp:10), so every
  * tvara_kv_* call -- fork (kv.hpp:123-129), snapshots, retain / release,
@@ -403,17 +423,21 @@ TVARA_API void tvara_prefill_plan_destroy(tvara_prefill_plan* plan);
  * parents [sum nodes] with -1 <= parents[j] < j within its tree.  precision
  * TVARA_ATTN_F32, or TVARA_ATTN_F32X3 as tvara_attn_prefill has it where the
  * layout has such tiles (head_dim 64 or 128, blocks of a power of two from 16
- * tokens) and f32 elsewhere; bf16 is refused.  Launching fails with TVARA_INVALID
- * once the cache has changed. */
+ * tokens) and f32 elsewhere; bf16 is refused.  f32x3 holds queries, keys and values
+ * alike as two fp16 parts: 22 bits, 2^-25 at the least, and what leaves fp16's range
+ * (65,504; queries times 1.44 / sqrt(head_dim)) is reported by tvara_tree_plan_check.
+ * Launching fails with TVARA_INVALID once the cache has changed.  All trees together
+ * have at most 16,700,000 nodes, and nodes * heads * head_dim stays below 2^32. */
 TVARA_API tvara_tree_plan* tvara_tree_plan_create(tvara_kv_cache* cache, const uint64_t* sequences, size_t count,
                                                   size_t heads, size_t context, const size_t* visible,
                                                   const size_t* nodes, const int32_t* parents, int precision);
 /* Attention of every node over its sequence's cached tokens, the nodes above it
  * and itself: q and out f32 [sum nodes][heads * head_dim], keys and values rows
- * of kv_width floats row_stride floats apart (0: kv_width; a multiple of 4),
- * device pointers, asynchronous on `stream` (NULL: the cache's).  What a node
- * does not see never reaches its row, whatever it holds.  Launches of one plan run
- * in stream order: they share its partial results. */
+ * of kv_width floats row_stride floats apart (0: kv_width; a multiple of 4, up to
+ * 2^23), device pointers, asynchronous on `stream` (NULL: the cache's).  What a node
+ * does not see never reaches its row, whatever it holds.  Launches and acceptances of
+ * one plan share its workspace: they run one after the other, on one stream or in
+ * the caller's order, captured ones too; two plans share nothing. */
 TVARA_API int tvara_tree_plan_launch(tvara_tree_plan* plan, size_t layer, const float* q, const float* keys,
                                      const float* values, size_t row_stride, float* out, void* stream);
 /* Greedy acceptance: e = first[i]; while a child of the current node (a root at
@@ -423,7 +447,8 @@ TVARA_API int tvara_tree_plan_launch(tvara_tree_plan* plan, size_t layer, const 
  * vocab); path [count][path_stride] receives the accepted nodes as packed rows and
  * -1 behind them, accepted [count] how many.  A NaN logit is never the largest.
  * It, or a path longer than path_stride (which ends there), is reported by
- * tvara_tree_plan_check.  Device pointers, asynchronous; needs no cache data, so the plan may be stale. */
+ * tvara_tree_plan_check.  Device pointers, asynchronous; needs no cache data, so the
+ * plan may be stale. */
 TVARA_API int tvara_tree_plan_accept(tvara_tree_plan* plan, const uint32_t* tokens, const uint32_t* first,
                                      const float* logits, size_t vocab, size_t logits_stride, int32_t* path,
                                      size_t path_stride, int32_t* accepted, uint32_t* next, void* stream);
@@ -459,9 +484,10 @@ TVARA_API int tvara_slot_plan_build(tvara_slot_plan* plan, const int32_t* starts
 /* K/V rows of every layer into slots, f32 as they are or encoded as appends
  * encode them: entry t (of n) takes row rows[t] (NULL: row t) of row_count rows to
  * slots[t]; an entry with slot -1 is skipped.  Element (row, layer, column) lies at
- * row * row_stride + layer * layer_stride + column floats.  A slot outside the pool
- * or a row outside the rows is skipped and reported by tvara_slot_plan_check.  Two entries of one slot
- * leave either's bytes.  Device pointers, asynchronous. */
+ * row * row_stride + layer * layer_stride + column floats (strides in multiples of 4
+ * for Q8_0 blocks).  A slot outside the pool or a row outside the rows is skipped and
+ * reported by tvara_slot_plan_check.  Two entries of one slot leave a mixture of their
+ * bytes.  At most 16,700,000 entries.  Device pointers, asynchronous. */
 TVARA_API int tvara_slot_plan_write(tvara_slot_plan* plan, const int64_t* slots, const int32_t* rows, size_t n,
                                     const float* keys, const float* values, size_t row_count, size_t row_stride,
                                     size_t layer_stride, void* stream);

@@ -9,10 +9,11 @@ than 258 * 2^-24 * 13 = 2e-4 relative in that worst case and sqrt(258) 2^-24 13 
 1.3e-5 as independent roundings go; an output is a mean of such terms around its
 own value, |v - o| <= 10, n_eff of them: 1e-4 * (1 + |ref|) holds the typical
 error eightfold.  In the 2-norm, over many outputs, the roundings are
-independent: 2e-6 relative.  f32x3: scores carry 2^-22 per product (fp16 parts)
-and the values and probabilities 2^-17 each (bf16 parts, the second rounded to
-nearest), 2^-17 * sqrt(2) / sqrt(3) = 6.2e-6 of a term's size as independent
-roundings; terms may cancel down to 1/2 of the output: the same 1e-4 and 1.3e-5.
+independent: 2e-6 relative.  f32x3: scores carry 2^-22 per product (fp16 parts);
+for values and probabilities in two parts of 8 bits each, the second rounded to
+nearest, 2^-17 * sqrt(2) / sqrt(3) = 6.2e-6 of a term's size as independent
+roundings; terms may cancel down to 1/2 of the output: the same 1e-4 and 1.3e-5
+(in fp16 parts, as they are, they are off by less).
 Whole numbers and stored bytes are equal.
 """
 
@@ -272,12 +273,58 @@ def test_plan_strides_and_layers(device, oracle, dim, tpb, precision):
         for bad in (lambda: plan.launch(3, d.q.ptr, d.k.ptr, d.v.ptr, d.out.ptr),
                     lambda: plan.launch(0, d.q.ptr, d.k.ptr, d.v.ptr, d.out.ptr, row_stride=b.w - 4),
                     lambda: plan.launch(0, d.q.ptr, d.k.ptr, d.v.ptr, d.out.ptr, row_stride=b.w + 1),
+                    lambda: plan.launch(0, d.q.ptr, d.k.ptr, d.v.ptr, d.out.ptr, row_stride=(1 << 23) + 4),
+                    lambda: plan.launch(0, d.q.ptr, d.k.ptr, d.v.ptr, d.out.ptr, row_stride=1 << 62),
                     lambda: plan.launch(0, d.q.ptr + 4, d.k.ptr, d.v.ptr, d.out.ptr)):
             with pytest.raises(_capi.InvalidArgument):
                 bad()
         b.cache.truncate(b.seqs[0], 70)
         with pytest.raises(_capi.InvalidArgument, match="stale"):
             plan.launch(0, d.q.ptr, d.k.ptr, d.v.ptr, d.out.ptr)
+
+
+@pytest.mark.parametrize("nodes", [3, 12, 40])  # 16, 32 and 128 rows a workgroup
+@pytest.mark.parametrize("where", ["q", "cached keys", "cached values", "keys", "values"])
+@pytest.mark.parametrize("q8", [False, True])
+def test_beyond_fp16_is_reported(device, oracle, where, nodes, q8):
+    """f32x3 reports inputs that its fp16 parts do not hold; f32 takes them."""
+    say("tree beyond fp16", where, nodes, q8)
+    b = Batch(device, oracle, 8, 2, 64, [70], [chain(nodes)], seed=3, spare=1)
+    if where.startswith("cached"):
+        if q8:  # (a Q8_0 element is at most 127 * 65,504: the scales are fp16)
+            b = Batch(device, oracle, 8, 2, 64, [70], [chain(nodes)], seed=3, spare=1, q8=True)
+        row = [np.array(x[0][69:70], np.float64) for x in (b.k, b.v)]
+        row["keys" not in where][:, 5] = 3e5
+        b.cache.truncate(b.seqs[0], 69)
+        b.cache.append(b.seqs[0], *(np.ascontiguousarray(x) for x in row))
+    else:
+        x = b.q if where == "q" else b.tk if where == "keys" else b.tv
+        x[0, 5] = 3e6
+    message = None
+    try:
+        b.run("f32x3")
+    except _capi.InvalidArgument as e:
+        message = str(e)
+    assert message == "invalid online attention input"
+    assert np.isfinite(b.run("f32")).all()
+
+
+@pytest.mark.parametrize("precision", PRECISIONS)
+def test_launches_repeat_to_the_bit(device, oracle, precision):
+    """Runs of a long context and their merge, one launch after the other in one plan."""
+    say("tree launches repeat", precision)
+    b = Batch(device, oracle, 8, 2, 64, [3000, 100], [bushy(9, 3), chain(30)], seed=6)
+    with hip_rows(b) as d:
+        plan = attention.TreePlan(b.cache, b.seqs, b.nodes, b.parents, b.heads, 1 << 20, precision=precision)
+        first = None
+        for _ in range(6):
+            d.out.zero()
+            plan.launch(0, d.q.ptr, d.k.ptr, d.v.ptr, d.out.ptr)
+            plan.check()
+            got = d.out.numpy()
+            first = got if first is None else first
+            assert np.array_equal(got, first)
+        agree(first[: b.rows], b.want(), precision)
 
 
 def test_one_sequence_in_several_trees(device, oracle):
@@ -622,7 +669,7 @@ def test_slot_write_reports(device):
         plan.check()
     assert np.array_equal(cache.read_all(s, 0).reshape(12, 4)[5:9], np.arange(16).reshape(4, 4))
     plan.write(None, None, 0, None, None, 0, 4, 4)
-    for a in ((ds.ptr, None, 5, k.ptr, v.ptr, 4, 3, 4), (None, None, 5, k.ptr, v.ptr, 4, 4, 4),
+    for a in ((ds.ptr, None, 5, k.ptr, v.ptr, 4, 3, 4), (ds.ptr, None, 1 << 24, k.ptr, v.ptr, 4, 4, 4), (None, None, 5, k.ptr, v.ptr, 4, 4, 4),
               (ds.ptr, None, 5, k.ptr + 4, v.ptr, 4, 4, 4), (ds.ptr, None, 1 << 40, k.ptr, v.ptr, 4, 4, 4)):
         with pytest.raises(_capi.InvalidArgument):
             plan.write(*a)

@@ -27,6 +27,12 @@ def test_closed_handles_are_refused():
     assert n[0] == 0
 
 
+def test_closed_model_is_refused():
+    lib = _capi.lib()
+    assert lib.tvara_sequences_verify_trees(None, None, 0, None, None, None, None, None, None, None) == -1
+    assert lib.tvara_last_error() == b"invalid batch buffers"
+
+
 def test_trees_of_unequal_lists_are_refused():
     for nodes, parents in (([1], [-1, 0]), ([1, 2], [-1, -1]), ([], [])):
         with pytest.raises(_capi.InvalidArgument):

@@ -41,6 +41,9 @@ SIGNATURES = {
     "tvara_sequence_prefill": (C.c_int, [_vp, _u64, C.POINTER(C.c_uint32), _sz, _fp, _sz]),
     "tvara_sequence_truncate": (C.c_int, [_vp, _u64, _sz]),
     "tvara_sequences_decode": (C.c_int, [_vp, C.POINTER(_u64), C.POINTER(C.c_uint32), _sz, _fp, _sz]),
+    "tvara_sequences_verify_trees": (C.c_int, [_vp, C.POINTER(_u64), _sz, C.POINTER(_sz), C.POINTER(C.c_int32),
+                                               C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_int32),
+                                               C.POINTER(_sz), C.POINTER(C.c_uint32)]),
     "tvara_model_cache": (_vp, [_vp]),
     "tvara_radix_create": (_vp, [_vp, C.c_char_p]),
     "tvara_radix_destroy": (None, [_vp]),

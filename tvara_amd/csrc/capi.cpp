@@ -721,6 +721,28 @@ int tvara_sequences_decode(tvara_model* model, const uint64_t* sequences, const 
     }
 }
 
+int tvara_sequences_verify_trees(tvara_model* model, const uint64_t* sequences, size_t count, const size_t* nodes,
+                                 const int32_t* parents, const uint32_t* tokens, const uint32_t* first, int32_t* path,
+                                 size_t* accepted, uint32_t* next) {
+    tvara_amd::abi::clear();
+    try {
+        if (!model || (count && (!sequences || !nodes || !first || !accepted || !next)))
+            throw std::invalid_argument("invalid batch buffers");
+        bool any = false;
+        for (size_t i = 0; i < count; ++i) any |= nodes[i] != 0;
+        if (any && (!parents || !tokens || !path)) throw std::invalid_argument("invalid batch buffers");
+        std::lock_guard<std::mutex> lock(model->mutex);
+        model->model->verify_trees(sequences, count, nodes, parents, tokens, first, path, accepted, next);
+        return 0;
+    } catch (const std::exception& e) {
+        failed(TVARA_ERROR, e.what());
+        return -1;
+    } catch (...) {
+        failed(TVARA_ERROR, "unknown batch error");
+        return -1;
+    }
+}
+
 tvara_kv_cache* tvara_model_cache(tvara_model* model) {
     if (!model) {
         failed(TVARA_INVALID, "closed model");

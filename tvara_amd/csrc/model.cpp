@@ -9,6 +9,7 @@
 #include <stdexcept>
 
 #include "gguf.hpp"
+#include "tree.hpp"
 
 namespace tvara_amd {
 
@@ -361,6 +362,109 @@ void DeviceModel::decode_many(const uint64_t* sequences, const uint32_t* tokens,
         throw;
     }
     copy_logits(bands, n, logits_host);
+}
+
+void DeviceModel::verify_trees(const uint64_t* sequences, size_t n, const size_t* nodes, const int32_t* parents,
+                               const uint32_t* tokens, const uint32_t* first, int32_t* path, size_t* accepted,
+                               uint32_t* next) {
+    if (!n) return;
+    const ModelConfig& c = cfg_;
+    {
+        std::vector<uint64_t> sorted(sequences, sequences + n);
+        std::sort(sorted.begin(), sorted.end());
+        if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
+            throw std::invalid_argument("duplicate sequence in decode batch");
+    }
+    std::vector<size_t> lengths(n), positions, depth;
+    size_t deepest = 0;
+    for (size_t i = 0; i < n; ++i) {
+        if (nodes[i] > kMaxTreeNodes) throw std::invalid_argument("a token tree has at most 1,024 nodes");
+        lengths[i] = cache_->sequence(sequences[i]).length;
+        if (first[i] >= c.vocab) throw std::invalid_argument("paged decode exceeds token/context limits");
+        tree_depths(parents + positions.size(), nodes[i], c.context - std::min(c.context, lengths[i]), depth);
+        for (size_t j = 0; j < nodes[i]; ++j) {
+            if (tokens[positions.size()] >= c.vocab) throw std::invalid_argument("paged decode exceeds token/context limits");
+            positions.push_back(lengths[i] + depth[j] - 1);
+            deepest = std::max(deepest, depth[j]);
+        }
+    }
+    const size_t rows = positions.size();
+    if (rows > static_cast<size_t>(std::numeric_limits<int>::max() / std::max<size_t>(c.vocab, c.hidden)) ||
+        n > static_cast<size_t>(std::numeric_limits<int>::max()) / std::max<size_t>(deepest, 1))
+        throw std::invalid_argument("decode batch too large");
+    if (!rows || !batched_widths()) {
+        // along the accepted nodes alone, token by token
+        std::vector<float> logits(c.vocab);
+        std::vector<int32_t> found(rows, -1);
+        std::vector<size_t> counts(n, 0);
+        std::vector<uint32_t> want(first, first + n);
+        size_t i = 0, row0 = 0;
+        try {
+            for (; i < n; row0 += nodes[i++]) {
+                int32_t at = -1;
+                for (int32_t j = 0; j < static_cast<int32_t>(nodes[i]); ++j) {
+                    if (parents[row0 + j] != at || tokens[row0 + j] != want[i]) continue;
+                    decode(sequences[i], want[i], logits.data());
+                    for (const float x : logits)
+                        if (std::isnan(x)) throw std::invalid_argument("invalid logits or path of a token tree");
+                    want[i] = static_cast<uint32_t>(std::max_element(logits.begin(), logits.end()) - logits.begin());
+                    found[row0 + counts[i]++] = at = j;
+                }
+            }
+        } catch (...) {
+            for (size_t k = 0; k <= i; ++k) cache_->truncate(sequences[k], lengths[k]);
+            throw;
+        }
+        std::copy(found.begin(), found.end(), path);
+        std::copy(counts.begin(), counts.end(), accepted);
+        std::copy(want.begin(), want.end(), next);
+        return;
+    }
+    ensure_batch(rows, rows);
+    hipStream_t s = cache_->stream();
+    // starts, expected tokens | accepted counts, next tokens, paths
+    const size_t part = (n + 3) / 4 * 4, words = 4 * part + n * deepest;
+    auto* d = static_cast<int32_t*>(verify_.ensure(words * sizeof(int32_t)));
+    auto* slots = static_cast<int64_t*>(verify_slots_.ensure(n * deepest * sizeof(int64_t)));
+    auto* host = static_cast<int32_t*>(verify_host_.acquire(words * sizeof(int32_t)));
+    for (size_t i = 0; i < n; ++i) {
+        host[i] = static_cast<int32_t>(lengths[i]);
+        host[part + i] = static_cast<int32_t>(first[i]);
+    }
+    TreePlan plan;
+    plan.build(cache_.get(), sequences, n, c.heads, c.context, nullptr, nodes, parents, 0);
+    TVARA_HIP(hipMemcpyAsync(d, host, 2 * part * sizeof(int32_t), hipMemcpyHostToDevice, s));
+    stage_rows(tokens, positions.data(), rows);
+    layer_stack(rows, [&](int l, const float* q, float* kl, float* vl, float* attn) {
+        plan.launch(l, q, kl, vl, 0, attn, s);
+    });
+    launch_logits(rows, 0);
+    int32_t *counts = d + 2 * part, *after = d + 3 * part, *paths = d + 4 * part;
+    plan.accept(static_cast<const uint32_t*>(btok_.ptr), reinterpret_cast<const uint32_t*>(d + part), at(blogits_, 0), c.vocab,
+                0, paths, deepest, counts, reinterpret_cast<uint32_t*>(after), s);
+    TVARA_HIP(hipMemcpyAsync(host + 2 * part, counts, (words - 2 * part) * sizeof(int32_t), hipMemcpyDeviceToHost, s));
+    verify_host_.release(s);
+    plan.check();  // (waits for the stream)
+    TVARA_HIP(hipStreamSynchronize(s));
+    std::vector<size_t> taken(host + 2 * part, host + 2 * part + n);
+    cache_->reserve(sequences, n, taken.data());
+    try {
+        SlotPlan map;
+        map.build(cache_.get(), sequences, n);
+        map.map(d, counts, deepest, n * deepest, nullptr, nullptr, slots, nullptr, 0, s);
+        map.write(slots, paths, n * deepest, at(bk_, 0), at(bv_, 0), rows, c.kv_width(), rows * c.kv_width(), s);
+        map.check();
+    } catch (...) {
+        for (size_t i = 0; i < n; ++i) cache_->truncate(sequences[i], lengths[i]);
+        throw;
+    }
+    size_t row0 = 0;
+    for (size_t i = 0; i < n; row0 += nodes[i++]) {
+        accepted[i] = taken[i];
+        next[i] = static_cast<uint32_t>(host[3 * part + i]);
+        for (size_t j = 0; j < nodes[i]; ++j)
+            path[row0 + j] = j < taken[i] ? host[4 * part + i * deepest + j] - static_cast<int32_t>(row0) : -1;
+    }
 }
 
 bool DeviceModel::batched_widths() const {

@@ -153,6 +153,14 @@ public:
     // Calls that return every token's logits keep kChunkRows, for the size of
     // the logits buffer, and so do passes on the f32 rows, for their partials.
     static constexpr size_t kChunkRows = 512, kPromptRows = 2048;
+    // Trees of drafted tokens at the ends of n distinct sequences (node lists packed,
+    // as TreePlan has them): one pass over all nodes, each at its depth's position and
+    // attending to its sequence, its ancestors and itself; greedy acceptance from
+    // first[i] on the GPU; the accepted nodes' K/V appended through a slot map.
+    // path (as long as the nodes, each tree's at its first node): the accepted nodes,
+    // numbered within their tree, -1 behind.  On failure no sequence changes.
+    void verify_trees(const uint64_t* sequences, size_t n, const size_t* nodes, const int32_t* parents,
+                      const uint32_t* tokens, const uint32_t* first, int32_t* path, size_t* accepted, uint32_t* next);
 
 private:
     struct Layer {
@@ -181,6 +189,9 @@ private:
     DeviceBuffer bx_, bnorm_, bq_, bk_, bv_, bkapp_, bvapp_, battn_, bgate_, blogits_, brope_, btok_, bpart_, bhalves_,
         bunscale_;
     PinnedBuffer bhost_;
+    // acceptance: each tree's sequence length and expected token, then what it gives
+    DeviceBuffer verify_, verify_slots_;
+    PinnedBuffer verify_host_;
     HostCopier copier_;
     // the batched step's synchronisation: an event after the last layer's
     // attention (the plan's check waits on it, not on the whole stream), one

@@ -12,6 +12,8 @@ namespace tvara_amd {
 
 namespace {
 constexpr size_t kIntMax = static_cast<size_t>(std::numeric_limits<int32_t>::max());
+// of a launch: 2^32 threads, here in workgroups of up to 256
+constexpr size_t kMaxThreads = std::numeric_limits<uint32_t>::max(), kMaxWorkgroups = kMaxThreads / 256;
 
 size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 }  // namespace
@@ -71,6 +73,16 @@ int PlanRegion::check() {
 
 // -------------------------------------------------------------- the trees
 
+void tree_depths(const int32_t* parents, size_t nodes, size_t room, std::vector<size_t>& depth) {
+    depth.resize(nodes);
+    for (size_t j = 0; j < nodes; ++j) {
+        const int32_t p = parents[j];
+        if (p < -1 || p >= static_cast<int32_t>(j)) throw std::invalid_argument("invalid token tree");
+        depth[j] = p < 0 ? 1 : depth[p] + 1;
+        if (depth[j] > room) throw std::invalid_argument("token tree exceeds the context");
+    }
+}
+
 void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t h, size_t context,
                      const size_t* visible, const size_t* nodes, const int32_t* parents, int prec) {
     cache = c;
@@ -78,6 +90,7 @@ void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t
     c->check_device();
     if (!n || !sequences || !nodes) throw std::invalid_argument("empty tree plan");
     if (prec != 0 && prec != 2) throw std::invalid_argument("tree attention is f32 or f32x3");
+    if (h > 65535) throw std::invalid_argument("invalid fused attention shape");  // (a grid's second dimension)
     heads = static_cast<int>(h);
     group = static_cast<int>(h / g.kv_heads);
     precision = prec;
@@ -88,7 +101,9 @@ void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t
         if (nodes[i] > kMaxTreeNodes) throw std::invalid_argument("a token tree has at most 1,024 nodes");
         rows += nodes[i];
         most = std::max(most, nodes[i]);
-        if (rows > kIntMax / h) throw std::invalid_argument("attention batch too large");
+        // (the merge has a thread for two columns, acceptance a workgroup a row and more)
+        if (rows > kMaxWorkgroups - kAcceptParts || rows > std::min(kIntMax, kMaxThreads / g.head_dim) / h)
+            throw std::invalid_argument("attention batch too large");
     }
     if (rows && !parents) throw std::invalid_argument("invalid token tree");
     words = static_cast<int>(std::max<size_t>(1, (most + 31) / 32));
@@ -97,21 +112,19 @@ void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t
     std::vector<uint32_t> mask(rows * words, 0);
     std::vector<int32_t> tab;
     std::map<uint64_t, int32_t> offset;
-    std::vector<size_t> depth(most);
+    std::vector<size_t> depth;
     size_t row0 = 0;
     for (size_t i = 0; i < n; ++i) {
         const Table& t = c->sequence(sequences[i]);
         const size_t seen = visible ? std::min(visible[i], t.length) : t.length;
         if (seen > kIntMax - kMaxTreeNodes) throw std::invalid_argument("sequence too long for the device kernels");
         if (seen > context) throw std::invalid_argument("invalid fused attention shape");
+        tree_depths(parents + row0, nodes[i], context - seen, depth);
         for (size_t j = 0; j < nodes[i]; ++j) {
             const int32_t p = parents[row0 + j];
-            if (p < -1 || p >= static_cast<int32_t>(j)) throw std::invalid_argument("invalid token tree");
             uint32_t* m = &mask[(row0 + j) * words];
             if (p >= 0) std::copy_n(&mask[(row0 + p) * words], words, m);
             m[j / 32] |= 1u << (j % 32);
-            depth[j] = p < 0 ? 1 : depth[p] + 1;
-            if (depth[j] > context - seen) throw std::invalid_argument("token tree exceeds the context");
         }
         if (!offset.count(sequences[i])) {
             offset[sequences[i]] = static_cast<int32_t>(tab.size());
@@ -131,7 +144,7 @@ void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t
         tile_work(trees, work, runs);
     else
         row_work(trees, work, runs);
-    if (slots > kIntMax / h || work.size() > kIntMax) throw std::invalid_argument("attention batch too large");
+    if (slots > kIntMax / h || work.size() > 3 * kMaxWorkgroups) throw std::invalid_argument("attention batch too large");
     items = static_cast<int>(tiles.rows ? work.size() / 3 : work.size());
 
     // acceptance's: each row's tree, and counters that start at zero
@@ -249,6 +262,7 @@ void TreePlan::launch(int layer, const float* q, const float* keys, const float*
     if (layer < 0 || static_cast<size_t>(layer) >= g.layers) throw std::invalid_argument("invalid fused attention shape");
     if (!row_stride) row_stride = g.kv_width();
     if (row_stride < g.kv_width()) throw std::invalid_argument("token rows overlap");
+    if (row_stride > kMaxRowStride) throw std::invalid_argument("token rows too far apart");
     if (!rows) return;
     cache->check_device();
     cache->flush();
@@ -385,7 +399,10 @@ void SlotPlan::write(const int64_t* slots, const int32_t* rows, size_t n, const 
                      size_t row_count, size_t row_stride, size_t layer_stride, hipStream_t s) {
     if (cache->epoch() != epoch) throw std::invalid_argument("slot plan is stale: the cache changed");
     const Geometry& g = cache->geometry();
-    if (n > kIntMax || row_count > kIntMax) throw std::invalid_argument("KV write too large");
+    // (a thread has up to four floats of a row, and 32 bits for their place in a block)
+    if (n > kMaxWorkgroups || row_count > kIntMax || 2 * g.layers * g.kv_width() > size_t(65535) * 256 ||
+        2 * g.layers * g.kv_width() * g.tokens_per_block > kMaxThreads)
+        throw std::invalid_argument("KV write too large");
     if (row_stride < g.kv_width() || (g.layers > 1 && layer_stride < g.kv_width()))
         throw std::invalid_argument("token rows overlap");
     if (cache->format() == kQ8 && (row_stride % 4 || (g.layers > 1 && layer_stride % 4)))

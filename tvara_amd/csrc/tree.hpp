@@ -14,6 +14,9 @@ namespace tvara_amd {
 
 // most nodes of one tree (its ancestor masks are 32 words a node)
 constexpr size_t kMaxTreeNodes = 1024;
+// most floats from one node's keys to the next one's: a tile's 32 rows lie within
+// the 32 bits of a buffer's offsets
+constexpr size_t kMaxRowStride = size_t(1) << 23;
 
 // A batch of trees as the kernels read it.  Node rows are packed, one tree
 // after the other; an attention row is a (node, query head) pair.
@@ -149,6 +152,10 @@ private:
     bool null_stream_ = true;
     hipStream_t last_ = nullptr;
 };
+
+// the nodes' depths, a root's 1; refuses a parent that does not come before its node
+// and depths above `room`
+void tree_depths(const int32_t* parents, size_t nodes, size_t room, std::vector<size_t>& depth);
 
 // Trees of drafted tokens over cached sequences (tvara_tree_plan_*).
 struct TreePlan {

@@ -161,6 +161,45 @@ class NativeModel:
                 self._raise_error()
         return output
 
+    def verify_trees(self, sequences, parents, tokens, first):
+        """One step of speculative decoding (tvara_sequences_verify_trees):
+        parents[i] and tokens[i] are the drafted tree at the end of
+        sequences[i], first[i] the token that its own logits chose.  Returns
+        each tree's accepted nodes, whose tokens are appended, and the tokens
+        expected after them."""
+        seqs = np.ascontiguousarray(sequences, dtype=np.uint64).reshape(-1)
+        if not len(parents) == len(tokens) == len(first) == seqs.size:
+            raise ValueError("one tree and one first token per sequence")
+        if any(len(p) != len(t) for p, t in zip(parents, tokens)):
+            raise ValueError("one parent per drafted token")
+        if any(not self._valid_token(t) for tree in [*tokens, first] for t in tree):
+            raise ValueError("Invalid token ID")
+        nodes = np.array([len(p) for p in parents], dtype=np.uintp)
+
+        def packed(lists, dtype):
+            flat = [x for one in lists for x in one]
+            return np.array(flat, dtype=np.int64).astype(dtype) if flat else np.zeros(0, dtype)
+
+        if any(not -1 <= p < len(tree) for tree in parents for p in tree):
+            raise ValueError("invalid token tree")
+        par, toks = packed(parents, np.int32), packed(tokens, np.uint32)
+        start = packed([first], np.uint32)
+        path, accepted = np.full(toks.size, -1, np.int32), np.zeros(seqs.size, np.uintp)
+        after = np.zeros(seqs.size, np.uint32)
+
+        def ptr(a, t):
+            return a.ctypes.data_as(ctypes.POINTER(t))
+
+        with self._lock:
+            self._check_open()
+            if self._library.tvara_sequences_verify_trees(
+                    self._handle, ptr(seqs, ctypes.c_uint64), seqs.size, ptr(nodes, ctypes.c_size_t),
+                    ptr(par, ctypes.c_int32), ptr(toks, ctypes.c_uint32), ptr(start, ctypes.c_uint32),
+                    ptr(path, ctypes.c_int32), ptr(accepted, ctypes.c_size_t), ptr(after, ctypes.c_uint32)):
+                self._raise_error()
+        ends = np.concatenate([[0], np.cumsum(nodes)]).astype(int)
+        return [path[a:a + int(k)].tolist() for a, k in zip(ends, accepted)], after.tolist()
+
     def cache(self):
         """The model's KV cache as a tvara_amd.kv.PagedCache (tvara_model_cache):
         fork, snapshots, retain / release, import and the prefix cache
