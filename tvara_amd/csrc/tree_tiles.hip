@@ -78,6 +78,18 @@ __device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned&
     lo = __builtin_bit_cast(unsigned, __builtin_convertvector(rest, f16x2));
 }
 
+// Two elements of Q8_0 blocks as hi + lo in fp16: bytes i and j (4 to 7: of w1) of a
+// pair of words times the fp16 scales d.  A byte in the low end of 1024 is q + 1152
+// exactly, and the scale times q less its rounding is exact as well: five
+// instructions a pair, eight by way of f32.
+template <int i, int j>
+__device__ __forceinline__ void scaled2(unsigned w0, unsigned w1, f16x2 d, unsigned& hi, unsigned& lo) {
+    const unsigned u = __builtin_amdgcn_perm(w1, w0, 0x0c000c00u | j << 16 | i) ^ 0x64806480u;
+    const f16x2 q = __builtin_bit_cast(f16x2, u) - f16x2{1152, 1152}, h = q * d;
+    hi = __builtin_bit_cast(unsigned, h);
+    lo = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(q, d, -h));
+}
+
 __device__ __forceinline__ bool all_finite(f32x4 x) {
     return __builtin_isfinite(x[0]) && __builtin_isfinite(x[1]) && __builtin_isfinite(x[2]) && __builtin_isfinite(x[3]);
 }
@@ -711,17 +723,46 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
         }
     };
     auto put = [&](int buf, int step) __attribute__((always_inline)) {
-        if constexpr (kQ8) {
-            f32x4 x[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const unsigned w = rawq[i / 4][i % 4];
-                const float d = half_bits_to_float(static_cast<uint16_t>(takes_keys ? rawd[i / 4] : rawd[i]));
-                x[i] = f32x4{sbyte_to_float<0>(w) * d, sbyte_to_float<1>(w) * d, sbyte_to_float<2>(w) * d, sbyte_to_float<3>(w) * d};
-            }
-            stage(buf, step, x);
-        } else {
+        if constexpr (!kQ8) {
             stage(buf, step, raw);
+        } else if (takes_keys) {
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {  // (words 0 to 3 are of the first key or half, 4 to 7 of the second)
+                const f16x2 d = __builtin_bit_cast(f16x2, rawd[p / 2] | rawd[p / 2] << 16);
+                u32x4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const unsigned w = rawq[p / 2][2 * (p % 2) + e];
+                    unsigned h0, h1, l0, l1;
+                    scaled2<0, 1>(w, 0, d, h0, l0);
+                    scaled2<2, 3>(w, 0, d, h1, l1);
+                    hi[2 * e] = h0;
+                    hi[2 * e + 1] = h1;
+                    lo[2 * e] = l0;
+                    lo[2 * e + 1] = l1;
+                }
+                const int o = D == 128 ? mt0 * KC + p : p;
+                parts[buf][sub][2 * o][lane] = hi;
+                parts[buf][sub][2 * o + 1][lane] = lo;
+            }
+        } else {
+            auto tile = [&](auto j) __attribute__((always_inline)) {
+                u32x4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f16x2 d = __builtin_bit_cast(f16x2, rawd[2 * e] | rawd[2 * e + 1] << 16);
+                    unsigned h1, l1;
+                    scaled2<j, 4 + j>(rawq[e / 2][2 * (e % 2)], rawq[e / 2][2 * (e % 2) + 1], d, h1, l1);
+                    hi[e] = h1;
+                    lo[e] = l1;
+                }
+                parts[buf][sub][VO + 2 * (4 * vh + j)][lane] = hi;
+                parts[buf][sub][VO + 2 * (4 * vh + j) + 1][lane] = lo;
+            };
+            tile(std::integral_constant<int, 0>{});
+            tile(std::integral_constant<int, 1>{});
+            tile(std::integral_constant<int, 2>{});
+            tile(std::integral_constant<int, 3>{});
         }
     };
 
