@@ -169,7 +169,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
     }
 
     f32x4 s[2][NT];  // scores, then probabilities, of keys 16mt + 4g + i
-    auto scores = [&](const f32x4 (&k)[2][C]) {
+    // key(mt, c): the lane's c-th four columns; key(mt, kc, hi, lo): eight in parts
+    auto scores = [&](auto&& key) __attribute__((always_inline)) {
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
@@ -178,14 +179,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
 #pragma unroll
                 for (int kc = 0; kc < KC; ++kc) {
                     u32x4 hi, lo;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const f32x4 x = k[mt][2 * kc + e / 2];
-                        unsigned h1, l1;
-                        split2(x[2 * (e % 2)], x[2 * (e % 2) + 1], h1, l1);
-                        hi[e] = h1;
-                        lo[e] = l1;
-                    }
+                    key(mt, kc, hi, lo);
                     const f16x8 kh8 = __builtin_bit_cast(f16x8, hi), kl8 = __builtin_bit_cast(f16x8, lo);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
@@ -198,14 +192,46 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                 }
             } else {
 #pragma unroll
-                for (int c = 0; c < C; ++c)
+                for (int c = 0; c < C; ++c) {
+                    const f32x4 k = key(mt, c);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
-                            s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[mt][c][i], qf[nt][c][i], s[mt][nt], 0, 0, 0);
+                            s[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i], qf[nt][c][i], s[mt][nt], 0, 0, 0);
+                }
             }
         }
+    };
+    // rows as f32 in registers, given so
+    auto from_f32 = [](const f32x4 (&k)[2][C]) __attribute__((always_inline)) {
+        if constexpr (kX3)
+            return [&k](int mt, int kc, u32x4& hi, u32x4& lo) __attribute__((always_inline)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f32x4 x = k[mt][2 * kc + e / 2];
+                    unsigned h1, l1;
+                    split2(x[2 * (e % 2)], x[2 * (e % 2) + 1], h1, l1);
+                    hi[e] = h1;
+                    lo[e] = l1;
+                }
+            };
+        else
+            return [&k](int mt, int c) __attribute__((always_inline)) { return k[mt][c]; };
+    };
+    auto values_from_f32 = [](const f32x4 (&v)[2][4][H]) __attribute__((always_inline)) {
+        if constexpr (kX3)
+            return [&v](int h, auto j, u32x4& hi, u32x4& lo) __attribute__((always_inline)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    unsigned h1, l1;
+                    split2(v[e / 2][2 * (e % 2)][h][j.value], v[e / 2][2 * (e % 2) + 1][h][j.value], h1, l1);
+                    hi[e] = h1;
+                    lo[e] = l1;
+                }
+            };
+        else
+            return [&v](int mt, int i, int h, auto j) __attribute__((always_inline)) { return v[mt][i][h][j.value]; };
     };
     // seen(mt, i, nt): whether the row sees the key
     auto softmax = [&](auto masked, auto&& seen) {
@@ -248,9 +274,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
             l[nt] += sum;
         }
     };
-    auto output = [&](const f32x4 (&v)[2][4][H]) {
+    // value(mt, i, h, j): column j of the h-th four of key 16mt + 4g + i;
+    // value(h, j, hi, lo): of the lane's eight keys in parts
+    auto output = [&](auto&& value) __attribute__((always_inline)) {
+        u32x4 ph[NT], pl[NT];
         if constexpr (kX3) {
-            u32x4 ph[NT], pl[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -260,48 +288,45 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                     ph[nt][e] = h1;
                     pl[nt][e] = l1;
                 }
+        }
+        auto tile = [&](int h, auto j) __attribute__((always_inline)) {
+            if constexpr (kX3) {
+                u32x4 hi, lo;
+                value(h, j, hi, lo);
+                const f16x8 vh = __builtin_bit_cast(f16x8, hi), vl = __builtin_bit_cast(f16x8, lo);
 #pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    u32x4 hi, lo;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        unsigned h1, l1;
-                        split2(v[e / 2][2 * (e % 2)][h][j], v[e / 2][2 * (e % 2) + 1][h][j], h1, l1);
-                        hi[e] = h1;
-                        lo[e] = l1;
-                    }
-                    const f16x8 vh = __builtin_bit_cast(f16x8, hi), vl = __builtin_bit_cast(f16x8, lo);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        f32x4& o = acc[4 * h + j][nt];
-                        const f16x8 p8 = __builtin_bit_cast(f16x8, ph[nt]);
-                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, p8, o, 0, 0, 0);
-                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(f16x8, pl[nt]), o, 0, 0, 0);
-                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, p8, o, 0, 0, 0);
-                    }
+                for (int nt = 0; nt < NT; ++nt) {
+                    f32x4& o = acc[4 * h + j][nt];
+                    const f16x8 p8 = __builtin_bit_cast(f16x8, ph[nt]);
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, p8, o, 0, 0, 0);
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(f16x8, pl[nt]), o, 0, 0, 0);
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, p8, o, 0, 0, 0);
                 }
-        } else {
-            // a step's part is a chain of eight from zero, added to the rest: as
-            // short as a long context's sums need it
+            } else {
+                // a step's part is a chain of eight from zero, added to the rest: as
+                // short as a long context's sums need it
+                f32x4 part[NT];
 #pragma unroll
-            for (int h = 0; h < H; ++h)
+                for (int nt = 0; nt < NT; ++nt) part[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    f32x4 part[NT];
+                for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) part[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    for (int i = 0; i < 4; ++i) {
+                        const float x = value(mt, i, h, j);
 #pragma unroll
-                    for (int mt = 0; mt < 2; ++mt)
+                        for (int nt = 0; nt < NT; ++nt)
+                            part[nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, s[mt][nt][i], part[nt], 0, 0, 0);
+                    }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                for (int nt = 0; nt < NT; ++nt) acc[4 * h + j][nt] += part[nt];
+            }
+        };
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-                                part[nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[mt][i][h][j], s[mt][nt][i], part[nt], 0, 0, 0);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) acc[4 * h + j][nt] += part[nt];
-                }
+        for (int h = 0; h < H; ++h) {
+            tile(h, std::integral_constant<int, 0>{});
+            tile(h, std::integral_constant<int, 1>{});
+            tile(h, std::integral_constant<int, 2>{});
+            tile(h, std::integral_constant<int, 3>{});
         }
     };
 
@@ -326,25 +351,24 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
             const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
             return a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes + static_cast<size_t>(slot) * rowb;
         };
-        f32x4 k[2][C], v[2][4][H];
-        auto load_k = [&](int stp) {
+        // f32 rows, or Q8_0 bytes and scales, which become values where they are used
+        f32x4 k[kQ8 ? 1 : 2][C], v[kQ8 ? 1 : 2][4][H];
+        u32x4 kw[kQ8 ? 2 : 1][H];
+        unsigned kd[kQ8 ? 2 : 1][H], vw[kQ8 ? 2 : 1][4][H], vd[kQ8 ? 2 : 1][4];
+        auto scales = [&](const char* b, int mt, int stp) {  // of the block's rows from the tile's first on
+            const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
+            return b + static_cast<size_t>(tpb - slot) * D + static_cast<size_t>(slot) * (D / 32) * 2;
+        };
+        auto load_k = [&](int stp) __attribute__((always_inline)) {
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
                 const char* b = block(mt, stp);
                 if constexpr (kQ8) {
-                    const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
-                    const char* sc = b + static_cast<size_t>(tpb - slot) * D + static_cast<size_t>(slot) * (D / 32) * 2;
+                    const char* sc = scales(b, mt, stp);
 #pragma unroll
                     for (int u = 0; u < H; ++u) {
-                        const u32x4 w = *reinterpret_cast<const u32x4*>(b + koff + 64 * u);
-                        const float d = half_bits_to_float(
-                            *reinterpret_cast<const uint16_t*>(sc + (r16 * (D / 32) + 2 * u + (g >> 1)) * 2));
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const unsigned b4 = w[c];
-                            k[mt][4 * u + c] = f32x4{sbyte_to_float<0>(b4) * d, sbyte_to_float<1>(b4) * d,
-                                                     sbyte_to_float<2>(b4) * d, sbyte_to_float<3>(b4) * d};
-                        }
+                        kw[mt][u] = *reinterpret_cast<const u32x4*>(b + koff + 64 * u);
+                        kd[mt][u] = *reinterpret_cast<const uint16_t*>(sc + (r16 * (D / 32) + 2 * u + (g >> 1)) * 2);
                     }
                 } else {
 #pragma unroll
@@ -352,23 +376,17 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                 }
             }
         };
-        auto load_v = [&](int stp) {
+        auto load_v = [&](int stp) __attribute__((always_inline)) {
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
                 const char* b = block(mt, stp) + vsec;
                 if constexpr (kQ8) {
-                    const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
-                    const char* sc = b + static_cast<size_t>(tpb - slot) * D + static_cast<size_t>(slot) * (D / 32) * 2;
+                    const char* sc = scales(b, mt, stp);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float d = half_bits_to_float(*reinterpret_cast<const uint16_t*>(
-                            sc + ((4 * g + i) * (D / 32) + (D / 16) * r16 / 32) * 2));
+                        vd[mt][i] = *reinterpret_cast<const uint16_t*>(sc + ((4 * g + i) * (D / 32) + (D / 16) * r16 / 32) * 2);
 #pragma unroll
-                        for (int h = 0; h < H; ++h) {
-                            const unsigned b4 = *reinterpret_cast<const unsigned*>(b + voff + i * D + 4 * h);
-                            v[mt][i][h] = f32x4{sbyte_to_float<0>(b4) * d, sbyte_to_float<1>(b4) * d,
-                                                sbyte_to_float<2>(b4) * d, sbyte_to_float<3>(b4) * d};
-                        }
+                        for (int h = 0; h < H; ++h) vw[mt][i][h] = *reinterpret_cast<const unsigned*>(b + voff + i * D + 4 * h);
                     }
                 } else {
 #pragma unroll
@@ -379,11 +397,57 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                 }
             }
         };
+        auto cached_scores = [&]() __attribute__((always_inline)) {
+            if constexpr (!kQ8)
+                scores(from_f32(k));
+            else if constexpr (kX3)
+                scores([&](int mt, int kc, u32x4& hi, u32x4& lo) __attribute__((always_inline)) {
+                    const unsigned one = kd[mt][kc / 2];
+                    const f16x2 d = __builtin_bit_cast(f16x2, one | one << 16);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const unsigned w = kw[mt][kc / 2][2 * (kc % 2) + e];
+                        unsigned h0, h1, l0, l1;
+                        scaled2<0, 1>(w, 0, d, h0, l0);
+                        scaled2<2, 3>(w, 0, d, h1, l1);
+                        hi[2 * e] = h0;
+                        hi[2 * e + 1] = h1;
+                        lo[2 * e] = l0;
+                        lo[2 * e + 1] = l1;
+                    }
+                });
+            else
+                scores([&](int mt, int c) __attribute__((always_inline)) {
+                    const float d = half_bits_to_float(static_cast<uint16_t>(kd[mt][c / 4]));
+                    const unsigned w = kw[mt][c / 4][c % 4];
+                    return f32x4{sbyte_to_float<0>(w) * d, sbyte_to_float<1>(w) * d, sbyte_to_float<2>(w) * d, sbyte_to_float<3>(w) * d};
+                });
+        };
+        auto cached_output = [&]() __attribute__((always_inline)) {
+            if constexpr (!kQ8)
+                output(values_from_f32(v));
+            else if constexpr (kX3)
+                output([&](int h, auto j, u32x4& hi, u32x4& lo) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int mt = e / 2, i = 2 * (e % 2);
+                        unsigned h1, l1;
+                        scaled2<j, 4 + j>(vw[mt][i][h], vw[mt][i + 1][h],
+                                          __builtin_bit_cast(f16x2, vd[mt][i] | vd[mt][i + 1] << 16), h1, l1);
+                        hi[e] = h1;
+                        lo[e] = l1;
+                    }
+                });
+            else
+                output([&](int mt, int i, int h, auto j) __attribute__((always_inline)) {
+                    return sbyte_to_float<j>(vw[mt][i][h]) * half_bits_to_float(static_cast<uint16_t>(vd[mt][i]));
+                });
+        };
         load_k(step);
         load_v(step);
         for (; step < end; step += WK) {
             const int next = step + WK;
-            scores(k);
+            cached_scores();
             // the loads of the next step go out as soon as a register is free (past
             // the end the last step's again: its blocks are there)
             if (++at == 32) {
@@ -400,11 +464,17 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                 for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (kStep * step + 16 * mt + 4 * g + i >= cached)
+                        if (kStep * step + 16 * mt + 4 * g + i >= cached) {
+                            if constexpr (kQ8) vd[mt][i] = 0;
 #pragma unroll
-                            for (int h = 0; h < H; ++h) v[mt][i][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+                            for (int h = 0; h < H; ++h)
+                                if constexpr (kQ8)
+                                    vw[mt][i][h] = 0;
+                                else
+                                    v[mt][i][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+                        }
             }
-            output(v);
+            cached_output();
             load_v(next);
         }
     }
@@ -436,7 +506,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                 }
             }
         }
-        scores(k);
+        scores(from_f32(k));
         softmax(std::true_type{}, [&](int mt, int i, int nt) { return (mask[nt] >> (16 * mt + 4 * g + i) & 1u) != 0; });
         const bool plain = !__any(odd != 0.f);  // (0, or NaN where a value is not finite)
         if (!plain) {
@@ -451,7 +521,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
 #pragma unroll
                         for (int j = 0; j < 4; ++j) v[mt][i][h][j] = finite_or_zero(v[mt][i][h][j]);
         }
-        output(v);
+        output(values_from_f32(v));
         if (plain) continue;
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
