@@ -110,30 +110,47 @@ __global__ __launch_bounds__(64) void tree_rows_kernel(const TreeArgs a) {
     if (!whole && lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(m, l);
 }
 
-// A row's runs combined in order: a thread per two columns.
+// A row's runs combined in order: a thread per four columns (two where head_dim is
+// no multiple of four), with the loads of four runs in flight.  Bound: the memory
+// behind the L2s, which the partials come from.  Four contexts of 20,000 to 32,768
+// tokens (84 rows of 32 heads of 128, 16 runs): 8.7 us, 2.7 TB/s; one run at a time
+// and two columns a thread took 15.0.
+template <int kVec>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
-    const int D = a.lay.head_dim, half = D / 2;
-    const size_t t = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x, at = t / half;
+    typedef float vec __attribute__((ext_vector_type(kVec)));
+    const int D = a.lay.head_dim, parts = D / kVec;
+    const size_t t = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x, at = t / parts;
     if (at >= static_cast<size_t>(a.rows) * a.heads) return;
     const int2 runs = a.runs[at / a.heads];
     if (runs.y == 1) return;
-    const int c = 2 * static_cast<int>(t % half), h = static_cast<int>(at % a.heads);
+    const int c = kVec * static_cast<int>(t % parts), h = static_cast<int>(at % a.heads);
+    constexpr int kTogether = 4;
     float m = -INFINITY, l = 0.f;
-    float2 sum = make_float2(0.f, 0.f);
-    for (int r = 0; r < runs.y; ++r) {
-        const size_t p = (static_cast<size_t>(runs.x) + r) * a.heads + h;
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
-        if (ml.x == -INFINITY) continue;
-        const float2 x = *reinterpret_cast<const float2*>(a.part_acc + p * D + c);
-        const float mn = fmaxf(m, ml.x), wm = fast_exp2(m - mn), wr = fast_exp2(ml.x - mn);
-        l = l * wm + ml.y * wr;
-        sum.x = sum.x * wm + x.x * wr;
-        sum.y = sum.y * wm + x.y * wr;
-        m = mn;
+    vec sum = 0.f;
+    for (int r0 = 0; r0 < runs.y; r0 += kTogether) {
+        float2 ml[kTogether];
+        vec x[kTogether];
+#pragma unroll
+        for (int r = 0; r < kTogether; ++r) {
+            const size_t p = (static_cast<size_t>(runs.x) + min(r0 + r, runs.y - 1)) * a.heads + h;
+            ml[r] = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
+            x[r] = *reinterpret_cast<const vec*>(a.part_acc + p * D + c);
+        }
+#pragma unroll
+        for (int r = 0; r < kTogether; ++r) {
+            if (r0 + r >= runs.y || ml[r].x == -INFINITY) continue;
+            const float mn = fmaxf(m, ml[r].x), wm = fast_exp2(m - mn), wr = fast_exp2(ml[r].x - mn);
+            l = l * wm + ml[r].y * wr;
+            sum = sum * wm + x[r] * wr;
+            m = mn;
+        }
     }
-    const float2 o = make_float2(sum.x / l, sum.y / l);
-    if (a.check && !(__builtin_isfinite(o.x) && __builtin_isfinite(o.y))) *a.err = 1;
-    *reinterpret_cast<float2*>(a.out + at * D + c) = o;
+    const vec o = sum / l;
+    bool finite = true;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) finite &= __builtin_isfinite(o[e]);
+    if (a.check && !finite) *a.err = 1;
+    *reinterpret_cast<vec*>(a.out + at * D + c) = o;
 }
 
 }  // namespace
@@ -145,8 +162,10 @@ void launch_tree_rows(const TreeArgs& a, int items, hipStream_t s) {
 }
 
 void launch_tree_merge(const TreeArgs& a, hipStream_t s) {
-    const size_t threads = static_cast<size_t>(a.rows) * a.heads * (a.lay.head_dim / 2);
-    launch("tree_attention_merge", tree_merge_kernel, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, s, a);
+    const int vec = a.lay.head_dim % 4 ? 2 : 4;
+    const size_t threads = static_cast<size_t>(a.rows) * a.heads * (a.lay.head_dim / vec);
+    launch("tree_attention_merge", vec == 4 ? tree_merge_kernel<4> : tree_merge_kernel<2>,
+           dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, s, a);
     TVARA_HIP(hipGetLastError());
 }
 

@@ -134,17 +134,98 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
     auto kcol = [&](int c) { return kQ8 ? 64 * (c / 4) + 16 * g + 4 * (c % 4) : 16 * c + 4 * g; };
     auto vcol = [](int h, int r) { return kQ8 ? (D / 16) * r + 4 * h : 64 * h + 4 * r; };
 
-    f32x4 qf[kX3 ? 1 : NT][kX3 ? 1 : C];
+    const int csteps = (cached + kStep - 1) / kStep, end = min(it.end, csteps);
+    const int tpb = a.lay.tpb, tsh = __builtin_ctz(static_cast<unsigned>(tpb));
+    const int32_t* tab = a.tables + tree.x;
+    const size_t kbytes = kQ8 ? static_cast<size_t>(a.layer) * 2 * a.lay.section + static_cast<size_t>(kh) * a.lay.head_bytes
+                              : (static_cast<size_t>(a.layer) * 2 * tpb * kvw + static_cast<size_t>(kh) * D) * sizeof(float);
+    const size_t vsec = kQ8 ? a.lay.section : static_cast<size_t>(tpb) * kvw * sizeof(float);
+    const int rowb = kQ8 ? D : kvw * static_cast<int>(sizeof(float));  // from one slot to the next
+    const unsigned koff = static_cast<unsigned>(r16 * rowb + kcol(0) * (kQ8 ? 1 : 4));
+    const unsigned voff = static_cast<unsigned>(4 * g * rowb + vcol(0, r16) * (kQ8 ? 1 : 4));
+    int step = it.step + wk;
+    const int last = max(cached - 1, 0) >> 4;  // 16 keys a table lookup; past the end the last again
+    // lane 2i + mt: the block of the wave's i-th step from here
+    auto lookup = [&](int from) { return cached ? tab[min(2 * (from + (lane >> 1) * WK) + (lane & 1), last) << 4 >> tsh] : 0; };
+    int ids = lookup(step), more = lookup(step + 32 * WK), at = 0;
+    auto block = [&](int mt, int stp) {
+        const int id = __builtin_amdgcn_readlane(ids, 2 * at + mt);
+        const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
+        return a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes + static_cast<size_t>(slot) * rowb;
+    };
+    // Loads are asked for as early as what they need is there, the table's first: a
+    // workgroup's start is a chain of waits for memory.
+    f32x4 qf[NT][C];
+    auto load_q = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const float* qp = a.q + (static_cast<size_t>(tree.w + node[nt]) * a.heads + head[nt]) * D;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                qf[nt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (live[nt]) qf[nt][c] = *reinterpret_cast<const f32x4*>(qp + kcol(c));
+            }
+        }
+    };
+    // f32 rows, or Q8_0 bytes and scales, which become values where they are used
+    f32x4 k[kQ8 ? 1 : 2][C], v[kQ8 ? 1 : 2][4][H];
+    u32x4 kw[kQ8 ? 2 : 1][H];
+    unsigned kd[kQ8 ? 2 : 1][H], vw[kQ8 ? 2 : 1][4][H], vd[kQ8 ? 2 : 1][4];
+    auto scales = [&](const char* b, int mt, int stp) {  // of the block's rows from the tile's first on
+        const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
+        return b + static_cast<size_t>(tpb - slot) * D + static_cast<size_t>(slot) * (D / 32) * 2;
+    };
+    auto load_k = [&](int stp) __attribute__((always_inline)) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+            const char* b = block(mt, stp);
+            if constexpr (kQ8) {
+                const char* sc = scales(b, mt, stp);
+#pragma unroll
+                for (int u = 0; u < H; ++u) {
+                    kw[mt][u] = *reinterpret_cast<const u32x4*>(b + koff + 64 * u);
+                    kd[mt][u] = *reinterpret_cast<const uint16_t*>(sc + (r16 * (D / 32) + 2 * u + (g >> 1)) * 2);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < C; ++c) k[mt][c] = *reinterpret_cast<const f32x4*>(b + koff + 64 * c);
+            }
+        }
+    };
+    auto load_v = [&](int stp) __attribute__((always_inline)) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+            const char* b = block(mt, stp) + vsec;
+            if constexpr (kQ8) {
+                const char* sc = scales(b, mt, stp);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    vd[mt][i] = *reinterpret_cast<const uint16_t*>(sc + ((4 * g + i) * (D / 32) + (D / 16) * r16 / 32) * 2);
+#pragma unroll
+                    for (int h = 0; h < H; ++h) vw[mt][i][h] = *reinterpret_cast<const unsigned*>(b + voff + i * D + 4 * h);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+                        v[mt][i][h] = *reinterpret_cast<const f32x4*>(b + static_cast<size_t>(i) * rowb + voff + 256 * h);
+            }
+        }
+    };
+    load_q();
+    if (step < end) {
+        load_k(step);
+        load_v(step);
+    }
     u32x4 qh[kX3 ? NT : 1][kX3 ? KC : 1], ql[kX3 ? NT : 1][kX3 ? KC : 1];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const float* qp = a.q + (static_cast<size_t>(tree.w + node[nt]) * a.heads + head[nt]) * D;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            f32x4 x = {0.f, 0.f, 0.f, 0.f};
-            if (live[nt]) x = *reinterpret_cast<const f32x4*>(qp + kcol(c));
-            x *= a.qscale;
+            qf[nt][c] *= a.qscale;
             if constexpr (kX3) {
+                const f32x4 x = qf[nt][c];
                 unsigned h0, h1, l0, l1;
                 split2(x[0], x[1], h0, l0);
                 split2(x[2], x[3], h1, l1);
@@ -152,11 +233,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                 qh[nt][c / 2][2 * (c % 2) + 1] = h1;
                 ql[nt][c / 2][2 * (c % 2)] = l0;
                 ql[nt][c / 2][2 * (c % 2) + 1] = l1;
-            } else {
-                qf[nt][c] = x;
             }
         }
-    }
 
     f32x4 acc[4 * H][NT];  // tile (h, j) at 4h + j
     float m[NT], l[NT], nonfinite = 0.f;  // nonfinite: NaN once a score is not finite
@@ -331,72 +409,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
     };
 
     // ---- cached steps: this wave's are step0 + wk, + WK, ...
-    const int csteps = (cached + kStep - 1) / kStep, end = min(it.end, csteps);
-    const int tpb = a.lay.tpb, tsh = __builtin_ctz(static_cast<unsigned>(tpb));
-    const int32_t* tab = a.tables + tree.x;
-    const size_t kbytes = kQ8 ? static_cast<size_t>(a.layer) * 2 * a.lay.section + static_cast<size_t>(kh) * a.lay.head_bytes
-                              : (static_cast<size_t>(a.layer) * 2 * tpb * kvw + static_cast<size_t>(kh) * D) * sizeof(float);
-    const size_t vsec = kQ8 ? a.lay.section : static_cast<size_t>(tpb) * kvw * sizeof(float);
-    const int rowb = kQ8 ? D : kvw * static_cast<int>(sizeof(float));  // from one slot to the next
-    const unsigned koff = static_cast<unsigned>(r16 * rowb + kcol(0) * (kQ8 ? 1 : 4));
-    const unsigned voff = static_cast<unsigned>(4 * g * rowb + vcol(0, r16) * (kQ8 ? 1 : 4));
-    int step = it.step + wk;
     if (step < end) {
-        const int last = (cached - 1) >> 4;  // 16 keys a table lookup; past the end the last again
-        // lane 2i + mt: the block of the wave's i-th step from here
-        auto lookup = [&](int from) { return tab[min(2 * (from + (lane >> 1) * WK) + (lane & 1), last) << 4 >> tsh]; };
-        int ids = lookup(step), more = lookup(step + 32 * WK), at = 0;
-        auto block = [&](int mt, int stp) {
-            const int id = __builtin_amdgcn_readlane(ids, 2 * at + mt);
-            const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
-            return a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes + static_cast<size_t>(slot) * rowb;
-        };
-        // f32 rows, or Q8_0 bytes and scales, which become values where they are used
-        f32x4 k[kQ8 ? 1 : 2][C], v[kQ8 ? 1 : 2][4][H];
-        u32x4 kw[kQ8 ? 2 : 1][H];
-        unsigned kd[kQ8 ? 2 : 1][H], vw[kQ8 ? 2 : 1][4][H], vd[kQ8 ? 2 : 1][4];
-        auto scales = [&](const char* b, int mt, int stp) {  // of the block's rows from the tile's first on
-            const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
-            return b + static_cast<size_t>(tpb - slot) * D + static_cast<size_t>(slot) * (D / 32) * 2;
-        };
-        auto load_k = [&](int stp) __attribute__((always_inline)) {
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-                const char* b = block(mt, stp);
-                if constexpr (kQ8) {
-                    const char* sc = scales(b, mt, stp);
-#pragma unroll
-                    for (int u = 0; u < H; ++u) {
-                        kw[mt][u] = *reinterpret_cast<const u32x4*>(b + koff + 64 * u);
-                        kd[mt][u] = *reinterpret_cast<const uint16_t*>(sc + (r16 * (D / 32) + 2 * u + (g >> 1)) * 2);
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < C; ++c) k[mt][c] = *reinterpret_cast<const f32x4*>(b + koff + 64 * c);
-                }
-            }
-        };
-        auto load_v = [&](int stp) __attribute__((always_inline)) {
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-                const char* b = block(mt, stp) + vsec;
-                if constexpr (kQ8) {
-                    const char* sc = scales(b, mt, stp);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        vd[mt][i] = *reinterpret_cast<const uint16_t*>(sc + ((4 * g + i) * (D / 32) + (D / 16) * r16 / 32) * 2);
-#pragma unroll
-                        for (int h = 0; h < H; ++h) vw[mt][i][h] = *reinterpret_cast<const unsigned*>(b + voff + i * D + 4 * h);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int h = 0; h < H; ++h)
-                            v[mt][i][h] = *reinterpret_cast<const f32x4*>(b + static_cast<size_t>(i) * rowb + voff + 256 * h);
-                }
-            }
-        };
         auto cached_scores = [&]() __attribute__((always_inline)) {
             if constexpr (!kQ8)
                 scores(from_f32(k));
@@ -443,8 +456,6 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                     return sbyte_to_float<j>(vw[mt][i][h]) * half_bits_to_float(static_cast<uint16_t>(vd[mt][i]));
                 });
         };
-        load_k(step);
-        load_v(step);
         for (; step < end; step += WK) {
             const int next = step + WK;
             cached_scores();
