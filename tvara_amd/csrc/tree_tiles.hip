@@ -109,7 +109,15 @@ __device__ __forceinline__ Item item_of(const TreeArgs& a) {
 template <int D, int NT, bool kQ8, bool kX3>
 __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel(const TreeArgs a) {
     constexpr int WK = kWaves, C = D / 16, KC = D / 32, H = D / 64;
+    constexpr int W = D / 4;  // 16-byte parts of a row
     __shared__ f32x4 sums[WK][4][NT][64];
+    // f32 keys come as whole rows, W lanes each, and turn into operands (16 lanes, 16
+    // rows) by way of LDS: read from memory as operands they take four times as long
+    // to come through the CU's cache (16 contexts of 2048, 32 heads on 8: f32 and
+    // head_dim 64, 64 rows 63.7 -> 56.9 us; f32x3 and head_dim 128 65.8 -> 61.5 us).
+    // The one wave a SIMD of f32 and head_dim 128 waits for LDS instead (100 -> 114 us).
+    constexpr bool kStaged = !kQ8 && (D == 64 || kX3);
+    __shared__ f32x4 staged[kStaged ? WK : 1][kStaged ? kStep * W : 1];  // a wave's keys of a step
     __shared__ float2 stats[WK][16 * NT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, r16 = lane & 15, wk = wave;
@@ -141,7 +149,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                               : (static_cast<size_t>(a.layer) * 2 * tpb * kvw + static_cast<size_t>(kh) * D) * sizeof(float);
     const size_t vsec = kQ8 ? a.lay.section : static_cast<size_t>(tpb) * kvw * sizeof(float);
     const int rowb = kQ8 ? D : kvw * static_cast<int>(sizeof(float));  // from one slot to the next
-    const unsigned koff = static_cast<unsigned>(r16 * rowb + kcol(0) * (kQ8 ? 1 : 4));
+    const unsigned koff = static_cast<unsigned>(kStaged ? lane / W * rowb + lane % W * 16 : r16 * rowb + kcol(0) * (kQ8 ? 1 : 4));
     const unsigned voff = static_cast<unsigned>(4 * g * rowb + vcol(0, r16) * (kQ8 ? 1 : 4));
     int step = it.step + wk;
     const int last = max(cached - 1, 0) >> 4;  // 16 keys a table lookup; past the end the last again
@@ -188,9 +196,23 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                 }
             } else {
 #pragma unroll
-                for (int c = 0; c < C; ++c) k[mt][c] = *reinterpret_cast<const f32x4*>(b + koff + 64 * c);
+                for (int c = 0; c < C; ++c)
+                    k[mt][c] = *reinterpret_cast<const f32x4*>(b + (kStaged ? static_cast<size_t>(64 / W * c) * rowb : 64 * c) + koff);
             }
         }
+    };
+    // (parts of a row are permuted by its number, so that neither side meets a bank twice)
+    auto stage_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < 2 * C; ++n) {
+            const int row = 64 / W * n + lane / W;
+            staged[wave][row * W + (lane % W ^ (row & 15))] = k[n / C][n % C];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    auto staged_k = [&](int mt, int c) __attribute__((always_inline)) {
+        return staged[wave][(16 * mt + r16) * W + ((4 * c + g) ^ r16)];
     };
     auto load_v = [&](int stp) __attribute__((always_inline)) {
 #pragma unroll
@@ -281,21 +303,24 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
             }
         }
     };
-    // rows as f32 in registers, given so
-    auto from_f32 = [](const f32x4 (&k)[2][C]) __attribute__((always_inline)) {
+    // f32 keys k(mt, c), and values in registers, given so
+    auto from_f32 = [](auto&& k) __attribute__((always_inline)) {
         if constexpr (kX3)
             return [&k](int mt, int kc, u32x4& hi, u32x4& lo) __attribute__((always_inline)) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const f32x4 x = k[mt][2 * kc + e / 2];
-                    unsigned h1, l1;
-                    split2(x[2 * (e % 2)], x[2 * (e % 2) + 1], h1, l1);
-                    hi[e] = h1;
-                    lo[e] = l1;
+                for (int half = 0; half < 2; ++half) {
+                    const f32x4 x = k(mt, 2 * kc + half);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        unsigned h1, l1;
+                        split2(x[2 * e], x[2 * e + 1], h1, l1);
+                        hi[2 * half + e] = h1;
+                        lo[2 * half + e] = l1;
+                    }
                 }
             };
         else
-            return [&k](int mt, int c) __attribute__((always_inline)) { return k[mt][c]; };
+            return [&k](int mt, int c) __attribute__((always_inline)) { return k(mt, c); };
     };
     auto values_from_f32 = [](const f32x4 (&v)[2][4][H]) __attribute__((always_inline)) {
         if constexpr (kX3)
@@ -411,8 +436,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
     // ---- cached steps: this wave's are step0 + wk, + WK, ...
     if (step < end) {
         auto cached_scores = [&]() __attribute__((always_inline)) {
-            if constexpr (!kQ8)
-                scores(from_f32(k));
+            if constexpr (kStaged)
+                scores(from_f32(staged_k));
+            else if constexpr (!kQ8)
+                scores(from_f32([&](int mt, int c) __attribute__((always_inline)) { return k[mt][c]; }));
             else if constexpr (kX3)
                 scores([&](int mt, int kc, u32x4& hi, u32x4& lo) __attribute__((always_inline)) {
                     const unsigned one = kd[mt][kc / 2];
@@ -458,7 +485,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
         };
         for (; step < end; step += WK) {
             const int next = step + WK;
-            cached_scores();
+            if constexpr (kStaged)
+                stage_k();
+            else
+                cached_scores();
             // the loads of the next step go out as soon as a register is free (past
             // the end the last step's again: its blocks are there)
             if (++at == 32) {
@@ -467,6 +497,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                 more = lookup(next + 32 * WK);
             }
             load_k(next);
+            if constexpr (kStaged) {
+                cached_scores();
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
             if (kStep * step + kStep <= cached) {
                 softmax(std::false_type{}, [](int, int, int) { return true; });
             } else {  // the last keys: what lies behind them is not seen, and its values are zeros
@@ -517,7 +552,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                 }
             }
         }
-        scores(from_f32(k));
+        scores(from_f32([&](int mt, int c) __attribute__((always_inline)) { return k[mt][c]; }));
         softmax(std::true_type{}, [&](int mt, int i, int nt) { return (mask[nt] >> (16 * mt + 4 * g + i) & 1u) != 0; });
         const bool plain = !__any(odd != 0.f);  // (0, or NaN where a value is not finite)
         if (!plain) {
