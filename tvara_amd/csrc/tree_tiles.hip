@@ -161,8 +161,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
         const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
         return a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes + static_cast<size_t>(slot) * rowb;
     };
-    // Loads are asked for as early as what they need is there, the table's first: a
-    // workgroup's start is a chain of waits for memory.
+    // A workgroup's start is a chain of waits for memory: table, then keys.  With
+    // head_dim 64 the first keys are asked for before the queries are waited for (16
+    // ragged contexts 50.2 -> 48.3 us); with 128 the registers do not reach for it (f32,
+    // 64 rows 100 -> 102 us, in blocks of 16 115 -> 137).
     f32x4 qf[NT][C];
     auto load_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -235,8 +237,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
             }
         }
     };
+    constexpr bool kEarly = D == 64;
     load_q();
-    if (step < end) {
+    if (kEarly && step < end) {
         load_k(step);
         load_v(step);
     }
@@ -483,6 +486,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                     return sbyte_to_float<j>(vw[mt][i][h]) * half_bits_to_float(static_cast<uint16_t>(vd[mt][i]));
                 });
         };
+        if constexpr (!kEarly) {
+            load_k(step);
+            load_v(step);
+        }
         for (; step < end; step += WK) {
             const int next = step + WK;
             if constexpr (kStaged)
@@ -1119,12 +1126,14 @@ bool tree_tiles_supported(const BlockLayout& lay) {
 }
 
 // 16 contexts of 2048 tokens, 32 query and 8 KV heads, microseconds with each block:
-//   f32x3, head_dim 128:  16 rows  16: 52.6  32: 55.0;  40 rows  32: 62.9  128: 63.9
-//                         64 rows  32: 65.6  128: 73.7;  96 rows  32: 115.8  128: 80.8
-//   f32x3, head_dim 64:   64 rows  32: 44.8  128: 48.5;  96 rows  32: 60.0  128: 51.2
-//   f32, head_dim 64:     16 rows  16: 36.3  32: 41.3;   64 rows  16: 64.4  32: 64.5
-//     (24 to 96 rows, ragged: 16: 56.1  32: 57.2;  one context of 512: 16: 11.2  32: 12.8)
-//   f32, head_dim 128:    32 rows  16: 63.7  32: 63.4;   64 rows  16: 115.2  32: 99.0
+//   f32x3, head_dim 128:  16 rows  16: 53.0  32: 55.3;  32 rows  16: 56.6  32: 57.9
+//                         64 rows  32: 60.6  128: 72.5;  80 rows  32: 113  128: 79.2
+//     Q8_0                16 rows  16: 25.3  32: 31.3;  32 rows  16: 35.3  32: 33.9
+//                         64 rows  32: 49.3  128: 64.0;  80 rows  32: 90.3  128: 70.1
+//   f32x3, head_dim 64:   64 rows  32: 40.5  128: 48.6;  80 rows  32: 58.5  128: 49.9
+//   f32, head_dim 64:     16 rows  16: 33.8  32: 41.3;   64 rows  16: 56.9  32: 64.5
+//   f32, head_dim 128:    16 rows  16: 53.3  32: 60.0;   32 rows  16: 65.2  32: 62.7
+//                         64 rows  16: 116  32: 100
 // Two workgroups share a CU where 256 registers hold a wave, or LDS a workgroup's keys.
 // A run has at least a step a wave, and no more where there are CUs: a wave's second
 // step waits for memory again (one context of 512 tokens in runs of 4 steps: 12.7,
