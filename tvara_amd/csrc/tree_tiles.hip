@@ -689,8 +689,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
     auto row_of = [&](int nt) { return row0 + 16 * kWaves * nt + r16; };
     auto node_of = [&](int nt) { return row_of(nt) / G; };
 
-    // the lane's c-th four columns of a key: as the staging lane holds them
-    auto kcol = [&](int c) { return kQ8 ? 64 * (c / 4) + 16 * g + 4 * (c % 4) : 16 * c + 4 * g; };
+    // the lane's c-th four columns of a key: as the staging lane holds them.  Of f32
+    // blocks that one loads parts of whole rows, two for each operand: part X of the
+    // row's first half and of its second make eight columns for the lane group X % 4
+    // of the products over X / 4.
+    constexpr int X = D / 8;  // lanes that load a row's half
+    auto kcol = [&](int c) { return kQ8 ? 64 * (c / 4) + 16 * g + 4 * (c % 4) : 16 * (c / 2) + 4 * g + D / 2 * (c % 2); };
+    // f32: where the operand of part x of row r goes among the 16 of its lane group, so
+    // that neither the lanes of a row nor those of a group meet a bank twice
+    auto swizzle = [&](int r, int x) { return kQ8 ? r : r ^ (16 / X * x); };
     u32x4 qh[NT][KC], ql[NT][KC];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -765,12 +772,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
         const __amdgpu_buffer_rsrc_t t0 = rows16.descriptor(ia), t1 = rows16.descriptor(ib);
         if constexpr (!kQ8) {
             const int pitch = step < csteps ? rowb : ownb;
-            const int far = takes_keys && D == 128 ? 256 : 0, by = takes_keys ? 64 : pitch;
-            const int off = takes_keys ? r16 * pitch + 16 * g : 4 * g * pitch + 256 * vh + 16 * r16;
+            const int off = takes_keys ? lane / X * pitch + lane % X * 16 : 4 * g * pitch + 256 * vh + 16 * r16;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                raw[i] = __builtin_amdgcn_raw_buffer_load_b128(t0, off, i * by, 0);
-                raw[4 + i] = __builtin_amdgcn_raw_buffer_load_b128(t1, off, i * by + far, 0);
+            for (int i = 0; i < 4; ++i) {  // (keys: 64 / X rows an instruction)
+                const int n = D == 128 ? i : i / 2, half = D == 128 ? 0 : i % 2;
+                const int at0 = takes_keys ? 64 / X * n * pitch + 2 * D * half : i * pitch;
+                raw[i] = __builtin_amdgcn_raw_buffer_load_b128(t0, off, at0, 0);
+                raw[4 + i] = __builtin_amdgcn_raw_buffer_load_b128(t1, off, at0 + (takes_keys && D == 128 ? 2 * D : 0), 0);
             }
         } else {
             const __amdgpu_buffer_rsrc_t s0 = scales16.descriptor(ia), s1 = scales16.descriptor(ib);
@@ -804,14 +812,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
                 u32x4 hi, lo;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
+                    const f32x4 y = x[kQ8 || D == 64 ? 2 * p + e / 2 : p + 4 * (e / 2)];
                     unsigned h1, l1;
-                    split2(x[2 * p + e / 2][2 * (e % 2)], x[2 * p + e / 2][2 * (e % 2) + 1], h1, l1);
+                    split2(y[2 * (e % 2)], y[2 * (e % 2) + 1], h1, l1);
                     hi[e] = h1;
                     lo[e] = l1;
                 }
-                const int o = D == 128 ? mt0 * KC + p : p;  // [mt][kc]
-                parts[buf][sub][2 * o][lane] = hi;
-                parts[buf][sub][2 * o + 1][lane] = lo;
+                u32x4* to;
+                if constexpr (kQ8) {
+                    const int o = D == 128 ? mt0 * KC + p : p;  // [mt][kc]
+                    to = &parts[buf][sub][2 * o][lane];
+                } else {
+                    const int part = lane % X, row = 64 / X * (D == 128 ? p : p % 2) + lane / X, mt = D == 128 ? mt0 : p / 2;
+                    to = &parts[buf][sub][2 * (mt * KC + part / 4)][16 * (part % 4) + swizzle(row, part)];
+                }
+                to[0] = hi;
+                to[64] = lo;
             }
         } else {
             const bool tail = step >= csteps;
@@ -897,15 +913,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
     };
     // (operands are read from LDS one ahead of their products)
     auto scores = [&](int buf, int t) __attribute__((always_inline)) {
-        const u32x4* op = operands(buf, t);
-        u32x4 hi = op[0], lo = op[64];
+        unsigned base = static_cast<unsigned>((buf * S + t) * OPS * 64 + 16 * g + swizzle(r16, g));
+        asm("" : "+v"(base));
+        auto operand = [&](int o) __attribute__((always_inline)) {  // (swizzle(r16, 4 kc + g): an exclusive or by 4 kc more)
+            return &parts[0][0][0][0] + (kQ8 ? base : base ^ (16 / X * 4 * (o % KC))) + 128 * o;
+        };
+        u32x4 hi = operand(0)[0], lo = operand(0)[64];
 #pragma unroll
         for (int o = 0; o < 2 * KC; ++o) {
             const int mt = o / KC, kc = o % KC;
             const f16x8 kh8 = __builtin_bit_cast(f16x8, hi), kl8 = __builtin_bit_cast(f16x8, lo);
             if (o + 1 < 2 * KC) {
-                hi = op[64 * (2 * o + 2)];
-                lo = op[64 * (2 * o + 3)];
+                hi = operand(o + 1)[0];
+                lo = operand(o + 1)[64];
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
