@@ -30,7 +30,8 @@ __device__ __forceinline__ float cached_element(const TreeArgs& a, int block, in
 // Any head_dim and block size, f32 arithmetic: a wave per (run of a node's
 // cached tokens, query head); lanes are keys for the scores and columns for the
 // output.  A work item is x: tree, y: node, z: run, w: runs; the last run takes
-// the tree's nodes.
+// the tree's nodes.  For the layouts that the matrix cores' tiles do not take; bound
+// by loads of single elements, every row for itself.
 __global__ __launch_bounds__(64) void tree_rows_kernel(const TreeArgs a) {
     __shared__ float qs[kMaxDim];
     const int lane = threadIdx.x, h = blockIdx.y, kh = h / a.group;
@@ -112,8 +113,8 @@ __global__ __launch_bounds__(64) void tree_rows_kernel(const TreeArgs a) {
 
 // A row's runs combined in order: a thread per four columns (two where head_dim is
 // no multiple of four), with the loads of four runs in flight.  Bound: the memory
-// behind the L2s, which the partials come from.  Four contexts of 20,000 to 32,768
-// tokens (84 rows of 32 heads of 128, 16 runs): 8.7 us, 2.7 TB/s; one run at a time
+// behind the L2s, which the partials come from.  Four contexts of 21,268 to 24,966
+// tokens (86 nodes, 32 heads of 128, 16 runs): 8.7 us, 2.7 TB/s; one run at a time
 // and two columns a thread took 15.0.
 template <int kVec>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {

@@ -7,7 +7,8 @@
 // in parts of a workgroup each, and a workgroup then walks a tree.  Bound: one read
 // of the logits.  A launch of few parts ends with the walk in the last workgroup of
 // a tree (one launch); larger ones take a second launch, since the last arriver's
-// release writes its XCD's L2 back, one workgroup after the other.
+// release writes its XCD's L2 back, one workgroup after the other.  MI355X, 32 trees
+// (503 nodes) over 128,256 tokens: 45.4 us, 5.7 TB/s, of which the walk is 4.6.
 #include <algorithm>
 
 #include "common.hpp"
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(kThreads) void tree_walk_kernel(const AcceptArgs a)
 
 // About kAcceptParts parts in all, of 1,024 logits or more and a multiple of them;
 // of at most kFusedParts where they are 32 KiB each at most (MI355X, one tree of
-// eight over 32,000: two launches 8.2 us, one in few parts 6.0).
+// eight over 32,000: two launches 8.25 us, one in few parts 7.34).
 void tree_accept_parts(AcceptArgs& a) {
     const size_t rows = std::max(a.rows, 1), all = rows * a.vocab;
     auto part = [&](size_t parts) { return std::max<size_t>(1, (all / parts + 1023) / 1024) * 1024; };
