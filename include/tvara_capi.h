@@ -128,7 +128,7 @@ TVARA_API int tvara_sequence_truncate(tvara_model* model, uint64_t sequence, siz
 TVARA_API int tvara_sequences_decode(tvara_model* model, const uint64_t* sequences, const uint32_t* tokens,
                                      size_t count, float* logits, size_t logits_count);
 
-/* One step of speculative decoding for `count` distinct sequences: every node of
+/* One step of speculative decoding for up to 65,535 distinct sequences: every node of
  * every tree of drafted tokens passes through the model at once, and the nodes that
  * greedy decoding would have taken are appended.  Tree i has nodes[i] (up to 1,024)
  * of the packed tokens; parents[] numbers them within their tree, a parent before

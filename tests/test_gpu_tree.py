@@ -575,6 +575,10 @@ def test_reserve(device):
         cache.reserve([a, b], [3, 40])
     with pytest.raises(_capi.CacheExhausted):
         cache.reserve([a, b], [3, 17])
+    with pytest.raises(_capi.CacheExhausted):  # each within the pool, together far beyond any memory
+        cache.reserve([a] * 100000, [32] * 100000)
+    with pytest.raises(_capi.CacheExhausted):
+        cache.reserve([a, b], [1, (1 << 64) - 1])
     after = cache.state()
     assert {s: t[0] for s, t in after["tables"].items()} == {s: t[0] for s, t in before["tables"].items()}
     cache.audit()

@@ -194,6 +194,49 @@ def test_fork_copies_on_write(tmp_path):
     assert close(model.logits(f, 9), plain.logits)
 
 
+def test_fork_and_its_origin_in_one_call(tmp_path):
+    spec = gf.LlamaSpec(matrix_type=gf.T_Q8_0, heads=8, kv_heads=2, hidden=128, intermediate=256)
+    model = native.NativeModel(spec.write(tmp_path / "m.gguf"), max_blocks=64, block_tokens=4)
+    prompt = [int(t) for t in np.random.default_rng(6).integers(0, spec.vocab, 9)]
+    plain = Greedy(model, prompt)
+    a = model.new_sequence()
+    first = choice(model.prefill(a, prompt))[0]
+    cache = model.cache()
+    f = cache.fork(a)
+    right = plain.choices(4)
+    assert len(right) > 2
+    chain = list(range(-1, len(right) - 1))
+    paths, after = model.verify_trees([a, f], [chain[:2], chain], [right[:2], right], [first, first])
+    assert paths == [[0, 1], list(range(len(right)))] and after[0] == right[2]
+    other = Greedy(model, prompt)
+    other.take(right[:2] + [5])
+    plain.take(right + [7])
+    got = model.decode_sequences([a, f], [5, 7])
+    assert close(got[0], other.logits) and close(got[1], plain.logits)
+    cache.audit()
+
+
+@pytest.mark.parametrize("nodes,vocab", [(1024, 300), (70, 34001)])
+def test_large_trees(tmp_path, nodes, vocab):
+    """The most nodes of a tree; logits that are computed in bands."""
+    say("verify large trees", nodes, vocab)
+    spec = gf.LlamaSpec(matrix_type=gf.T_Q8_0, embed_type=gf.T_Q8_0, output=False, hidden=256, intermediate=512, heads=4,
+                        kv_heads=2, vocab=vocab, context=256)
+    model = native.NativeModel(spec.write(tmp_path / "m.gguf"), max_blocks=64, block_tokens=16)
+    rng = np.random.default_rng(nodes)
+    prompt = [int(t) for t in rng.integers(0, vocab, 40)]
+    g = Greedy(model, prompt)
+    seq = model.new_sequence()
+    first = choice(model.prefill(seq, prompt))[0]
+    ahead = g.choices(9)
+    right = ahead[:-1]
+    parents, tokens, want = drafted(rng, right, nodes - len(right), vocab)
+    (path,), (after,) = model.verify_trees([seq], [parents], [tokens], [first])
+    assert path == want and after == ahead[-1] and len(want) > 3
+    g.take(right + [1])
+    assert close(model.logits(seq, 1), g.logits)
+
+
 def message(fn, *args):
     with pytest.raises((RuntimeError, ValueError)) as e:
         fn(*args)

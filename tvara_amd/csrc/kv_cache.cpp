@@ -238,11 +238,12 @@ void DeviceCache::reserve(const uint64_t* seqs, size_t n, const size_t* tokens) 
     if (n && (!seqs || !tokens)) throw std::invalid_argument("invalid KV reservation");
     std::vector<uint64_t> list;
     std::vector<size_t> lengths(n);
-    const Geometry& g = geometry();
+    // (more than the pool holds: refused before a list of that size is made)
+    size_t room = geometry().max_blocks * geometry().tokens_per_block;
     for (size_t i = 0; i < n; ++i) {
         lengths[i] = sequence(seqs[i]).length;
-        // (more than the pool holds: refused before a list of that size is made)
-        if (tokens[i] > g.max_blocks * g.tokens_per_block) throw CacheExhausted();
+        if (tokens[i] > room) throw CacheExhausted();
+        room -= tokens[i];
         list.insert(list.end(), tokens[i], seqs[i]);
     }
     AppendWork w = meta_.plan_appends(list.data(), list.size());

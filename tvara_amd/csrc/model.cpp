@@ -368,6 +368,8 @@ void DeviceModel::verify_trees(const uint64_t* sequences, size_t n, const size_t
                                const uint32_t* tokens, const uint32_t* first, int32_t* path, size_t* accepted,
                                uint32_t* next) {
     if (!n) return;
+    cache_->check_device();
+    if (n > 65535) throw std::invalid_argument("decode batch too large");  // (a slot plan's)
     const ModelConfig& c = cfg_;
     {
         std::vector<uint64_t> sorted(sequences, sequences + n);
