@@ -146,6 +146,8 @@ void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t
         row_work(trees, work, runs);
     if (slots > kIntMax / h || work.size() > 3 * kMaxWorkgroups) throw std::invalid_argument("attention batch too large");
     items = static_cast<int>(tiles.rows ? work.size() / 3 : work.size());
+    most_runs = 1;
+    for (const int2& r : runs) most_runs = std::max(most_runs, r.y);
 
     // acceptance's: each row's tree, and counters that start at zero
     std::vector<int32_t> tree_of(rows), zeros(n, 0);
@@ -296,7 +298,7 @@ void TreePlan::launch(int layer, const float* q, const float* keys, const float*
         launch_tree_tiles(a, tiles.rows, items, precision == 2, s);
     else
         launch_tree_rows(a, items, s);
-    if (slots) launch_tree_merge(a, s);
+    if (slots) launch_tree_merge(a, most_runs, s);
     cache->leave(s);
     region.launched(s);
 }

@@ -3,6 +3,8 @@
 //   o = sum_k p_k v_k,  p = softmax_k(q . k / sqrt(d)),
 // with the nodes' K/V in rows of their own, outside the cache (they join it only
 // when they are accepted).
+#include <algorithm>
+
 #include "common.hpp"
 #include "device_util.hpp"
 #include "q8.hpp"
@@ -12,6 +14,11 @@ namespace tvara_amd {
 namespace {
 
 constexpr int kMaxDim = 512;
+// Groups of a row's runs where the rows alone leave CUs idle.  MI355X, one context of
+// 32,400 tokens with 5 nodes (10 workgroups, 64 runs): the whole call 32.1 us without
+// and 22.1 with; 86 nodes of 32 heads of 128 (344 workgroups, 16 runs): 8.5 and 9.0.
+constexpr int kMergeGroups = 8;
+constexpr size_t kMergeFew = 256;
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -111,41 +118,54 @@ __global__ __launch_bounds__(64) void tree_rows_kernel(const TreeArgs a) {
     if (!whole && lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(m, l);
 }
 
-// A row's runs combined in order: a thread per four columns (two where head_dim is
-// no multiple of four), with the loads of four runs in flight.  Bound: the memory
-// behind the L2s, which the partials come from.  Four contexts of 21,268 to 24,966
-// tokens (86 nodes, 32 heads of 128, 16 runs): 8.7 us, 2.7 TB/s; one run at a time
-// and two columns a thread took 15.0.
-template <int kVec>
-__global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
+// A row's runs combined: a thread per four columns (two where head_dim is no
+// multiple of four) and per `groups` runs, the loads of four of its runs in flight;
+// the groups meet in LDS, in order.  Bound: the memory behind the L2s, which the
+// partials come from (86 nodes of 32 heads of 128, 16 runs: 8.5 us, 2.8 TB/s; 512
+// nodes, 4 runs: 9.1 us, 4.6 TB/s).
+template <int kVec, bool kGroups>
+__global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a, int groups) {
     typedef float vec __attribute__((ext_vector_type(kVec)));
-    const int D = a.lay.head_dim, parts = D / kVec;
-    const size_t t = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x, at = t / parts;
-    if (at >= static_cast<size_t>(a.rows) * a.heads) return;
-    const int2 runs = a.runs[at / a.heads];
-    if (runs.y == 1) return;
-    const int c = kVec * static_cast<int>(t % parts), h = static_cast<int>(at % a.heads);
+    __shared__ float2 stats[kGroups ? 256 : 1];
+    __shared__ vec sums[kGroups ? 256 : 1];
+    const int D = a.lay.head_dim, parts = D / kVec, unit = parts * groups, each = 256 / unit;
+    const int tid = threadIdx.x, mine = tid / unit, group = tid % unit / parts;
+    const size_t at = static_cast<size_t>(blockIdx.x) * each + mine;
+    const bool in = mine < each && at < static_cast<size_t>(a.rows) * a.heads;
+    const int2 runs = in ? a.runs[at / a.heads] : make_int2(0, 1);
+    const int c = kVec * (tid % parts), h = static_cast<int>(at % a.heads);
     constexpr int kTogether = 4;
     float m = -INFINITY, l = 0.f;
     vec sum = 0.f;
-    for (int r0 = 0; r0 < runs.y; r0 += kTogether) {
-        float2 ml[kTogether];
-        vec x[kTogether];
+    auto add = [&](float2 ml, vec x) __attribute__((always_inline)) {
+        if (ml.x == -INFINITY) return;
+        const float mn = fmaxf(m, ml.x), wm = fast_exp2(m - mn), wr = fast_exp2(ml.x - mn);
+        l = l * wm + ml.y * wr;
+        sum = sum * wm + x * wr;
+        m = mn;
+    };
+    if (runs.y > 1)
+        for (int r0 = group; r0 < runs.y; r0 += kTogether * groups) {
+            float2 ml[kTogether];
+            vec x[kTogether];
 #pragma unroll
-        for (int r = 0; r < kTogether; ++r) {
-            const size_t p = (static_cast<size_t>(runs.x) + min(r0 + r, runs.y - 1)) * a.heads + h;
-            ml[r] = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
-            x[r] = *reinterpret_cast<const vec*>(a.part_acc + p * D + c);
-        }
+            for (int r = 0; r < kTogether; ++r) {
+                const size_t p = (static_cast<size_t>(runs.x) + min(r0 + r * groups, runs.y - 1)) * a.heads + h;
+                ml[r] = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
+                x[r] = *reinterpret_cast<const vec*>(a.part_acc + p * D + c);
+            }
 #pragma unroll
-        for (int r = 0; r < kTogether; ++r) {
-            if (r0 + r >= runs.y || ml[r].x == -INFINITY) continue;
-            const float mn = fmaxf(m, ml[r].x), wm = fast_exp2(m - mn), wr = fast_exp2(ml[r].x - mn);
-            l = l * wm + ml[r].y * wr;
-            sum = sum * wm + x[r] * wr;
-            m = mn;
+            for (int r = 0; r < kTogether; ++r)
+                if (r0 + r * groups < runs.y) add(ml[r], x[r]);
         }
+    if constexpr (kGroups) {
+        stats[tid] = make_float2(m, l);
+        sums[tid] = sum;
+        __syncthreads();
+        if (group || !in) return;
+        for (int g = 1; g < groups; ++g) add(stats[tid + g * parts], sums[tid + g * parts]);
     }
+    if (runs.y == 1) return;  // (written by the attention itself, or no row)
     const vec o = sum / l;
     bool finite = true;
 #pragma unroll
@@ -162,11 +182,21 @@ void launch_tree_rows(const TreeArgs& a, int items, hipStream_t s) {
     TVARA_HIP(hipGetLastError());
 }
 
-void launch_tree_merge(const TreeArgs& a, hipStream_t s) {
-    const int vec = a.lay.head_dim % 4 ? 2 : 4;
-    const size_t threads = static_cast<size_t>(a.rows) * a.heads * (a.lay.head_dim / vec);
-    launch("tree_attention_merge", vec == 4 ? tree_merge_kernel<4> : tree_merge_kernel<2>,
-           dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, s, a);
+void launch_tree_merge(const TreeArgs& a, int most_runs, hipStream_t s) {
+    const int vec = a.lay.head_dim % 4 ? 2 : 4, parts = a.lay.head_dim / vec;
+    auto workgroups = [&](int groups) {
+        const size_t each = 256 / (parts * groups);
+        return (static_cast<size_t>(a.rows) * a.heads + each - 1) / each;
+    };
+    const int groups = workgroups(1) < kMergeFew ? std::max(1, std::min({(most_runs + 3) / 4, 256 / parts, kMergeGroups})) : 1;
+    const size_t blocks = workgroups(groups);
+    auto go = [&](auto kernel) {
+        launch("tree_attention_merge", kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, groups);
+    };
+    if (vec == 4)
+        groups > 1 ? go(tree_merge_kernel<4, true>) : go(tree_merge_kernel<4, false>);
+    else
+        groups > 1 ? go(tree_merge_kernel<2, true>) : go(tree_merge_kernel<2, false>);
     TVARA_HIP(hipGetLastError());
 }
 

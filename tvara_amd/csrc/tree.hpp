@@ -97,7 +97,7 @@ struct WriteArgs {
 
 // tree.hip
 void launch_tree_rows(const TreeArgs& a, int items, hipStream_t s);
-void launch_tree_merge(const TreeArgs& a, hipStream_t s);
+void launch_tree_merge(const TreeArgs& a, int most_runs, hipStream_t s);
 // tree_tiles.hip: head_dim 64 and 128.  Work has three entries a workgroup: the tree
 // (as trees); KV head, first row, first step, end; run, runs, the tree's first partial.
 bool tree_tiles_supported(const BlockLayout& lay);
@@ -163,6 +163,7 @@ struct TreePlan {
     uint64_t epoch = 0;
     int heads = 0, group = 0, precision = 0, words = 1, items = 0, split_tokens = 0;
     TreeTileShape tiles{};  // rows 0: the row kernel
+    int most_runs = 1;
     size_t count = 0, rows = 0, slots = 0;
     PlanRegion region;
     size_t tables_at = 0, trees_at = 0, mask_at = 0, work_at = 0, runs_at = 0, parents_at = 0, acc_at = 0, ml_at = 0,
