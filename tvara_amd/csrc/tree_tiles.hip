@@ -69,6 +69,20 @@ struct Spans {
 // ahead too (they return in order).
 __device__ __forceinline__ void wait_for_loads() { __builtin_amdgcn_s_waitcnt(0); }
 
+// Until at most n loads are on their way (they return in order), or every read of LDS
+// is done; no access to memory moves across either.
+template <int n>
+__device__ __forceinline__ void wait_until_left() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((n & 15) | n >> 4 << 14 | 0xf70);
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_lds() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    asm volatile("" ::: "memory");
+}
+
 // Two values as hi + lo in fp16, each rounded to nearest (22 bits; beyond fp16's
 // range one is infinite and the other its opposite).  `one` is 1, hidden from the
 // compiler, so that x - hi stays a mixed-precision fma: four instructions a pair
@@ -112,17 +126,20 @@ __device__ __forceinline__ Item item_of(const TreeArgs& a) {
 }
 
 template <int D, int NT, bool kQ8, bool kX3>
-__global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel(const TreeArgs a) {
+__global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_tile_kernel(const TreeArgs a) {
     constexpr int WK = kWaves, C = D / 16, KC = D / 32, H = D / 64;
     constexpr int W = D / 4;  // 16-byte parts of a row
-    __shared__ f32x4 sums[WK][4][NT][64];
     // f32 keys come as whole rows, W lanes each, and turn into operands (16 lanes, 16
     // rows) by way of LDS: read from memory as operands they take four times as long
-    // to come through the CU's cache (16 contexts of 2048, 32 heads on 8: f32 and
-    // head_dim 64, 64 rows 63.7 -> 56.9 us; f32x3 and head_dim 128 65.8 -> 61.5 us).
-    // The one wave a SIMD of f32 and head_dim 128 waits for LDS instead (100 -> 114 us).
-    constexpr bool kStaged = !kQ8 && (D == 64 || kX3);
-    __shared__ f32x4 staged[kStaged ? WK : 1][kStaged ? kStep * W : 1];  // a wave's keys of a step
+    // to come through the CU's cache.  They go there without passing registers, so
+    // that 128 columns leave room for two waves a SIMD (16 contexts of 2048, 32 heads on
+    // 8: f32 and head_dim 64, 64 rows 63.7 us as operands, 56.9 by way of registers and
+    // LDS, 55.0 so; head_dim 128, 32 rows 63, 73, 58.7; f32x3 and head_dim 128, 64 rows
+    // 65.8, 60.6, 58.7).
+    constexpr bool kStaged = !kQ8;
+    // a wave's keys of a step; at the end its results, for the others
+    __shared__ f32x4 staged[WK][kStaged ? kStep * W : 4 * NT * 64];
+    auto result = [&](int w, int i, int nt) -> f32x4& { return staged[w][(i * NT + nt) * 64 + static_cast<int>(threadIdx.x & 63)]; };
     __shared__ float2 stats[WK][16 * NT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, r16 = lane & 15, wk = wave;
@@ -154,7 +171,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                               : (static_cast<size_t>(a.layer) * 2 * tpb * kvw + static_cast<size_t>(kh) * D) * sizeof(float);
     const size_t vsec = kQ8 ? a.lay.section : static_cast<size_t>(tpb) * kvw * sizeof(float);
     const int rowb = kQ8 ? D : kvw * static_cast<int>(sizeof(float));  // from one slot to the next
-    const unsigned koff = static_cast<unsigned>(kStaged ? lane / W * rowb + lane % W * 16 : r16 * rowb + kcol(0) * (kQ8 ? 1 : 4));
+    const unsigned koff = static_cast<unsigned>(kStaged ? lane / W * rowb + (lane % W ^ lane / W) * 16 : r16 * rowb + kcol(0));
     const unsigned voff = static_cast<unsigned>(4 * g * rowb + vcol(0, r16) * (kQ8 ? 1 : 4));
     int step = it.step + wk;
     const int last = max(cached - 1, 0) >> 4;  // 16 keys a table lookup; past the end the last again
@@ -168,8 +185,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
     };
     // A workgroup's start is a chain of waits for memory: table, then keys.  With
     // head_dim 64 the first keys are asked for before the queries are waited for (16
-    // ragged contexts 50.2 -> 48.3 us); with 128 the registers do not reach for it (f32,
-    // 64 rows 100 -> 102 us, in blocks of 16 115 -> 137).
+    // ragged contexts 50.2 -> 48.3 us).
     f32x4 qf[NT][C];
     auto load_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -183,7 +199,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
         }
     };
     // f32 rows, or Q8_0 bytes and scales, which become values where they are used
-    f32x4 k[kQ8 ? 1 : 2][C], v[kQ8 ? 1 : 2][4][H];
+    f32x4 v[kQ8 ? 1 : 2][4][H];
     u32x4 kw[kQ8 ? 2 : 1][H];
     unsigned kd[kQ8 ? 2 : 1][H], vw[kQ8 ? 2 : 1][4][H], vd[kQ8 ? 2 : 1][4];
     auto scales = [&](const char* b, int mt, int stp) {  // of the block's rows from the tile's first on
@@ -202,21 +218,16 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
                     kd[mt][u] = *reinterpret_cast<const uint16_t*>(sc + (r16 * (D / 32) + 2 * u + (g >> 1)) * 2);
                 }
             } else {
+                // straight into LDS, lane after lane; what a lane loads is permuted by its
+                // row, so that the operands' reads meet no bank twice
+                const __amdgpu_buffer_rsrc_t rows =
+                    __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(b), 0, 15 * rowb + 4 * D, kBufferWord3);
 #pragma unroll
                 for (int c = 0; c < C; ++c)
-                    k[mt][c] = *reinterpret_cast<const f32x4*>(b + (kStaged ? static_cast<size_t>(64 / W * c) * rowb : 64 * c) + koff);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (__attribute__((address_space(3))) void*)&staged[wave][(mt * C + c) * 64],
+                                                             16, koff ^ 1024 / W * c, 64 / W * c * rowb, 0, 0);
             }
         }
-    };
-    // (parts of a row are permuted by its number, so that neither side meets a bank twice)
-    auto stage_k = [&]() __attribute__((always_inline)) {
-#pragma unroll
-        for (int n = 0; n < 2 * C; ++n) {
-            const int row = 64 / W * n + lane / W;
-            staged[wave][row * W + (lane % W ^ (row & 15))] = k[n / C][n % C];
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
     };
     auto staged_k = [&](int mt, int c) __attribute__((always_inline)) {
         return staged[wave][(16 * mt + r16) * W + ((4 * c + g) ^ r16)];
@@ -246,6 +257,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
     load_q();
     if (kEarly && step < end) {
         load_k(step);
+        if constexpr (kStaged) asm volatile("" ::: "memory");
         load_v(step);
     }
     u32x4 qh[kX3 ? NT : 1][kX3 ? KC : 1], ql[kX3 ? NT : 1][kX3 ? KC : 1];
@@ -446,8 +458,6 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
         auto cached_scores = [&]() __attribute__((always_inline)) {
             if constexpr (kStaged)
                 scores(from_f32(staged_k));
-            else if constexpr (!kQ8)
-                scores(from_f32([&](int mt, int c) __attribute__((always_inline)) { return k[mt][c]; }));
             else if constexpr (kX3)
                 scores([&](int mt, int kc, u32x4& hi, u32x4& lo) __attribute__((always_inline)) {
                     const unsigned one = kd[mt][kc / 2];
@@ -493,27 +503,23 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
         };
         if constexpr (!kEarly) {
             load_k(step);
+            if constexpr (kStaged) asm volatile("" ::: "memory");
             load_v(step);
         }
         for (; step < end; step += WK) {
             const int next = step + WK;
-            if constexpr (kStaged)
-                stage_k();
-            else
-                cached_scores();
-            // the loads of the next step go out as soon as a register is free (past
-            // the end the last step's again: its blocks are there)
+            if constexpr (kStaged) wait_until_left<8 * H>();  // the values'
+            cached_scores();
+            if constexpr (kStaged) wait_for_lds();
+            // the loads of the next step go out as soon as there is room (past the end the
+            // last step's again: its blocks are there)
             if (++at == 32) {
                 at = 0;
                 ids = more;
                 more = lookup(next + 32 * WK);
             }
             load_k(next);
-            if constexpr (kStaged) {
-                cached_scores();
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-            }
+            if constexpr (kStaged) asm volatile("" ::: "memory");
             if (kStep * step + kStep <= cached) {
                 softmax(std::false_type{}, [](int, int, int) { return true; });
             } else {  // the last keys: what lies behind them is not seen, and its values are zeros
@@ -535,6 +541,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
             cached_output();
             load_v(next);
         }
+        if constexpr (kStaged) wait_until_left<0>();  // (LDS is used again)
     }
 
     // ---- the tree's own nodes
@@ -641,15 +648,14 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void tree_tile_kernel
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-                sums[wave][i][nt][lane] =
-                    f32x4{acc[4 * h][nt][i], acc[4 * h + 1][nt][i], acc[4 * h + 2][nt][i], acc[4 * h + 3][nt][i]};
+                result(wave, i, nt) = f32x4{acc[4 * h][nt][i], acc[4 * h + 1][nt][i], acc[4 * h + 2][nt][i], acc[4 * h + 3][nt][i]};
         __syncthreads();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int i = wave;
-            f32x4 x = sums[0][i][nt][lane];
+            f32x4 x = result(0, i, nt);
 #pragma unroll
-            for (int w = 1; w < WK; ++w) x += sums[w][i][nt][lane];
+            for (int w = 1; w < WK; ++w) x += result(w, i, nt);
             if (!live[nt]) continue;
             const size_t row = static_cast<size_t>(tree.w) + node[nt];
             if (it.runs == 1) {
@@ -1143,8 +1149,6 @@ void launch_shape(const TreeArgs& a, int rows, int workgroups, hipStream_t s) {
         go(tree_tile_kernel<D, 1, kQ8, kX3>);
     else if constexpr (kX3)
         rows == 32 ? go(tree_tile_kernel<D, 2, kQ8, kX3>) : go(tree_shared_kernel<D, kQ8>);
-    else if constexpr (D == 128)
-        go(tree_tile_kernel<D, 2, kQ8, kX3>);
     else
         throw std::logic_error("no f32 tree kernel for these rows");
 }
@@ -1157,25 +1161,27 @@ bool tree_tiles_supported(const BlockLayout& lay) {
 }
 
 // 16 contexts of 2048 tokens, 32 query and 8 KV heads, microseconds with each block:
-//   f32x3, head_dim 128:  16 rows  16: 53.0  32: 55.3;  32 rows  16: 56.6  32: 57.9
-//                         64 rows  32: 60.6  128: 72.5;  80 rows  32: 113  128: 79.2
+//   f32x3, head_dim 128:  16 rows  16: 51.6  32: 55.3;  32 rows  16: 55.6  32: 57.9
+//                         64 rows  32: 58.7  128: 72.5;  80 rows  32: 113  128: 79.2
 //     Q8_0                16 rows  16: 25.3  32: 31.3;  32 rows  16: 35.3  32: 33.9
 //                         64 rows  32: 49.3  128: 64.0;  80 rows  32: 90.3  128: 70.1
 //   f32x3, head_dim 64:   64 rows  32: 40.5  128: 48.6;  80 rows  32: 58.5  128: 49.9
-//   f32, head_dim 64:     16 rows  16: 33.8  32: 41.3;   64 rows  16: 56.9  32: 64.5
-//   f32, head_dim 128:    16 rows  16: 53.3  32: 60.0;   32 rows  16: 65.2  32: 62.7
-//                         64 rows  16: 116  32: 100
-// Two workgroups share a CU where 256 registers hold a wave, or LDS a workgroup's keys.
+//   f32, head_dim 64:     16 rows  16: 33.8  32: 41.3;   64 rows  16: 54.8  32: 64.5
+//   f32, head_dim 128:    32 rows  16: 58.7  32: 65.6;   96 rows  16: 150   32: 186
+// Workgroups that a CU is dealt: what its registers (f32x3 of 128 columns one, of 64
+// two) or LDS (128 rows: two) hold.  f32 holds more than pay for their merges: of 64
+// columns (four) three (ragged contexts 2: 47.1  3: 45.4  4: 46.9), of 128 (two) over
+// f32 blocks one (32 rows 1: 58.7  2: 67.0), over Q8_0 two (1: 70.0  2: 63.2).
 // A run has at least a step a wave, and no more where there are CUs: a wave's second
 // step waits for memory again (one context of 512 tokens in runs of 4 steps: 12.7,
 // of 8: 14.0, of 12: 15.3, each with its merge).
 TreeTileShape tree_tile_shape(const BlockLayout& lay, size_t most, bool x3) {
     TreeTileShape t{};
+    t.rows = !x3 || most <= 16 ? 16 : most <= 64 ? 32 : 128;
     if (x3)
-        t.rows = most <= 16 ? 16 : most <= 64 ? 32 : 128;
+        t.units = t.rows == 128 || lay.head_dim == 64 ? 2 : 1;
     else
-        t.rows = most <= 16 || lay.head_dim == 64 ? 16 : 32;
-    t.units = t.rows == 128 || lay.head_dim == 64 ? 2 : 1;
+        t.units = lay.head_dim == 64 ? 3 : lay.format == kQ8 ? 2 : 1;
     t.least = kWaves;
     return t;
 }
