@@ -15,6 +15,9 @@ constexpr size_t kIntMax = static_cast<size_t>(std::numeric_limits<int32_t>::max
 // of a launch: 2^32 threads, here in workgroups of up to 256
 constexpr size_t kMaxThreads = std::numeric_limits<uint32_t>::max(), kMaxWorkgroups = kMaxThreads / 256;
 
+// steps from which on a run is a long one, and those that its start and merge are worth
+constexpr size_t kLongRun = 64, kRunStart = 5;
+
 size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 }  // namespace
 
@@ -208,17 +211,33 @@ void TreePlan::tile_work(const std::vector<int4>& trees, std::vector<int4>& work
         for (int r0 = 0; r0 < t.z * group; r0 += tiles.rows)
             total += static_cast<size_t>(kv_heads) * (cached_steps(t) + own_steps(t, r0));
     // Steps of a run: an even share, or up to twice that if the chip then holds all
-    // workgroups at once: a second round for a few of them costs more.
-    const size_t units = static_cast<size_t>(cache->compute_units()) * tiles.units;
-    const size_t even = std::max<size_t>(tiles.least, (total + units - 1) / units);
-    size_t per = even;
-    for (size_t p = even; p <= 2 * even; p += (even + 15) / 16) {
-        size_t workgroups = 0;
-        for (const int4& t : trees)
-            if (t.z) workgroups += ((steps_of(t) + p - 1) / p) * ((t.z * group - 1) / tiles.rows + 1) * kv_heads;
-        if (workgroups <= units) {
+    // workgroups at once.  Where the share is long, the length with the least rounds of
+    // workgroups * their mean steps: a second round for a few of them costs a share
+    // (MI355X, f32, head_dim 128: six trees of 23 nodes after 6,263 tokens in 288
+    // workgroups for 256 places 240 us, cut so 179); short ones would pay more for the
+    // launch of a merge (62 trees of 7 nodes after 191: 20.2 us, cut so 26.9).
+    const size_t units = static_cast<size_t>(cache->compute_units()) * tiles.units, least = tiles.least;
+    const size_t even = std::max(least, (total + units - 1) / units);
+    const bool lengthy = even >= kLongRun;
+    size_t per = even, best = std::numeric_limits<size_t>::max();
+    for (size_t p = lengthy ? even / 6 : even; p <= 2 * even; p += (p + 15) / 16) {
+        size_t workgroups = 0, longest = 0;
+        for (const int4& t : trees) {
+            if (!t.z) continue;
+            const size_t steps = steps_of(t), parts = (steps + p - 1) / p;
+            workgroups += parts * ((t.z * group - 1) / tiles.rows + 1) * kv_heads;
+            longest = std::max(longest, (steps + parts - 1) / parts);
+        }
+        if (!lengthy) {
+            if (workgroups > units) continue;
             per = p;
             break;
+        }
+        const size_t rounds = (workgroups + units - 1) / units;
+        const size_t end = std::max((longest + kRunStart) * units, rounds * (total * units / workgroups + kRunStart * units));
+        if (end < best) {
+            best = end;
+            per = p;
         }
     }
     struct Group {  // the row blocks of a run
