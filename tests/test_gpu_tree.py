@@ -283,7 +283,7 @@ def test_plan_strides_and_layers(device, oracle, dim, tpb, precision):
             plan.launch(0, d.q.ptr, d.k.ptr, d.v.ptr, d.out.ptr)
 
 
-@pytest.mark.parametrize("nodes", [3, 12, 40])  # 16, 32 and 128 rows a workgroup
+@pytest.mark.parametrize("nodes", [3, 12, 40])
 @pytest.mark.parametrize("where", ["q", "cached keys", "cached values", "keys", "values"])
 @pytest.mark.parametrize("q8", [False, True])
 def test_beyond_fp16_is_reported(device, oracle, where, nodes, q8):
@@ -344,6 +344,65 @@ def test_chain_is_the_prompt_chunk(device, oracle):
     b.cache.append_many(b.seqs[0], b.tk, b.tv)
     chunk = attention.prefill_batch(b.cache, b.q, b.seqs, [100], [12], 0, 8, 1 << 20)
     assert refmath.close(got, chunk, BAR)
+
+
+@pytest.mark.parametrize("rows", ["16", "32", "128"])
+class TestRowBlocks:
+    """Each number of rows that a workgroup of f32x3 may have, whatever the batch."""
+
+    @pytest.fixture(autouse=True)
+    def choose(self, monkeypatch, rows):
+        monkeypatch.setenv("TVARA_TREE_ROWS", rows)
+
+    @pytest.mark.parametrize("fmt", ["f32", "q8_0"])
+    @pytest.mark.parametrize("dim", [64, 128])
+    @pytest.mark.parametrize("group", [1, 3, 4, 8])
+    def test_groups(self, device, oracle, rows, group, dim, fmt):
+        test_groups(device, oracle, group, dim, fmt, "f32x3")
+
+    @pytest.mark.parametrize("fmt", ["f32", "q8_0"])
+    @pytest.mark.parametrize("length", [0, 1, 16, 31, 32, 33, 300])
+    def test_lengths(self, device, oracle, rows, length, fmt):
+        test_lengths(device, oracle, length, fmt, "f32x3")
+
+    @pytest.mark.parametrize("dim", [64, 128])
+    @pytest.mark.parametrize("nodes", [1, 8, 31, 33, 65, 200])
+    def test_tree_sizes(self, device, oracle, rows, nodes, dim):
+        test_tree_sizes(device, oracle, nodes, dim, "f32x3")
+
+    @pytest.mark.parametrize("fmt", ["f32", "q8_0"])
+    @pytest.mark.parametrize("dim,tpb", [(64, 32), (128, 16), (128, 128), (64, 2048)])
+    def test_layouts(self, device, oracle, rows, dim, tpb, fmt):
+        test_layouts(device, oracle, dim, tpb, fmt, "f32x3")
+
+    @pytest.mark.parametrize("dim", [64, 128])
+    def test_long_contexts_strides_and_visible(self, device, oracle, rows, dim):
+        test_long_contexts(device, oracle, dim, "f32", "f32x3")
+        test_long_contexts(device, oracle, dim, "q8_0", "f32x3")
+        test_plan_strides_and_layers(device, oracle, dim, 16, "f32x3")
+        test_visible(device, oracle, dim, "f32x3")
+        test_sharp_scores(device, oracle, "f32x3")
+
+    @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+    @pytest.mark.parametrize("dim", [64, 128])
+    def test_what_is_not_seen_does_not_count(self, device, oracle, rows, dim, bad):
+        test_what_is_not_seen_does_not_count(device, oracle, dim, "f32x3", bad)
+
+    @pytest.mark.parametrize("where", ["q", "cached keys", "cached values", "keys", "values"])
+    @pytest.mark.parametrize("q8", [False, True])
+    def test_beyond_fp16_is_reported(self, device, oracle, rows, where, q8):
+        test_beyond_fp16_is_reported(device, oracle, where, 12, q8)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("trees", [12, 70, 300])
+def test_rows_by_the_batch(device, oracle, trees, dim):
+    """Batches of few, of more and of many short trees, which take other rows a workgroup."""
+    say("tree rows by the batch", trees, dim)
+    lengths = [(7 * i) % 50 for i in range(trees)]
+    b = Batch(device, oracle, 8, 2, dim, lengths, [bushy(1 + i % 17, 4, seed=i) for i in range(trees)], seed=trees)
+    agree(b.run("f32x3"), b.want(), "f32x3")
+    agree(b.run("f32"), b.want(), "f32")
 
 
 def test_tree_refusals(device, oracle):

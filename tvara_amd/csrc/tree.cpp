@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 #include <limits>
 #include <map>
@@ -17,6 +18,7 @@ constexpr size_t kMaxThreads = std::numeric_limits<uint32_t>::max(), kMaxWorkgro
 
 // steps from which on a run is a long one, and those that its start and merge are worth
 constexpr size_t kLongRun = 64, kRunStart = 5;
+constexpr int kWavesOfTiles = 4;  // that share a workgroup's steps
 
 size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 }  // namespace
@@ -142,7 +144,7 @@ void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t
     std::vector<int4> work;
     std::vector<int2> runs(rows);
     slots = 0;
-    tiles = tree_tiles_supported(c->layout()) ? tree_tile_shape(c->layout(), most * group, precision == 2) : TreeTileShape{};
+    tiles = tree_tiles_supported(c->layout()) ? tile_shape(trees) : TreeTileShape{};
     if (tiles.rows)
         tile_work(trees, work, runs);
     else
@@ -192,24 +194,73 @@ void TreePlan::row_work(const std::vector<int4>& trees, std::vector<int4>& work,
     }
 }
 
+namespace {
+int cached_steps(const int4& t) { return (t.y + kTreeStep - 1) / kTreeStep; }
+// steps over the tree's own nodes of the row block from row r0
+int own_steps(const int4& t, int r0, int rows, int group) {
+    return (std::min(t.z * group, r0 + rows) - 1) / group / kTreeStep + 1;
+}
+}  // namespace
+
+// Rows of a workgroup.  f32: 16 (MI355X, 16 contexts of 2048, 32 heads on 8, head_dim 64,
+// 64 rows a KV head 16: 54.8 us  32: 64.5; head_dim 128, 32 rows 58.7 and 65.6).  f32x3
+// can share a key's two parts among 32 rows in registers or 128 in LDS.  Many rows need
+// that, but as long as the work is short, the fewest rows are best for which the chip
+// holds all workgroups at once (eight trees of 16 nodes after 250 tokens 16: 11.8  32: 17.4
+// 128: 20.1; 60 such 90.3, 67.4, 42.5), and then blocks that fill it.  Else by the
+// most rows of a tree (16 contexts of 2048, 16 rows 16: 51.6  32: 55.3; 64 rows 32: 58.7
+// 128: 72.5; 80 rows 32: 113  128: 79).  Over 404 shapes (1 to 60 trees of 4 to 28
+// nodes after 30 to 16,000 tokens, both widths and formats) this is 0.6% from the
+// best of the three on average, 45% at worst; by rows alone it would be 11%.  16 uneven
+// contexts (200 to 2,000 tokens) fill the chip with blocks of 16 in one run each, which
+// end with the longest: 27.3 us, 23.0 in blocks of 32.
+// TVARA_TREE_ROWS (16, 32 or 128) chooses for f32x3 instead.
+TreeTileShape TreePlan::tile_shape(const std::vector<int4>& trees) const {
+    constexpr size_t kShort = 40;  // steps of a place for a workgroup
+    const bool x3 = precision == 2;
+    if (!x3) return tree_tile_shape(cache->layout(), 16, x3);
+    int most = 0;
+    for (const int4& t : trees) most = std::max(most, t.z * group);
+    const char* choice = std::getenv("TVARA_TREE_ROWS");
+    for (const int high : {16, 32, 128})
+        if (choice && std::atoi(choice) == high) return tree_tile_shape(cache->layout(), high, x3);
+    bool crowded = false;  // few steps, and not in one round
+    for (const int high : {16, 32, 128}) {
+        const TreeTileShape shape = tree_tile_shape(cache->layout(), high, x3);
+        const size_t units = static_cast<size_t>(cache->compute_units()) * shape.units;
+        size_t workgroups = 0, steps = 0;
+        int longest = 0;
+        for (const int4& t : trees) {
+            if (!t.z) continue;
+            const int blocks = (t.z * group - 1) / high + 1, each = cached_steps(t) + own_steps(t, t.z * group - 1, high, group);
+            workgroups += static_cast<size_t>(blocks) * cache->layout().kv_heads;
+            steps += static_cast<size_t>(blocks) * cache->layout().kv_heads * each;
+            longest = std::max(longest, each);
+        }
+        // (where a run a tree fills the chip, the longest may not end much later than the rest)
+        const bool even = longest <= 8 || 2 * workgroups <= units || 2 * longest * workgroups <= 3 * steps;
+        // (in blocks of 128, 32 rows leave half of the waves without any)
+        const size_t most_steps = high == 128 && most <= 32 ? kShort / 4 : kShort;
+        if (workgroups <= units && steps <= most_steps * units && even && (high < 128 || (most > 16 && 2 * workgroups >= units)))
+            return shape;
+        crowded |= high == 32 && workgroups > units && longest < kWavesOfTiles;
+    }
+    return tree_tile_shape(cache->layout(), most <= 16 ? 16 : most <= 64 && !crowded ? 32 : 128, x3);
+}
+
 // Runs of steps of the tiles, as many as give every CU its workgroups.  Ids go to the
 // XCDs round-robin: the row blocks of one run, which read the same keys, go to one
 // XCD, whose L2 then has them, and the XCDs' lists are filled by the fewest steps so
 // far, each ordered from the longest run to the shortest.
 void TreePlan::tile_work(const std::vector<int4>& trees, std::vector<int4>& work, std::vector<int2>& runs) {
-    const int kv_heads = cache->layout().kv_heads, xcds = std::max(1, cache->xcds());
-    auto cached_steps = [](const int4& t) { return (t.y + kTreeStep - 1) / kTreeStep; };
-    // steps over the tree's own nodes of the row block from row r0
-    auto own_steps = [&](const int4& t, int r0) {
-        return (std::min(t.z * group, r0 + tiles.rows) - 1) / group / kTreeStep + 1;
-    };
+    const int kv_heads = cache->layout().kv_heads, xcds = std::max(1, cache->xcds()), high = tiles.rows;
     auto steps_of = [&](const int4& t) {  // of its last row block, which has the most
-        return cached_steps(t) + own_steps(t, (t.z * group - 1) / tiles.rows * tiles.rows);
+        return cached_steps(t) + own_steps(t, t.z * group - 1, high, group);
     };
     size_t total = 0;
     for (const int4& t : trees)
-        for (int r0 = 0; r0 < t.z * group; r0 += tiles.rows)
-            total += static_cast<size_t>(kv_heads) * (cached_steps(t) + own_steps(t, r0));
+        for (int r0 = 0; r0 < t.z * group; r0 += high)
+            total += static_cast<size_t>(kv_heads) * (cached_steps(t) + own_steps(t, r0, high, group));
     // Steps of a run: an even share, or up to twice that if the chip then holds all
     // workgroups at once.  Where the share is long, the length with the least rounds of
     // workgroups * their mean steps: a second round for a few of them costs a share
@@ -225,7 +276,7 @@ void TreePlan::tile_work(const std::vector<int4>& trees, std::vector<int4>& work
         for (const int4& t : trees) {
             if (!t.z) continue;
             const size_t steps = steps_of(t), parts = (steps + p - 1) / p;
-            workgroups += parts * ((t.z * group - 1) / tiles.rows + 1) * kv_heads;
+            workgroups += parts * ((t.z * group - 1) / high + 1) * kv_heads;
             longest = std::max(longest, (steps + parts - 1) / parts);
         }
         if (!lengthy) {
@@ -262,8 +313,8 @@ void TreePlan::tile_work(const std::vector<int4>& trees, std::vector<int4>& work
     for (const Group& x : groups) {
         const int4& t = trees[x.tree];
         const size_t to = std::min_element(load.begin(), load.end()) - load.begin();
-        for (int r0 = 0; r0 < t.z * group; r0 += tiles.rows) {
-            const int all = cached_steps(t) + own_steps(t, r0);
+        for (int r0 = 0; r0 < t.z * group; r0 += high) {
+            const int all = cached_steps(t) + own_steps(t, r0, high, group);
             const int step = std::min(x.step, all), end = std::min(x.end, all);
             lists[to].insert(lists[to].end(), {t, make_int4(x.head, r0, step, end), make_int4(x.run, x.runs, x.slot, 0)});
             load[to] += end - step + 1;

@@ -107,8 +107,8 @@ struct TreeTileShape {
     int units;  // workgroups that share a CU
     int least;  // steps of a run
 };
-// for trees of up to `most` rows a KV head
-TreeTileShape tree_tile_shape(const BlockLayout& lay, size_t most, bool x3);
+// of 16 rows, or for f32x3 32 or 128 too
+TreeTileShape tree_tile_shape(const BlockLayout& lay, int rows, bool x3);
 void launch_tree_tiles(const TreeArgs& a, int rows, int workgroups, bool x3, hipStream_t s);
 // tree_accept.hip: chooses part, splits and whether done stays; rows * splits is at
 // most rows + kAcceptParts
@@ -172,6 +172,7 @@ struct TreePlan {
 
     void build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t heads, size_t context,
                const size_t* visible, const size_t* nodes, const int32_t* parents, int precision);
+    TreeTileShape tile_shape(const std::vector<int4>& trees) const;
     // the workgroups of the kernel, and each node row's first partial and runs
     void row_work(const std::vector<int4>& trees, std::vector<int4>& work, std::vector<int2>& runs);
     void tile_work(const std::vector<int4>& trees, std::vector<int4>& work, std::vector<int2>& runs);

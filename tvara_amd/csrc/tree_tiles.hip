@@ -1160,26 +1160,19 @@ bool tree_tiles_supported(const BlockLayout& lay) {
            lay.stride <= static_cast<size_t>(1) << 31;
 }
 
-// 16 contexts of 2048 tokens, 32 query and 8 KV heads, microseconds with each block:
-//   f32x3, head_dim 128:  16 rows  16: 51.6  32: 55.3;  32 rows  16: 55.6  32: 57.9
-//                         64 rows  32: 58.7  128: 72.5;  80 rows  32: 113  128: 79.2
-//     Q8_0                16 rows  16: 25.3  32: 31.3;  32 rows  16: 35.3  32: 33.9
-//                         64 rows  32: 49.3  128: 64.0;  80 rows  32: 90.3  128: 70.1
-//   f32x3, head_dim 64:   64 rows  32: 40.5  128: 48.6;  80 rows  32: 58.5  128: 49.9
-//   f32, head_dim 64:     16 rows  16: 33.8  32: 41.3;   64 rows  16: 54.8  32: 64.5
-//   f32, head_dim 128:    32 rows  16: 58.7  32: 65.6;   96 rows  16: 150   32: 186
 // Workgroups that a CU is dealt: what its registers (f32x3 of 128 columns one, of 64
 // two) or LDS (128 rows: two) hold.  f32 holds more than pay for their merges: of 64
-// columns (four) three (ragged contexts 2: 47.1  3: 45.4  4: 46.9), of 128 (two) over
-// f32 blocks one (32 rows 1: 58.7  2: 67.0), over Q8_0 two (1: 70.0  2: 63.2).
+// columns (four) three (MI355X, 16 ragged contexts 2: 47.1 us  3: 45.4  4: 46.9), of
+// 128 (two) over f32 blocks one (16 contexts of 2048, 32 rows 1: 58.7  2: 67.0), over
+// Q8_0 two (1: 70.0  2: 63.2).
 // A run has at least a step a wave, and no more where there are CUs: a wave's second
 // step waits for memory again (one context of 512 tokens in runs of 4 steps: 12.7,
 // of 8: 14.0, of 12: 15.3, each with its merge).
-TreeTileShape tree_tile_shape(const BlockLayout& lay, size_t most, bool x3) {
+TreeTileShape tree_tile_shape(const BlockLayout& lay, int rows, bool x3) {
     TreeTileShape t{};
-    t.rows = !x3 || most <= 16 ? 16 : most <= 64 ? 32 : 128;
+    t.rows = rows;
     if (x3)
-        t.units = t.rows == 128 || lay.head_dim == 64 ? 2 : 1;
+        t.units = rows == 128 || lay.head_dim == 64 ? 2 : 1;
     else
         t.units = lay.head_dim == 64 ? 3 : lay.format == kQ8 ? 2 : 1;
     t.least = kWaves;
