@@ -405,6 +405,30 @@ def test_rows_by_the_batch(device, oracle, trees, dim):
     agree(b.run("f32"), b.want(), "f32")
 
 
+@pytest.mark.parametrize("bad", [None, np.nan, np.inf])
+@pytest.mark.parametrize("fmt,most", [("f32", 340), ("q8_0", 90)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_short_trees(device, oracle, dim, fmt, most, bad):
+    """Batches whose waves work on their own; values that few nodes see."""
+    say("many short trees", dim, fmt, bad)
+    trees = [[-1, 0, 0, 1] if i % 50 == 7 else bushy(1 + i % 21, 4, seed=i) for i in range(360)]
+    b = Batch(device, oracle, 8, 2, dim, [(37 * i) % most for i in range(360)], trees, q8=fmt == "q8_0", seed=dim)
+    want, clean = b.want(), b.run("f32")
+    agree(clean, want, "f32")
+    if bad is None:
+        with hip_rows(b) as d:  # (rows behind the last stay)
+            plan = attention.TreePlan(b.cache, b.seqs, b.nodes, b.parents, b.heads, 1 << 20)
+            plan.launch(0, d.q.ptr, d.k.ptr, d.v.ptr, d.out.ptr)
+            plan.check()
+            assert np.array_equal(d.out.numpy()[: b.rows], clean) and (d.out.numpy()[b.rows:] == 7).all()
+        return
+    hit = [sum(map(len, trees[:i])) + 2 for i in range(7, 360, 50)]  # node 2 of such a tree: only it sees itself
+    b.tv[hit] = bad
+    got = b.run("f32")
+    keep = np.setdiff1d(np.arange(b.rows), hit)
+    assert np.array_equal(got[keep], clean[keep]) and not np.isfinite(got[hit]).any()
+
+
 def test_tree_refusals(device, oracle):
     say("tree refusals")
     b = Batch(device, oracle, 4, 2, 64, [20, 5], [chain(3), [-1, 0]], seed=2)

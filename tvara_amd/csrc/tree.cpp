@@ -150,7 +150,7 @@ void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t
     else
         row_work(trees, work, runs);
     if (slots > kIntMax / h || work.size() > 3 * kMaxWorkgroups) throw std::invalid_argument("attention batch too large");
-    items = static_cast<int>(tiles.rows ? work.size() / 3 : work.size());
+    items = static_cast<int>(tiles.rows ? work.size() / (alone ? 3 * kWavesOfTiles : 3) : work.size());
     most_runs = 1;
     for (const int2& r : runs) most_runs = std::max(most_runs, r.y);
 
@@ -291,6 +291,14 @@ void TreePlan::tile_work(const std::vector<int4>& trees, std::vector<int4>& work
             per = p;
         }
     }
+    size_t workgroups = 0, most_steps = 0;
+    for (const int4& t : trees) {
+        if (!t.z) continue;
+        workgroups += (steps_of(t) + per - 1) / per * ((t.z * group - 1) / high + 1) * kv_heads;
+        most_steps = std::max(most_steps, std::min<size_t>(per, steps_of(t)));
+    }
+    alone = workgroups / cache->compute_units() >= static_cast<size_t>(tiles.alone_from) &&
+           most_steps <= static_cast<size_t>(tiles.alone_to);
     struct Group {  // the row blocks of a run
         int tree, head, run, runs, slot, step, end;
     };
@@ -320,11 +328,13 @@ void TreePlan::tile_work(const std::vector<int4>& trees, std::vector<int4>& work
             load[to] += end - step + 1;
         }
     }
+    // an XCD's list becomes that of every xcds-th workgroup
+    const size_t chunk = alone ? 3 * kWavesOfTiles : 3;
     size_t longest = 0;
-    for (const auto& l : lists) longest = std::max(longest, l.size());
+    for (const auto& l : lists) longest = std::max(longest, round_up(l.size(), chunk));
     work.assign(longest * xcds, make_int4(0, 0, 0, 0));  // (padding has no nodes)
     for (int x = 0; x < xcds; ++x)
-        for (size_t k = 0; k < lists[x].size(); ++k) work[3 * (k / 3 * xcds + x) + k % 3] = lists[x][k];
+        for (size_t k = 0; k < lists[x].size(); ++k) work[chunk * (k / chunk * xcds + x) + k % chunk] = lists[x][k];
 }
 
 void TreePlan::launch(int layer, const float* q, const float* keys, const float* values, size_t row_stride, float* out,
@@ -351,6 +361,7 @@ void TreePlan::launch(int layer, const float* q, const float* keys, const float*
     a.mask = reinterpret_cast<const uint32_t*>(d + mask_at);
     a.words = words;
     a.work = reinterpret_cast<const int4*>(d + work_at);
+    a.alone = alone;
     a.split_tokens = split_tokens;
     a.runs = reinterpret_cast<const int2*>(d + runs_at);
     a.rows = static_cast<int>(rows);

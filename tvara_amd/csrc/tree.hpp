@@ -28,6 +28,7 @@ struct TreeArgs {
     const int4* trees;     // x: table offset, y: cached tokens seen, z: nodes, w: first node row
     const uint32_t* mask;  // [node rows][words]: bit k of word s: the node sees node 32s + k of its tree
     int words;
+    bool alone;            // tiles: an entry of work for each wave, not each workgroup
     const int4* work;      // see the kernels
     int split_tokens;      // row kernel: cached tokens of a run
     const int2* runs;      // per node row: first partial, runs (one run: written to out)
@@ -106,6 +107,7 @@ struct TreeTileShape {
     int rows;   // of a workgroup
     int units;  // workgroups that share a CU
     int least;  // steps of a run
+    int alone_from, alone_to;  // workgroups a CU from which, steps of one to which waves work alone
 };
 // of 16 rows, or for f32x3 32 or 128 too
 TreeTileShape tree_tile_shape(const BlockLayout& lay, int rows, bool x3);
@@ -163,6 +165,7 @@ struct TreePlan {
     uint64_t epoch = 0;
     int heads = 0, group = 0, precision = 0, words = 1, items = 0, split_tokens = 0;
     TreeTileShape tiles{};  // rows 0: the row kernel
+    bool alone = false;     // an entry of work for each wave of the tiles
     int most_runs = 1;
     size_t count = 0, rows = 0, slots = 0;
     PlanRegion region;

@@ -23,6 +23,7 @@
 // workgroups (a CU is at work 60% of the time) and the f32 products (half of that).
 // f32x3, 16 contexts of 2,048 with 16 nodes, head_dim 128: 60.6 us, 4.4 TB/s.
 #include <algorithm>
+#include <limits>
 
 #include "common.hpp"
 #include "device_util.hpp"
@@ -120,12 +121,12 @@ struct Item {
     int4 tree;
     int head, row0, step, end, run, runs, slot;
 };
-__device__ __forceinline__ Item item_of(const TreeArgs& a) {
-    const int4 t = a.work[3 * blockIdx.x], x = a.work[3 * blockIdx.x + 1], y = a.work[3 * blockIdx.x + 2];
+__device__ __forceinline__ Item item_of(const TreeArgs& a, unsigned i) {
+    const int4 t = a.work[3 * static_cast<size_t>(i)], x = a.work[3 * static_cast<size_t>(i) + 1], y = a.work[3 * static_cast<size_t>(i) + 2];
     return {t, x.x, x.y, x.z, x.w, y.x, y.y, y.z};
 }
 
-template <int D, int NT, bool kQ8, bool kX3>
+template <int D, int NT, bool kQ8, bool kX3, bool kAlone = false>
 __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_tile_kernel(const TreeArgs a) {
     constexpr int WK = kWaves, C = D / 16, KC = D / 32, H = D / 64;
     constexpr int W = D / 4;  // 16-byte parts of a row
@@ -142,8 +143,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
     auto result = [&](int w, int i, int nt) -> f32x4& { return staged[w][(i * NT + nt) * 64 + static_cast<int>(threadIdx.x & 63)]; };
     __shared__ float2 stats[WK][16 * NT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g = lane >> 4, r16 = lane & 15, wk = wave;
-    const Item it = item_of(a);
+    const int g = lane >> 4, r16 = lane & 15;
+    // one entry of work a workgroup, whose steps the waves share, or (kAlone) one a wave
+    constexpr int stride = kAlone ? 1 : WK;
+    const Item it = item_of(a, kAlone ? blockIdx.x * WK + wave : blockIdx.x);
     if (!it.tree.z) return;  // the list's padding
     const int4 tree = it.tree;
     const int cached = tree.y, nodes = tree.z, kh = it.head, G = a.group, kvw = a.lay.kv_width;
@@ -173,11 +176,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
     const int rowb = kQ8 ? D : kvw * static_cast<int>(sizeof(float));  // from one slot to the next
     const unsigned koff = static_cast<unsigned>(kStaged ? lane / W * rowb + (lane % W ^ lane / W) * 16 : r16 * rowb + kcol(0));
     const unsigned voff = static_cast<unsigned>(4 * g * rowb + vcol(0, r16) * (kQ8 ? 1 : 4));
-    int step = it.step + wk;
+    int step = it.step + (kAlone ? 0 : wave);
     const int last = max(cached - 1, 0) >> 4;  // 16 keys a table lookup; past the end the last again
     // lane 2i + mt: the block of the wave's i-th step from here
-    auto lookup = [&](int from) { return cached ? tab[min(2 * (from + (lane >> 1) * WK) + (lane & 1), last) << 4 >> tsh] : 0; };
-    int ids = lookup(step), more = lookup(step + 32 * WK), at = 0;
+    auto lookup = [&](int from) { return cached ? tab[min(2 * (from + (lane >> 1) * stride) + (lane & 1), last) << 4 >> tsh] : 0; };
+    int ids = lookup(step), more = lookup(step + 32 * stride), at = 0;
     auto block = [&](int mt, int stp) {
         const int id = __builtin_amdgcn_readlane(ids, 2 * at + mt);
         const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
@@ -453,7 +456,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
         }
     };
 
-    // ---- cached steps: this wave's are step0 + wk, + WK, ...
+    // ---- cached steps
     if (step < end) {
         auto cached_scores = [&]() __attribute__((always_inline)) {
             if constexpr (kStaged)
@@ -506,8 +509,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
             if constexpr (kStaged) asm volatile("" ::: "memory");
             load_v(step);
         }
-        for (; step < end; step += WK) {
-            const int next = step + WK;
+        for (; step < end; step += stride) {
+            const int next = step + stride;
             if constexpr (kStaged) wait_until_left<8 * H>();  // the values'
             cached_scores();
             if constexpr (kStaged) wait_for_lds();
@@ -516,7 +519,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
             if (++at == 32) {
                 at = 0;
                 ids = more;
-                more = lookup(next + 32 * WK);
+                more = lookup(next + 32 * stride);
             }
             load_k(next);
             if constexpr (kStaged) asm volatile("" ::: "memory");
@@ -545,7 +548,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
     }
 
     // ---- the tree's own nodes
-    for (; step < it.end; step += WK) {
+    for (; step < it.end; step += stride) {
         const int n0 = kStep * (step - csteps);
         const float* kb = a.keys + static_cast<size_t>(tree.w) * a.row_stride + static_cast<size_t>(kh) * D;
         const float* vb = a.values + static_cast<size_t>(tree.w) * a.row_stride + static_cast<size_t>(kh) * D;
@@ -618,12 +621,15 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
     float total[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) total[nt] = cross_row_sum(l[nt]);
-    if (g == 0)
+    if constexpr (!kAlone) {
+        if (g == 0)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) stats[wave][16 * nt + r16] = make_float2(m[nt], total[nt]);
-    __syncthreads();
+            for (int nt = 0; nt < NT; ++nt) stats[wave][16 * nt + r16] = make_float2(m[nt], total[nt]);
+        __syncthreads();
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+        if constexpr (kAlone) continue;
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int w = 0; w < WK; ++w) top = fmaxf(top, stats[w][16 * nt + r16].x);
@@ -643,20 +649,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
     bool bad = false;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-        if (h) __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                result(wave, i, nt) = f32x4{acc[4 * h][nt][i], acc[4 * h + 1][nt][i], acc[4 * h + 2][nt][i], acc[4 * h + 3][nt][i]};
-        __syncthreads();
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int i = wave;
-            f32x4 x = result(0, i, nt);
-#pragma unroll
-            for (int w = 1; w < WK; ++w) x += result(w, i, nt);
-            if (!live[nt]) continue;
+        auto mine = [&](int i, int nt) {
+            return f32x4{acc[4 * h][nt][i], acc[4 * h + 1][nt][i], acc[4 * h + 2][nt][i], acc[4 * h + 3][nt][i]};
+        };
+        auto put = [&](int i, int nt, f32x4 x) __attribute__((always_inline)) {
+            if (!live[nt]) return;
             const size_t row = static_cast<size_t>(tree.w) + node[nt];
             if (it.runs == 1) {
                 x /= total[nt];
@@ -667,6 +664,26 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
                 *reinterpret_cast<f32x4*>(a.part_acc + p * D + vcol(h, 4 * g + i)) = x;
                 if (h == 0 && i == 0 && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m[nt], total[nt]);
             }
+        };
+        if constexpr (kAlone) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) put(i, nt, mine(i, nt));
+            continue;
+        }
+        if (h) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) result(wave, i, nt) = mine(i, nt);
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            f32x4 x = result(0, wave, nt);
+#pragma unroll
+            for (int w = 1; w < WK; ++w) x += result(w, wave, nt);
+            put(wave, nt, x);
         }
     }
     if (bad) *a.err = 1;
@@ -696,7 +713,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
     __shared__ int odds[2][S][H];    // the tree's own values: some are not finite
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, r16 = lane & 15;
-    const Item it = item_of(a);
+    const Item it = item_of(a, blockIdx.x);
     if (!it.tree.z) return;  // the list's padding
     const int4 tree = it.tree;
     const int cached = tree.y, nodes = tree.z, kh = it.head, G = a.group, kvw = a.lay.kv_width;
@@ -1145,6 +1162,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
 template <int D, bool kQ8, bool kX3>
 void launch_shape(const TreeArgs& a, int rows, int workgroups, hipStream_t s) {
     auto go = [&](auto kernel) { launch("tree_attention_tiles", kernel, dim3(workgroups), dim3(64 * kWaves), 0, s, a); };
+    if constexpr (!kX3)
+        if (a.alone) return go(tree_tile_kernel<D, 1, kQ8, false, true>);
     if (rows == 16)
         go(tree_tile_kernel<D, 1, kQ8, kX3>);
     else if constexpr (kX3)
@@ -1165,6 +1184,11 @@ bool tree_tiles_supported(const BlockLayout& lay) {
 // columns (four) three (MI355X, 16 ragged contexts 2: 47.1 us  3: 45.4  4: 46.9), of
 // 128 (two) over f32 blocks one (16 contexts of 2048, 32 rows 1: 58.7  2: 67.0), over
 // Q8_0 two (1: 70.0  2: 63.2).
+// Where workgroups are many and their steps few, the waves of f32 take an entry of work
+// each (alone): a workgroup's start, not its steps, is what passes then (60 trees of 24
+// nodes after 3 tokens, head_dim 128: 57.6 us shared  31.5 alone; after 250: 118 and 89,
+// but 16 of 12 nodes 22.2 and 30.7; over Q8_0, whose steps wait less, 61 trees of 11 nodes
+// after 295, head_dim 64: 29.3 and 41.3).
 // A run has at least a step a wave, and no more where there are CUs: a wave's second
 // step waits for memory again (one context of 512 tokens in runs of 4 steps: 12.7,
 // of 8: 14.0, of 12: 15.3, each with its merge).
@@ -1176,6 +1200,8 @@ TreeTileShape tree_tile_shape(const BlockLayout& lay, int rows, bool x3) {
     else
         t.units = lay.head_dim == 64 ? 3 : lay.format == kQ8 ? 2 : 1;
     t.least = kWaves;
+    t.alone_from = x3 ? std::numeric_limits<int>::max() : lay.head_dim == 64 ? 4 : 3;
+    t.alone_to = lay.format == kQ8 ? 4 : 12;
     return t;
 }
 
