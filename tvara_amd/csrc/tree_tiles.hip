@@ -19,9 +19,9 @@
 // running maximum that moves only where a step exceeds it by 2^8.
 //
 // MI355X: f32, 16 contexts of 123 to 2,793 tokens with 6 to 24 nodes, 32 heads on 8
-// of 64: 48.4 us (floor 21: one read of K and V at a copy's rate), bound by the longest
-// workgroups (a CU is at work 60% of the time) and the f32 products (half of that).
-// f32x3, 16 contexts of 2,048 with 16 nodes, head_dim 128: 60.6 us, 4.4 TB/s.
+// of 64: 45.3 us with the merge (floor 21: one read of K and V at a copy's rate), bound
+// by the longest workgroups and the f32 products (25 us, padded to 16 rows).
+// f32x3, 16 contexts of 2,048 with 16 nodes, head_dim 128: 58.2 us, 4.6 TB/s.
 #include <algorithm>
 #include <limits>
 
@@ -697,9 +697,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
 // an iteration of S steps.  Loads go through descriptors that end with the last
 // key, so that what lies behind it reads as zeros.
 //
-// MI355X, 16 contexts of 4,096 with 32 nodes, 32 heads on 8 of 128: 142 us with the
-// merge, 3.9 TB/s (a copy reads and writes 4.8); 8 contexts of 4,096 with 64 nodes, 64
-// heads on 8: 217 us, 3 x 318 TFLOP/s of fp16 products: the matrix pipe is busy half
+// MI355X, 16 contexts of 4,096 with 32 nodes, 32 heads on 8 of 128: 136 us with the
+// merge, 4.1 TB/s (a copy reads and writes 4.8); 8 contexts of 4,096 with 64 nodes, 64
+// heads on 8: 220 us, 3 x 314 TFLOP/s of fp16 products: the matrix pipe is busy half
 // of the time, and the vector instructions of two waves a SIMD (230 a step, beside
 // 96 products) do not hide behind it.
 template <int D, bool kQ8>
