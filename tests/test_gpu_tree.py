@@ -405,6 +405,36 @@ def test_rows_by_the_batch(device, oracle, trees, dim):
     agree(b.run("f32"), b.want(), "f32")
 
 
+@pytest.mark.parametrize("precision,rows", [("f32", ""), ("f32x3", "16"), ("f32x3", "32"), ("f32x3", "128")])
+@pytest.mark.parametrize("fmt", ["f32", "q8_0"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_runs(device, oracle, monkeypatch, dim, fmt, precision, rows):
+    """Enough trees that a workgroup walks a long context alone, through a table of
+    blocks in no order: one sequence of 16,003 tokens under 500 trees of a node."""
+    say("tree long runs", dim, fmt, precision, rows)
+    monkeypatch.setenv("TVARA_TREE_ROWS", rows)
+    n, trees, heads, w = 16003, 500, 4, 2 * dim
+    cache = device.PagedCache(1, 2, dim, 16, 1800, fmt=device.Q8_0 if fmt == "q8_0" else device.F32)
+    k, v = (synth.normal(dim, x, n * w).reshape(n, w) for x in "kv")
+    a, b = cache.create_sequence(), cache.create_sequence()
+    for i in range(0, n, 48):  # the other sequence's blocks lie between
+        cache.append_many(a, k[i:i + 48], v[i:i + 48])
+        cache.append_many(b, k[:16 * (1 + i // 48 % 2)], v[:16 * (1 + i // 48 % 2)])
+    if fmt == "q8_0":
+        k, v = (oracle.dequantize_q8_0(oracle.quantize_q8_0(x)).reshape(n, w) for x in (k, v))
+    q, tk, tv = (synth.normal(dim, x, trees * c).reshape(trees, c) for x, c in (("q", heads * dim), ("tk", w), ("tv", w)))
+    got = attention.tree_batch(cache, q, [a] * trees, [1] * trees, [-1] * trees, tk, tv, 0, heads, 1 << 20, precision=precision)
+    want = np.empty((trees, heads, dim))
+    for h in range(heads):
+        cols = slice(h // 2 * dim, (h // 2 + 1) * dim)
+        x = q.reshape(trees, heads, dim)[:, h].astype(np.float64)
+        s = np.concatenate([x @ k[:, cols].astype(np.float64).T, (x * tk[:, cols]).sum(1, keepdims=True)], 1) / np.sqrt(dim)
+        p = np.exp(s - s.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        want[:, h] = p[:, :n] @ v[:, cols].astype(np.float64) + p[:, n:] * tv[:, cols]
+    agree(got, want.reshape(trees, heads * dim), precision)
+
+
 @pytest.mark.parametrize("bad", [None, np.nan, np.inf])
 @pytest.mark.parametrize("fmt,most", [("f32", 340), ("q8_0", 90)])
 @pytest.mark.parametrize("dim", [64, 128])
