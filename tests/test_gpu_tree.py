@@ -435,6 +435,43 @@ def test_long_runs(device, oracle, monkeypatch, dim, fmt, precision, rows):
     agree(got, want.reshape(trees, heads * dim), precision)
 
 
+@pytest.mark.parametrize("dim,kv_heads", [(128, 8), (64, 16), (96, 10)])
+def test_pool_beyond_32_bits(device, oracle, monkeypatch, dim, kv_heads):
+    """Blocks more than 4 GiB into the pool: attention, slots, writes."""
+    say("tree, pool beyond 4 GiB", dim)
+    w, heads, n = kv_heads * dim, 2 * kv_heads, 100
+    per = (5 << 30) // (16 * w * 8) + 1
+    cache = device.PagedCache(1, kv_heads, dim, 16, per + 20)
+    filler, a = cache.create_sequence(), cache.create_sequence()
+    cache.reserve([filler], [16 * per])
+    k, v = (synth.normal(dim, x, n * w).reshape(n, w) for x in "kv")
+    cache.reserve([a], [n])
+    up = hip.DeviceArray.from_numpy
+    base, stride = cache.pool_address()
+    assert min(h[0] for h in cache.blocks(a)) * stride > 1 << 32
+    plan = SlotPlan(cache, [a])
+    slots, starts, counts = hip.DeviceArray((n,), np.int64), up(np.zeros(1, np.int32)), up(np.full(1, n, np.int32))
+    plan.build(starts.ptr, counts.ptr, 0, n, slots_ptr=slots.ptr)
+    dk, dv = up(k.astype(np.float32)), up(v.astype(np.float32))
+    plan.write(slots.ptr, None, n, dk.ptr, dv.ptr, n, w, w)
+    plan.check()
+    assert np.array_equal(cache.read_all(a, 0).reshape(n, w), k.astype(np.float32))
+    q, tk, tv = (synth.normal(dim, x, 2 * c).reshape(2, c) for x, c in (("q", heads * dim), ("tk", w), ("tv", w)))
+    want = np.empty((2, heads, dim))
+    for h in range(heads):
+        cols = slice(h // 2 * dim, (h // 2 + 1) * dim)
+        for r in range(2):  # node 1 sees node 0 and itself
+            kk = np.concatenate([k[:, cols], tk[: r + 1, cols]]).astype(np.float64)
+            vv = np.concatenate([v[:, cols], tv[: r + 1, cols]]).astype(np.float64)
+            s = kk @ q[r].reshape(heads, dim)[h].astype(np.float64) / np.sqrt(dim)
+            p = np.exp(s - s.max())
+            want[r, h] = p @ vv / p.sum()
+    for precision, rows in (("f32", ""), ("f32x3", "16"), ("f32x3", "32"), ("f32x3", "128")):
+        monkeypatch.setenv("TVARA_TREE_ROWS", rows)
+        got = attention.tree_batch(cache, q, [a], [2], [-1, 0], tk, tv, 0, heads, 1 << 20, precision=precision)
+        agree(got, want.reshape(2, heads * dim), precision)
+
+
 @pytest.mark.parametrize("bad", [None, np.nan, np.inf])
 @pytest.mark.parametrize("fmt,most", [("f32", 340), ("q8_0", 90)])
 @pytest.mark.parametrize("dim", [64, 128])

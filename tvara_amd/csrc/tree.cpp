@@ -18,7 +18,6 @@ constexpr size_t kMaxThreads = std::numeric_limits<uint32_t>::max(), kMaxWorkgro
 
 // steps from which on a run is a long one, and those that its start and merge are worth
 constexpr size_t kLongRun = 64, kRunStart = 5;
-constexpr int kWavesOfTiles = 4;  // that share a workgroup's steps
 
 size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 }  // namespace
@@ -150,7 +149,7 @@ void TreePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t
     else
         row_work(trees, work, runs);
     if (slots > kIntMax / h || work.size() > 3 * kMaxWorkgroups) throw std::invalid_argument("attention batch too large");
-    items = static_cast<int>(tiles.rows ? work.size() / (alone ? 3 * kWavesOfTiles : 3) : work.size());
+    items = static_cast<int>(tiles.rows ? work.size() / (alone ? 3 * kTreeWaves : 3) : work.size());
     most_runs = 1;
     for (const int2& r : runs) most_runs = std::max(most_runs, r.y);
 
@@ -243,7 +242,7 @@ TreeTileShape TreePlan::tile_shape(const std::vector<int4>& trees) const {
         const size_t most_steps = high == 128 && most <= 32 ? kShort / 4 : kShort;
         if (workgroups <= units && steps <= most_steps * units && even && (high < 128 || (most > 16 && 2 * workgroups >= units)))
             return shape;
-        crowded |= high == 32 && workgroups > units && longest < kWavesOfTiles;
+        crowded |= high == 32 && workgroups > units && longest < kTreeWaves;
     }
     return tree_tile_shape(cache->layout(), most <= 16 ? 16 : most <= 64 && !crowded ? 32 : 128, x3);
 }
@@ -329,7 +328,7 @@ void TreePlan::tile_work(const std::vector<int4>& trees, std::vector<int4>& work
         }
     }
     // an XCD's list becomes that of every xcds-th workgroup
-    const size_t chunk = alone ? 3 * kWavesOfTiles : 3;
+    const size_t chunk = alone ? 3 * kTreeWaves : 3;
     size_t longest = 0;
     for (const auto& l : lists) longest = std::max(longest, round_up(l.size(), chunk));
     work.assign(longest * xcds, make_int4(0, 0, 0, 0));  // (padding has no nodes)

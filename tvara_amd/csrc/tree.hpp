@@ -99,10 +99,12 @@ struct WriteArgs {
 // tree.hip
 void launch_tree_rows(const TreeArgs& a, int items, hipStream_t s);
 void launch_tree_merge(const TreeArgs& a, int most_runs, hipStream_t s);
-// tree_tiles.hip: head_dim 64 and 128.  Work has three entries a workgroup: the tree
-// (as trees); KV head, first row, first step, end; run, runs, the tree's first partial.
+// tree_tiles.hip: head_dim 64 and 128.  Work has three entries a workgroup (TreeArgs::
+// alone: a wave): the tree (as trees); KV head, first row, first step, end; run, runs, the
+// tree's first partial.
 bool tree_tiles_supported(const BlockLayout& lay);
 constexpr int kTreeStep = 32;  // keys of a step
+constexpr int kTreeWaves = 4;  // of a workgroup
 struct TreeTileShape {
     int rows;   // of a workgroup
     int units;  // workgroups that share a CU

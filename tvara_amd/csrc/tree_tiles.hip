@@ -40,7 +40,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kThreshold = 8.0f;
-constexpr int kStep = 32, kWaves = 4;
+constexpr int kStep = kTreeStep, kWaves = kTreeWaves;
 constexpr int kBufferWord3 = 0x00020000;  // gfx9 buffer descriptor, dword 3
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
