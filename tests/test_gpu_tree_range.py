@@ -1,0 +1,67 @@
+"""Tree attention over the whole range of its inputs: weights far below a row's
+largest.  The bars are test_gpu_tree's unless a test derives its own."""
+
+import numpy as np
+import pytest
+
+import test_gpu_tree as tt
+from tvara_amd import attention, synth
+
+pytestmark = pytest.mark.gpu
+
+
+class Sink:
+    """One sequence under 256 trees of a node: its first key's score is `gap`, the
+    others' are N(0,1).  256 trees of two KV heads give every CU its workgroups, so
+    each walks the whole context alone."""
+
+    TREES, KV, GROUP, CHECKED = 256, 2, 2, 24
+
+    def __init__(self, device, oracle, dim, n, gap, q8, sink_value=1.0):
+        w, self.dim, self.n = self.KV * dim, dim, n
+        u = synth.normal(dim, "u", w).reshape(self.KV, dim).astype(np.float64)
+        u /= np.linalg.norm(u, axis=1, keepdims=True)
+        k, v, q, tk, tv = (synth.normal(n, x, rows * c).reshape(rows, -1, dim).astype(np.float64) for x, rows, c in (
+            ("k", n, w), ("v", n, w), ("q", self.TREES, self.GROUP * w), ("tk", self.TREES, w), ("tv", self.TREES, w)))
+        along = np.repeat(u, self.GROUP, 0)
+        q += (np.sqrt(dim) - (q * along).sum(2, keepdims=True)) * along  # sqrt(dim) along u
+        for x in (k, tk):
+            x -= (x * u).sum(2, keepdims=True) * u
+        k[0], v[0] = gap * u, sink_value * v[0]
+        k, v, tk, tv = (np.ascontiguousarray(x.reshape(-1, w), np.float32) for x in (k, v, tk, tv))
+        self.q = np.ascontiguousarray(q.reshape(self.TREES, -1), np.float32)
+        self.cache = device.PagedCache(1, self.KV, dim, 64, n // 64 + 1, fmt=device.Q8_0 if q8 else device.F32)
+        self.seq = self.cache.create_sequence()
+        self.cache.append_many(self.seq, k, v)
+        if q8:
+            k, v = (oracle.dequantize_q8_0(oracle.quantize_q8_0(x)).reshape(n, w) for x in (k, v))
+        self.k, self.v, self.tk, self.tv = k, v, tk, tv
+
+    def run(self, precision):
+        n = self.TREES
+        got = attention.tree_batch(self.cache, self.q, [self.seq] * n, [1] * n, [-1] * n, self.tk, self.tv, 0,
+                                   self.KV * self.GROUP, 1 << 20, precision=precision)
+        return got[: self.CHECKED].reshape(self.CHECKED, -1, self.dim).astype(np.float64)
+
+    def want(self):
+        out = np.empty((self.CHECKED, self.KV * self.GROUP, self.dim))
+        for h in range(out.shape[1]):
+            cols = slice(h // self.GROUP * self.dim, (h // self.GROUP + 1) * self.dim)
+            x = self.q.reshape(self.TREES, -1, self.dim)[: self.CHECKED, h].astype(np.float64)
+            tk, tv = (y[: self.CHECKED, cols].astype(np.float64) for y in (self.tk, self.tv))
+            s = np.concatenate([x @ self.k[:, cols].astype(np.float64).T, (x * tk).sum(1, keepdims=True)], 1) / np.sqrt(self.dim)
+            p = np.exp(s - s.max(1, keepdims=True))
+            p /= p.sum(1, keepdims=True)
+            out[:, h] = p[:, :-1] @ self.v[:, cols].astype(np.float64) + p[:, -1:] * tv
+        return out
+
+
+@pytest.mark.parametrize("gap", [12, 18, 19.5, 21])
+@pytest.mark.parametrize("fmt", ["f32", "q8_0"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_small_weights_add_up(device, oracle, dim, fmt, gap):
+    """Beside the largest weight each step's others may be less than half an ulp of the
+    normaliser, and together many."""
+    tt.say("tree, one key far above, f32", dim, fmt, gap)
+    b = Sink(device, oracle, dim, 32768, gap, fmt == "q8_0")
+    tt.agree(b.run("f32"), b.want(), "f32")
