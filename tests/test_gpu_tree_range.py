@@ -8,6 +8,7 @@ import test_gpu_tree as tt
 from tvara_amd import attention, synth
 
 pytestmark = pytest.mark.gpu
+ROWS = ["16", "32", "128"]  # that a workgroup of f32x3 may have
 
 
 class Sink:
@@ -65,3 +66,33 @@ def test_small_weights_add_up(device, oracle, dim, fmt, gap):
     tt.say("tree, one key far above, f32", dim, fmt, gap)
     b = Sink(device, oracle, dim, 32768, gap, fmt == "q8_0")
     tt.agree(b.run("f32"), b.want(), "f32")
+
+
+@pytest.mark.parametrize("gap", [12, 16, 18, 19.5])
+@pytest.mark.parametrize("n", [4096, 32768])
+@pytest.mark.parametrize("fmt", ["f32", "q8_0"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_key_far_above_many(device, oracle, monkeypatch, dim, fmt, n, gap):
+    tt.say("tree, one key far above", dim, fmt, n, gap)
+    b = Sink(device, oracle, dim, n, gap, fmt == "q8_0")
+    want = b.want()
+    for rows in ROWS:
+        monkeypatch.setenv("TVARA_TREE_ROWS", rows)
+        tt.agree(b.run("f32x3"), want, "f32x3")
+
+
+@pytest.mark.parametrize("gap", [12, 18])
+@pytest.mark.parametrize("fmt", ["f32", "q8_0"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_key_far_above_without_a_value(device, oracle, monkeypatch, dim, fmt, gap):
+    """Only the small weights count.  Each is off by up to 2^-36 of the largest, by
+    itself: 2^-36 / sqrt(3) sqrt(sum v^2) as a deviation, six of which no output
+    passes, beside the module's relative bar."""
+    tt.say("tree, one key far above, no value", dim, fmt, gap)
+    b = Sink(device, oracle, dim, 32768, gap, fmt == "q8_0", sink_value=0.0)
+    want = b.want()
+    floor = 6 * 2.0 ** -36 / np.sqrt(3) * np.sqrt(np.square(b.v.astype(np.float64)).sum(0).max())
+    for rows in ROWS:
+        monkeypatch.setenv("TVARA_TREE_ROWS", rows)
+        off = np.abs(b.run("f32x3") - want)
+        assert (off <= floor + tt.BAR * np.abs(want).max()).all(), (off.max(), np.abs(want).max())

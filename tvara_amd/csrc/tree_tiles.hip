@@ -16,7 +16,7 @@
 //
 // f32: v_mfma_f32_16x16x4_f32.  f32x3 (kX3): 16x16x32 on operands in two fp16
 // parts, hi * hi + hi * lo + lo * hi.  Softmax in log2 units with a
-// running maximum that moves only where a step exceeds it by 2^8.
+// running maximum that moves only where a step exceeds it by 2^8 (f32x3: 2^4).
 //
 // MI355X: f32, 16 contexts of 123 to 2,793 tokens with 6 to 24 nodes, 32 heads on 8
 // of 64: 45.3 us with the merge (floor 21: one read of K and V at a copy's rate), bound
@@ -40,6 +40,15 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kThreshold = 8.0f;
+// f32x3: what two fp16 parts hold of a probability ends at 2^-25, and a row may have
+// its largest one beside thousands of small ones that count together (the first token
+// of a text draws such weight, and may have little value itself).  So m is kept 2^11
+// below the running maximum, which every probability, sum and partial is then relative
+// to, and the maximum may pass it by 2^4: the largest lies between 2^11 and 2^15, fp16
+// ends at 2^16, and a small one is off by 2^-36 of it.  MI355X, one key without value 18
+// above 32,768 of N(0,1): 2-norm 0.19 (m the maximum, which may move by 2^8),
+// 1.6e-3 (2^7 and 2^8), 1e-4 so (128 rows a workgroup: 2e-4).
+constexpr float kPartsThreshold = 4.0f, kPartsLift = 11.0f;
 constexpr int kStep = kTreeStep, kWaves = kTreeWaves;
 constexpr int kBufferWord3 = 0x00020000;  // gfx9 buffer descriptor, dword 3
 
@@ -292,7 +301,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
         }
 
     f32x4 acc[4 * H][NT];  // tile (h, j) at 4h + j
-    float m[NT], l[NT], rounded[NT], nonfinite = 0.f;  // nonfinite: NaN once a score is not finite
+    constexpr float kLift = kX3 ? kPartsLift : 0.f, kMove = (kX3 ? kPartsThreshold : kThreshold) + kLift;
+    float m[NT], l[NT], rounded[NT], nonfinite = 0.f;  // m: the maximum less kLift; nonfinite: NaN once a score is not finite
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         m[nt] = -INFINITY;
@@ -389,8 +399,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
                     }
                     mx = fmaxf(mx, x);
                 }
-            if (__any(mx > m[nt] + kThreshold)) {
-                const float mn = fmaxf(m[nt], cross_row_max(mx));
+            if (__any(mx > m[nt] + kMove)) {
+                const float mn = fmaxf(m[nt], cross_row_max(mx) - kLift);
                 const float alpha = m[nt] == -INFINITY ? 0.f : fast_exp2(m[nt] - mn);
                 m[nt] = mn;
                 l[nt] *= alpha;
@@ -763,7 +773,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
         }
     }
     f32x4 acc[4 * H][NT];
-    float m[NT], l[NT], rounded[NT];
+    float m[NT], l[NT], rounded[NT];  // m: the maximum less kPartsLift
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         m[nt] = -INFINITY;
@@ -1013,8 +1023,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[mt][nt][i]);
-            if (__any(mx > m[nt] + kThreshold)) {
-                const float mn = fmaxf(m[nt], cross_row_max(mx));
+            if (__any(mx > m[nt] + (kPartsThreshold + kPartsLift))) {
+                const float mn = fmaxf(m[nt], cross_row_max(mx) - kPartsLift);
                 const float alpha = m[nt] == -INFINITY ? 0.f : fast_exp2(m[nt] - mn);
                 m[nt] = mn;
                 l[nt] *= alpha;
