@@ -1,11 +1,11 @@
 """Tree attention over the whole range of its inputs: weights far below a row's
-largest.  The bars are test_gpu_tree's unless a test derives its own."""
+largest, values that f32x3's fp16 parts do not hold.  The bars are test_gpu_tree's unless a test derives its own."""
 
 import numpy as np
 import pytest
 
 import test_gpu_tree as tt
-from tvara_amd import attention, synth
+from tvara_amd import _capi, attention, synth
 
 pytestmark = pytest.mark.gpu
 ROWS = ["16", "32", "128"]  # that a workgroup of f32x3 may have
@@ -96,3 +96,43 @@ def test_one_key_far_above_without_a_value(device, oracle, monkeypatch, dim, fmt
         monkeypatch.setenv("TVARA_TREE_ROWS", rows)
         off = np.abs(b.run("f32x3") - want)
         assert (off <= floor + tt.BAR * np.abs(want).max()).all(), (off.max(), np.abs(want).max())
+
+
+@pytest.mark.parametrize("bad", [65520.0, -1e5, 3e6, -3e38, np.nan, np.inf])
+@pytest.mark.parametrize("fmt", ["f32", "q8_0"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_unseen_values_beyond_the_parts(device, oracle, monkeypatch, dim, fmt, bad):
+    """f32x3: a node's value that fp16 does not hold leaves the rows that do not see it
+    to the bit as they are, and is reported for those that do."""
+    tt.say("tree, unseen beyond fp16", dim, fmt, bad)
+    trees = [[-1, 0, 1, 1, 0, 4], tt.chain(2), [-1] * 20 + [3] * 20]
+    for rows in ROWS:
+        monkeypatch.setenv("TVARA_TREE_ROWS", rows)
+        b = tt.Batch(device, oracle, 4, 2, dim, [35, 20, 700], trees, q8=fmt == "q8_0", seed=8)
+        clean = b.run("f32x3")
+        tt.agree(clean, b.want(), "f32x3")
+        b.tv[4, 3] = b.tv[8 + 3, dim + 5] = bad  # seen by rows 4, 5 of the first tree; 3 and 20 to 39 of the third
+        hit = np.array([4, 5, 8 + 3, *range(8 + 20, 8 + 40)])
+        keep = np.setdiff1d(np.arange(b.rows), hit)
+        with tt.hip_rows(b) as d:
+            plan = attention.TreePlan(b.cache, b.seqs, b.nodes, b.parents, 4, 1 << 20, precision="f32x3")
+            plan.launch(0, d.q.ptr, d.k.ptr, d.v.ptr, d.out.ptr)
+            with pytest.raises(_capi.InvalidArgument, match="invalid online attention input"):
+                plan.check()
+            got = d.out.numpy()[: b.rows]
+        assert np.array_equal(got[keep], clean[keep])
+        heads = got[hit].reshape(hit.size, 4, dim)
+        assert not np.isfinite(heads[:2, :2, 3]).any() and not np.isfinite(heads[2:, 2:, 5]).any()
+        other = np.isfinite(got[hit]).sum()
+        assert other == got[hit].size - 2 * hit.size  # one column of the two heads of that KV head
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_largest_values_of_the_parts(device, oracle, monkeypatch, dim):
+    """f32x3 takes values up to fp16's own range."""
+    tt.say("tree, largest values of fp16", dim)
+    for rows in ROWS:
+        monkeypatch.setenv("TVARA_TREE_ROWS", rows)
+        b = tt.Batch(device, oracle, 4, 2, dim, [35, 700], [tt.bushy(6, 2), [-1] * 20], seed=9)
+        b.tv[3, 7], b.tv[8, 2] = 65519.0, -65519.0
+        tt.agree(b.run("f32x3"), b.want(), "f32x3")

@@ -54,7 +54,18 @@ constexpr int kBufferWord3 = 0x00020000;  // gfx9 buffer descriptor, dword 3
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-__device__ __forceinline__ float finite_or_zero(float x) { return __builtin_isfinite(x) ? x : 0.f; }
+// Whether a product with x passes zeros on: x is finite, and (kParts) so is the nearest
+// fp16 number, x's first part.
+template <bool kParts>
+__device__ __forceinline__ bool fits(float x) {
+    return kParts ? __builtin_fabsf(x) < 65520.f : __builtin_isfinite(x);
+}
+// What a row that sees such a value is given of it: in parts, something that is not
+// finite, which the launch reports.
+template <bool kParts>
+__device__ __forceinline__ float unfit(float x) {
+    return kParts ? x * INFINITY : x;
+}
 
 // Where 64 runs of bytes start and how far they go, one a lane.
 struct Spans {
@@ -578,7 +589,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
             mask[nt] = live[nt] ? a.mask[static_cast<size_t>(tree.w + node[nt]) * a.words + (step - csteps)] : 0u;
-        float odd = 0.f;
+        bool odd = false;
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
             const float* kr = kb + static_cast<size_t>(min(n0 + 16 * mt + r16, nodes - 1)) * a.row_stride;
@@ -591,13 +602,13 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
                 for (int h = 0; h < H; ++h) {
                     v[mt][i][h] = *reinterpret_cast<const f32x4*>(vr + vcol(h, r16));
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) odd = fmaf(v[mt][i][h][j], 0.f, odd);
+                    for (int j = 0; j < 4; ++j) odd |= !fits<kX3>(v[mt][i][h][j]);
                 }
             }
         }
         scores(from_f32([&](int mt, int c) __attribute__((always_inline)) { return k[mt][c]; }));
         softmax(std::true_type{}, [&](int mt, int i, int nt) { return (mask[nt] >> (16 * mt + 4 * g + i) & 1u) != 0; });
-        const bool plain = !__any(odd != 0.f);  // (0, or NaN where a value is not finite)
+        const bool plain = !__any(odd);
         if (!plain) {
             // Zero times such a value would reach rows that do not see it: it is
             // zero in the product, and added below to the rows that do.
@@ -608,7 +619,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
 #pragma unroll
                     for (int h = 0; h < H; ++h)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) v[mt][i][h][j] = finite_or_zero(v[mt][i][h][j]);
+                        for (int j = 0; j < 4; ++j) v[mt][i][h][j] = fits<kX3>(v[mt][i][h][j]) ? v[mt][i][h][j] : 0.f;
         }
         output(values_from_f32(v));
         if (plain) continue;
@@ -631,7 +642,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
                             const f32x4 x = *reinterpret_cast<const f32x4*>(vr + vcol(h, 4 * g + o));
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                if (on && !__builtin_isfinite(x[j])) acc[4 * h + j][nt][o] = fmaf(p, x[j], acc[4 * h + j][nt][o]);
+                                if (on && !fits<kX3>(x[j]))
+                                    acc[4 * h + j][nt][o] = fmaf(p, unfit<kX3>(x[j]), acc[4 * h + j][nt][o]);
                         }
                 }
             }
@@ -731,7 +743,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
     constexpr int TK = 128 / D;      // key tiles of 16 a wave takes
     constexpr int VO = 4 * KC, OPS = VO + 8 * H;  // operands of a step: hi, lo of [mt][kc] keys, then of the value tiles
     __shared__ u32x4 parts[2][S][OPS][64];
-    __shared__ int odds[2][S][H];    // the tree's own values: some are not finite
+    __shared__ int odds[2][S][H];    // the tree's own values: some do not fit
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, r16 = lane & 15;
     const Item it = item_of(a, blockIdx.x);
@@ -886,17 +898,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
             }
         } else {
             const bool tail = step >= csteps;
-            float odd = 0.f;
+            bool odd = false;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 f32x4 y[2] = {{x[0][j], x[1][j], x[2][j], x[3][j]}, {x[4][j], x[5][j], x[6][j], x[7][j]}};
                 if (tail) {
-                    // Zero times a value that is not finite would reach rows that do not
+                    // Zero times a value that does not fit would reach rows that do not
                     // see it: it is zero in the product, and added to the rows that do.
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        odd = fmaf(y[e / 4][e % 4], 0.f, odd);
-                        y[e / 4][e % 4] = finite_or_zero(y[e / 4][e % 4]);
+                        const bool in = fits<true>(y[e / 4][e % 4]);
+                        odd |= !in;
+                        y[e / 4][e % 4] = in ? y[e / 4][e % 4] : 0.f;
                     }
                 }
                 u32x4 hi, lo;
@@ -911,7 +924,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
                 parts[buf][sub][VO + 2 * (4 * vh + j) + 1][lane] = lo;
             }
             if (tail) {
-                const bool any = __any(odd != 0.f);
+                const bool any = __any(odd);
                 if (lane == 0) odds[buf][sub][vh] = any;
             }
         }
@@ -1071,7 +1084,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeA
                                 const f32x4 y = *reinterpret_cast<const f32x4*>(vr + 64 * h + 4 * (4 * g + o));
 #pragma unroll
                                 for (int j = 0; j < 4; ++j)
-                                    if (on && !__builtin_isfinite(y[j])) acc[4 * h + j][nt][o] = fmaf(p, y[j], acc[4 * h + j][nt][o]);
+                                    if (on && !fits<true>(y[j]))
+                                        acc[4 * h + j][nt][o] = fmaf(p, unfit<true>(y[j]), acc[4 * h + j][nt][o]);
                             }
                     }
             }
