@@ -136,3 +136,13 @@ def test_largest_values_of_the_parts(device, oracle, monkeypatch, dim):
         b = tt.Batch(device, oracle, 4, 2, dim, [35, 700], [tt.bushy(6, 2), [-1] * 20], seed=9)
         b.tv[3, 7], b.tv[8, 2] = 65519.0, -65519.0
         tt.agree(b.run("f32x3"), b.want(), "f32x3")
+
+
+@pytest.mark.parametrize("gap", [0.5, 12, 21])
+@pytest.mark.parametrize("dim", [32, 96])
+def test_long_sums_of_the_row_kernel(device, oracle, monkeypatch, dim, gap):
+    """Layouts without tiles: as many waves as take a whole context each."""
+    tt.say("tree, rows, long sums", dim, gap)
+    monkeypatch.setattr(Sink, "TREES", 1024)
+    b = Sink(device, oracle, dim, 32768, gap, False)
+    tt.agree(b.run("f32"), b.want(), "f32")
