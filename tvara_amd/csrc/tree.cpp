@@ -29,6 +29,9 @@ PlanRegion::~PlanRegion() {
 }
 
 void PlanRegion::place(DeviceCache& c, std::vector<Section>& sections) {
+    // blocks that wait for their zeros get them now: none is handed out while a plan is
+    // not stale, and a launch may be captured, whose replays would clear them again
+    c.flush();
     size_t total = 0, copied = 0;
     for (Section& s : sections) {
         s.at = total;
@@ -346,7 +349,6 @@ void TreePlan::launch(int layer, const float* q, const float* keys, const float*
     if (row_stride > kMaxRowStride) throw std::invalid_argument("token rows too far apart");
     if (!rows) return;
     cache->check_device();
-    cache->flush();
     cache->enter(s);
     char* d = region.device();
     TreeArgs a{};
@@ -491,7 +493,6 @@ void SlotPlan::write(const int64_t* slots, const int32_t* rows, size_t n, const 
         throw std::invalid_argument("device buffers must be 16-byte aligned");
     if (!n) return;
     cache->check_device();
-    cache->flush();
     cache->enter(s);
     WriteArgs a{};
     a.pool = cache->pool();
