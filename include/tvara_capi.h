@@ -215,7 +215,10 @@ TVARA_API void tvara_kv_cache_destroy(tvara_kv_cache* cache);
  * CacheGeometry::elements_per_block (kv.hpp:18-23) floats; Q8_0 blocks are 34
  * bytes per 32 elements. */
 TVARA_API size_t tvara_kv_block_bytes(tvara_kv_cache* cache);
-/* Issue device work on `stream` (a hipStream_t; NULL = null stream). */
+/* Issue device work on `stream` (a hipStream_t; NULL = null stream).  A launch of a
+ * plan on another stream waits for this one, and this one for it; so launches are
+ * captured on this stream, or one that has joined its capture, and fail with
+ * TVARA_INVALID in any other capture. */
 TVARA_API int tvara_kv_set_stream(tvara_kv_cache* cache, void* stream);
 /* Wait for the handle's stream. */
 TVARA_API int tvara_kv_synchronize(tvara_kv_cache* cache);
@@ -437,7 +440,8 @@ TVARA_API tvara_tree_plan* tvara_tree_plan_create(tvara_kv_cache* cache, const u
  * 2^23), device pointers, asynchronous on `stream` (NULL: the cache's).  What a node
  * does not see never reaches its row, whatever it holds.  Launches and acceptances of
  * one plan share its workspace: they run one after the other, on one stream or in
- * the caller's order, captured ones too; two plans share nothing. */
+ * the caller's order, captured ones too (on the cache's stream: tvara_kv_set_stream);
+ * two plans share nothing. */
 TVARA_API int tvara_tree_plan_launch(tvara_tree_plan* plan, size_t layer, const float* q, const float* keys,
                                      const float* values, size_t row_stride, float* out, void* stream);
 /* Greedy acceptance: e = first[i]; while a child of the current node (a root at

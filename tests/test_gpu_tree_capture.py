@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import test_gpu_tree as tt
-from tvara_amd import attention, hip
+from tvara_amd import _capi, attention, hip
 from tvara_amd.kv import SlotPlan
 
 pytestmark = pytest.mark.gpu
@@ -38,5 +38,60 @@ def test_replays_leave_blocks_handed_out_before(device, oracle, what):
             assert np.array_equal(b.cache.block_data(h), mine)
         if what == "attention":
             tt.agree(d.out.numpy()[: b.rows], b.want(), "f32")
+        del graph
+    b.cache.set_stream(None)
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_captures_on_another_stream_are_refused(device, oracle, own):
+    """The cache's stream takes no part in such a capture: every launch is refused, the
+    capture goes on, and so does eager work."""
+    tt.say("captures on another stream", own)
+    b = tt.Batch(device, oracle, 4, 2, 64, [40, 30], [tt.chain(3), [-1]], seed=2)
+    streams = hip.Stream(), hip.Stream()
+    b.cache.set_stream(streams[1].h if own else None)
+    up, s = hip.DeviceArray.from_numpy, streams[0].h
+    with tt.hip_rows(b) as d:
+        tree, slots = attention.TreePlan(b.cache, b.seqs, b.nodes, b.parents, 4, 1 << 20), SlotPlan(b.cache, b.seqs)
+        decode = attention.DecodePlan(b.cache, b.seqs, 4, 1 << 20)
+        prefill = attention.PrefillPlan(b.cache, b.seqs, [0, 0], [2, 2], 4, 1 << 20, precision="f32")
+        ints, words, logits = up(np.zeros(64, np.int32)), up(np.full(16, -1, np.int64)), up(np.zeros((4, 8), np.float32))
+        calls = [lambda: tree.launch(0, d.q.ptr, d.k.ptr, d.v.ptr, d.out.ptr, stream=s),
+                 lambda: tree.accept(ints.ptr, ints.ptr, logits.ptr, 8, ints.ptr + 64, 4, ints.ptr + 128, ints.ptr + 192, stream=s),
+                 lambda: slots.build(ints.ptr, ints.ptr, 4, 8, slots_ptr=words.ptr, stream=s),
+                 lambda: slots.write(words.ptr, None, 4, d.k.ptr, d.v.ptr, 4, b.w, b.w, stream=s),
+                 lambda: decode.launch(0, d.q.ptr, d.out.ptr, stream=s),
+                 lambda: prefill.launch(0, d.q.ptr, d.out.ptr, stream=s)]
+
+        def body():
+            for call in calls:
+                with pytest.raises(_capi.InvalidArgument, match="captured on the cache's stream"):
+                    call()
+
+        graph = tt.Graph(s, body)
+        for call in calls:
+            call()
+        tree.check(), slots.check(), decode.check(), prefill.check()
+        del graph
+    tt.agree(b.run(), b.want(), "f32")
+    b.cache.set_stream(None)
+
+
+def test_a_capture_that_forks_and_joins(device, oracle):
+    """Captured from the cache's stream, launches on another one join the capture and
+    come back to it."""
+    tt.say("tree captured, two streams")
+    b = tt.Batch(device, oracle, 4, 2, 64, [400, 30], [tt.chain(3), [-1]], seed=2)
+    own, other = hip.Stream(), hip.Stream()
+    b.cache.set_stream(own.h)
+    with tt.hip_rows(b) as d:
+        plan = attention.TreePlan(b.cache, b.seqs, b.nodes, b.parents, 4, 1 << 20)
+        graph = tt.Graph(own.h, lambda: plan.launch(0, d.q.ptr, d.k.ptr, d.v.ptr, d.out.ptr, stream=other.h))
+        for _ in range(3):
+            d.out.zero()
+            hip.synchronize()
+            graph.replay()
+            tt.agree(d.out.numpy()[: b.rows], b.want(), "f32")
+            tt.agree(b.run(), b.want(), "f32")
         del graph
     b.cache.set_stream(None)

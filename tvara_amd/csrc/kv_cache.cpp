@@ -109,6 +109,15 @@ void DeviceCache::flush() {
 
 void DeviceCache::enter(hipStream_t s) {
     if (s == stream_) return;
+    // The cache's stream waits for s afterwards: were s captured and this stream not, that
+    // would draw it into a capture that never joins it again, which ends the process.
+    hipStreamCaptureStatus on = hipStreamCaptureStatusNone, own = hipStreamCaptureStatusNone;
+    unsigned long long id = 0, own_id = 0;
+    TVARA_HIP(hipStreamGetCaptureInfo(s, &on, &id));
+    if (on != hipStreamCaptureStatusNone) {
+        if (stream_) TVARA_HIP(hipStreamGetCaptureInfo(stream_, &own, &own_id));
+        if (own != on || own_id != id) throw std::invalid_argument("launches are captured on the cache's stream only");
+    }
     if (!ordered_[0]) TVARA_HIP(hipEventCreateWithFlags(&ordered_[0], hipEventDisableTiming));
     TVARA_HIP(hipEventRecord(ordered_[0], stream_));
     TVARA_HIP(hipStreamWaitEvent(s, ordered_[0], 0));
