@@ -285,3 +285,42 @@ def test_refusals_change_nothing(tmp_path, hidden):
     assert paths == [[0, 1]] and (cache.length(a), cache.length(b)) == (10, 11)
     model.close()
     assert message(verify, [a], [[-1]], [[1]], [fa]) == "Model is closed"
+
+
+def test_one_deep_tree_among_many_sequences(tmp_path):
+    """Sequences times the deepest tree beyond any launch: what is written goes by the
+    accepted nodes."""
+    spec = gf.LlamaSpec(matrix_type=gf.T_Q8_0, hidden=256, intermediate=512, heads=4, kv_heads=2, vocab=300, context=1100)
+    model = native.NativeModel(spec.write(tmp_path / "m.gguf"), max_blocks=64, block_tokens=16)
+    n, prompt = 16400, [int(t) for t in np.random.default_rng(7).integers(0, spec.vocab, 20)]
+    seqs = [model.new_sequence() for _ in range(n)]
+    plain = Greedy(model, prompt)
+    first = [0] * n
+    for i in (0, n - 1):
+        first[i] = choice(model.prefill(seqs[i], prompt))[0]
+    right = plain.choices(6)
+    assert len(right) == 6
+    wrong = [(right[5] + 1) % spec.vocab] * (1024 - 5)
+    parents, tokens = [[] for _ in range(n)], [[] for _ in range(n)]
+    parents[0], tokens[0] = [-1, 0], right[:2]
+    parents[-1], tokens[-1] = list(range(-1, 1023)), right[:5] + wrong
+    paths, after = model.verify_trees(seqs, parents, tokens, first)
+    assert paths[0] == [0, 1] and after[0] == right[2]
+    assert paths[-1] == list(range(5)) and after[-1] == right[5]
+    assert not any(paths[1:-1]) and after[1:-1] == [0] * (n - 2)
+    cache = model.cache()
+    assert [cache.length(s) for s in (seqs[0], seqs[1], seqs[-1])] == [22, 0, 25]
+    plain.take(right[:5] + [9])
+    assert close(model.logits(seqs[-1], 9), plain.logits)
+    cache.audit()
+
+
+def test_no_node_accepted(tmp_path):
+    spec = gf.LlamaSpec(matrix_type=gf.T_Q8_0, heads=8, kv_heads=2, hidden=128, intermediate=256)
+    model = native.NativeModel(spec.write(tmp_path / "m.gguf"), max_blocks=8, block_tokens=4)
+    prompt = [int(t) for t in np.random.default_rng(5).integers(0, spec.vocab, 10)]
+    a = model.new_sequence()
+    first = choice(model.prefill(a, prompt))[0]
+    wrong = (first + 1) % spec.vocab
+    assert model.verify_trees([a], [[-1, 0, -1]], [[wrong] * 3], [first]) == ([[]], [first])
+    assert model.cache().length(a) == 10

@@ -424,11 +424,11 @@ void DeviceModel::verify_trees(const uint64_t* sequences, size_t n, const size_t
     }
     ensure_batch(rows, rows);
     hipStream_t s = cache_->stream();
-    // starts, expected tokens | accepted counts, next tokens, paths
-    const size_t part = (n + 3) / 4 * 4, words = 4 * part + n * deepest;
-    auto* d = static_cast<int32_t*>(verify_.ensure(words * sizeof(int32_t)));
-    auto* slots = static_cast<int64_t*>(verify_slots_.ensure(n * deepest * sizeof(int64_t)));
-    auto* host = static_cast<int32_t*>(verify_host_.acquire(words * sizeof(int32_t)));
+    // starts, expected tokens | accepted counts, next tokens, paths | the paths' rows, one after the other
+    const size_t part = (n + 3) / 4 * 4, words = 4 * part + n * deepest, rows_at = (words + 3) / 4 * 4;
+    auto* d = static_cast<int32_t*>(verify_.ensure((rows_at + rows) * sizeof(int32_t)));
+    auto* slots = static_cast<int64_t*>(verify_slots_.ensure(rows * sizeof(int64_t)));
+    auto* host = static_cast<int32_t*>(verify_host_.acquire((rows_at + rows) * sizeof(int32_t)));
     for (size_t i = 0; i < n; ++i) {
         host[i] = static_cast<int32_t>(lengths[i]);
         host[part + i] = static_cast<int32_t>(first[i]);
@@ -447,15 +447,20 @@ void DeviceModel::verify_trees(const uint64_t* sequences, size_t n, const size_t
     TVARA_HIP(hipMemcpyAsync(host + 2 * part, counts, (words - 2 * part) * sizeof(int32_t), hipMemcpyDeviceToHost, s));
     verify_host_.release(s);
     plan.check();  // (waits for the stream)
-    TVARA_HIP(hipStreamSynchronize(s));
     std::vector<size_t> taken(host + 2 * part, host + 2 * part + n);
+    size_t total = 0;
+    for (size_t i = 0; i < n; total += taken[i++]) std::copy_n(host + 4 * part + i * deepest, taken[i], host + rows_at + total);
     cache_->reserve(sequences, n, taken.data());
     try {
-        SlotPlan map;
-        map.build(cache_.get(), sequences, n);
-        map.map(d, counts, deepest, n * deepest, nullptr, nullptr, slots, nullptr, 0, s);
-        map.write(slots, paths, n * deepest, at(bk_, 0), at(bv_, 0), rows, c.kv_width(), rows * c.kv_width(), s);
-        map.check();
+        if (total) {
+            TVARA_HIP(hipMemcpyAsync(d + rows_at, host + rows_at, total * sizeof(int32_t), hipMemcpyHostToDevice, s));
+            verify_host_.release(s);
+            SlotPlan map;
+            map.build(cache_.get(), sequences, n);
+            map.map(d, counts, 0, total, nullptr, nullptr, slots, nullptr, 0, s);
+            map.write(slots, d + rows_at, total, at(bk_, 0), at(bv_, 0), rows, c.kv_width(), rows * c.kv_width(), s);
+            map.check();
+        }
     } catch (...) {
         for (size_t i = 0; i < n; ++i) cache_->truncate(sequences[i], lengths[i]);
         throw;
