@@ -37,3 +37,19 @@ def test_trees_of_unequal_lists_are_refused():
     for nodes, parents in (([1], [-1, 0]), ([1, 2], [-1, -1]), ([], [])):
         with pytest.raises(_capi.InvalidArgument):
             attention._trees([1, 2], nodes, parents, None)
+
+
+@pytest.mark.parametrize("parents,visible", [([-1, 2**32 - 1], None), (np.array([-1, 2**32]), None), ([-1, 0.5], None),
+                                             ([-1, 0], -1), ([-1, 0], np.array([-1])), ([-1, 0], np.array([3.5]))])
+def test_numbers_that_would_change_are_refused(parents, visible):
+    """A parent of 2^32 - 1 is no -1, a visible length of -1 not all of the sequence."""
+    with pytest.raises(_capi.InvalidArgument):
+        attention._trees([1], [2], parents, visible)
+
+
+def test_whole_numbers_of_any_type_are_taken():
+    for dtype in (np.int64, np.int32, np.int8, np.float64):
+        (seqs, nodes, parents, visible), _ = attention._trees([1, 2], np.array([2, 0], dtype), np.array([-1, 0], dtype), [7, 0])
+        assert nodes.tolist() == [2, 0] and parents.tolist() == [-1, 0] and visible.tolist() == [7, 0]
+    (_, nodes, parents, _), _ = attention._trees([1], [0], [], None)
+    assert nodes.tolist() == [0] and parents.size == 0

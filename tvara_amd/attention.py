@@ -166,14 +166,24 @@ class PrefillPlan:
         self.close()
 
 
+def _whole(values, dtype, what):
+    """values as an array of dtype, none of which it changes."""
+    given = np.asarray(values)
+    with np.errstate(invalid="ignore"):
+        out = np.ascontiguousarray(given.astype(dtype))
+    if not (given == out).all():
+        raise InvalidArgument(f"{what} are not whole numbers of their range")
+    return out
+
+
 def _trees(seqs, nodes, parents, visible):
     seqs = np.ascontiguousarray(seqs, dtype=np.uint64).reshape(-1)
-    nodes = np.ascontiguousarray(nodes, dtype=np.uintp).reshape(-1)
-    parents = np.ascontiguousarray(parents, dtype=np.int32).reshape(-1)
+    nodes = _whole(nodes, np.uintp, "nodes").reshape(-1)
+    parents = _whole(parents, np.int32, "parents").reshape(-1)
     if nodes.size != seqs.size or int(nodes.sum()) != parents.size:
         raise InvalidArgument("sequences, nodes and parents differ in length")
     if visible is not None:
-        visible = np.ascontiguousarray(np.broadcast_to(np.asarray(visible, dtype=np.uintp), seqs.shape))
+        visible = np.ascontiguousarray(np.broadcast_to(_whole(visible, np.uintp, "visible lengths"), seqs.shape))
     vp = visible.ctypes.data_as(C.POINTER(_sz)) if visible is not None else None
     keep = (seqs, nodes, parents, visible)
     return keep, (seqs.ctypes.data_as(C.POINTER(C.c_uint64)), nodes.ctypes.data_as(C.POINTER(_sz)),
