@@ -424,11 +424,15 @@ TVARA_API void tvara_prefill_plan_destroy(tvara_prefill_plan* plan);
 /* The listed trees, resident: sequences[i] (which may be listed again) is seen up
  * to visible[i] tokens (NULL: all of it) and has nodes[i] nodes (0 to 1,024),
  * parents [sum nodes] with -1 <= parents[j] < j within its tree.  precision
- * TVARA_ATTN_F32, or TVARA_ATTN_F32X3 as tvara_attn_prefill has it where the
- * layout has such tiles (head_dim 64 or 128, blocks of a power of two from 16
- * tokens) and f32 elsewhere; bf16 is refused.  f32x3 holds queries, keys and values
- * alike as two fp16 parts: 22 bits, 2^-25 at the least, and what leaves fp16's range
- * (65,504; queries times 1.44 / sqrt(head_dim)) is reported by tvara_tree_plan_check.
+ * TVARA_ATTN_F32, or TVARA_ATTN_F32X3 where the layout has such tiles (head_dim 64 or
+ * 128, blocks of a power of two from 16 tokens) and f32 elsewhere; bf16 is refused.
+ * f32x3 holds queries (times 1.44 / sqrt(head_dim)), keys, values and weights alike as
+ * two fp16 parts, where tvara_attn_prefill has bf16 parts of the last two.  That is 22
+ * bits of each, but nothing finer than 2^-25 (of a weight: 2^-36 of its row's largest),
+ * so it is meant for values of an ordinary size (root mean square) of 0.003 or more and
+ * keys of one up to 70: values of 0.001 are off by 1.7e-5 of it, of 0.0001 by 1.7e-4,
+ * where f32 knows no such limits.  What leaves fp16's range (65,504) is reported by
+ * tvara_tree_plan_check.
  * Launching fails with TVARA_INVALID once the cache has changed.  All trees together
  * have at most 16,700,000 nodes, and nodes * heads * head_dim stays below 2^32. */
 TVARA_API tvara_tree_plan* tvara_tree_plan_create(tvara_kv_cache* cache, const uint64_t* sequences, size_t count,

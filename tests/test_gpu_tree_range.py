@@ -1,5 +1,5 @@
 """Tree attention over the whole range of its inputs: weights far below a row's
-largest, values that f32x3's fp16 parts do not hold.  The bars are test_gpu_tree's unless a test derives its own."""
+largest, values far from one, values that f32x3's fp16 parts do not hold.  The bars are test_gpu_tree's unless a test derives its own."""
 
 import numpy as np
 import pytest
@@ -146,3 +146,45 @@ def test_long_sums_of_the_row_kernel(device, oracle, monkeypatch, dim, gap):
     monkeypatch.setattr(Sink, "TREES", 1024)
     b = Sink(device, oracle, dim, 32768, gap, False)
     tt.agree(b.run("f32"), b.want(), "f32")
+
+
+@pytest.mark.parametrize("size", [1e4, 100.0, 0.01, 1e-3, 1e-4])
+@pytest.mark.parametrize("fmt", ["f32", "q8_0"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_sizes_of_values(device, oracle, monkeypatch, dim, fmt, size):
+    """f32 is as near at any size.  f32x3 holds a value to 2^-25 at the finest, off by
+    2^-25 / sqrt(3) as a deviation: outputs are the same means of values and of their
+    roundings, which are independent, so that they are off by 2^-25 / (sqrt(3) size)
+    more, here with half as much again for outputs that happen to be small."""
+    tt.say("tree, sizes of values", dim, fmt, size)
+    b = tt.Batch(device, oracle, 8, 2, dim, [300, 33, 1500], [tt.bushy(12, 4), tt.chain(20), tt.bushy(40, 9)], seed=dim, layers=1)
+    w, q8 = b.w, fmt == "q8_0"
+    b.cache = device.PagedCache(1, 2, dim, 16, 200, fmt=device.Q8_0 if q8 else device.F32)
+    b.seqs = []
+    for i, n in enumerate(b.lengths):
+        k, v = b.k[i], np.ascontiguousarray(b.v[i] * size, np.float32)
+        b.seqs.append(b.cache.create_sequence())
+        b.cache.append_many(b.seqs[i], k, v)
+        if q8:
+            k, v = (oracle.dequantize_q8_0(oracle.quantize_q8_0(np.ascontiguousarray(x, np.float32))).reshape(n, w) for x in (k, v))
+        b.k[i], b.v[i] = k, v
+    b.tv = np.ascontiguousarray(b.tv * size, np.float32)
+    want = b.want()
+    bars = {"f32": tt.NORM["f32"], "f32x3": tt.NORM["f32x3"] + 1.5 * 2.0 ** -25 / (np.sqrt(3) * size)}
+    for precision, rows in [("f32", "")] + [("f32x3", r) for r in ROWS]:
+        monkeypatch.setenv("TVARA_TREE_ROWS", rows)
+        off = np.linalg.norm(b.run(precision) - want) / np.linalg.norm(want)
+        assert off <= bars[precision], (precision, rows, off)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_sizes_of_keys(device, oracle, monkeypatch, dim, rows):
+    """Keys of 70 beside queries of 1/70: the scores are those of N(0,1), each off by
+    2^-25 / sqrt(3) * 70 sqrt(dim) * ln 2 as a deviation, 1e-5, which the mean of a
+    row's values is off by less than."""
+    tt.say("tree, sizes of keys", dim, rows)
+    monkeypatch.setenv("TVARA_TREE_ROWS", rows)
+    b = tt.Batch(device, oracle, 8, 2, dim, [300, 33], [tt.bushy(12, 4), tt.chain(20)], seed=dim, scale=70.0)
+    b.q = np.ascontiguousarray(b.q / 70, np.float32)
+    tt.agree(b.run("f32x3"), b.want(), "f32x3")
