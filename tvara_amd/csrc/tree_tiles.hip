@@ -2,14 +2,16 @@
 // or Q8_0 blocks of a power of two from 16 tokens.
 //
 // A row is a (node, query head) pair; the rows of one (tree, KV head) share its
-// keys.  A wave takes 16 * NT rows and walks keys 32 at a time ("a step"), all of
-// its operands in registers: no LDS and no barrier until its keys are done.
-//  S^T = K Q^T: the lane (g, r) = (l / 16, l % 16) loads four columns at a time of
-//    key r, which are the operands as they come, since the numbering of a
-//    contraction's terms is free as long as Q has the same.
-//  O^T = V^T P^T: lane (g, r) loads four columns of the keys 4g + i of each 16,
-//    so it holds V^T's operand for four output tiles (tile j: column j of every
-//    lane's four) and its own scores are P^T's.
+// keys.  A wave takes 16 * NT rows, whose queries, output and statistics stay in its
+// registers, and walks keys 32 at a time ("a step"), with no barrier until they are done.
+//  S^T = K Q^T: the lane (g, r) = (l / 16, l % 16) has four columns at a time of key r
+//    as operands, in an order of its own, since the numbering of a contraction's terms
+//    is free as long as Q has the same.  Q8_0 bytes are loaded so; keys of f32 blocks
+//    go as whole rows from memory into the wave's own part of LDS and are read from
+//    there so.
+//  O^T = V^T P^T: lane (g, r) loads four columns of the keys 4g + i of each 16 into
+//    registers, so it holds V^T's operand for four output tiles (tile j: column j of
+//    every lane's four) and its own scores are P^T's.
 // Steps are dealt in turn to the workgroup's waves, whose results meet in LDS.  A
 // long context is cut into runs, a workgroup each, that leave partials for a merge.
 // After the cached steps come those over the tree's own nodes, with a mask word a row.
@@ -19,8 +21,9 @@
 // running maximum that moves only where a step exceeds it by 2^8 (f32x3: 2^4).
 //
 // MI355X: f32, 16 contexts of 123 to 2,793 tokens with 6 to 24 nodes, 32 heads on 8
-// of 64: 45.3 us with the merge (floor 21: one read of K and V at a copy's rate), bound
-// by the longest workgroups and the f32 products (25 us, padded to 16 rows).
+// of 64: 45.6 us with the merge (floor 21: one read of K and V at a copy's rate), bound
+// by the longest workgroups and the f32 products (25 us, padded to 16 rows: the matrix
+// pipe is busy 58% of the time, the CUs' caches 88%).
 // f32x3, 16 contexts of 2,048 with 16 nodes, head_dim 128: 58.2 us, 4.6 TB/s.
 #include <algorithm>
 #include <limits>
@@ -730,10 +733,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 || !kX3 ? 2 : 1) void tree_til
 // an iteration of S steps.  Loads go through descriptors that end with the last
 // key, so that what lies behind it reads as zeros.
 //
-// MI355X, 16 contexts of 4,096 with 32 nodes, 32 heads on 8 of 128: 136 us with the
-// merge, 4.1 TB/s (a copy reads and writes 4.8); 8 contexts of 4,096 with 64 nodes, 64
-// heads on 8: 220 us, 3 x 314 TFLOP/s of fp16 products: the matrix pipe is busy half
-// of the time, and the vector instructions of two waves a SIMD (230 a step, beside
+// MI355X, 16 contexts of 4,096 with 32 nodes, 32 heads on 8 of 128: 140 us with the
+// merge, 4.0 TB/s (a copy reads and writes 4.8); 8 contexts of 4,096 with 64 nodes, 64
+// heads on 8: 224 us, 3 x 308 TFLOP/s of fp16 products: the matrix pipe is busy half
+// of the time, and the vector instructions of two waves a SIMD (250 a step, beside
 // 96 products) do not hide behind it.
 template <int D, bool kQ8>
 __global__ __launch_bounds__(64 * kWaves, 2) void tree_shared_kernel(const TreeArgs a) {
