@@ -218,7 +218,8 @@ TVARA_API size_t tvara_kv_block_bytes(tvara_kv_cache* cache);
 /* Issue device work on `stream` (a hipStream_t; NULL = null stream).  A launch of a
  * plan on another stream waits for this one, and this one for it; so launches are
  * captured on this stream, or one that has joined its capture, and fail with
- * TVARA_INVALID in any other capture. */
+ * TVARA_INVALID in any other capture.  What was issued on the stream before is not
+ * waited for: tvara_kv_synchronize first. */
 TVARA_API int tvara_kv_set_stream(tvara_kv_cache* cache, void* stream);
 /* Wait for the handle's stream. */
 TVARA_API int tvara_kv_synchronize(tvara_kv_cache* cache);

@@ -10,7 +10,7 @@ from tvara_amd.kv import SlotPlan
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("what", ["attention", "write"])
+@pytest.mark.parametrize("what", ["attention", "write", "decode", "prefill"])
 def test_replays_leave_blocks_handed_out_before(device, oracle, what):
     """A block that still waits for its zeros when a plan is made: a graph of the plan's
     launches does not clear it, however often it is replayed."""
@@ -24,6 +24,12 @@ def test_replays_leave_blocks_handed_out_before(device, oracle, what):
         if what == "attention":
             plan = attention.TreePlan(b.cache, b.seqs, b.nodes, b.parents, 4, 1 << 20)
             launch = lambda: plan.launch(0, d.q.ptr, d.k.ptr, d.v.ptr, d.out.ptr, stream=stream.h)  # noqa: E731
+        elif what == "decode":
+            plan = attention.DecodePlan(b.cache, b.seqs, 4, 1 << 20)
+            launch = lambda: plan.launch(0, d.q.ptr, d.out.ptr, stream=stream.h)  # noqa: E731
+        elif what == "prefill":
+            plan = attention.PrefillPlan(b.cache, b.seqs, [0], [3], 4, 1 << 20)
+            launch = lambda: plan.launch(0, d.q.ptr, d.out.ptr, stream=stream.h)  # noqa: E731
         else:
             plan = SlotPlan(b.cache, b.seqs)
             slots = up(np.full(4, -1, np.int64))

@@ -335,6 +335,9 @@ void attention_rows(const DeviceCache& c, const uint64_t* seqs, size_t count, si
 
 void AttnPlan::compute(DeviceCache* c, const std::vector<uint64_t>& seq_of_row, const std::vector<size_t>& cached,
                      const std::vector<uint8_t>& tail_rows, int h, size_t split_override) {
+    // blocks that wait for their zeros get them now: none is handed out while a plan is
+    // not stale, and a launch may be captured, whose replays would clear them again
+    c->flush();
     cache = c;
     epoch = c->epoch();
     heads = h;
@@ -639,7 +642,6 @@ void AttnPlan::launch(int layer, const float* q, const float* tail_k, const floa
         throw std::invalid_argument("invalid fused attention shape");
     if (with_tail && (!tail_k || !tail_v)) throw std::invalid_argument("plan expects tail K/V");
     if (!dev.tables) throw std::invalid_argument("attention plan is not placed");
-    cache->flush();
     cache->enter(s);
     DecodeArgs a{};
     a.pool = cache->pool();
@@ -907,6 +909,7 @@ void PrefillPlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, siz
         throw std::invalid_argument(
             "bf16 prefill needs f32 or Q8_0 blocks of 16 to 1,024 tokens (a power of two, under 2 GiB) and head_dim "
             "64 or 128");
+    c->flush();  // (as AttnPlan::compute)
     std::vector<int32_t> tab;
     std::vector<int4> sq(n);
     size_t row0 = 0;
@@ -944,7 +947,6 @@ void PrefillPlan::launch(int layer, const float* q, float* out, hipStream_t s) {
         return;
     }
     if (cache->epoch() != epoch) throw std::invalid_argument("attention plan is stale: the cache changed");
-    cache->flush();
     cache->enter(s);
     PrefillArgs a{};
     a.pool = cache->pool();

@@ -29,9 +29,7 @@ PlanRegion::~PlanRegion() {
 }
 
 void PlanRegion::place(DeviceCache& c, std::vector<Section>& sections) {
-    // blocks that wait for their zeros get them now: none is handed out while a plan is
-    // not stale, and a launch may be captured, whose replays would clear them again
-    c.flush();
+    c.flush();  // (as AttnPlan::compute)
     size_t total = 0, copied = 0;
     for (Section& s : sections) {
         s.at = total;
