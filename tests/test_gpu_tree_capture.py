@@ -17,6 +17,7 @@ def test_replays_leave_blocks_handed_out_before(device, oracle, what):
     tt.say("tree captured, block handed out", what)
     b = tt.Batch(device, oracle, 4, 2, 64, [40], [tt.chain(3)], seed=2, spare=2)
     stream = hip.Stream()
+    hip.synchronize()
     b.cache.set_stream(stream.h)
     h = b.cache.allocate()
     up = hip.DeviceArray.from_numpy
@@ -45,6 +46,7 @@ def test_replays_leave_blocks_handed_out_before(device, oracle, what):
         if what == "attention":
             tt.agree(d.out.numpy()[: b.rows], b.want(), "f32")
         del graph
+    hip.synchronize()
     b.cache.set_stream(None)
 
 
@@ -55,6 +57,7 @@ def test_captures_on_another_stream_are_refused(device, oracle, own):
     tt.say("captures on another stream", own)
     b = tt.Batch(device, oracle, 4, 2, 64, [40, 30], [tt.chain(3), [-1]], seed=2)
     streams = hip.Stream(), hip.Stream()
+    hip.synchronize()
     b.cache.set_stream(streams[1].h if own else None)
     up, s = hip.DeviceArray.from_numpy, streams[0].h
     with tt.hip_rows(b) as d:
@@ -80,6 +83,7 @@ def test_captures_on_another_stream_are_refused(device, oracle, own):
         tree.check(), slots.check(), decode.check(), prefill.check()
         del graph
     tt.agree(b.run(), b.want(), "f32")
+    hip.synchronize()
     b.cache.set_stream(None)
 
 
@@ -89,6 +93,7 @@ def test_a_capture_that_forks_and_joins(device, oracle):
     tt.say("tree captured, two streams")
     b = tt.Batch(device, oracle, 4, 2, 64, [400, 30], [tt.chain(3), [-1]], seed=2)
     own, other = hip.Stream(), hip.Stream()
+    hip.synchronize()
     b.cache.set_stream(own.h)
     with tt.hip_rows(b) as d:
         plan = attention.TreePlan(b.cache, b.seqs, b.nodes, b.parents, 4, 1 << 20)
@@ -100,4 +105,5 @@ def test_a_capture_that_forks_and_joins(device, oracle):
             tt.agree(d.out.numpy()[: b.rows], b.want(), "f32")
             tt.agree(b.run(), b.want(), "f32")
         del graph
+    hip.synchronize()
     b.cache.set_stream(None)
