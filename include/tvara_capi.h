@@ -63,6 +63,7 @@ typedef struct tvara_prefill_plan tvara_prefill_plan;
 typedef struct tvara_radix tvara_radix;
 typedef struct tvara_tree_plan tvara_tree_plan;
 typedef struct tvara_slot_plan tvara_slot_plan;
+typedef struct tvara_score_plan tvara_score_plan;
 
 /* BlockHandle (kv.hpp:35) */
 typedef struct {
@@ -471,6 +472,44 @@ TVARA_API int tvara_attn_tree(tvara_kv_cache* cache, const uint64_t* sequences, 
                               size_t context, const size_t* visible, const size_t* nodes, const int32_t* parents,
                               const float* q, const float* keys, const float* values, float* out, int precision,
                               int device_ptrs);
+
+/* ----------------------------------------------------------- scored attention
+ *
+ * Attention of cached rows whose scores are more than a product: row r of position p
+ * (packed, one sequence after the other: start[i] .. start[i] + rows[i] - 1 of
+ * sequences[i], one row for a decoded token, many for a prompt's chunk, both in one
+ * batch) and query head h have, over the keys first[r] <= k < end[r],
+ *   s_k = scale * q . k;  where cap > 0: s_k = cap * tanh(s_k / cap);
+ *   s_k -= slopes[h] * |p - k|;  out = sum_k softmax(s)_k v_k
+ * and zeros where a row sees no key.  The rows' own tokens are in the cache
+ * (tvara_slot_plan_rotate, _write, or appends put them there).  first NULL: 0, end
+ * NULL: p + 1; with both, windows, prefixes that see all of themselves, and packed
+ * documents are ranges.  scale 0: 1 / sqrt(head_dim); slopes NULL: none.  f32
+ * arithmetic, or products of as many bits; any layout (fast: head_dim 64 or 128,
+ * blocks of a power of two from 16 tokens).  What a row does not see never reaches
+ * it, whatever it holds; a value that is not finite makes its column of the rows that
+ * see it not finite.  The reference has causal attention alone (attention.hpp:57-89).
+ *
+ * Launching fails with TVARA_INVALID once the cache has changed.  rows * heads *
+ * head_dim stays below 2^32 in all. */
+TVARA_API tvara_score_plan* tvara_score_plan_create(tvara_kv_cache* cache, const uint64_t* sequences, size_t count,
+                                                    size_t heads, size_t context, const size_t* start,
+                                                    const size_t* rows, const size_t* first, const size_t* end,
+                                                    float scale, float cap, const float* slopes);
+/* q and out f32 [sum rows][heads * head_dim], device pointers, asynchronous on
+ * `stream` (NULL: the cache's).  Launches of one plan share its workspace: they run
+ * one after the other, on one stream or in the caller's order, captured ones too (on
+ * the cache's stream: tvara_kv_set_stream); two plans share nothing. */
+TVARA_API int tvara_score_plan_launch(tvara_score_plan* plan, size_t layer, const float* q, float* out, void* stream);
+/* Synchronise the plan's last launch and report a score that was not finite. */
+TVARA_API int tvara_score_plan_check(tvara_score_plan* plan);
+TVARA_API void tvara_score_plan_destroy(tvara_score_plan* plan);
+/* A plan, one launch and its check in one synchronous call: host pointers, or
+ * device pointers where device_ptrs is nonzero. */
+TVARA_API int tvara_attn_score(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, size_t layer, size_t heads,
+                               size_t context, const size_t* start, const size_t* rows, const size_t* first,
+                               const size_t* end, float scale, float cap, const float* slopes, const float* q, float* out,
+                               int device_ptrs);
 
 /* The block ids of the listed sequences, resident (at most 65,535); calls fail
  * with TVARA_INVALID once the cache's tables have changed. */

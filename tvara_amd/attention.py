@@ -7,7 +7,9 @@
   MFMA tiles;
 * ``DecodePlan`` -- resident block tables for repeated device launches;
 * ``TreePlan`` / ``tree_batch`` -- trees of drafted tokens over cached
-  sequences: their attention and their greedy acceptance.
+  sequences: their attention and their greedy acceptance;
+* ``ScorePlan`` / ``score_batch`` -- attention with capped or biased scores,
+  each row within a range of keys of its own (``visible_ranges``).
 """
 
 from __future__ import annotations
@@ -239,6 +241,108 @@ class TreePlan:
     def close(self):
         if getattr(self, "h", None):
             self.lib.tvara_tree_plan_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        self.close()
+
+
+def visible_ranges(starts, counts, window=None, prefix=None, document=None):
+    """(first, end) of the keys that each row sees, for ScorePlan: the text up to
+    itself and, where given, of that
+
+    * window: itself and the window - 1 tokens before it;
+    * prefix (one for each sequence): rows of a sequence's first prefix tokens
+      see all of those;
+    * document (one for each row): no token before the first of its document.
+    """
+    starts = _whole(starts, np.uintp, "starts").reshape(-1)
+    counts = _whole(counts, np.uintp, "counts").reshape(-1)
+    if starts.size != counts.size:
+        raise InvalidArgument("starts and counts differ in length")
+    seq = np.repeat(np.arange(counts.size), counts.astype(np.int64))
+    before = np.concatenate([[0], np.cumsum(counts)[:-1]]).astype(np.int64) if counts.size else np.zeros(0, np.int64)
+    pos = starts.astype(np.int64)[seq] + np.arange(seq.size) - before[seq]
+    first, end = np.zeros(seq.size, np.int64), pos + 1
+    if window is not None:
+        if window < 1:
+            raise InvalidArgument("a window has at least the row itself")
+        first = np.maximum(first, end - int(min(window, 1 << 62)))
+    if document is not None:
+        document = _whole(document, np.int64, "documents").reshape(-1)
+        if document.size != seq.size:
+            raise InvalidArgument("one document start for each row")
+        first = np.maximum(first, document)
+    if prefix is not None:
+        whole = np.broadcast_to(_whole(prefix, np.int64, "prefixes"), counts.shape)[seq]
+        end = np.where(pos < whole, whole, end)
+    return first.astype(np.uintp), end.astype(np.uintp)
+
+
+def _scored(seqs, starts, counts, heads, first, end, slopes):
+    seqs = np.ascontiguousarray(seqs, dtype=np.uint64).reshape(-1)
+    starts = _whole(starts, np.uintp, "starts").reshape(-1)
+    counts = _whole(counts, np.uintp, "counts").reshape(-1)
+    if not seqs.size == starts.size == counts.size:
+        raise InvalidArgument("sequences, starts and counts differ in length")
+    rows = int(counts.sum())
+    if first is not None:
+        first = _whole(first, np.uintp, "first keys").reshape(-1)
+    if end is not None:
+        end = _whole(end, np.uintp, "ends of keys").reshape(-1)
+    if any(x is not None and x.size != rows for x in (first, end)):
+        raise InvalidArgument("one range of keys for each row")
+    if slopes is not None:
+        slopes = _f32(slopes).reshape(-1)
+        if slopes.size != heads:
+            raise InvalidArgument("one slope for each query head")
+
+    def sizes(x):
+        return x.ctypes.data_as(C.POINTER(_sz)) if x is not None else None
+
+    keep = (seqs, starts, counts, first, end, slopes)
+    return rows, keep, (seqs.ctypes.data_as(C.POINTER(C.c_uint64)), sizes(starts), sizes(counts), sizes(first), sizes(end),
+                        _ptr(slopes))
+
+
+def score_batch(cache, q, seqs, starts, counts, layer, heads, context, first=None, end=None, scale=None, cap=0.0,
+                slopes=None):
+    """Scored attention (tvara_attn_score) of the cached rows starts[i] ..
+    starts[i] + counts[i] - 1 of seqs[i], packed: q [rows, heads * head_dim]."""
+    rows, keep, (sp, st, ct, fp, ep, bp) = _scored(seqs, starts, counts, heads, first, end, slopes)
+    hidden = heads * cache.head_dim
+    q = _f32(q).reshape(rows, hidden)
+    out = np.empty((max(rows, 1), hidden), np.float32)
+    _capi.check(cache.lib.tvara_attn_score(cache.h, sp, keep[0].size, layer, heads, context, st, ct, fp, ep, scale or 0.0,
+                                           cap, bp, _ptr(q), _ptr(out), 0))
+    return out[:rows]
+
+
+class ScorePlan:
+    """Resident rows of scored attention over cached sequences
+    (tvara_score_plan_*): scores are scale * q.k, capped as cap * tanh(s / cap)
+    where cap is above 0, less slopes[head] times the distance of key and row;
+    row r sees the keys first[r] .. end[r] - 1 (None: from 0, to itself)."""
+
+    def __init__(self, cache, seqs, starts, counts, heads, context, first=None, end=None, scale=None, cap=0.0, slopes=None):
+        self.cache = cache
+        self.lib = cache.lib
+        self.rows, keep, (sp, st, ct, fp, ep, bp) = _scored(seqs, starts, counts, heads, first, end, slopes)
+        self.h = self.lib.tvara_score_plan_create(cache.h, sp, keep[0].size, heads, context, st, ct, fp, ep, scale or 0.0, cap,
+                                                  bp)
+        if not self.h:
+            _capi.raise_last()
+
+    def launch(self, layer, q_ptr, out_ptr, stream=None):
+        """Asynchronous attention over device pointers (ints)."""
+        _capi.check(self.lib.tvara_score_plan_launch(self.h, layer, q_ptr, out_ptr, stream))
+
+    def check(self):
+        _capi.check(self.lib.tvara_score_plan_check(self.h))
+
+    def close(self):
+        if getattr(self, "h", None):
+            self.lib.tvara_score_plan_destroy(self.h)
             self.h = None
 
     def __del__(self):

@@ -18,6 +18,7 @@
 #include "host_copy.hpp"
 #include "kv_cache.hpp"
 #include "model.hpp"
+#include "score.hpp"
 #include "tree.hpp"
 
 using tvara_amd::AttnPlan;
@@ -67,6 +68,10 @@ struct tvara_tree_plan {
 
 struct tvara_slot_plan {
     tvara_amd::SlotPlan plan;
+};
+
+struct tvara_score_plan {
+    tvara_amd::ScorePlan plan;
 };
 
 namespace tvara_amd {
@@ -525,6 +530,78 @@ int tvara_slot_plan_check(tvara_slot_plan* plan) {
 }
 
 void tvara_slot_plan_destroy(tvara_slot_plan* plan) { delete plan; }
+
+// ------------------------------------------------------- scored attention
+
+tvara_score_plan* tvara_score_plan_create(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, size_t heads,
+                                          size_t context, const size_t* start, const size_t* rows, const size_t* first,
+                                          const size_t* end, float scale, float cap, const float* slopes) {
+    tvara_score_plan* out = nullptr;
+    guard([&] {
+        auto& c = live(cache);
+        tvara_amd::check_attention_config(c, heads, context);
+        auto p = std::make_unique<tvara_score_plan>();
+        p->plan.build(&c, sequences, count, heads, context, start, rows, first, end, scale, cap, slopes);
+        out = p.release();
+    });
+    return out;
+}
+
+int tvara_score_plan_launch(tvara_score_plan* plan, size_t layer, const float* q, float* out, void* stream) {
+    return guard([&] {
+        if (!plan) throw std::invalid_argument("null score plan");
+        if (plan->plan.rows && (!q || !out)) throw std::invalid_argument("invalid fused attention shape");
+        if (!aligned16(q) || !aligned16(out)) throw std::invalid_argument("device buffers must be 16-byte aligned");
+        if (layer > static_cast<size_t>(std::numeric_limits<int>::max()))
+            throw std::invalid_argument("invalid fused attention shape");
+        hipStream_t s = stream ? static_cast<hipStream_t>(stream) : plan->plan.cache->stream();
+        plan->plan.launch(static_cast<int>(layer), q, out, s);
+    });
+}
+
+int tvara_score_plan_check(tvara_score_plan* plan) {
+    return guard([&] {
+        if (!plan) throw std::invalid_argument("null score plan");
+        plan->plan.check();
+    });
+}
+
+void tvara_score_plan_destroy(tvara_score_plan* plan) { delete plan; }
+
+int tvara_attn_score(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, size_t layer, size_t heads,
+                     size_t context, const size_t* start, const size_t* rows, const size_t* first, const size_t* end,
+                     float scale, float cap, const float* slopes, const float* q, float* out, int device_ptrs) {
+    return guard([&] {
+        auto& c = live(cache);
+        tvara_amd::check_attention_config(c, heads, context);
+        if (!count) return;
+        if (layer >= c.geometry().layers) throw std::invalid_argument("invalid fused attention shape");
+        tvara_amd::ScorePlan plan;
+        plan.build(&c, sequences, count, heads, context, start, rows, first, end, scale, cap, slopes);
+        if (!plan.rows) return;
+        if (!q || !out) throw std::invalid_argument("invalid fused attention shape");
+        hipStream_t s = c.stream();
+        if (device_ptrs) {
+            if (!aligned16(q) || !aligned16(out)) throw std::invalid_argument("device buffers must be 16-byte aligned");
+            plan.launch(static_cast<int>(layer), q, out, s);
+            plan.check();
+            return;
+        }
+        const size_t n = plan.rows * heads * c.geometry().head_dim, at = (n + 3) / 4 * 4;
+        tvara_amd::HostCopier& copier = tvara_amd::HostCopier::shared();
+        std::lock_guard<std::mutex> hold(copier.lock());
+        auto* in = static_cast<float*>(cache->io_in.acquire(n * sizeof(float)));
+        copier.parallel_copy(reinterpret_cast<char*>(in), reinterpret_cast<const char*>(q), n * sizeof(float));
+        auto* d = static_cast<float*>(cache->io.ensure(2 * at * sizeof(float)));
+        TVARA_HIP(hipMemcpyAsync(d, in, n * sizeof(float), hipMemcpyHostToDevice, s));
+        cache->io_in.release(s);
+        plan.launch(static_cast<int>(layer), d, d + at, s);
+        auto* back = static_cast<float*>(cache->io_out.acquire(n * sizeof(float)));
+        TVARA_HIP(hipMemcpyAsync(back, d + at, n * sizeof(float), hipMemcpyDeviceToHost, s));
+        plan.check();
+        copier.parallel_copy(reinterpret_cast<char*>(out), reinterpret_cast<const char*>(back), n * sizeof(float));
+    });
+}
 
 // ------------------------------------------------------- model-level exports
 // c_api.cpp:35-78: return conventions (nullptr / 0 / -1), messages and the

@@ -1,0 +1,775 @@
+// Scored attention (score.hip) on the matrix cores, for head_dim 64 and 128 over f32
+// or Q8_0 blocks of a power of two from 16 tokens.
+//
+// An attention row is a (row, query head) pair; the rows of a block share the keys of
+// their KV head.  Scores S^T = K Q^T and outputs O^T = V^T P^T both have the row in
+// lane % 16, so that what the softmax does to a row stays in its four lanes, and the
+// probabilities are the second product's operand where they are.  Steps that some row
+// sees only a part of are masked by the rows' ranges; in them a value that is not
+// finite is taken out of the product, in which zero times it would reach every row,
+// and added to the rows that see it.
+#include <type_traits>
+
+#include "score_util.hpp"
+
+namespace tvara_amd {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kThreshold = 8.0f;
+constexpr int kBufferWord3 = 0x00020000;  // gfx9 buffer descriptor, dword 3
+
+// A workgroup's work (ScoreArgs::work)
+struct Item {
+    int table, tokens, rows, row0, head, heads, step, end, run, runs, slot, position;
+};
+__device__ __forceinline__ Item item_of(const ScoreArgs& a, unsigned i) {
+    const int4 x = a.work[3 * static_cast<size_t>(i)], y = a.work[3 * static_cast<size_t>(i) + 1], z = a.work[3 * static_cast<size_t>(i) + 2];
+    return {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+}
+
+// max / min over the 16 lanes of a row of a wave, to a scalar
+__device__ __forceinline__ int uniform_max(int v) {
+    for (int o = 8; o >= 1; o >>= 1) v = max(v, __shfl_xor(v, o));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+// ------------------------------------------------------------- few rows
+
+constexpr int kFewStep = 32, kFewWaves = 4;
+
+// Up to 16 attention rows in f32 (v_mfma_f32_16x16x4_f32): four waves take steps of
+// 32 keys in turn, with no barrier until the end, where their results meet in LDS.
+// Bound: HBM; keys of f32 blocks come as whole rows into the wave's own part of LDS
+// without passing registers (as operands they take four times as long through the CU's
+// cache), values straight into registers as the product has them.
+template <int D, bool kQ8>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_kernel(const ScoreArgs a) {
+    constexpr int WK = kFewWaves, C = D / 16, H = D / 64;
+    constexpr int W = D / 4;  // 16-byte parts of a row
+    __shared__ f32x4 staged[WK][kQ8 ? 4 * 64 : kFewStep * W];
+    auto result = [&](int w, int i) -> f32x4& { return staged[w][i * 64 + static_cast<int>(threadIdx.x & 63)]; };
+    __shared__ float2 stats[WK][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, r16 = lane & 15;
+    const Item it = item_of(a, blockIdx.x);
+    if (!it.rows) return;  // the list's padding
+    const int kh = it.head / a.group, kvw = a.lay.kv_width, tokens = it.tokens;
+
+    // this lane's row
+    const int index = r16 / it.heads, head = it.head + r16 - index * it.heads;
+    const bool live = index < it.rows;
+    const int position = it.position + index;
+    const size_t row = static_cast<size_t>(it.row0) + index;
+    const int2 range = live ? a.ranges[row] : make_int2(0, 0);
+    const float slope = a.slopes && live ? a.slopes[head] : 0.f;
+    const int lo = uniform_max(range.x), hi = -uniform_max(live ? -range.y : -0x7fffffff);  // keys that all rows see: [lo, hi)
+
+    // column of element 0 of a lane's c-th four of a key, and of the h-th four of
+    // a value (r: the loading lane's r16, or an output row of the tiles)
+    auto kcol = [&](int c) { return kQ8 ? 64 * (c / 4) + 16 * g + 4 * (c % 4) : 16 * c + 4 * g; };
+    auto vcol = [](int h, int r) { return kQ8 ? (D / 16) * r + 4 * h : 64 * h + 4 * r; };
+
+    const int tpb = a.lay.tpb, tsh = __builtin_ctz(static_cast<unsigned>(tpb));
+    const int32_t* tab = a.tables + it.table;
+    const size_t kbytes = kQ8 ? static_cast<size_t>(a.layer) * 2 * a.lay.section + static_cast<size_t>(kh) * a.lay.head_bytes
+                              : (static_cast<size_t>(a.layer) * 2 * tpb * kvw + static_cast<size_t>(kh) * D) * sizeof(float);
+    const size_t vsec = kQ8 ? a.lay.section : static_cast<size_t>(tpb) * kvw * sizeof(float);
+    const int rowb = kQ8 ? D : kvw * static_cast<int>(sizeof(float));  // from one slot to the next
+    const unsigned koff = static_cast<unsigned>(!kQ8 ? lane / W * rowb + (lane % W ^ lane / W) * 16 : r16 * rowb + kcol(0));
+    const unsigned voff = static_cast<unsigned>(4 * g * rowb + vcol(0, r16) * (kQ8 ? 1 : 4));
+    int step = it.step + wave;
+    const int last = max(tokens - 1, 0) >> 4;  // 16 keys a table lookup; past the end the last again
+    // lane 2i + mt: the block of the wave's i-th step from here
+    auto lookup = [&](int from) { return tokens ? tab[min(2 * (from + (lane >> 1) * WK) + (lane & 1), last) << 4 >> tsh] : 0; };
+    int ids = lookup(step), more = lookup(step + 32 * WK), at = 0;
+    auto block = [&](int mt, int stp) {
+        const int id = __builtin_amdgcn_readlane(ids, 2 * at + mt);
+        const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
+        return a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes + static_cast<size_t>(slot) * rowb;
+    };
+    f32x4 qf[C];
+    // f32 rows, or Q8_0 bytes and scales, which become values where they are used
+    f32x4 v[kQ8 ? 1 : 2][4][H];
+    u32x4 kw[kQ8 ? 2 : 1][H];
+    unsigned kd[kQ8 ? 2 : 1][H], vw[kQ8 ? 2 : 1][4][H], vd[kQ8 ? 2 : 1][4];
+    auto scales = [&](const char* b, int mt, int stp) {  // of the block's rows from the tile's first on
+        const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
+        return b + static_cast<size_t>(tpb - slot) * D + static_cast<size_t>(slot) * (D / 32) * 2;
+    };
+    auto load_k = [&](int stp) __attribute__((always_inline)) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+            const char* b = block(mt, stp);
+            if constexpr (kQ8) {
+                const char* sc = scales(b, mt, stp);
+#pragma unroll
+                for (int u = 0; u < H; ++u) {
+                    kw[mt][u] = *reinterpret_cast<const u32x4*>(b + koff + 64 * u);
+                    kd[mt][u] = *reinterpret_cast<const uint16_t*>(sc + (r16 * (D / 32) + 2 * u + (g >> 1)) * 2);
+                }
+            } else {
+                // straight into LDS, lane after lane; what a lane loads is permuted by its
+                // row, so that the operands' reads meet no bank twice
+                const __amdgpu_buffer_rsrc_t rows =
+                    __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(b), 0, 15 * rowb + 4 * D, kBufferWord3);
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (__attribute__((address_space(3))) void*)&staged[wave][(mt * C + c) * 64],
+                                                             16, koff ^ 1024 / W * c, 64 / W * c * rowb, 0, 0);
+            }
+        }
+    };
+    auto load_v = [&](int stp) __attribute__((always_inline)) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+            const char* b = block(mt, stp) + vsec;
+            if constexpr (kQ8) {
+                const char* sc = scales(b, mt, stp);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    vd[mt][i] = *reinterpret_cast<const uint16_t*>(sc + ((4 * g + i) * (D / 32) + (D / 16) * r16 / 32) * 2);
+#pragma unroll
+                    for (int h = 0; h < H; ++h) vw[mt][i][h] = *reinterpret_cast<const unsigned*>(b + voff + i * D + 4 * h);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+                        v[mt][i][h] = *reinterpret_cast<const f32x4*>(b + static_cast<size_t>(i) * rowb + voff + 256 * h);
+            }
+        }
+    };
+    {
+        const float* qp = a.q + (row * a.heads + head) * D;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            qf[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (live) qf[c] = *reinterpret_cast<const f32x4*>(qp + kcol(c));
+        }
+    }
+    if (step < it.end) {
+        load_k(step);
+        if constexpr (!kQ8) asm volatile("" ::: "memory");
+        load_v(step);
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) qf[c] *= a.qscale;
+
+    f32x4 acc[4 * H];  // tile (h, j) at 4h + j
+    float m = -INFINITY, l = 0.f, rounded = 0.f, nonfinite = 0.f;  // nonfinite: NaN once a score is not finite
+#pragma unroll
+    for (int dt = 0; dt < 4 * H; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 s[2];  // scores, then probabilities, of keys 16mt + 4g + i
+    auto key_part = [&](int mt, int c) __attribute__((always_inline)) {
+        if constexpr (kQ8) {
+            const float d = half_bits_to_float(static_cast<uint16_t>(kd[mt][c / 4]));
+            const unsigned w = kw[mt][c / 4][c % 4];
+            return f32x4{sbyte_to_float<0>(w) * d, sbyte_to_float<1>(w) * d, sbyte_to_float<2>(w) * d, sbyte_to_float<3>(w) * d};
+        } else {
+            return staged[wave][(16 * mt + r16) * W + ((4 * c + g) ^ r16)];
+        }
+    };
+    auto value = [&](int mt, int i, int h, auto j) __attribute__((always_inline)) {
+        if constexpr (kQ8)
+            return sbyte_to_float<j.value>(vw[mt][i][h]) * half_bits_to_float(static_cast<uint16_t>(vd[mt][i]));
+        else
+            return v[mt][i][h][j.value];
+    };
+    auto every_tile = [&](auto&& f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            f(h, std::integral_constant<int, 0>{});
+            f(h, std::integral_constant<int, 1>{});
+            f(h, std::integral_constant<int, 2>{});
+            f(h, std::integral_constant<int, 3>{});
+        }
+    };
+    // the lane's columns of key 16mt + 4g + i
+    auto finite_value = [&](int mt, int i) __attribute__((always_inline)) {
+        if constexpr (kQ8) {
+            return __builtin_isfinite(half_bits_to_float(static_cast<uint16_t>(vd[mt][i])));
+        } else {
+            bool fine = true;
+#pragma unroll
+            for (int h = 0; h < H; ++h) fine &= all_finite(v[mt][i][h]);
+            return fine;
+        }
+    };
+    auto drop_odd = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (kQ8) {
+                    if (!finite_value(mt, i)) vd[mt][i] = 0;
+                } else {
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[mt][i][h][j] = __builtin_isfinite(v[mt][i][h][j]) ? v[mt][i][h][j] : 0.f;
+                }
+            }
+    };
+    for (; step < it.end; step += WK) {
+        const int next = step + WK, key0 = kFewStep * step;
+        if constexpr (!kQ8) wait_until_left<8 * H>();  // the values'
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+            s[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const f32x4 k = key_part(mt, c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i], qf[c][i], s[mt], 0, 0, 0);
+            }
+        }
+        if constexpr (!kQ8) wait_for_lds();
+        // the loads of the next step go out as soon as there is room (past the end the
+        // last step's again: its blocks are there)
+        if (++at == 32) {
+            at = 0;
+            ids = more;
+            more = lookup(next + 32 * WK);
+        }
+        load_k(next);
+        if constexpr (!kQ8) asm volatile("" ::: "memory");
+        const bool whole = key0 >= lo && key0 + kFewStep <= hi;  // every row sees every key
+        const int first = range.x - key0 - 4 * g, end = range.y - key0 - 4 * g;  // of the lane's keys 16mt + i
+        if (whole) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) nonfinite = fmaf(s[mt][i], 0.f, nonfinite);
+        } else {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool on = 16 * mt + i >= first && 16 * mt + i < end;
+                    s[mt][i] = on ? s[mt][i] : 0.f;
+                    nonfinite = fmaf(s[mt][i], 0.f, nonfinite);
+                }
+        }
+        if (a.cap != 0.f) {
+            float most = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most = fmaxf(most, __builtin_fabsf(s[mt][i]));
+            const bool small = !__any(most > kSmallTanh);
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[mt][i] = a.cap * (small ? small_tanh(s[mt][i]) : any_tanh(s[mt][i]));
+        }
+        if (a.slopes) {
+            const int away = position - key0 - 4 * g;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[mt][i] = fmaf(-slope, static_cast<float>(abs(away - 16 * mt - i)), s[mt][i]);
+        }
+        if (!whole) {
+            bool odd = false;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (16 * mt + i < first || 16 * mt + i >= end) s[mt][i] = -INFINITY;
+                    odd |= !finite_value(mt, i);
+                }
+            if (__any(odd)) {
+                // A row that sees such a value has a column that is not finite: their
+                // product as ones and zeros counts them.
+                auto count = [&](int h, auto j) __attribute__((always_inline)) {
+                    f32x4 part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool on = 16 * mt + i >= first && 16 * mt + i < end;
+                            part = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_isfinite(value(mt, i, h, j)) ? 0.f : 1.f, on ? 1.f : 0.f,
+                                                                        part, 0, 0, 0);
+                        }
+#pragma unroll
+                    for (int o = 0; o < 4; ++o) acc[4 * h + j.value][o] += part[o] != 0.f ? NAN : 0.f;
+                };
+                every_tile(count);
+                drop_odd();
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[mt][i]);
+        if (__any(mx > m + kThreshold)) {
+            const float mn = fmaxf(m, cross_row_max(mx));
+            const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+            m = mn;
+            l *= alpha;
+            rounded *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < 4 * H; ++dt) acc[dt] *= alpha;
+        }
+        const float base = m == -INFINITY ? 0.f : m;  // (no key seen yet: probabilities 0)
+        float sum = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[mt][i] = fast_exp2(s[mt][i] - base);
+                sum += s[mt][i];
+            }
+        add_to(l, rounded, sum);
+        // a step's part is a chain of eight from zero, added to the rest: as short as a
+        // long context's sums need it
+        auto tile = [&](int h, auto j) __attribute__((always_inline)) {
+            f32x4 part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part = __builtin_amdgcn_mfma_f32_16x16x4f32(value(mt, i, h, j), s[mt][i], part, 0, 0, 0);
+            acc[4 * h + j.value] += part;
+        };
+        every_tile(tile);
+        load_v(next);
+    }
+    if constexpr (!kQ8) wait_until_left<0>();  // (LDS is used again)
+    if (__any(nonfinite != 0.f) && lane == 0) *a.err = 1;
+
+    // ---- the waves that shared these rows' keys, together
+    float total = cross_row_sum(l);
+    if (g == 0) stats[wave][r16] = make_float2(m, total);
+    __syncthreads();
+    {
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) top = fmaxf(top, stats[w][r16].x);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) sum = fmaf(fast_exp2(stats[w][r16].x - base), stats[w][r16].y, sum);
+        const float scale = fast_exp2(m - base);
+#pragma unroll
+        for (int dt = 0; dt < 4 * H; ++dt) acc[dt] *= scale;
+        m = top;
+        total = sum;
+    }
+    // four columns of output row 4g + i of the tiles
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        if (h) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) result(wave, i) = f32x4{acc[4 * h][i], acc[4 * h + 1][i], acc[4 * h + 2][i], acc[4 * h + 3][i]};
+        __syncthreads();
+        f32x4 x = result(0, wave);
+#pragma unroll
+        for (int w = 1; w < WK; ++w) x += result(w, wave);
+        if (!live) continue;
+        if (it.runs == 1) {
+            *reinterpret_cast<f32x4*>(a.out + (row * a.heads + head) * D + vcol(h, 4 * g + wave)) = x / (total != 0.f ? total : 1.f);
+        } else {
+            const size_t p = (static_cast<size_t>(it.slot) + static_cast<size_t>(index) * it.runs + it.run) * a.heads + head;
+            *reinterpret_cast<f32x4*>(a.part_acc + p * D + vcol(h, 4 * g + wave)) = x;
+            if (h == 0 && wave == 0 && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m, total);
+        }
+    }
+}
+
+// ------------------------------------------------------------ many rows
+
+constexpr int kManyWaves = 8;
+
+// ds_read_b64_tr_b16: within 16 lanes, lane i receives element i % 4 of the four that
+// lane 4j + i / 4 addresses, as its element j
+__device__ __forceinline__ bf16x4 transposed_read(const __bf16* p) {
+    typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+    const i16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p));
+    return __builtin_bit_cast(bf16x4, v);
+}
+
+// Four values as three parts in bf16, each the rest's nearest: 24 bits and more, f32's
+// whole range but what lies below 2^-126 (a value that rounds beyond bf16's largest,
+// 3.39e38, is infinite in the first).
+__device__ __forceinline__ void split3(f32x4 x, bf16x4& p0, bf16x4& p1, bf16x4& p2) {
+    p0 = __builtin_convertvector(x, bf16x4);
+    const f32x4 r1 = x - __builtin_convertvector(p0, f32x4);
+    p1 = __builtin_convertvector(r1, bf16x4);
+    p2 = __builtin_convertvector(r1 - __builtin_convertvector(p1, f32x4), bf16x4);
+}
+__device__ __forceinline__ bf16x8 both(bf16x4 x, bf16x4 y) {
+    return bf16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+}
+// the largest value that keeps a finite first part
+constexpr float kMostParts = 3.38e38f;
+
+// Up to 256 attention rows, eight waves of 32.  f32 products as six of bf16 parts
+// (16x16x32, 16 times the f32 instruction's rate): of x = x0 + x1 + x2 and y likewise
+// x0 y0 + x0 y1 + x1 y0 + x1 y1 + x0 y2 + x2 y0, what is left out being 2^-25 of the
+// product, with no range of its own.  All waves load and split a step's keys and values
+// once, into the other of two buffers in LDS; one barrier a step.
+template <int D, bool kQ8>
+__global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const ScoreArgs a) {
+    constexpr int NT = 2, KC = D / 32, DT = D / 16;
+    constexpr int KEYS = 4096 / D, MT = KEYS / 16;  // keys of a step: eight columns a thread
+    constexpr int LPR = D / 8;                      // lanes of a key's row
+    constexpr int STR = D + 16;                     // LDS row pitch: no bank twice
+    __shared__ __attribute__((aligned(16))) __bf16 kparts[2][3][KEYS * STR];
+    __shared__ __attribute__((aligned(16))) __bf16 vparts[2][3][KEYS * STR];
+    __shared__ int odds[2][kManyWaves];          // some value of the wave's keys is not finite:
+    __shared__ uint8_t which[2][KEYS][D / 8];    // bit c % 8 of [key][c / 8]: the value of column c
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, r16 = lane & 15;
+    const Item it = item_of(a, blockIdx.x);
+    if (!it.rows) return;  // the list's padding
+    const int kh = it.head / a.group, kvw = a.lay.kv_width, tokens = it.tokens;
+
+    int index[NT], head[NT], position[NT];
+    bool live[NT];
+    int2 range[NT];
+    float slope[NT];
+    int seen_lo = 0x7fffffff, seen_hi = 0, all_lo = 0, all_hi = 0x7fffffff;  // what some row of the wave sees, and all do
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = 32 * wave + 16 * nt + r16;
+        index[nt] = r / it.heads;
+        head[nt] = it.head + r - index[nt] * it.heads;
+        live[nt] = index[nt] < it.rows;
+        position[nt] = it.position + index[nt];
+        range[nt] = live[nt] ? a.ranges[static_cast<size_t>(it.row0) + index[nt]] : make_int2(0, 0);
+        slope[nt] = a.slopes && live[nt] ? a.slopes[head[nt]] : 0.f;
+        if (range[nt].x < range[nt].y) {
+            seen_lo = min(seen_lo, range[nt].x);
+            seen_hi = max(seen_hi, range[nt].y);
+        }
+        if (live[nt]) {
+            all_lo = max(all_lo, range[nt].x);
+            all_hi = min(all_hi, range[nt].y);
+        }
+    }
+    seen_lo = -uniform_max(-seen_lo);
+    seen_hi = uniform_max(seen_hi);
+    all_lo = uniform_max(all_lo);
+    all_hi = -uniform_max(-all_hi);
+
+    bf16x8 qp[NT][KC][3];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+            f32x4 x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0;
+            if (live[nt]) {
+                const float* q = a.q + ((static_cast<size_t>(it.row0) + index[nt]) * a.heads + head[nt]) * D + 32 * kc + 8 * g;
+                x0 = *reinterpret_cast<const f32x4*>(q) * a.qscale;
+                x1 = *reinterpret_cast<const f32x4*>(q + 4) * a.qscale;
+            }
+            bf16x4 p[2][3];
+            split3(x0, p[0][0], p[0][1], p[0][2]);
+            split3(x1, p[1][0], p[1][1], p[1][2]);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) qp[nt][kc][i] = both(p[0][i], p[1][i]);
+        }
+
+    // staging: eight columns of a key; a wave's keys lie in one block
+    const int skey = tid / LPR, col = 8 * (tid % LPR);
+    const int tpb = a.lay.tpb, tsh = __builtin_ctz(static_cast<unsigned>(tpb));
+    const int32_t* tab = a.tables + it.table;
+    const size_t kbytes = kQ8 ? static_cast<size_t>(a.layer) * 2 * a.lay.section + static_cast<size_t>(kh) * a.lay.head_bytes
+                              : (static_cast<size_t>(a.layer) * 2 * tpb * kvw + static_cast<size_t>(kh) * D) * sizeof(float);
+    const size_t vsec = kQ8 ? a.lay.section : static_cast<size_t>(tpb) * kvw * sizeof(float);
+    // (past the last key: its block again, whose slots are there whatever they hold)
+    auto lookup = [&](int stp) { return tab[min(KEYS * stp + skey, tokens - 1) >> tsh]; };
+    f32x4 kreg[2], vreg[2];
+    u32x2 kraw, vraw;
+    unsigned kdraw, vdraw;
+    auto load = [&](int stp, int id) __attribute__((always_inline)) {
+        const int slot = (KEYS * stp + skey) & (tpb - 1);
+        const char* b = a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes;
+        if constexpr (kQ8) {
+            const char* sc = b + static_cast<size_t>(tpb) * D + static_cast<size_t>(slot * (D / 32) + col / 32) * 2;
+            b += static_cast<size_t>(slot) * D + col;
+            kraw = *reinterpret_cast<const u32x2*>(b);
+            kdraw = *reinterpret_cast<const uint16_t*>(sc);
+            vraw = *reinterpret_cast<const u32x2*>(b + vsec);
+            vdraw = *reinterpret_cast<const uint16_t*>(sc + vsec);
+        } else {
+            b += (static_cast<size_t>(slot) * kvw + col) * sizeof(float);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                kreg[i] = *reinterpret_cast<const f32x4*>(b + 16 * i);
+                vreg[i] = *reinterpret_cast<const f32x4*>(b + vsec + 16 * i);
+            }
+        }
+    };
+    auto stage = [&](int buf) __attribute__((always_inline)) {
+        if constexpr (kQ8) {
+            const float kd = half_bits_to_float(static_cast<uint16_t>(kdraw)), vd = half_bits_to_float(static_cast<uint16_t>(vdraw));
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const unsigned kw = kraw[i], vw = vraw[i];
+                kreg[i] = f32x4{sbyte_to_float<0>(kw) * kd, sbyte_to_float<1>(kw) * kd, sbyte_to_float<2>(kw) * kd, sbyte_to_float<3>(kw) * kd};
+                vreg[i] = f32x4{sbyte_to_float<0>(vw) * vd, sbyte_to_float<1>(vw) * vd, sbyte_to_float<2>(vw) * vd, sbyte_to_float<3>(vw) * vd};
+            }
+        }
+        unsigned odd = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!(__builtin_fabsf(vreg[i][e]) < kMostParts)) {
+                    odd |= 1u << (4 * i + e);
+                    vreg[i][e] = 0.f;
+                }
+        const bool any = __any(odd != 0);
+        if (lane == 0) odds[buf][wave] = any;
+        if (any) which[buf][skey][col / 8] = static_cast<uint8_t>(odd);
+        const int at = skey * STR + col;
+        bf16x4 p[2][3];
+        split3(kreg[0], p[0][0], p[0][1], p[0][2]);
+        split3(kreg[1], p[1][0], p[1][1], p[1][2]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) *reinterpret_cast<bf16x8*>(&kparts[buf][i][at]) = both(p[0][i], p[1][i]);
+        split3(vreg[0], p[0][0], p[0][1], p[0][2]);
+        split3(vreg[1], p[1][0], p[1][1], p[1][2]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) *reinterpret_cast<bf16x8*>(&vparts[buf][i][at]) = both(p[0][i], p[1][i]);
+    };
+
+    f32x4 acc[DT][NT];
+    float m[NT], l[NT], rounded[NT], nonfinite = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        m[nt] = -INFINITY;
+        l[nt] = rounded[nt] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // the products of three parts each, small ones first
+    auto six = [](const bf16x8 (&x)[3], const bf16x8 (&y)[3], f32x4 c) __attribute__((always_inline)) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[2], y[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[2], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[1], y[1], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[1], y[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[1], c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[0], c, 0, 0, 0);
+    };
+    auto compute = [&](int buf, int stp) __attribute__((always_inline)) {
+        const int key0 = KEYS * stp;
+        if (key0 >= seen_hi || key0 + KEYS <= seen_lo) return;
+        const bool whole = key0 >= all_lo && key0 + KEYS <= all_hi;
+        f32x4 s[MT][NT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[mt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                bf16x8 k[3];
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+                    k[i] = *reinterpret_cast<const bf16x8*>(&kparts[buf][i][(16 * mt + r16) * STR + 32 * kc + 8 * g]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) s[mt][nt] = six(k, qp[nt][kc], s[mt][nt]);
+            }
+        float alpha[NT];
+        bf16x8 pp[NT][MT / 2][3];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int first = range[nt].x - key0 - 4 * g, end = range[nt].y - key0 - 4 * g;
+            if (!whole) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[mt][nt][i] = 16 * mt + i >= first && 16 * mt + i < end ? s[mt][nt][i] : 0.f;
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) nonfinite = fmaf(s[mt][nt][i], 0.f, nonfinite);
+            if (a.cap != 0.f) {
+                float most = 0.f;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) most = fmaxf(most, __builtin_fabsf(s[mt][nt][i]));
+                if (!__any(most > kSmallTanh)) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[mt][nt][i] = a.cap * small_tanh(s[mt][nt][i]);
+                } else {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[mt][nt][i] = a.cap * any_tanh(s[mt][nt][i]);
+                }
+            }
+            if (a.slopes) {
+                const int away = position[nt] - key0 - 4 * g;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        s[mt][nt][i] = fmaf(-slope[nt], static_cast<float>(abs(away - 16 * mt - i)), s[mt][nt][i]);
+            }
+            if (!whole) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (16 * mt + i < first || 16 * mt + i >= end) s[mt][nt][i] = -INFINITY;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[mt][nt][i]);
+            const float mn = fmaxf(m[nt], cross_row_max(mx)), base = mn == -INFINITY ? 0.f : mn;
+            alpha[nt] = fast_exp2(m[nt] - base);
+            m[nt] = mn;
+            float sum = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[mt][nt][i] = fast_exp2(s[mt][nt][i] - base);
+                    sum += s[mt][nt][i];
+                }
+            l[nt] *= alpha[nt];
+            rounded[nt] *= alpha[nt];
+            add_to(l[nt], rounded[nt], sum);
+#pragma unroll
+            for (int h = 0; h < MT / 2; ++h) {
+                bf16x4 p[2][3];
+                split3(s[2 * h][nt], p[0][0], p[0][1], p[0][2]);
+                split3(s[2 * h + 1][nt], p[1][0], p[1][1], p[1][2]);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) pp[nt][h][i] = both(p[0][i], p[1][i]);
+            }
+        }
+        // lane (g, i): column 16dt + i of keys 4g .. 4g + 3 and 16 + 4g .. of each 32, as the
+        // probabilities have them; a step's part from zero, then added to the rest
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            f32x4 part[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) part[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int h = 0; h < MT / 2; ++h) {
+                bf16x8 v[3];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    const __bf16* p = &vparts[buf][i][(32 * h + 4 * g + (r16 >> 2)) * STR + 16 * dt + 4 * (r16 & 3)];
+                    v[i] = both(transposed_read(p), transposed_read(p + 16 * STR));
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) part[nt] = six(v, pp[nt][h], part[nt]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[dt][nt][i] = fmaf(acc[dt][nt][i], alpha[nt], part[nt][i]);
+        }
+        if (__any(odds[buf][lane % kManyWaves] != 0)) {
+            // A row that sees such a value has a column that is not finite: their
+            // product as ones and zeros counts them.
+            bf16x8 on[NT][MT / 2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < 8 * (MT / 2); ++k) {
+                    const int key = key0 + 16 * (k / 4) + 4 * g + k % 4;
+                    on[nt][k / 8][k % 8] = static_cast<__bf16>(key >= range[nt].x && key < range[nt].y ? 1.f : 0.f);
+                }
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                f32x4 part[NT];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) part[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < MT / 2; ++h) {
+                    bf16x8 v;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int key = 32 * h + 16 * (k / 4) + 4 * g + k % 4;
+                        const bool marked = odds[buf][key * LPR / 64] && (which[buf][key][2 * dt + r16 / 8] >> (r16 % 8) & 1);
+                        v[k] = static_cast<__bf16>(marked ? 1.f : 0.f);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) part[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, on[nt][h], part[nt], 0, 0, 0);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int o = 0; o < 4; ++o) acc[dt][nt][o] += part[nt][o] != 0.f ? NAN : 0.f;
+            }
+        }
+    };
+
+    if (it.step < it.end) {
+        load(it.step, lookup(it.step));
+        int id = lookup(it.step + 1);
+        stage(0);
+        __syncthreads();
+        int buf = 0;
+        for (int step = it.step; step < it.end; ++step, buf ^= 1) {
+            load(step + 1, id);
+            id = lookup(step + 2);
+            compute(buf, step);
+            stage(buf ^ 1);
+            __syncthreads();
+        }
+    }
+    if (__any(nonfinite != 0.f) && lane == 0) *a.err = 1;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const float total = cross_row_sum(l[nt]);
+        if (!live[nt]) continue;
+        const bool whole = it.runs == 1;
+        const size_t at = (whole ? static_cast<size_t>(it.row0) + index[nt]
+                                 : static_cast<size_t>(it.slot) + static_cast<size_t>(index[nt]) * it.runs + it.run) * a.heads + head[nt];
+        float* o = (whole ? a.out : a.part_acc) + at * D + 4 * g;
+        const float div = whole && total != 0.f ? total : 1.f;
+        if (!whole && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(m[nt], total);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(o + 16 * dt) = acc[dt][nt] / div;
+    }
+}
+
+}  // namespace
+
+int score_step(const BlockLayout& lay, int block) { return block == kScoreFew ? kFewStep : 4096 / lay.head_dim; }
+
+int score_units(const BlockLayout& lay, int block) {
+    return block == kScoreMany ? 1 : lay.head_dim == 64 ? 3 : lay.format == kQ8 ? 2 : 1;
+}
+
+void launch_score_tiles(const ScoreArgs& a, int block, int workgroups, hipStream_t s) {
+    const bool q8 = a.lay.format == kQ8;
+    auto go = [&](const char* name, auto kernel, int waves) { launch(name, kernel, dim3(workgroups), dim3(64 * waves), 0, s, a); };
+    if (block == kScoreFew) {
+        const char* name = "score_attention_tiles";
+        if (a.lay.head_dim == 128)
+            q8 ? go(name, score_tile_kernel<128, true>, kFewWaves) : go(name, score_tile_kernel<128, false>, kFewWaves);
+        else
+            q8 ? go(name, score_tile_kernel<64, true>, kFewWaves) : go(name, score_tile_kernel<64, false>, kFewWaves);
+    } else {
+        const char* name = "score_attention_shared";
+        if (a.lay.head_dim == 128)
+            q8 ? go(name, score_shared_kernel<128, true>, kManyWaves) : go(name, score_shared_kernel<128, false>, kManyWaves);
+        else
+            q8 ? go(name, score_shared_kernel<64, true>, kManyWaves) : go(name, score_shared_kernel<64, false>, kManyWaves);
+    }
+    TVARA_HIP(hipGetLastError());
+}
+
+}  // namespace tvara_amd

@@ -36,7 +36,6 @@
 namespace tvara_amd {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -54,8 +53,6 @@ constexpr float kThreshold = 8.0f;
 constexpr float kPartsThreshold = 4.0f, kPartsLift = 11.0f;
 constexpr int kStep = kTreeStep, kWaves = kTreeWaves;
 constexpr int kBufferWord3 = 0x00020000;  // gfx9 buffer descriptor, dword 3
-
-__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Whether a product with x passes zeros on: x is finite, and (kParts) so is the nearest
 // fp16 number, x's first part.
@@ -93,20 +90,6 @@ struct Spans {
 // ahead too (they return in order).
 __device__ __forceinline__ void wait_for_loads() { __builtin_amdgcn_s_waitcnt(0); }
 
-// Until at most n loads are on their way (they return in order), or every read of LDS
-// is done; no access to memory moves across either.
-template <int n>
-__device__ __forceinline__ void wait_until_left() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt((n & 15) | n >> 4 << 14 | 0xf70);
-    asm volatile("" ::: "memory");
-}
-__device__ __forceinline__ void wait_for_lds() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xc07f);
-    asm volatile("" ::: "memory");
-}
-
 // Two values as hi + lo in fp16, each rounded to nearest (22 bits; beyond fp16's
 // range one is infinite and the other its opposite).  `one` is 1, hidden from the
 // compiler, so that x - hi stays a mixed-precision fma: four instructions a pair
@@ -131,20 +114,6 @@ __device__ __forceinline__ void scaled2(unsigned w0, unsigned w1, f16x2 d, unsig
     const f16x2 q = __builtin_bit_cast(f16x2, u) - f16x2{1152, 1152}, h = q * d;
     hi = __builtin_bit_cast(unsigned, h);
     lo = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(q, d, -h));
-}
-
-// A step's probabilities join a row's normaliser, with what the additions before have
-// rounded away (Kahan's sum): beside one large probability each step's part may be
-// less than half an ulp, and they are all of one sign.  MI355X, one key 19.5 above 131,072
-// of N(0,1), f32: every output off by 2.4e-5 of itself without, 7e-7 with it.
-__device__ __forceinline__ void add_to(float& l, float& rounded, float sum) {
-    const float y = sum - rounded, t = l + y;
-    rounded = (t - l) - y;
-    l = t;
-}
-
-__device__ __forceinline__ bool all_finite(f32x4 x) {
-    return __builtin_isfinite(x[0]) && __builtin_isfinite(x[1]) && __builtin_isfinite(x[2]) && __builtin_isfinite(x[3]);
 }
 
 // A workgroup's work: a tree (TreeArgs::trees), the KV head and first row of a row
