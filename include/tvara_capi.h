@@ -64,6 +64,7 @@ typedef struct tvara_radix tvara_radix;
 typedef struct tvara_tree_plan tvara_tree_plan;
 typedef struct tvara_slot_plan tvara_slot_plan;
 typedef struct tvara_score_plan tvara_score_plan;
+typedef struct tvara_sample_plan tvara_sample_plan;
 
 /* BlockHandle (kv.hpp:35) */
 typedef struct {
@@ -148,6 +149,17 @@ TVARA_API int tvara_sequences_decode(tvara_model* model, const uint64_t* sequenc
 TVARA_API int tvara_sequences_verify_trees(tvara_model* model, const uint64_t* sequences, size_t count,
                                            const size_t* nodes, const int32_t* parents, const uint32_t* tokens,
                                            const uint32_t* first, int32_t* path, size_t* accepted, uint32_t* next);
+
+/* tvara_sequences_decode with the logits left on the GPU and the next token of each
+ * sequence drawn there, as tvara_sample_plan_launch draws it (host arrays of `count`,
+ * NULL as there): next[i], and in probability[i] (or NULL) its probability.  What
+ * crosses to the host is eight bytes a sequence in place of its logits.  All or
+ * nothing: on failure, NaN logits or parameters out of range among it, no sequence
+ * changes.  Returns 0 / -1.  The reference samples on the host
+ * (python/tvara/native.py:301-334). */
+TVARA_API int tvara_sequences_sample(tvara_model* model, const uint64_t* sequences, const uint32_t* tokens, size_t count,
+                                     const float* uniforms, const float* temperature, const int32_t* top_k,
+                                     const float* top_p, const float* min_p, uint32_t* next, float* probability);
 
 /* The model's KV cache as a tvara_kv_cache handle owned by the model (the
  * in-process PagedModelExecutor::cache(), paged_model.hpp:10), so every
@@ -511,6 +523,37 @@ TVARA_API int tvara_attn_score(tvara_kv_cache* cache, const uint64_t* sequences,
                                const size_t* end, float scale, float cap, const float* slopes, const float* q, float* out,
                                int device_ptrs);
 
+/* ---------------------------------------------------------------- sampling
+ *
+ * The next token of each row of logits x by a given random number u in [0, 1):
+ *   w_i = exp((x_i - max x) / temperature)                  temperature >= 0
+ *   top-k  the top_k largest x, the lowest index first among equals (0: all)
+ *   top-p  of those, from the largest down, as many as it takes to reach top_p of their
+ *          mass; one at the least
+ *   min-p  of those, w_i >= min_p
+ * and then the first index up to which the kept mass exceeds u times all of it.
+ * temperature 0 takes the lowest index of the largest.  -inf is never drawn, and
+ * neither is a weight below 2^-45.  The same logits, numbers and parameters give the
+ * same token whatever the batch: masses are summed as whole numbers of 64 bits. */
+/* Workspace for up to `rows` rows of `vocab` logits on the current device (rows * vocab
+ * up to 2^33, vocab below 2^30). */
+TVARA_API tvara_sample_plan* tvara_sample_plan_create(size_t rows, size_t vocab);
+/* logits f32 [rows] rows of vocab, logits_stride floats apart (0: vocab); uniforms
+ * [rows]; temperature, top_k, top_p, min_p [rows], or NULL for 1, 0, 1 and 0; tokens
+ * [rows] receives the token, probability [rows] (or NULL) its share of the kept mass.
+ * A NaN logit counts as -inf; it, and a row with no token left (0xffffffff and 0 are
+ * written), or parameters out of range (the same), are reported by
+ * tvara_sample_plan_check.  Device pointers, asynchronous on `stream` (NULL: the null
+ * stream).  Launches of one plan share its workspace: one after the other, captured
+ * ones too. */
+TVARA_API int tvara_sample_plan_launch(tvara_sample_plan* plan, size_t rows, const float* logits, size_t logits_stride,
+                                       const float* uniforms, const float* temperature, const int32_t* top_k,
+                                       const float* top_p, const float* min_p, uint32_t* tokens, float* probability,
+                                       void* stream);
+/* Synchronise the plan's last launch and report what it found. */
+TVARA_API int tvara_sample_plan_check(tvara_sample_plan* plan);
+TVARA_API void tvara_sample_plan_destroy(tvara_sample_plan* plan);
+
 /* The block ids of the listed sequences, resident (at most 65,535); calls fail
  * with TVARA_INVALID once the cache's tables have changed. */
 TVARA_API tvara_slot_plan* tvara_slot_plan_create(tvara_kv_cache* cache, const uint64_t* sequences, size_t count);
@@ -539,6 +582,32 @@ TVARA_API int tvara_slot_plan_build(tvara_slot_plan* plan, const int32_t* starts
 TVARA_API int tvara_slot_plan_write(tvara_slot_plan* plan, const int64_t* slots, const int32_t* rows, size_t n,
                                     const float* keys, const float* values, size_t row_count, size_t row_stride,
                                     size_t layer_stride, void* stream);
+/* A layer's queries and keys on their way to attention, in one pass: of each head x,
+ *   y = x * weight / sqrt(mean x^2 + eps)            where q_norm / k_norm are given
+ *   (y_a, y_b) -> (y_a cos t - y_b sin t, y_a sin t + y_b cos t),  t = positions[i] * freqs[j]
+ * for the pairs j of its first `rotary` columns: columns 2j and 2j + 1 where
+ * interleaved, else j and j + rotary / 2; computed in f64, rounded once.  Token i's rows
+ * are at q + i * q_stride (heads * head_dim floats; 0: packed) and keys, values + i *
+ * kv_stride (kv_width; 0: packed), such as the parts of a fused product.  Queries go to
+ * q_out [n][heads * head_dim]; keys and values into slots[i] of `layer`, f32 as they are
+ * or encoded as appends encode them (-1: nowhere; NULL: none is written); rotated keys
+ * to k_out [n][kv_width] too, for rows that stay outside the cache (tree plans).
+ * q_out and k_out may be NULL, or q_out q itself where q is packed.  A slot outside the
+ * pool is skipped and reported by tvara_slot_plan_check; two entries of one slot leave
+ * a mixture.  head_dim and rotary are even, head_dim up to 512.  Device pointers,
+ * asynchronous.  The reference rotates on the host (model.hpp:67-76). */
+TVARA_API int tvara_slot_plan_rotate(tvara_slot_plan* plan, const int64_t* slots, size_t n, size_t layer, size_t heads,
+                                     const float* q, size_t q_stride, const float* keys, const float* values,
+                                     size_t kv_stride, const int32_t* positions, const float* freqs, size_t rotary,
+                                     int interleaved, const float* q_norm, const float* k_norm, float eps, float* q_out,
+                                     float* k_out, void* stream);
+/* K/V of layers layer .. layer + layers - 1 out of slots, as f32 (Q8_0 blocks: scale *
+ * byte): entry t to element (t, layer, column) as tvara_slot_plan_write has them, the
+ * first layer at 0; an entry with slot -1 leaves its rows as they are, a slot outside
+ * the pool too and is reported by tvara_slot_plan_check.  Strides in multiples of 4 for
+ * Q8_0 blocks.  Device pointers, asynchronous. */
+TVARA_API int tvara_slot_plan_read(tvara_slot_plan* plan, const int64_t* slots, size_t n, size_t layer, size_t layers,
+                                   float* keys, float* values, size_t row_stride, size_t layer_stride, void* stream);
 TVARA_API int tvara_slot_plan_check(tvara_slot_plan* plan);
 TVARA_API void tvara_slot_plan_destroy(tvara_slot_plan* plan);
 

@@ -10,4 +10,4 @@ include/tvara_capi.h); this package is its Python surface:
 * tvara_amd.build      -- the in-tree hipcc build
 """
 
-__all__ = ["kv", "attention", "synth", "workloads"]
+__all__ = ["kv", "attention", "sampling", "synth", "workloads"]

@@ -44,6 +44,8 @@ SIGNATURES = {
     "tvara_sequences_verify_trees": (C.c_int, [_vp, C.POINTER(_u64), _sz, C.POINTER(_sz), C.POINTER(C.c_int32),
                                                C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_int32),
                                                C.POINTER(_sz), C.POINTER(C.c_uint32)]),
+    "tvara_sequences_sample": (C.c_int, [_vp, C.POINTER(_u64), C.POINTER(C.c_uint32), _sz, _fp, _fp, C.POINTER(C.c_int32), _fp,
+                                         _fp, C.POINTER(C.c_uint32), _fp]),
     "tvara_model_cache": (_vp, [_vp]),
     "tvara_radix_create": (_vp, [_vp, C.c_char_p]),
     "tvara_radix_destroy": (None, [_vp]),
@@ -120,6 +122,10 @@ SIGNATURES = {
     "tvara_tree_plan_destroy": (None, [_vp]),
     "tvara_attn_tree": (C.c_int, [_vp, C.POINTER(_u64), _sz, _sz, _sz, _sz, C.POINTER(_sz), C.POINTER(_sz),
                                   C.POINTER(C.c_int32), _fp, _fp, _fp, _fp, C.c_int, C.c_int]),
+    "tvara_sample_plan_create": (_vp, [_sz, _sz]),
+    "tvara_sample_plan_launch": (C.c_int, [_vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "tvara_sample_plan_check": (C.c_int, [_vp]),
+    "tvara_sample_plan_destroy": (None, [_vp]),
     "tvara_score_plan_create": (_vp, [_vp, C.POINTER(_u64), _sz, _sz, _sz, C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz),
                                       C.POINTER(_sz), C.c_float, C.c_float, _fp]),
     "tvara_score_plan_launch": (C.c_int, [_vp, _sz, _vp, _vp, _vp]),
@@ -130,6 +136,9 @@ SIGNATURES = {
     "tvara_slot_plan_create": (_vp, [_vp, C.POINTER(_u64), _sz]),
     "tvara_slot_plan_build": (C.c_int, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _vp]),
     "tvara_slot_plan_write": (C.c_int, [_vp, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp]),
+    "tvara_slot_plan_rotate": (C.c_int, [_vp, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz, C.c_int, _vp, _vp,
+                                         C.c_float, _vp, _vp, _vp]),
+    "tvara_slot_plan_read": (C.c_int, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _sz, _vp]),
     "tvara_slot_plan_check": (C.c_int, [_vp]),
     "tvara_slot_plan_destroy": (None, [_vp]),
     "tvara_profile_enable": (C.c_int, [C.c_int]),

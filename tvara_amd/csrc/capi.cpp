@@ -18,6 +18,7 @@
 #include "host_copy.hpp"
 #include "kv_cache.hpp"
 #include "model.hpp"
+#include "sample.hpp"
 #include "score.hpp"
 #include "tree.hpp"
 
@@ -68,6 +69,10 @@ struct tvara_tree_plan {
 
 struct tvara_slot_plan {
     tvara_amd::SlotPlan plan;
+};
+
+struct tvara_sample_plan {
+    tvara_amd::SamplePlan plan;
 };
 
 struct tvara_score_plan {
@@ -522,6 +527,66 @@ int tvara_slot_plan_write(tvara_slot_plan* plan, const int64_t* slots, const int
     });
 }
 
+int tvara_slot_plan_rotate(tvara_slot_plan* plan, const int64_t* slots, size_t n, size_t layer, size_t heads, const float* q,
+                           size_t q_stride, const float* keys, const float* values, size_t kv_stride,
+                           const int32_t* positions, const float* freqs, size_t rotary, int interleaved,
+                           const float* q_norm, const float* k_norm, float eps, float* q_out, float* k_out, void* stream) {
+    return guard([&] {
+        if (!plan) throw std::invalid_argument("null slot plan");
+        if (n && ((q_out && !q) || (k_out && !keys) || (slots && (!keys || !values)) || (rotary && (!positions || !freqs))))
+            throw std::invalid_argument("null rotation buffers");
+        if (!aligned16(slots) || !aligned16(q) || !aligned16(keys) || !aligned16(values) || !aligned16(positions) ||
+            !aligned16(freqs) || !aligned16(q_norm) || !aligned16(k_norm) || !aligned16(q_out) || !aligned16(k_out))
+            throw std::invalid_argument("device buffers must be 16-byte aligned");
+        const size_t most = static_cast<size_t>(std::numeric_limits<int>::max());
+        if (layer > most || heads > most || rotary > most) throw std::invalid_argument("invalid rotation shape");
+        hipStream_t s = stream ? static_cast<hipStream_t>(stream) : plan->plan.cache->stream();
+        tvara_amd::RotateArgs a{};
+        a.layer = static_cast<int>(layer);
+        a.heads = static_cast<int>(heads);
+        a.rotary = static_cast<int>(rotary);
+        a.interleaved = interleaved != 0;
+        a.n = n;
+        a.slots = slots;
+        a.q = q;
+        a.keys = keys;
+        a.values = values;
+        a.q_stride = q_stride;
+        a.kv_stride = kv_stride;
+        a.positions = positions;
+        a.freqs = freqs;
+        a.q_norm = q_norm;
+        a.k_norm = k_norm;
+        a.eps = eps;
+        a.q_out = q_out;
+        a.k_out = k_out;
+        plan->plan.rotate(a, s);
+    });
+}
+
+int tvara_slot_plan_read(tvara_slot_plan* plan, const int64_t* slots, size_t n, size_t layer, size_t layers, float* keys,
+                         float* values, size_t row_stride, size_t layer_stride, void* stream) {
+    return guard([&] {
+        if (!plan) throw std::invalid_argument("null slot plan");
+        if (n && layers && (!slots || !keys || !values)) throw std::invalid_argument("null KV read buffers");
+        if (!aligned16(slots) || !aligned16(keys) || !aligned16(values))
+            throw std::invalid_argument("device buffers must be 16-byte aligned");
+        const size_t most = static_cast<size_t>(std::numeric_limits<int>::max());
+        if (layer > most || layers > most) throw std::invalid_argument("layers outside the cache");
+        hipStream_t s = stream ? static_cast<hipStream_t>(stream) : plan->plan.cache->stream();
+        tvara_amd::ReadArgs a{};
+        a.layer = static_cast<int>(layer);
+        a.layers = static_cast<int>(layers);
+        a.slots = slots;
+        a.n = n;
+        a.keys = keys;
+        a.values = values;
+        a.row_stride = row_stride;
+        a.layer_stride = layer_stride;
+        plan->plan.read(a, s);
+    });
+}
+
 int tvara_slot_plan_check(tvara_slot_plan* plan) {
     return guard([&] {
         if (!plan) throw std::invalid_argument("null slot plan");
@@ -602,6 +667,41 @@ int tvara_attn_score(tvara_kv_cache* cache, const uint64_t* sequences, size_t co
         copier.parallel_copy(reinterpret_cast<char*>(out), reinterpret_cast<const char*>(back), n * sizeof(float));
     });
 }
+
+// --------------------------------------------------------------- sampling
+
+tvara_sample_plan* tvara_sample_plan_create(size_t rows, size_t vocab) {
+    tvara_sample_plan* out = nullptr;
+    guard([&] {
+        auto p = std::make_unique<tvara_sample_plan>();
+        p->plan.build(rows, vocab);
+        out = p.release();
+    });
+    return out;
+}
+
+int tvara_sample_plan_launch(tvara_sample_plan* plan, size_t rows, const float* logits, size_t logits_stride,
+                             const float* uniforms, const float* temperature, const int32_t* top_k, const float* top_p,
+                             const float* min_p, uint32_t* tokens, float* probability, void* stream) {
+    return guard([&] {
+        if (!plan) throw std::invalid_argument("null sample plan");
+        if (rows && (!logits || !uniforms || !tokens)) throw std::invalid_argument("null sampling buffers");
+        if (!aligned16(logits) || !aligned16(uniforms) || !aligned16(temperature) || !aligned16(top_k) || !aligned16(top_p) ||
+            !aligned16(min_p) || !aligned16(tokens) || !aligned16(probability))
+            throw std::invalid_argument("device buffers must be 16-byte aligned");
+        plan->plan.launch(rows, logits, logits_stride, uniforms, temperature, top_k, top_p, min_p, tokens, probability,
+                          static_cast<hipStream_t>(stream));
+    });
+}
+
+int tvara_sample_plan_check(tvara_sample_plan* plan) {
+    return guard([&] {
+        if (!plan) throw std::invalid_argument("null sample plan");
+        plan->plan.check();
+    });
+}
+
+void tvara_sample_plan_destroy(tvara_sample_plan* plan) { delete plan; }
 
 // ------------------------------------------------------- model-level exports
 // c_api.cpp:35-78: return conventions (nullptr / 0 / -1), messages and the
@@ -810,6 +910,25 @@ int tvara_sequences_verify_trees(tvara_model* model, const uint64_t* sequences, 
         if (any && (!parents || !tokens || !path)) throw std::invalid_argument("invalid batch buffers");
         std::lock_guard<std::mutex> lock(model->mutex);
         model->model->verify_trees(sequences, count, nodes, parents, tokens, first, path, accepted, next);
+        return 0;
+    } catch (const std::exception& e) {
+        failed(TVARA_ERROR, e.what());
+        return -1;
+    } catch (...) {
+        failed(TVARA_ERROR, "unknown batch error");
+        return -1;
+    }
+}
+
+int tvara_sequences_sample(tvara_model* model, const uint64_t* sequences, const uint32_t* tokens, size_t count,
+                           const float* uniforms, const float* temperature, const int32_t* top_k, const float* top_p,
+                           const float* min_p, uint32_t* next, float* probability) {
+    tvara_amd::abi::clear();
+    try {
+        if (!model || (count && (!sequences || !tokens || !uniforms || !next)))
+            throw std::invalid_argument("invalid batch buffers");
+        std::lock_guard<std::mutex> lock(model->mutex);
+        model->model->sample_many(sequences, tokens, count, uniforms, temperature, top_k, top_p, min_p, next, probability);
         return 0;
     } catch (const std::exception& e) {
         failed(TVARA_ERROR, e.what());

@@ -176,6 +176,11 @@ DeviceModel::DeviceModel(const std::string& path, size_t max_blocks, size_t bloc
 }
 
 void DeviceModel::decode(uint64_t sequence, size_t token, float* logits_host) {
+    decode_step(sequence, token);
+    copier_.from_device(logits_host, logits_.ptr, cfg_.vocab * sizeof(float), cache_->stream());
+}
+
+void DeviceModel::decode_step(uint64_t sequence, size_t token) {
     const ModelConfig& c = cfg_;
     const size_t position = cache_->sequence(sequence).length;
     if (token >= c.vocab || position >= c.context)
@@ -247,7 +252,6 @@ void DeviceModel::decode(uint64_t sequence, size_t token, float* logits_host) {
     // the token's K/V for every layer, appended after all layers succeeded
     // (paged_model.hpp:27)
     cache_->append_batch(&sequence, 1, at(kall_, 0), at(vall_, 0), true);
-    copier_.from_device(logits_host, logits_.ptr, c.vocab * sizeof(float), s);
 }
 
 void DeviceModel::matvec(const Weight& w, const float* v, const MatvecSegment* seg, int nseg, hipStream_t s,
@@ -312,34 +316,46 @@ DeviceModel::StepEvents::~StepEvents() {
     if (copy) (void)hipStreamDestroy(copy);
 }
 
-void DeviceModel::decode_many(const uint64_t* sequences, const uint32_t* tokens, size_t n, float* logits_host) {
-    if (!n) return;
+std::vector<size_t> DeviceModel::check_step(const uint64_t* sequences, const uint32_t* tokens, size_t n) const {
     const ModelConfig& c = cfg_;
-    std::vector<uint64_t> seqs(sequences, sequences + n);
     std::vector<size_t> positions(n);
     {
-        std::vector<uint64_t> sorted = seqs;
+        std::vector<uint64_t> sorted(sequences, sequences + n);
         std::sort(sorted.begin(), sorted.end());
         if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
             throw std::invalid_argument("duplicate sequence in decode batch");
     }
     for (size_t i = 0; i < n; ++i) {
-        positions[i] = cache_->sequence(seqs[i]).length;
+        positions[i] = cache_->sequence(sequences[i]).length;
         if (tokens[i] >= c.vocab || positions[i] >= c.context)
             throw std::invalid_argument("paged decode exceeds token/context limits");
     }
     if (n > static_cast<size_t>(std::numeric_limits<int>::max() / std::max<size_t>(c.vocab, c.hidden)))
         throw std::invalid_argument("decode batch too large");
+    return positions;
+}
+
+void DeviceModel::decode_many(const uint64_t* sequences, const uint32_t* tokens, size_t n, float* logits_host) {
+    if (!n) return;
     if (!batched_widths()) {
+        const std::vector<size_t> positions = check_step(sequences, tokens, n);
         size_t done = 0;
         try {
-            for (; done < n; ++done) decode(seqs[done], tokens[done], logits_host + done * c.vocab);
+            for (; done < n; ++done) decode(sequences[done], tokens[done], logits_host + done * cfg_.vocab);
         } catch (...) {
-            for (size_t i = 0; i < done; ++i) cache_->truncate(seqs[i], positions[i]);
+            for (size_t i = 0; i < done; ++i) cache_->truncate(sequences[i], positions[i]);
             throw;
         }
         return;
     }
+    const LogitsBands bands = decode_many_step(sequences, tokens, n);
+    copy_logits(bands, n, logits_host);
+}
+
+DeviceModel::LogitsBands DeviceModel::decode_many_step(const uint64_t* sequences, const uint32_t* tokens, size_t n) {
+    const ModelConfig& c = cfg_;
+    const std::vector<uint64_t> seqs(sequences, sequences + n);
+    const std::vector<size_t> positions = check_step(sequences, tokens, n);
     ensure_batch(n, n);
     hipStream_t s = cache_->stream();
     const int N = static_cast<int>(n), KV = static_cast<int>(c.kv_width());
@@ -361,7 +377,57 @@ void DeviceModel::decode_many(const uint64_t* sequences, const uint32_t* tokens,
         for (size_t i = 0; i < applied; ++i) cache_->truncate(seqs[i], positions[i]);  // all or nothing
         throw;
     }
-    copy_logits(bands, n, logits_host);
+    return bands;
+}
+
+void DeviceModel::sample_many(const uint64_t* sequences, const uint32_t* tokens, size_t n, const float* uniforms,
+                              const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                              uint32_t* next, float* probability) {
+    if (!n) return;
+    cache_->check_device();
+    const ModelConfig& c = cfg_;
+    const std::vector<size_t> positions = check_step(sequences, tokens, n);
+    hipStream_t s = cache_->stream();
+    if (!sampler_ || static_cast<size_t>(sampler_->rows) < n) {
+        auto plan = std::make_unique<SamplePlan>();
+        plan->build(n, c.vocab);
+        sampler_ = std::move(plan);
+    }
+    // uniforms | temperature | top_k | top_p | min_p, then tokens | probability, each on 16 bytes
+    const size_t part = (n + 3) / 4 * 4;
+    auto* d = static_cast<float*>(sample_.ensure(7 * part * sizeof(float)));
+    auto* host = static_cast<float*>(sample_host_.acquire(7 * part * sizeof(float)));
+    const void* given[] = {uniforms, temperature, top_k, top_p, min_p};
+    for (int i = 0; i < 5; ++i)
+        if (given[i]) std::memcpy(host + i * part, given[i], n * sizeof(float));
+    TVARA_HIP(hipMemcpyAsync(d, host, 5 * part * sizeof(float), hipMemcpyHostToDevice, s));
+    sample_host_.release(s);
+    size_t done = 0;
+    try {
+        auto draw = [&](const float* logits, size_t row, size_t rows) {
+            auto in = [&](int i) { return given[i] ? d + i * part + row : nullptr; };
+            sampler_->launch(rows, logits, 0, in(0), in(1), reinterpret_cast<const int32_t*>(in(2)), in(3), in(4),
+                             reinterpret_cast<uint32_t*>(d + 5 * part + row), d + 6 * part + row, s);
+        };
+        if (n == 1 || !batched_widths()) {
+            for (; done < n; ++done) {
+                decode_step(sequences[done], tokens[done]);
+                draw(at(logits_, 0), done, 1);
+            }
+        } else {
+            decode_many_step(sequences, tokens, n);
+            done = n;
+            draw(at(blogits_, 0), 0, n);
+        }
+        TVARA_HIP(hipMemcpyAsync(host + 5 * part, d + 5 * part, 2 * part * sizeof(float), hipMemcpyDeviceToHost, s));
+        sample_host_.release(s);
+        sampler_->check();  // (waits for the stream)
+    } catch (...) {
+        for (size_t i = 0; i < std::min(done + 1, n); ++i) cache_->truncate(sequences[i], positions[i]);
+        throw;
+    }
+    std::memcpy(next, host + 5 * part, n * sizeof(uint32_t));
+    if (probability) std::memcpy(probability, host + 6 * part, n * sizeof(float));
 }
 
 void DeviceModel::verify_trees(const uint64_t* sequences, size_t n, const size_t* nodes, const int32_t* parents,

@@ -12,6 +12,7 @@
 #include "common.hpp"
 #include "host_copy.hpp"
 #include "kv_cache.hpp"
+#include "sample.hpp"
 
 namespace tvara_amd {
 
@@ -134,6 +135,12 @@ public:
     // one token for each of n distinct sequences in one pass: the logits of n
     // independent decode() calls; on failure no sequence changes
     void decode_many(const uint64_t* sequences, const uint32_t* tokens, size_t n, float* logits_host);
+    // the same step with its logits left on the GPU and a token drawn from each row of
+    // them there (sample.hpp; host arrays, null as SampleArgs has it); on failure, a row
+    // without a token among it, no sequence changes
+    void sample_many(const uint64_t* sequences, const uint32_t* tokens, size_t n, const float* uniforms,
+                     const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, uint32_t* next,
+                     float* probability);
     // n consecutive tokens at the end of `sequence` in one pass per chunk of
     // up to kChunkRows or kPromptRows tokens (the batched products, each layer's K/V written
     // into the cache, then the rows' causal attention over it): the logits of
@@ -167,6 +174,8 @@ private:
         DeviceBuffer attn_norm, ffn_norm;
         Weight qkv, out, gate_up, down;
     };
+    // decode() up to the logits, which stay in logits_
+    void decode_step(uint64_t sequence, size_t token);
     // y = W v, or W rms_norm(x) * norm_w when norm_w is given (v is then x)
     void matvec(const Weight& w, const float* v, const MatvecSegment* seg, int nseg, hipStream_t s,
                 const float* norm_w = nullptr);
@@ -192,6 +201,10 @@ private:
     // acceptance: each tree's sequence length and expected token, then what it gives
     DeviceBuffer verify_, verify_slots_;
     PinnedBuffer verify_host_;
+    // sampling: what the rows ask for, then what they get
+    std::unique_ptr<SamplePlan> sampler_;
+    DeviceBuffer sample_;
+    PinnedBuffer sample_host_;
     HostCopier copier_;
     // the batched step's synchronisation: an event after the last layer's
     // attention (the plan's check waits on it, not on the whole stream), one
@@ -209,6 +222,11 @@ private:
     };
     StepEvents step_events_;
     size_t batch_cap_ = 0, logits_cap_ = 0;
+    // decode_many() up to the logits, which stay in blogits_, and the appends
+    struct LogitsBands;
+    LogitsBands decode_many_step(const uint64_t* sequences, const uint32_t* tokens, size_t n);
+    // distinct sequences of the model, valid tokens, room for them: their lengths
+    std::vector<size_t> check_step(const uint64_t* sequences, const uint32_t* tokens, size_t n) const;
     // work buffers for n rows, of which `logits` rows give logits
     void ensure_batch(size_t n, size_t logits);
     // the widths the batched products and epilogues take

@@ -1,0 +1,67 @@
+// Plans of sampling (sample.hpp): what the host checks and lays out.
+#include "sample.hpp"
+
+#include <limits>
+#include <stdexcept>
+
+namespace tvara_amd {
+
+void SamplePlan::build(size_t n, size_t v) {
+    constexpr size_t kIntMax = static_cast<size_t>(std::numeric_limits<int32_t>::max());
+    if (!n || !v) throw std::invalid_argument("empty sample plan");
+    // (a workgroup a row, and a thread for every four logits)
+    if (v > kIntMax / 2 || n > kIntMax / 1024 || n > (size_t(1) << 33) / v) throw std::invalid_argument("sample plan too large");
+    TVARA_HIP(hipGetDevice(&device));
+    rows = static_cast<int>(n);
+    vocab = static_cast<int>(v);
+    chunk = 256;
+    while (v > static_cast<size_t>(chunk) * kSampleChunks) chunk *= 2;
+    chunks = static_cast<int>((v + chunk - 1) / chunk);
+    space.ensure(n * chunks * (sizeof(float) + sizeof(double)));
+    auto* f = static_cast<volatile int*>(flag.acquire(2 * sizeof(int)));
+    f[0] = 0;
+    f[1] = 0;
+}
+
+void SamplePlan::launch(size_t n, const float* logits, size_t stride, const float* uniforms, const float* temperature,
+                        const int32_t* top_k, const float* top_p, const float* min_p, uint32_t* tokens, float* probability,
+                        hipStream_t s) {
+    if (n > static_cast<size_t>(rows)) throw std::invalid_argument("more rows than the sample plan has");
+    if (!stride) stride = vocab;
+    if (stride < static_cast<size_t>(vocab)) throw std::invalid_argument("logit rows overlap");
+    if (!n) return;
+    int dev = 0;
+    TVARA_HIP(hipGetDevice(&dev));
+    if (dev != device) throw std::invalid_argument("the sample plan is on another device");
+    SampleArgs a{};
+    a.logits = logits;
+    a.stride = stride;
+    a.rows = static_cast<int>(n);
+    a.vocab = vocab;
+    a.chunk = chunk;
+    a.chunks = chunks;
+    a.uniforms = uniforms;
+    a.temperature = temperature;
+    a.top_k = top_k;
+    a.top_p = top_p;
+    a.min_p = min_p;
+    a.tokens = tokens;
+    a.probability = probability;
+    a.chunk_mass = static_cast<double*>(space.ptr);
+    a.chunk_max = reinterpret_cast<float*>(a.chunk_mass + static_cast<size_t>(rows) * chunks);
+    a.err = static_cast<int*>(flag.ptr);
+    launch_sample(a, s);
+    last = s;
+}
+
+void SamplePlan::check() {
+    TVARA_HIP(hipStreamSynchronize(last));
+    auto* f = static_cast<volatile int*>(flag.ptr);
+    const bool logits = f[0], asked = f[1];
+    f[0] = 0;
+    f[1] = 0;
+    if (asked) throw std::invalid_argument("invalid sampling parameters");
+    if (logits) throw std::invalid_argument("invalid logits to sample from");
+}
+
+}  // namespace tvara_amd

@@ -510,10 +510,61 @@ void SlotPlan::write(const int64_t* slots, const int32_t* rows, size_t n, const 
     region.launched(s);
 }
 
+void SlotPlan::rotate(RotateArgs a, hipStream_t s) {
+    if (cache->epoch() != epoch) throw std::invalid_argument("slot plan is stale: the cache changed");
+    const Geometry& g = cache->geometry();
+    if (a.layer < 0 || static_cast<size_t>(a.layer) >= g.layers || a.heads < 1 || a.heads % static_cast<int>(g.kv_heads) ||
+        a.heads + 2 * g.kv_heads > 65535 || g.head_dim % 2 || g.head_dim > 512 || a.rotary < 0 || a.rotary % 2 ||
+        static_cast<size_t>(a.rotary) > g.head_dim)
+        throw std::invalid_argument("invalid rotation shape");
+    if (!(a.eps >= 0) || !std::isfinite(a.eps)) throw std::invalid_argument("invalid norm epsilon");
+    const size_t hidden = a.heads * g.head_dim;
+    if (!a.q_stride) a.q_stride = hidden;
+    if (!a.kv_stride) a.kv_stride = g.kv_width();
+    if (a.q_stride < hidden || a.kv_stride < g.kv_width()) throw std::invalid_argument("token rows overlap");
+    if (a.n > kMaxWorkgroups || 2 * g.layers * g.kv_width() * g.tokens_per_block > kMaxThreads)
+        throw std::invalid_argument("KV write too large");
+    if (!a.n) return;
+    cache->check_device();
+    cache->enter(s);
+    a.pool = cache->pool();
+    a.lay = cache->layout();
+    a.slot_count = static_cast<int64_t>(g.max_blocks * g.tokens_per_block);
+    a.err = region.flags() + 2;
+    launch_rotate(a, s);
+    cache->leave(s);
+    region.launched(s);
+}
+
+void SlotPlan::read(ReadArgs a, hipStream_t s) {
+    if (cache->epoch() != epoch) throw std::invalid_argument("slot plan is stale: the cache changed");
+    const Geometry& g = cache->geometry();
+    if (a.layer < 0 || a.layers < 0 || static_cast<size_t>(a.layer) > g.layers || static_cast<size_t>(a.layers) > g.layers - a.layer)
+        throw std::invalid_argument("layers outside the cache");
+    if (a.row_stride < g.kv_width() || (a.layers > 1 && a.layer_stride < g.kv_width()))
+        throw std::invalid_argument("token rows overlap");
+    if (a.n > kMaxWorkgroups || 2 * g.layers * g.kv_width() > size_t(65535) * 256 ||
+        2 * g.layers * g.kv_width() * g.tokens_per_block > kMaxThreads)
+        throw std::invalid_argument("KV read too large");
+    if (cache->format() == kQ8 && (a.row_stride % 4 || (a.layers > 1 && a.layer_stride % 4)))
+        throw std::invalid_argument("device buffers must be 16-byte aligned");
+    if (!a.n || !a.layers) return;
+    cache->check_device();
+    cache->enter(s);
+    a.pool = cache->pool();
+    a.lay = cache->layout();
+    a.slot_count = static_cast<int64_t>(g.max_blocks * g.tokens_per_block);
+    a.err = region.flags() + 2;
+    launch_slot_read(a, s);
+    cache->leave(s);
+    region.launched(s);
+}
+
 void SlotPlan::check() {
     const int set = region.check();
     if (set & 1) throw std::invalid_argument("slot map outside the sequences' own blocks");
     if (set & 2) throw std::invalid_argument("KV write outside the pool or the rows");
+    if (set & 4) throw std::invalid_argument("slot outside the pool");
 }
 
 }  // namespace tvara_amd

@@ -96,6 +96,43 @@ struct WriteArgs {
     int* err;
 };
 
+// queries and keys normalised and rotated, keys and values into slots (launch_rotate)
+struct RotateArgs {
+    char* pool;
+    BlockLayout lay;
+    int64_t slot_count;
+    int layer, heads, rotary;  // rotary: columns of a head that turn, the first ones
+    bool interleaved;          // pair j: columns 2j and 2j + 1, or j and j + rotary / 2
+    size_t n;
+    const int64_t* slots;      // [n] or null, -1: nothing to write
+    const float* q;            // [n] rows of heads * head_dim, q_stride apart
+    const float* keys;         // [n] rows of kv_width, kv_stride apart
+    const float* values;
+    size_t q_stride, kv_stride;
+    const int32_t* positions;  // [n]
+    const float* freqs;        // [rotary / 2]
+    const float* q_norm;       // [head_dim] or null: as they are
+    const float* k_norm;
+    float eps;
+    float* q_out;              // [n][heads * head_dim] or null
+    float* k_out;              // [n][kv_width] or null
+    int* err;
+};
+
+// cached rows of layers layer .. layer + layers - 1 (launch_slot_read)
+struct ReadArgs {
+    const char* pool;
+    BlockLayout lay;
+    int64_t slot_count;
+    int layer, layers;
+    const int64_t* slots;  // [n], -1: its rows stay as they are
+    size_t n;
+    float* keys;           // element (row, layer, column) as WriteArgs has it
+    float* values;
+    size_t row_stride, layer_stride;
+    int* err;
+};
+
 // tree.hip
 void launch_tree_rows(const TreeArgs& a, int items, hipStream_t s);
 void launch_tree_merge(const TreeArgs& a, int most_runs, hipStream_t s);
@@ -122,6 +159,9 @@ void launch_tree_accept(const AcceptArgs& a, hipStream_t s);
 // slots.hip
 void launch_slot_map(const SlotArgs& a, hipStream_t s);
 void launch_slot_write(const WriteArgs& a, hipStream_t s);
+// rotate.hip
+void launch_rotate(const RotateArgs& a, hipStream_t s);
+void launch_slot_read(const ReadArgs& a, hipStream_t s);
 
 // The device memory of a plan: sections of one region, the first of them
 // uploaded in one copy on the cache's stream.  Plans that stayed on the null
@@ -144,7 +184,7 @@ public:
     char* device() const { return static_cast<char*>(buf_->region.ptr); }
     // the kernels' error words, in pinned host memory
     int* flags() const { return static_cast<int*>(buf_->flag.ptr); }
-    static constexpr int kFlags = 2;
+    static constexpr int kFlags = 3;
     void launched(hipStream_t s);
     // waits for the last launch's stream; the words that were set (bit i: word
     // i), which are cleared
@@ -200,6 +240,9 @@ struct SlotPlan {
              int32_t* positions, int64_t* slots, int32_t* tables, size_t width, hipStream_t s);
     void write(const int64_t* slots, const int32_t* rows, size_t n, const float* keys, const float* values,
                size_t row_count, size_t row_stride, size_t layer_stride, hipStream_t s);
+    // fills in the cache's part of the arguments
+    void rotate(RotateArgs a, hipStream_t s);
+    void read(ReadArgs a, hipStream_t s);
     void check();
 };
 

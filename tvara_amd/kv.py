@@ -353,7 +353,8 @@ class PagedCache:
 
 class SlotPlan:
     """Resident block ids of listed sequences (tvara_slot_plan_*): slot maps and
-    block tables from device lengths, and K/V writes through them.  Pointers
+    block tables from device lengths, and K/V writes (rotated ones too) and reads
+    through them.  Pointers
     are device addresses (ints); launches are asynchronous."""
 
     def __init__(self, cache, seqs):
@@ -377,6 +378,23 @@ class SlotPlan:
         row rows[t] (int32; None: row t) of row_count."""
         _capi.check(self.lib.tvara_slot_plan_write(self.h, slots_ptr, rows_ptr, n, keys_ptr, values_ptr, row_count,
                                                    row_stride, layer_stride, stream), self.lib)
+
+    def rotate(self, slots_ptr, n, layer, q_ptr, keys_ptr, values_ptr, positions_ptr, freqs_ptr, rotary, heads, q_out_ptr,
+               k_out_ptr=None, q_stride=0, kv_stride=0, q_norm_ptr=None, k_norm_ptr=None, eps=1e-6, interleaved=False,
+               stream=None):
+        """A layer's queries and keys normalised head by head (where weights are
+        given) and rotated by position * freqs in their first ``rotary`` columns;
+        queries to rows at q_out, keys and values into slots (int64; -1: skipped;
+        None: none is written), rotated keys to rows at k_out if given."""
+        _capi.check(self.lib.tvara_slot_plan_rotate(self.h, slots_ptr, n, layer, heads, q_ptr, q_stride, keys_ptr, values_ptr,
+                                                    kv_stride, positions_ptr, freqs_ptr, rotary, int(interleaved), q_norm_ptr,
+                                                    k_norm_ptr, eps, q_out_ptr, k_out_ptr, stream), self.lib)
+
+    def read(self, slots_ptr, n, layer, layers, keys_ptr, values_ptr, row_stride, layer_stride, stream=None):
+        """K/V of layers layer .. layer + layers - 1 out of slots (int64; -1: its
+        rows stay as they are) into f32 rows, laid out as write has them."""
+        _capi.check(self.lib.tvara_slot_plan_read(self.h, slots_ptr, n, layer, layers, keys_ptr, values_ptr, row_stride,
+                                                  layer_stride, stream), self.lib)
 
     def check(self):
         _capi.check(self.lib.tvara_slot_plan_check(self.h), self.lib)

@@ -161,6 +161,41 @@ class NativeModel:
                 self._raise_error()
         return output
 
+    def sample_sequences(self, sequences, tokens, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """One token for each of several distinct sequences, and the next of each
+        drawn on the GPU (tvara_sequences_sample): uniforms in [0, 1), one for
+        each; the parameters one for all or one for each (temperature 0: the
+        largest logit, top_k 0: all).  Returns the next tokens and their
+        probabilities."""
+        seqs = np.ascontiguousarray(sequences, dtype=np.uint64).reshape(-1)
+        if not len(tokens) == len(uniforms) == seqs.size:
+            raise ValueError("one token and one random number per sequence")
+        if any(not self._valid_token(t) for t in tokens):
+            raise ValueError("Invalid token ID")
+        toks = np.array([int(t) for t in tokens], dtype=np.uint32)
+
+        def each(values, dtype):
+            return np.ascontiguousarray(np.broadcast_to(np.asarray(values, dtype=dtype), seqs.shape))
+
+        given = np.asarray(top_k)
+        if given.dtype.kind not in "iu" or (given < 0).any() or (given > 2**31 - 1).any():
+            raise ValueError("top_k is a whole number from 0")
+        u, t, p, m = (each(x, np.float32) for x in (uniforms, temperature, top_p, min_p))
+        k = each(given, np.int32)
+        after, chances = np.zeros(seqs.size, np.uint32), np.zeros(seqs.size, np.float32)
+
+        def ptr(a, kind):
+            return a.ctypes.data_as(ctypes.POINTER(kind))
+
+        with self._lock:
+            self._check_open()
+            if self._library.tvara_sequences_sample(
+                    self._handle, ptr(seqs, ctypes.c_uint64), ptr(toks, ctypes.c_uint32), seqs.size, ptr(u, ctypes.c_float),
+                    ptr(t, ctypes.c_float), ptr(k, ctypes.c_int32), ptr(p, ctypes.c_float), ptr(m, ctypes.c_float),
+                    ptr(after, ctypes.c_uint32), ptr(chances, ctypes.c_float)):
+                self._raise_error()
+        return after.tolist(), chances
+
     def verify_trees(self, sequences, parents, tokens, first):
         """One step of speculative decoding (tvara_sequences_verify_trees):
         parents[i] and tokens[i] are the drafted tree at the end of
