@@ -1,8 +1,10 @@
 // Plans of sampling (sample.hpp): what the host checks and lays out.
 #include "sample.hpp"
 
+#include <algorithm>
 #include <limits>
 #include <stdexcept>
+#include <type_traits>
 
 namespace tvara_amd {
 
@@ -17,10 +19,30 @@ void SamplePlan::build(size_t n, size_t v) {
     chunk = 256;
     while (v > static_cast<size_t>(chunk) * kSampleChunks) chunk *= 2;
     chunks = static_cast<int>((v + chunk - 1) / chunk);
-    space.ensure(n * chunks * (sizeof(float) + sizeof(double)));
+    room = static_cast<int>(std::min<size_t>(v, kSampleList));
+    carve(nullptr, nullptr);
+    space.ensure(bytes);
     auto* f = static_cast<volatile int*>(flag.acquire(2 * sizeof(int)));
     f[0] = 0;
     f[1] = 0;
+}
+
+// the workspace's parts, into `a` where it is given; bytes: all of them
+void SamplePlan::carve(char* base, SampleArgs* a) {
+    bytes = 0;
+    auto part = [&](auto*& p, size_t each) {
+        if (a) p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(base + bytes);
+        bytes = (bytes + each * rows * sizeof(*p) + 255) / 256 * 256;
+    };
+    SampleArgs none{}, &to = a ? *a : none;
+    part(to.group_mass, kSampleGroups);
+    part(to.chunk_mass, chunks);
+    part(to.chunk_max, chunks);
+    part(to.list, room);
+    part(to.rows_state, 1);
+    if (vocab <= kSampleList) return;
+    part(to.bin_mass, kSampleBins);
+    part(to.bin_count, kSampleBins);
 }
 
 void SamplePlan::launch(size_t n, const float* logits, size_t stride, const float* uniforms, const float* temperature,
@@ -47,8 +69,8 @@ void SamplePlan::launch(size_t n, const float* logits, size_t stride, const floa
     a.min_p = min_p;
     a.tokens = tokens;
     a.probability = probability;
-    a.chunk_mass = static_cast<double*>(space.ptr);
-    a.chunk_max = reinterpret_cast<float*>(a.chunk_mass + static_cast<size_t>(rows) * chunks);
+    a.room = room;
+    carve(static_cast<char*>(space.ptr), &a);
     a.err = static_cast<int*>(flag.ptr);
     launch_sample(a, s);
     last = s;
