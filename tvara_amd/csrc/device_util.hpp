@@ -51,6 +51,8 @@ __device__ __forceinline__ float cross_row_max(float v) {
 }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -80,6 +82,20 @@ __device__ __forceinline__ void add_to(float& l, float& rounded, float sum) {
 
 __device__ __forceinline__ bool all_finite(f32x4 x) {
     return __builtin_isfinite(x[0]) && __builtin_isfinite(x[1]) && __builtin_isfinite(x[2]) && __builtin_isfinite(x[3]);
+}
+
+// Two values as hi + lo in fp16, each rounded to nearest (22 bits; beyond fp16's
+// range one is infinite and the other its opposite).  `one` is 1, hidden from the
+// compiler, so that x - hi stays a mixed-precision fma: four instructions a pair
+// where converting hi back takes six.
+__device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned& lo) {
+    float one = 1.f;
+    asm("" : "+s"(one));
+    const f32x2 v = {x, y};
+    const f16x2 h = __builtin_convertvector(v, f16x2);
+    const f32x2 rest = {fmaf(-static_cast<float>(h[0]), one, x), fmaf(-static_cast<float>(h[1]), one, y)};
+    hi = __builtin_bit_cast(unsigned, h);
+    lo = __builtin_bit_cast(unsigned, __builtin_convertvector(rest, f16x2));
 }
 
 }  // namespace tvara_amd

@@ -15,8 +15,8 @@
 namespace tvara_amd {
 namespace {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
@@ -37,6 +37,21 @@ __device__ __forceinline__ Item item_of(const ScoreArgs& a, unsigned i) {
 __device__ __forceinline__ int uniform_max(int v) {
     for (int o = 8; o >= 1; o >>= 1) v = max(v, __shfl_xor(v, o));
     return __builtin_amdgcn_readfirstlane(v);
+}
+
+// maximum over the n lanes (8 or 16, from a multiple of n) of a key's row
+template <int kControl>
+__device__ __forceinline__ float moved(float v) {
+    const int b = __builtin_bit_cast(int, v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(b, b, kControl, 0xf, 0xf, false));
+}
+template <int n>
+__device__ __forceinline__ float row_max(float v) {
+    constexpr int kSwap1 = 0xb1, kSwap2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;
+    v = fmaxf(v, moved<kSwap1>(v));
+    v = fmaxf(v, moved<kSwap2>(v));
+    v = fmaxf(v, moved<kHalfMirror>(v));
+    return n == 16 ? fmaxf(v, moved<kMirror>(v)) : v;
 }
 
 // ------------------------------------------------------------- few rows
@@ -389,42 +404,60 @@ constexpr int kManyWaves = 8;
 
 // ds_read_b64_tr_b16: within 16 lanes, lane i receives element i % 4 of the four that
 // lane 4j + i / 4 addresses, as its element j
-__device__ __forceinline__ bf16x4 transposed_read(const __bf16* p) {
+__device__ __forceinline__ f16x4 transposed_read(const _Float16* p) {
     typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
     const i16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p));
-    return __builtin_bit_cast(bf16x4, v);
+    return __builtin_bit_cast(f16x4, v);
 }
 
-// Four values as three parts in bf16, each the rest's nearest: 24 bits and more, f32's
-// whole range but what lies below 2^-126 (a value that rounds beyond bf16's largest,
-// 3.39e38, is infinite in the first).
-__device__ __forceinline__ void split3(f32x4 x, bf16x4& p0, bf16x4& p1, bf16x4& p2) {
-    p0 = __builtin_convertvector(x, bf16x4);
-    const f32x4 r1 = x - __builtin_convertvector(p0, f32x4);
-    p1 = __builtin_convertvector(r1, bf16x4);
-    p2 = __builtin_convertvector(r1 - __builtin_convertvector(p1, f32x4), bf16x4);
+// Eight values as two fp16 parts, hi + lo = x to 22 bits.
+struct Parts {
+    u32x4 hi, lo;
+    __device__ __forceinline__ f16x8 high() const { return __builtin_bit_cast(f16x8, hi); }
+    __device__ __forceinline__ f16x8 low() const { return __builtin_bit_cast(f16x8, lo); }
+};
+__device__ __forceinline__ Parts split8(f32x4 x, f32x4 y) {
+    Parts p;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        unsigned hi, lo;
+        split2(x[2 * e], x[2 * e + 1], hi, lo);
+        p.hi[e] = hi;
+        p.lo[e] = lo;
+        split2(y[2 * e], y[2 * e + 1], hi, lo);
+        p.hi[2 + e] = hi;
+        p.lo[2 + e] = lo;
+    }
+    return p;
 }
-__device__ __forceinline__ bf16x8 both(bf16x4 x, bf16x4 y) {
-    return bf16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-}
-// the largest value that keeps a finite first part
-constexpr float kMostParts = 3.38e38f;
 
-// Up to 256 attention rows, eight waves of 32.  f32 products as six of bf16 parts
-// (16x16x32, 16 times the f32 instruction's rate): of x = x0 + x1 + x2 and y likewise
-// x0 y0 + x0 y1 + x1 y0 + x1 y1 + x0 y2 + x2 y0, what is left out being 2^-25 of the
-// product, with no range of its own.  All waves load and split a step's keys and values
-// once, into the other of two buffers in LDS; one barrier a step.
+// Rows go into parts multiplied by a power of two that brings their largest element to
+// 2^14 .. 2^15: then an element is off by 2^-23 of itself or 2^-40 of the row's largest,
+// whatever the row's size.  The exponent (0 for 2^0 .. 2^1) of a magnitude, kept where
+// both that power and its inverse, times 2^15 more, are normal numbers.
+__device__ __forceinline__ int exponent_of(float most) {
+    return max(static_cast<int>(__builtin_bit_cast(unsigned, most) >> 23 & 255) - 127, -97);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (e + 127) << 23); }
+constexpr int kHigh = 14;  // the exponent of a row's largest element in parts
+
+// Up to 256 attention rows, eight waves of 32.  f32 products as three of fp16 parts
+// (16x16x32, 16 times the f32 instruction's rate): lo hi + hi lo + hi hi, of rows
+// brought to one size by powers of two (queries by lanes, keys and values when they are
+// staged), which the scores, and the probabilities before their own parts, are multiplied
+// by again.  All waves load and split a step's keys and values once, into the other of two
+// buffers in LDS; one barrier a step.
 template <int D, bool kQ8>
 __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const ScoreArgs a) {
     constexpr int NT = 2, KC = D / 32, DT = D / 16;
     constexpr int KEYS = 4096 / D, MT = KEYS / 16;  // keys of a step: eight columns a thread
     constexpr int LPR = D / 8;                      // lanes of a key's row
     constexpr int STR = D + 16;                     // LDS row pitch: no bank twice
-    __shared__ __attribute__((aligned(16))) __bf16 kparts[2][3][KEYS * STR];
-    __shared__ __attribute__((aligned(16))) __bf16 vparts[2][3][KEYS * STR];
-    __shared__ int odds[2][kManyWaves];          // some value of the wave's keys is not finite:
-    __shared__ uint8_t which[2][KEYS][D / 8];    // bit c % 8 of [key][c / 8]: the value of column c
+    __shared__ __attribute__((aligned(16))) _Float16 kparts[2][2][KEYS * STR];
+    __shared__ __attribute__((aligned(16))) _Float16 vparts[2][2][KEYS * STR];
+    __shared__ __attribute__((aligned(16))) float kscale[2][KEYS];  // what a key's scores are multiplied by
+    __shared__ __attribute__((aligned(16))) float vscale[2][KEYS];  // and its probability
+    __shared__ int odd_values;  // some value is not finite
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, r16 = lane & 15;
     const Item it = item_of(a, blockIdx.x);
@@ -459,23 +492,29 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
     all_lo = uniform_max(all_lo);
     all_hi = -uniform_max(-all_hi);
 
-    bf16x8 qp[NT][KC][3];
+    Parts q[NT][KC];
+    float qsize[NT];  // what a row's scores are multiplied by
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+        f32x4 x[KC][2];
+        float most = 0.f;
 #pragma unroll
-        for (int kc = 0; kc < KC; ++kc) {
-            f32x4 x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0;
-            if (live[nt]) {
-                const float* q = a.q + ((static_cast<size_t>(it.row0) + index[nt]) * a.heads + head[nt]) * D + 32 * kc + 8 * g;
-                x0 = *reinterpret_cast<const f32x4*>(q) * a.qscale;
-                x1 = *reinterpret_cast<const f32x4*>(q + 4) * a.qscale;
+        for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                x[kc][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (live[nt])
+                    x[kc][i] = *reinterpret_cast<const f32x4*>(
+                        a.q + ((static_cast<size_t>(it.row0) + index[nt]) * a.heads + head[nt]) * D + 32 * kc + 8 * g + 4 * i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) most = fmaxf(most, __builtin_fabsf(x[kc][i][e]));
             }
-            bf16x4 p[2][3];
-            split3(x0, p[0][0], p[0][1], p[0][2]);
-            split3(x1, p[1][0], p[1][1], p[1][2]);
+        const int size = exponent_of(cross_row_max(most));
+        const float up = power_of_two(kHigh - size);
+        qsize[nt] = power_of_two(size - kHigh) * a.qscale;
 #pragma unroll
-            for (int i = 0; i < 3; ++i) qp[nt][kc][i] = both(p[0][i], p[1][i]);
-        }
+        for (int kc = 0; kc < KC; ++kc) q[nt][kc] = split8(x[kc][0] * up, x[kc][1] * up);
+    }
 
     // staging: eight columns of a key; a wave's keys lie in one block
     const int skey = tid / LPR, col = 8 * (tid % LPR);
@@ -518,28 +557,34 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
                 vreg[i] = f32x4{sbyte_to_float<0>(vw) * vd, sbyte_to_float<1>(vw) * vd, sbyte_to_float<2>(vw) * vd, sbyte_to_float<3>(vw) * vd};
             }
         }
-        unsigned odd = 0;
+        float kmost = 0.f, vmost = 0.f;
+        bool odd = false;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (!(__builtin_fabsf(vreg[i][e]) < kMostParts)) {
-                    odd |= 1u << (4 * i + e);
-                    vreg[i][e] = 0.f;
-                }
-        const bool any = __any(odd != 0);
-        if (lane == 0) odds[buf][wave] = any;
-        if (any) which[buf][skey][col / 8] = static_cast<uint8_t>(odd);
+            for (int e = 0; e < 4; ++e) {
+                const bool fine = __builtin_isfinite(vreg[i][e]);
+                odd |= !fine;
+                vreg[i][e] = fine ? vreg[i][e] : 0.f;
+                kmost = fmaxf(kmost, __builtin_fabsf(kreg[i][e]));
+                vmost = fmaxf(vmost, __builtin_fabsf(vreg[i][e]));
+            }
+        if (odd) odd_values = 1;
+        // over the row's lanes: 8, or 16
+        kmost = row_max<LPR>(kmost);
+        vmost = row_max<LPR>(vmost);
+        const int ksize = exponent_of(kmost), size = exponent_of(vmost);
+        if (tid % LPR == 0) {
+            kscale[buf][skey] = power_of_two(ksize - kHigh);
+            vscale[buf][skey] = power_of_two(size);
+        }
         const int at = skey * STR + col;
-        bf16x4 p[2][3];
-        split3(kreg[0], p[0][0], p[0][1], p[0][2]);
-        split3(kreg[1], p[1][0], p[1][1], p[1][2]);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) *reinterpret_cast<bf16x8*>(&kparts[buf][i][at]) = both(p[0][i], p[1][i]);
-        split3(vreg[0], p[0][0], p[0][1], p[0][2]);
-        split3(vreg[1], p[1][0], p[1][1], p[1][2]);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) *reinterpret_cast<bf16x8*>(&vparts[buf][i][at]) = both(p[0][i], p[1][i]);
+        const float kup = power_of_two(kHigh - min(ksize, 127)), vup = power_of_two(kHigh - size);
+        const Parts k = split8(kreg[0] * kup, kreg[1] * kup), v = split8(vreg[0] * vup, vreg[1] * vup);
+        *reinterpret_cast<u32x4*>(&kparts[buf][0][at]) = k.hi;
+        *reinterpret_cast<u32x4*>(&kparts[buf][1][at]) = k.lo;
+        *reinterpret_cast<u32x4*>(&vparts[buf][0][at]) = v.hi;
+        *reinterpret_cast<u32x4*>(&vparts[buf][1][at]) = v.lo;
     };
 
     f32x4 acc[DT][NT];
@@ -551,14 +596,11 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[dt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // the products of three parts each, small ones first
-    auto six = [](const bf16x8 (&x)[3], const bf16x8 (&y)[3], f32x4 c) __attribute__((always_inline)) {
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[2], y[0], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[2], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[1], y[1], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[1], y[0], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[1], c, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[0], c, 0, 0, 0);
+    // the products of two parts each, small ones first
+    auto three = [](const Parts& x, const Parts& y, f32x4 c) __attribute__((always_inline)) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.low(), y.high(), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.high(), y.low(), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(x.high(), y.high(), c, 0, 0, 0);
     };
     auto compute = [&](int buf, int stp) __attribute__((always_inline)) {
         const int key0 = KEYS * stp;
@@ -569,22 +611,28 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s[mt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // (operands are read from LDS one ahead of their products)
+        auto key_parts = [&](int o) __attribute__((always_inline)) {
+            const int at = (16 * (o % MT) + r16) * STR + 32 * (o / MT) + 8 * g;
+            return Parts{*reinterpret_cast<const u32x4*>(&kparts[buf][0][at]), *reinterpret_cast<const u32x4*>(&kparts[buf][1][at])};
+        };
+        Parts k = key_parts(0);
 #pragma unroll
-        for (int kc = 0; kc < KC; ++kc)
+        for (int o = 0; o < KC * MT; ++o) {
+            const Parts now = k;
+            if (o + 1 < KC * MT) k = key_parts(o + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                bf16x8 k[3];
-#pragma unroll
-                for (int i = 0; i < 3; ++i)
-                    k[i] = *reinterpret_cast<const bf16x8*>(&kparts[buf][i][(16 * mt + r16) * STR + 32 * kc + 8 * g]);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) s[mt][nt] = six(k, qp[nt][kc], s[mt][nt]);
-            }
-        float alpha[NT];
-        bf16x8 pp[NT][MT / 2][3];
+            for (int nt = 0; nt < NT; ++nt) s[o % MT][nt] = three(now, q[nt][o / MT], s[o % MT][nt]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        float alpha[NT], down[NT];
+        Parts p[NT][MT / 2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int first = range[nt].x - key0 - 4 * g, end = range[nt].y - key0 - 4 * g;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) s[mt][nt] *= *reinterpret_cast<const f32x4*>(&kscale[buf][16 * mt + 4 * g]) * qsize[nt];
             if (!whole) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
@@ -596,12 +644,12 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
 #pragma unroll
                 for (int i = 0; i < 4; ++i) nonfinite = fmaf(s[mt][nt][i], 0.f, nonfinite);
             if (a.cap != 0.f) {
-                float most = 0.f;
+                float top = 0.f;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) most = fmaxf(most, __builtin_fabsf(s[mt][nt][i]));
-                if (!__any(most > kSmallTanh)) {
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, __builtin_fabsf(s[mt][nt][i]));
+                if (!__any(top > kSmallTanh)) {
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -636,28 +684,39 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
             const float mn = fmaxf(m[nt], cross_row_max(mx)), base = mn == -INFINITY ? 0.f : mn;
             alpha[nt] = fast_exp2(m[nt] - base);
             m[nt] = mn;
-            float sum = 0.f;
+            // probabilities times their values' sizes, brought to one size in turn
+            float sum = 0.f, most = 0.f;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int mt = 0; mt < MT; ++mt) {
+                const f32x4 sizes = *reinterpret_cast<const f32x4*>(&vscale[buf][16 * mt + 4 * g]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     s[mt][nt][i] = fast_exp2(s[mt][nt][i] - base);
                     sum += s[mt][nt][i];
+                    s[mt][nt][i] *= sizes[i];
+                    most = fmaxf(most, s[mt][nt][i]);
                 }
+            }
+            const int size = exponent_of(cross_row_max(most));
+            const float up = power_of_two(kHigh - size);
+            down[nt] = power_of_two(size - 2 * kHigh);
             l[nt] *= alpha[nt];
             rounded[nt] *= alpha[nt];
             add_to(l[nt], rounded[nt], sum);
 #pragma unroll
-            for (int h = 0; h < MT / 2; ++h) {
-                bf16x4 p[2][3];
-                split3(s[2 * h][nt], p[0][0], p[0][1], p[0][2]);
-                split3(s[2 * h + 1][nt], p[1][0], p[1][1], p[1][2]);
-#pragma unroll
-                for (int i = 0; i < 3; ++i) pp[nt][h][i] = both(p[0][i], p[1][i]);
-            }
+            for (int h = 0; h < MT / 2; ++h) p[nt][h] = split8(s[2 * h][nt] * up, s[2 * h + 1][nt] * up);
         }
         // lane (g, i): column 16dt + i of keys 4g .. 4g + 3 and 16 + 4g .. of each 32, as the
         // probabilities have them; a step's part from zero, then added to the rest
+        auto value_parts = [&](int o) __attribute__((always_inline)) {
+            const int at = (32 * (o % (MT / 2)) + 4 * g + (r16 >> 2)) * STR + 16 * (o / (MT / 2)) + 4 * (r16 & 3);
+            auto both = [&](int part) __attribute__((always_inline)) {
+                const f16x4 x = transposed_read(&vparts[buf][part][at]), y = transposed_read(&vparts[buf][part][at + 16 * STR]);
+                return __builtin_bit_cast(u32x4, f16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
+            };
+            return Parts{both(0), both(1)};
+        };
+        Parts v = value_parts(0);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             f32x4 part[NT];
@@ -665,59 +724,25 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
             for (int nt = 0; nt < NT; ++nt) part[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int h = 0; h < MT / 2; ++h) {
-                bf16x8 v[3];
+                const Parts now = v;
+                if (dt * (MT / 2) + h + 1 < DT * (MT / 2)) v = value_parts(dt * (MT / 2) + h + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < 3; ++i) {
-                    const __bf16* p = &vparts[buf][i][(32 * h + 4 * g + (r16 >> 2)) * STR + 16 * dt + 4 * (r16 & 3)];
-                    v[i] = both(transposed_read(p), transposed_read(p + 16 * STR));
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) part[nt] = six(v, pp[nt][h], part[nt]);
+                for (int nt = 0; nt < NT; ++nt) part[nt] = three(now, p[nt][h], part[nt]);
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[dt][nt][i] = fmaf(acc[dt][nt][i], alpha[nt], part[nt][i]);
-        }
-        if (__any(odds[buf][lane % kManyWaves] != 0)) {
-            // A row that sees such a value has a column that is not finite: their
-            // product as ones and zeros counts them.
-            bf16x8 on[NT][MT / 2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < 8 * (MT / 2); ++k) {
-                    const int key = key0 + 16 * (k / 4) + 4 * g + k % 4;
-                    on[nt][k / 8][k % 8] = static_cast<__bf16>(key >= range[nt].x && key < range[nt].y ? 1.f : 0.f);
-                }
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                f32x4 part[NT];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) part[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int h = 0; h < MT / 2; ++h) {
-                    bf16x8 v;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const int key = 32 * h + 16 * (k / 4) + 4 * g + k % 4;
-                        const bool marked = odds[buf][key * LPR / 64] && (which[buf][key][2 * dt + r16 / 8] >> (r16 % 8) & 1);
-                        v[k] = static_cast<__bf16>(marked ? 1.f : 0.f);
-                    }
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) part[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, on[nt][h], part[nt], 0, 0, 0);
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int o = 0; o < 4; ++o) acc[dt][nt][o] += part[nt][o] != 0.f ? NAN : 0.f;
-            }
+                for (int i = 0; i < 4; ++i) acc[dt][nt][i] = fmaf(acc[dt][nt][i], alpha[nt], part[nt][i] * down[nt]);
         }
     };
 
+    if (tid == 0) odd_values = 0;
     if (it.step < it.end) {
         load(it.step, lookup(it.step));
         int id = lookup(it.step + 1);
+        __syncthreads();
         stage(0);
         __syncthreads();
         int buf = 0;
@@ -727,6 +752,37 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
             compute(buf, step);
             stage(buf ^ 1);
             __syncthreads();
+        }
+    }
+    // Values that are not finite were zeros above.  A row that sees one has a column that is
+    // not finite: their product as ones and zeros counts them.
+    if (it.step < it.end && odd_values) {
+#pragma unroll 1
+        for (int key0 = max(KEYS * it.step, seen_lo / 32 * 32); key0 < min(KEYS * it.end, seen_hi); key0 += 32) {
+            f16x8 on[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int key = key0 + 16 * (k / 4) + 4 * g + k % 4;
+                    on[nt][k] = static_cast<_Float16>(key >= range[nt].x && key < range[nt].y ? 1.f : 0.f);
+                }
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                f16x8 v;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int key = min(key0 + 16 * (k / 4) + 4 * g + k % 4, tokens - 1);
+                    const float x = score_element(a, tab[key >> tsh], 1, key & (tpb - 1), kh * D + 16 * dt + r16);
+                    v[k] = static_cast<_Float16>(__builtin_isfinite(x) ? 0.f : 1.f);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const f32x4 part = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, on[nt], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                    for (int o = 0; o < 4; ++o) acc[dt][nt][o] += part[o] != 0.f ? NAN : 0.f;
+                }
+            }
         }
     }
     if (__any(nonfinite != 0.f) && lane == 0) *a.err = 1;

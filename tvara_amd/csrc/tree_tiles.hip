@@ -36,9 +36,7 @@
 namespace tvara_amd {
 namespace {
 
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kThreshold = 8.0f;
@@ -89,20 +87,6 @@ struct Spans {
 // flight, so that no wait for it is put there, which would wait for the loads
 // ahead too (they return in order).
 __device__ __forceinline__ void wait_for_loads() { __builtin_amdgcn_s_waitcnt(0); }
-
-// Two values as hi + lo in fp16, each rounded to nearest (22 bits; beyond fp16's
-// range one is infinite and the other its opposite).  `one` is 1, hidden from the
-// compiler, so that x - hi stays a mixed-precision fma: four instructions a pair
-// where converting hi back takes six.
-__device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned& lo) {
-    float one = 1.f;
-    asm("" : "+s"(one));
-    const f32x2 v = {x, y};
-    const f16x2 h = __builtin_convertvector(v, f16x2);
-    const f32x2 rest = {fmaf(-static_cast<float>(h[0]), one, x), fmaf(-static_cast<float>(h[1]), one, y)};
-    hi = __builtin_bit_cast(unsigned, h);
-    lo = __builtin_bit_cast(unsigned, __builtin_convertvector(rest, f16x2));
-}
 
 // Two elements of Q8_0 blocks as hi + lo in fp16: bytes i and j (4 to 7: of w1) of a
 // pair of words times the fp16 scales d.  A byte in the low end of 1024 is q + 1152
