@@ -457,63 +457,83 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
     __shared__ __attribute__((aligned(16))) _Float16 vparts[2][2][KEYS * STR];
     __shared__ __attribute__((aligned(16))) float kscale[2][KEYS];  // what a key's scores are multiplied by
     __shared__ __attribute__((aligned(16))) float vscale[2][KEYS];  // and its probability
-    __shared__ int odd_values;  // some value is not finite
+    // the queries' low parts, where registers do not hold them beside 128 columns of output
+    constexpr bool kFar = D == 128;
+    __shared__ u32x4 qlow[kFar ? kManyWaves : 1][kFar ? NT * KC : 1][64];
+    __shared__ int odd_values;   // some value is not finite
+    __shared__ int most_query;   // the exponent of the queries' largest element, scaled
+    __shared__ int large_keys;   // some key may take a score out of f32
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, r16 = lane & 15;
     const Item it = item_of(a, blockIdx.x);
     if (!it.rows) return;  // the list's padding
     const int kh = it.head / a.group, kvw = a.lay.kv_width, tokens = it.tokens;
 
-    int index[NT], head[NT], position[NT];
-    bool live[NT];
+    auto row_of = [&](int nt, int& head) {  // of the block's rows; behind them there are none
+        const int r = 32 * wave + 16 * nt + r16, row = r / it.heads;
+        head = it.head + r - row * it.heads;
+        return row;
+    };
+    int position[NT];
     int2 range[NT];
     float slope[NT];
-    int seen_lo = 0x7fffffff, seen_hi = 0, all_lo = 0, all_hi = 0x7fffffff;  // what some row of the wave sees, and all do
+    int all_lo = 0, all_hi = 0x7fffffff, from = 0x7fffffff;  // keys that all rows of the wave see; its first position
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int r = 32 * wave + 16 * nt + r16;
-        index[nt] = r / it.heads;
-        head[nt] = it.head + r - index[nt] * it.heads;
-        live[nt] = index[nt] < it.rows;
-        position[nt] = it.position + index[nt];
-        range[nt] = live[nt] ? a.ranges[static_cast<size_t>(it.row0) + index[nt]] : make_int2(0, 0);
-        slope[nt] = a.slopes && live[nt] ? a.slopes[head[nt]] : 0.f;
-        if (range[nt].x < range[nt].y) {
-            seen_lo = min(seen_lo, range[nt].x);
-            seen_hi = max(seen_hi, range[nt].y);
-        }
-        if (live[nt]) {
+        int head;
+        const int row = row_of(nt, head);
+        const bool live = row < it.rows;
+        position[nt] = it.position + row;
+        range[nt] = live ? a.ranges[static_cast<size_t>(it.row0) + row] : make_int2(0, 0);
+        slope[nt] = a.slopes && live ? a.slopes[head] : 0.f;
+        if (live) {
             all_lo = max(all_lo, range[nt].x);
             all_hi = min(all_hi, range[nt].y);
+            from = min(from, position[nt]);
         }
     }
-    seen_lo = -uniform_max(-seen_lo);
-    seen_hi = uniform_max(seen_hi);
     all_lo = uniform_max(all_lo);
     all_hi = -uniform_max(-all_hi);
+    from = -uniform_max(-from);
+    if (tid == 0) {
+        odd_values = 0;
+        large_keys = 0;
+        most_query = -1000;
+    }
+    __syncthreads();
 
-    Parts q[NT][KC];
+    u32x4 qh[NT][KC], ql[kFar ? 1 : NT][kFar ? 1 : KC];
     float qsize[NT];  // what a row's scores are multiplied by
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         f32x4 x[KC][2];
         float most = 0.f;
+        int head;
+        const int row = row_of(nt, head);
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 x[kc][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (live[nt])
-                    x[kc][i] = *reinterpret_cast<const f32x4*>(
-                        a.q + ((static_cast<size_t>(it.row0) + index[nt]) * a.heads + head[nt]) * D + 32 * kc + 8 * g + 4 * i);
+                if (row < it.rows)
+                    x[kc][i] = *reinterpret_cast<const f32x4*>(a.q + ((static_cast<size_t>(it.row0) + row) * a.heads + head) * D +
+                                                               32 * kc + 8 * g + 4 * i);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) most = fmaxf(most, __builtin_fabsf(x[kc][i][e]));
             }
         const int size = exponent_of(cross_row_max(most));
         const float up = power_of_two(kHigh - size);
-        qsize[nt] = power_of_two(size - kHigh) * a.qscale;
+        qsize[nt] = fmaxf(power_of_two(size - kHigh) * a.qscale, 1.17549435e-38f);
+        atomicMax(&most_query, size + exponent_of(a.qscale) + 1);
 #pragma unroll
-        for (int kc = 0; kc < KC; ++kc) q[nt][kc] = split8(x[kc][0] * up, x[kc][1] * up);
+        for (int kc = 0; kc < KC; ++kc) {
+            const Parts p = split8(x[kc][0] * up, x[kc][1] * up);
+            qh[nt][kc] = p.hi;
+            if constexpr (kFar)
+                qlow[wave][nt * KC + kc][lane] = p.lo;
+            else
+                ql[nt][kc] = p.lo;
+        }
     }
 
     // staging: eight columns of a key; a wave's keys lie in one block
@@ -524,26 +544,28 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
                               : (static_cast<size_t>(a.layer) * 2 * tpb * kvw + static_cast<size_t>(kh) * D) * sizeof(float);
     const size_t vsec = kQ8 ? a.lay.section : static_cast<size_t>(tpb) * kvw * sizeof(float);
     // (past the last key: its block again, whose slots are there whatever they hold)
-    auto lookup = [&](int stp) { return tab[min(KEYS * stp + skey, tokens - 1) >> tsh]; };
+    const int wkey = __builtin_amdgcn_readfirstlane(skey);  // the wave's first
+    auto lookup = [&](int stp) { return tab[min(KEYS * stp + wkey, tokens - 1) >> tsh]; };
+    const unsigned in_row = kQ8 ? (skey - wkey) * D + col : ((skey - wkey) * kvw + col) * static_cast<unsigned>(sizeof(float));
+    const unsigned in_scales = ((skey - wkey) * (D / 32) + col / 32) * 2;
     f32x4 kreg[2], vreg[2];
     u32x2 kraw, vraw;
     unsigned kdraw, vdraw;
     auto load = [&](int stp, int id) __attribute__((always_inline)) {
-        const int slot = (KEYS * stp + skey) & (tpb - 1);
-        const char* b = a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes;
+        const int slot = (KEYS * stp + wkey) & (tpb - 1);
+        const char* block = a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes;
         if constexpr (kQ8) {
-            const char* sc = b + static_cast<size_t>(tpb) * D + static_cast<size_t>(slot * (D / 32) + col / 32) * 2;
-            b += static_cast<size_t>(slot) * D + col;
-            kraw = *reinterpret_cast<const u32x2*>(b);
-            kdraw = *reinterpret_cast<const uint16_t*>(sc);
-            vraw = *reinterpret_cast<const u32x2*>(b + vsec);
-            vdraw = *reinterpret_cast<const uint16_t*>(sc + vsec);
+            const char *k = block + static_cast<size_t>(slot) * D, *sc = block + static_cast<size_t>(tpb) * D + static_cast<size_t>(slot * (D / 32)) * 2;
+            kraw = *reinterpret_cast<const u32x2*>(k + in_row);
+            kdraw = *reinterpret_cast<const uint16_t*>(sc + in_scales);
+            vraw = *reinterpret_cast<const u32x2*>(k + vsec + in_row);
+            vdraw = *reinterpret_cast<const uint16_t*>(sc + vsec + in_scales);
         } else {
-            b += (static_cast<size_t>(slot) * kvw + col) * sizeof(float);
+            const char *k = block + static_cast<size_t>(slot) * kvw * sizeof(float), *v = k + vsec;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                kreg[i] = *reinterpret_cast<const f32x4*>(b + 16 * i);
-                vreg[i] = *reinterpret_cast<const f32x4*>(b + vsec + 16 * i);
+                kreg[i] = *reinterpret_cast<const f32x4*>(k + in_row + 16 * i);
+                vreg[i] = *reinterpret_cast<const f32x4*>(v + in_row + 16 * i);
             }
         }
     };
@@ -574,6 +596,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
         kmost = row_max<LPR>(kmost);
         vmost = row_max<LPR>(vmost);
         const int ksize = exponent_of(kmost), size = exponent_of(vmost);
+        if (ksize + most_query >= 110) large_keys = 1;
         if (tid % LPR == 0) {
             kscale[buf][skey] = power_of_two(ksize - kHigh);
             vscale[buf][skey] = power_of_two(size);
@@ -589,10 +612,12 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
 
     f32x4 acc[DT][NT];
     float m[NT], l[NT], rounded[NT], nonfinite = 0.f;
+    int asize[NT];  // acc is in units of 2^(asize - 2 kHigh)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         m[nt] = -INFINITY;
         l[nt] = rounded[nt] = 0.f;
+        asize[nt] = -97;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[dt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -602,11 +627,8 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
         c = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.high(), y.low(), c, 0, 0, 0);
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(x.high(), y.high(), c, 0, 0, 0);
     };
-    auto compute = [&](int buf, int stp) __attribute__((always_inline)) {
-        const int key0 = KEYS * stp;
-        if (key0 >= seen_hi || key0 + KEYS <= seen_lo) return;
-        const bool whole = key0 >= all_lo && key0 + KEYS <= all_hi;
-        f32x4 s[MT][NT];
+    f32x4 s[MT][NT];  // scores, then probabilities, of keys 16mt + 4g + i
+    auto scores = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -616,58 +638,86 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
             const int at = (16 * (o % MT) + r16) * STR + 32 * (o / MT) + 8 * g;
             return Parts{*reinterpret_cast<const u32x4*>(&kparts[buf][0][at]), *reinterpret_cast<const u32x4*>(&kparts[buf][1][at])};
         };
+        u32x4 low[NT];
+        auto query_parts = [&](int kc) __attribute__((always_inline)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                if constexpr (kFar)
+                    low[nt] = qlow[wave][nt * KC + kc][lane];
+                else
+                    low[nt] = ql[nt][kc];
+            }
+        };
         Parts k = key_parts(0);
+        query_parts(0);
 #pragma unroll
         for (int o = 0; o < KC * MT; ++o) {
             const Parts now = k;
             if (o + 1 < KC * MT) k = key_parts(o + 1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[o % MT][nt] = three(now, q[nt][o / MT], s[o % MT][nt]);
+            for (int nt = 0; nt < NT; ++nt) s[o % MT][nt] = three(now, Parts{qh[nt][o / MT], low[nt]}, s[o % MT][nt]);
+            if (o % MT == MT - 1 && o + 1 < KC * MT) query_parts(o / MT + 1);
             __builtin_amdgcn_sched_barrier(0);
         }
-        float alpha[NT], down[NT];
+    };
+    auto output = [&](int buf, int stp) __attribute__((always_inline)) {
+        const int key0 = KEYS * stp;
+        const bool whole = key0 >= all_lo && key0 + KEYS <= all_hi;
+        float alpha[NT];
         Parts p[NT][MT / 2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int first = range[nt].x - key0 - 4 * g, end = range[nt].y - key0 - 4 * g;
+            // scores are s * by
+            float by = qsize[nt];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) s[mt][nt] *= *reinterpret_cast<const f32x4*>(&kscale[buf][16 * mt + 4 * g]) * qsize[nt];
-            if (!whole) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[mt][nt][i] = 16 * mt + i >= first && 16 * mt + i < end ? s[mt][nt][i] : 0.f;
-            }
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) nonfinite = fmaf(s[mt][nt][i], 0.f, nonfinite);
-            if (a.cap != 0.f) {
-                float top = 0.f;
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, __builtin_fabsf(s[mt][nt][i]));
-                if (!__any(top > kSmallTanh)) {
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[mt][nt][i] = a.cap * small_tanh(s[mt][nt][i]);
-                } else {
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[mt][nt][i] = a.cap * any_tanh(s[mt][nt][i]);
-                }
-            }
-            if (a.slopes) {
-                const int away = position[nt] - key0 - 4 * g;
+            for (int mt = 0; mt < MT; ++mt) s[mt][nt] *= *reinterpret_cast<const f32x4*>(&kscale[buf][16 * mt + 4 * g]);
+            if (large_keys) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        s[mt][nt][i] = fmaf(-slope[nt], static_cast<float>(abs(away - 16 * mt - i)), s[mt][nt][i]);
+                        nonfinite = fmaf(16 * mt + i >= first && 16 * mt + i < end ? s[mt][nt][i] * by : 0.f, 0.f, nonfinite);
+            }
+            if (a.cap != 0.f) {
+                float top = 0.f;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    s[mt][nt] *= by;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, __builtin_fabsf(s[mt][nt][i]));
+                }
+                by = a.cap;
+                if (!__any(top > kSmallTanh)) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[mt][nt][i] = small_tanh(s[mt][nt][i]);
+                } else {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[mt][nt][i] = any_tanh(s[mt][nt][i]);
+                }
+            }
+            if (a.slopes) {
+                const int away = position[nt] - key0 - 4 * g;
+                if (key0 + KEYS <= from) {  // every key lies before every row
+                    const float far = -slope[nt] * static_cast<float>(away);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[mt][nt][i] = fmaf(s[mt][nt][i], by, fmaf(slope[nt], static_cast<float>(16 * mt + i), far));
+                } else {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[mt][nt][i] = fmaf(s[mt][nt][i], by, -slope[nt] * static_cast<float>(abs(away - 16 * mt - i)));
+                }
+                by = 1.f;
             }
             if (!whole) {
 #pragma unroll
@@ -681,28 +731,30 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[mt][nt][i]);
-            const float mn = fmaxf(m[nt], cross_row_max(mx)), base = mn == -INFINITY ? 0.f : mn;
+            const float mn = fmaxf(m[nt], cross_row_max(mx) * by), base = mn == -INFINITY ? 0.f : mn;
             alpha[nt] = fast_exp2(m[nt] - base);
             m[nt] = mn;
-            // probabilities times their values' sizes, brought to one size in turn
+            // probabilities times their values' sizes, brought to one size in turn: the
+            // largest one's, or that of what was added before
             float sum = 0.f, most = 0.f;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 const f32x4 sizes = *reinterpret_cast<const f32x4*>(&vscale[buf][16 * mt + 4 * g]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    s[mt][nt][i] = fast_exp2(s[mt][nt][i] - base);
+                    s[mt][nt][i] = fast_exp2(fmaf(s[mt][nt][i], by, -base));
                     sum += s[mt][nt][i];
                     s[mt][nt][i] *= sizes[i];
                     most = fmaxf(most, s[mt][nt][i]);
                 }
             }
-            const int size = exponent_of(cross_row_max(most));
-            const float up = power_of_two(kHigh - size);
-            down[nt] = power_of_two(size - 2 * kHigh);
             l[nt] *= alpha[nt];
             rounded[nt] *= alpha[nt];
             add_to(l[nt], rounded[nt], sum);
+            const int size = max(exponent_of(cross_row_max(most)), max(asize[nt] + exponent_of(alpha[nt]), -97));
+            alpha[nt] *= power_of_two(max(asize[nt] - size, -126));
+            asize[nt] = size;
+            const float up = power_of_two(kHigh - size);
 #pragma unroll
             for (int h = 0; h < MT / 2; ++h) p[nt][h] = split8(s[2 * h][nt] * up, s[2 * h + 1][nt] * up);
         }
@@ -734,11 +786,10 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[dt][nt][i] = fmaf(acc[dt][nt][i], alpha[nt], part[nt][i] * down[nt]);
+                for (int i = 0; i < 4; ++i) acc[dt][nt][i] = fmaf(acc[dt][nt][i], alpha[nt], part[nt][i]);
         }
     };
 
-    if (tid == 0) odd_values = 0;
     if (it.step < it.end) {
         load(it.step, lookup(it.step));
         int id = lookup(it.step + 1);
@@ -747,57 +798,49 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
         __syncthreads();
         int buf = 0;
         for (int step = it.step; step < it.end; ++step, buf ^= 1) {
+            scores(buf);
             load(step + 1, id);
             id = lookup(step + 2);
-            compute(buf, step);
+            output(buf, step);
             stage(buf ^ 1);
             __syncthreads();
         }
     }
-    // Values that are not finite were zeros above.  A row that sees one has a column that is
-    // not finite: their product as ones and zeros counts them.
-    if (it.step < it.end && odd_values) {
-#pragma unroll 1
-        for (int key0 = max(KEYS * it.step, seen_lo / 32 * 32); key0 < min(KEYS * it.end, seen_hi); key0 += 32) {
-            f16x8 on[NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int key = key0 + 16 * (k / 4) + 4 * g + k % 4;
-                    on[nt][k] = static_cast<_Float16>(key >= range[nt].x && key < range[nt].y ? 1.f : 0.f);
-                }
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                f16x8 v;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int key = min(key0 + 16 * (k / 4) + 4 * g + k % 4, tokens - 1);
-                    const float x = score_element(a, tab[key >> tsh], 1, key & (tpb - 1), kh * D + 16 * dt + r16);
-                    v[k] = static_cast<_Float16>(__builtin_isfinite(x) ? 0.f : 1.f);
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const f32x4 part = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, on[nt], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-                    for (int o = 0; o < 4; ++o) acc[dt][nt][o] += part[o] != 0.f ? NAN : 0.f;
-                }
-            }
-        }
-    }
-    if (__any(nonfinite != 0.f) && lane == 0) *a.err = 1;
+    // (a score that is NaN is in its row's sum)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const float total = cross_row_sum(l[nt]);
-        if (!live[nt]) continue;
+        int head;
+        const int row = row_of(nt, head);
+        if (row >= it.rows) continue;
+        nonfinite = fmaf(total, 0.f, nonfinite);
         const bool whole = it.runs == 1;
-        const size_t at = (whole ? static_cast<size_t>(it.row0) + index[nt]
-                                 : static_cast<size_t>(it.slot) + static_cast<size_t>(index[nt]) * it.runs + it.run) * a.heads + head[nt];
+        const size_t at = (whole ? static_cast<size_t>(it.row0) + row
+                                 : static_cast<size_t>(it.slot) + static_cast<size_t>(row) * it.runs + it.run) * a.heads + head;
         float* o = (whole ? a.out : a.part_acc) + at * D + 4 * g;
-        const float div = whole && total != 0.f ? total : 1.f;
+        const float unit = power_of_two(asize[nt] - 2 * kHigh), div = whole && total != 0.f ? total : 1.f;
         if (!whole && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(m[nt], total);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(o + 16 * dt) = acc[dt][nt] / div;
+        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(o + 16 * dt) = acc[dt][nt] * unit / div;
+    }
+    if (nonfinite != 0.f) *a.err = 1;
+    if (it.step >= it.end || !odd_values) return;
+    // Values that are not finite were zeros above: a row that sees one is given a column that
+    // is not finite, over what was written.
+    __threadfence_block();
+    __syncthreads();
+    const int keys = min(KEYS * it.end, tokens) - KEYS * it.step;
+    for (int i = tid; i < keys * D; i += 64 * kManyWaves) {
+        const int key = KEYS * it.step + i / D, c = i % D;
+        if (__builtin_isfinite(score_element(a, tab[key >> tsh], 1, key & (tpb - 1), kh * D + c))) continue;
+        for (int row = 0; row < it.rows; ++row) {
+            const int2 seen = a.ranges[static_cast<size_t>(it.row0) + row];
+            if (key < seen.x || key >= seen.y) continue;
+            const size_t at = it.runs == 1 ? static_cast<size_t>(it.row0) + row
+                                           : static_cast<size_t>(it.slot) + static_cast<size_t>(row) * it.runs + it.run;
+            for (int head = it.head; head < it.head + it.heads; ++head)
+                (it.runs == 1 ? a.out : a.part_acc)[(at * a.heads + head) * D + c] = NAN;
+        }
     }
 }
 
