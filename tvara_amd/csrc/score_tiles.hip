@@ -15,6 +15,8 @@
 namespace tvara_amd {
 namespace {
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
@@ -31,6 +33,26 @@ struct Item {
 __device__ __forceinline__ Item item_of(const ScoreArgs& a, unsigned i) {
     const int4 x = a.work[3 * static_cast<size_t>(i)], y = a.work[3 * static_cast<size_t>(i) + 1], z = a.work[3 * static_cast<size_t>(i) + 2];
     return {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+}
+
+__device__ __forceinline__ bf16x8 both(bf16x4 x, bf16x4 y) { return bf16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}; }
+__device__ __forceinline__ bf16x8 eight(f32x4 x, f32x4 y) {
+    return both(__builtin_convertvector(x, bf16x4), __builtin_convertvector(y, bf16x4));
+}
+// Eight values as three parts in bf16, each the rest's nearest.
+__device__ __forceinline__ void split3(f32x4 x, f32x4 y, bf16x8 (&p)[3]) {
+    bf16x4 part[2][3];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        f32x4 rest = half ? y : x;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            part[half][i] = __builtin_convertvector(rest, bf16x4);
+            rest -= __builtin_convertvector(part[half][i], f32x4);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) p[i] = both(part[0][i], part[1][i]);
 }
 
 // max / min over the 16 lanes of a row of a wave, to a scalar
@@ -63,11 +85,11 @@ constexpr int kFewStep = 32, kFewWaves = 4;
 // Bound: HBM; keys of f32 blocks come as whole rows into the wave's own part of LDS
 // without passing registers (as operands they take four times as long through the CU's
 // cache), values straight into registers as the product has them.
-template <int D, bool kQ8>
+template <int D>
 __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_kernel(const ScoreArgs a) {
     constexpr int WK = kFewWaves, C = D / 16, H = D / 64;
     constexpr int W = D / 4;  // 16-byte parts of a row
-    __shared__ f32x4 staged[WK][kQ8 ? 4 * 64 : kFewStep * W];
+    __shared__ f32x4 staged[WK][kFewStep * W];
     auto result = [&](int w, int i) -> f32x4& { return staged[w][i * 64 + static_cast<int>(threadIdx.x & 63)]; };
     __shared__ float2 stats[WK][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -87,17 +109,16 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_kernel(const Sco
 
     // column of element 0 of a lane's c-th four of a key, and of the h-th four of
     // a value (r: the loading lane's r16, or an output row of the tiles)
-    auto kcol = [&](int c) { return kQ8 ? 64 * (c / 4) + 16 * g + 4 * (c % 4) : 16 * c + 4 * g; };
-    auto vcol = [](int h, int r) { return kQ8 ? (D / 16) * r + 4 * h : 64 * h + 4 * r; };
+    auto kcol = [&](int c) { return 16 * c + 4 * g; };
+    auto vcol = [](int h, int r) { return 64 * h + 4 * r; };
 
     const int tpb = a.lay.tpb, tsh = __builtin_ctz(static_cast<unsigned>(tpb));
     const int32_t* tab = a.tables + it.table;
-    const size_t kbytes = kQ8 ? static_cast<size_t>(a.layer) * 2 * a.lay.section + static_cast<size_t>(kh) * a.lay.head_bytes
-                              : (static_cast<size_t>(a.layer) * 2 * tpb * kvw + static_cast<size_t>(kh) * D) * sizeof(float);
-    const size_t vsec = kQ8 ? a.lay.section : static_cast<size_t>(tpb) * kvw * sizeof(float);
-    const int rowb = kQ8 ? D : kvw * static_cast<int>(sizeof(float));  // from one slot to the next
-    const unsigned koff = static_cast<unsigned>(!kQ8 ? lane / W * rowb + (lane % W ^ lane / W) * 16 : r16 * rowb + kcol(0));
-    const unsigned voff = static_cast<unsigned>(4 * g * rowb + vcol(0, r16) * (kQ8 ? 1 : 4));
+    const size_t kbytes = (static_cast<size_t>(a.layer) * 2 * tpb * kvw + static_cast<size_t>(kh) * D) * sizeof(float);
+    const size_t vsec = static_cast<size_t>(tpb) * kvw * sizeof(float);
+    const int rowb = kvw * static_cast<int>(sizeof(float));  // from one slot to the next
+    const unsigned koff = static_cast<unsigned>(lane / W * rowb + (lane % W ^ lane / W) * 16);
+    const unsigned voff = static_cast<unsigned>(4 * g * rowb + vcol(0, r16) * 4);
     int step = it.step + wave;
     const int last = max(tokens - 1, 0) >> 4;  // 16 keys a table lookup; past the end the last again
     // lane 2i + mt: the block of the wave's i-th step from here
@@ -109,56 +130,30 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_kernel(const Sco
         return a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes + static_cast<size_t>(slot) * rowb;
     };
     f32x4 qf[C];
-    // f32 rows, or Q8_0 bytes and scales, which become values where they are used
-    f32x4 v[kQ8 ? 1 : 2][4][H];
-    u32x4 kw[kQ8 ? 2 : 1][H];
-    unsigned kd[kQ8 ? 2 : 1][H], vw[kQ8 ? 2 : 1][4][H], vd[kQ8 ? 2 : 1][4];
-    auto scales = [&](const char* b, int mt, int stp) {  // of the block's rows from the tile's first on
-        const int slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
-        return b + static_cast<size_t>(tpb - slot) * D + static_cast<size_t>(slot) * (D / 32) * 2;
-    };
+    f32x4 v[2][4][H];
     auto load_k = [&](int stp) __attribute__((always_inline)) {
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
             const char* b = block(mt, stp);
-            if constexpr (kQ8) {
-                const char* sc = scales(b, mt, stp);
+            // straight into LDS, lane after lane; what a lane loads is permuted by its
+            // row, so that the operands' reads meet no bank twice
+            const __amdgpu_buffer_rsrc_t rows =
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(b), 0, 15 * rowb + 4 * D, kBufferWord3);
 #pragma unroll
-                for (int u = 0; u < H; ++u) {
-                    kw[mt][u] = *reinterpret_cast<const u32x4*>(b + koff + 64 * u);
-                    kd[mt][u] = *reinterpret_cast<const uint16_t*>(sc + (r16 * (D / 32) + 2 * u + (g >> 1)) * 2);
-                }
-            } else {
-                // straight into LDS, lane after lane; what a lane loads is permuted by its
-                // row, so that the operands' reads meet no bank twice
-                const __amdgpu_buffer_rsrc_t rows =
-                    __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(b), 0, 15 * rowb + 4 * D, kBufferWord3);
-#pragma unroll
-                for (int c = 0; c < C; ++c)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (__attribute__((address_space(3))) void*)&staged[wave][(mt * C + c) * 64],
-                                                             16, koff ^ 1024 / W * c, 64 / W * c * rowb, 0, 0);
-            }
+            for (int c = 0; c < C; ++c)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (__attribute__((address_space(3))) void*)&staged[wave][(mt * C + c) * 64],
+                                                         16, koff ^ 1024 / W * c, 64 / W * c * rowb, 0, 0);
         }
     };
     auto load_v = [&](int stp) __attribute__((always_inline)) {
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
             const char* b = block(mt, stp) + vsec;
-            if constexpr (kQ8) {
-                const char* sc = scales(b, mt, stp);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    vd[mt][i] = *reinterpret_cast<const uint16_t*>(sc + ((4 * g + i) * (D / 32) + (D / 16) * r16 / 32) * 2);
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int h = 0; h < H; ++h) vw[mt][i][h] = *reinterpret_cast<const unsigned*>(b + voff + i * D + 4 * h);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int h = 0; h < H; ++h)
-                        v[mt][i][h] = *reinterpret_cast<const f32x4*>(b + static_cast<size_t>(i) * rowb + voff + 256 * h);
-            }
+                for (int h = 0; h < H; ++h)
+                    v[mt][i][h] = *reinterpret_cast<const f32x4*>(b + static_cast<size_t>(i) * rowb + voff + 256 * h);
         }
     };
     {
@@ -171,7 +166,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_kernel(const Sco
     }
     if (step < it.end) {
         load_k(step);
-        if constexpr (!kQ8) asm volatile("" ::: "memory");
+        asm volatile("" ::: "memory");
         load_v(step);
     }
 #pragma unroll
@@ -182,21 +177,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_kernel(const Sco
 #pragma unroll
     for (int dt = 0; dt < 4 * H; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     f32x4 s[2];  // scores, then probabilities, of keys 16mt + 4g + i
-    auto key_part = [&](int mt, int c) __attribute__((always_inline)) {
-        if constexpr (kQ8) {
-            const float d = half_bits_to_float(static_cast<uint16_t>(kd[mt][c / 4]));
-            const unsigned w = kw[mt][c / 4][c % 4];
-            return f32x4{sbyte_to_float<0>(w) * d, sbyte_to_float<1>(w) * d, sbyte_to_float<2>(w) * d, sbyte_to_float<3>(w) * d};
-        } else {
-            return staged[wave][(16 * mt + r16) * W + ((4 * c + g) ^ r16)];
-        }
-    };
-    auto value = [&](int mt, int i, int h, auto j) __attribute__((always_inline)) {
-        if constexpr (kQ8)
-            return sbyte_to_float<j.value>(vw[mt][i][h]) * half_bits_to_float(static_cast<uint16_t>(vd[mt][i]));
-        else
-            return v[mt][i][h][j.value];
-    };
+    auto key_part = [&](int mt, int c) __attribute__((always_inline)) { return staged[wave][(16 * mt + r16) * W + ((4 * c + g) ^ r16)]; };
+    auto value = [&](int mt, int i, int h, auto j) __attribute__((always_inline)) { return v[mt][i][h][j.value]; };
     auto every_tile = [&](auto&& f) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < H; ++h) {
@@ -208,33 +190,25 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_kernel(const Sco
     };
     // the lane's columns of key 16mt + 4g + i
     auto finite_value = [&](int mt, int i) __attribute__((always_inline)) {
-        if constexpr (kQ8) {
-            return __builtin_isfinite(half_bits_to_float(static_cast<uint16_t>(vd[mt][i])));
-        } else {
-            bool fine = true;
+        bool fine = true;
 #pragma unroll
-            for (int h = 0; h < H; ++h) fine &= all_finite(v[mt][i][h]);
-            return fine;
-        }
+        for (int h = 0; h < H; ++h) fine &= all_finite(v[mt][i][h]);
+        return fine;
     };
     auto drop_odd = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if constexpr (kQ8) {
-                    if (!finite_value(mt, i)) vd[mt][i] = 0;
-                } else {
 #pragma unroll
-                    for (int h = 0; h < H; ++h)
+                for (int h = 0; h < H; ++h)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) v[mt][i][h][j] = __builtin_isfinite(v[mt][i][h][j]) ? v[mt][i][h][j] : 0.f;
-                }
+                    for (int j = 0; j < 4; ++j) v[mt][i][h][j] = __builtin_isfinite(v[mt][i][h][j]) ? v[mt][i][h][j] : 0.f;
             }
     };
     for (; step < it.end; step += WK) {
         const int next = step + WK, key0 = kFewStep * step;
-        if constexpr (!kQ8) wait_until_left<8 * H>();  // the values'
+        wait_until_left<8 * H>();  // the values'
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
             s[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -245,7 +219,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_kernel(const Sco
                 for (int i = 0; i < 4; ++i) s[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i], qf[c][i], s[mt], 0, 0, 0);
             }
         }
-        if constexpr (!kQ8) wait_for_lds();
+        wait_for_lds();
         // the loads of the next step go out as soon as there is room (past the end the
         // last step's again: its blocks are there)
         if (++at == 32) {
@@ -254,7 +228,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_kernel(const Sco
             more = lookup(next + 32 * WK);
         }
         load_k(next);
-        if constexpr (!kQ8) asm volatile("" ::: "memory");
+        asm volatile("" ::: "memory");
         const bool whole = key0 >= lo && key0 + kFewStep <= hi;  // every row sees every key
         const int first = range.x - key0 - 4 * g, end = range.y - key0 - 4 * g;  // of the lane's keys 16mt + i
         if (whole) {
@@ -357,7 +331,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_kernel(const Sco
         every_tile(tile);
         load_v(next);
     }
-    if constexpr (!kQ8) wait_until_left<0>();  // (LDS is used again)
+    wait_until_left<0>();  // (LDS is used again)
     if (__any(nonfinite != 0.f) && lane == 0) *a.err = 1;
 
     // ---- the waves that shared these rows' keys, together
@@ -393,6 +367,254 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_kernel(const Sco
         } else {
             const size_t p = (static_cast<size_t>(it.slot) + static_cast<size_t>(index) * it.runs + it.run) * a.heads + head;
             *reinterpret_cast<f32x4*>(a.part_acc + p * D + vcol(h, 4 * g + wave)) = x;
+            if (h == 0 && wave == 0 && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m, total);
+        }
+    }
+}
+
+// The same over Q8_0 blocks, whose bytes are operands as they are: 16x16x32 products of
+// bf16, which holds a byte exactly, with queries and probabilities in three bf16 parts
+// (24 bits, f32's range).  A product over 32 columns is one group's: scores are multiplied
+// by the group's scale behind it, probabilities before, one column group after the other.
+// Bound: HBM (in f32 products it is the matrix pipe: eight contexts of 16,000 to 32,768
+// tokens, 32 heads on 8 of 128: 224 us, and TIME so).
+template <int D>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_q8_kernel(const ScoreArgs a) {
+    constexpr int WK = kFewWaves, KC = D / 32, H = D / 64;
+    __shared__ f32x4 staged[WK][4 * 64];
+    auto result = [&](int w, int i) -> f32x4& { return staged[w][i * 64 + static_cast<int>(threadIdx.x & 63)]; };
+    __shared__ float2 stats[WK][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, r16 = lane & 15;
+    const Item it = item_of(a, blockIdx.x);
+    if (!it.rows) return;  // the list's padding
+    const int kh = it.head / a.group, tokens = it.tokens;
+
+    // this lane's row
+    const int index = r16 / it.heads, head = it.head + r16 - index * it.heads;
+    const bool live = index < it.rows;
+    const int position = it.position + index;
+    const size_t row = static_cast<size_t>(it.row0) + index;
+    const int2 range = live ? a.ranges[row] : make_int2(0, 0);
+    const float slope = a.slopes && live ? a.slopes[head] : 0.f;
+    const int lo = uniform_max(range.x), hi = -uniform_max(live ? -range.y : -0x7fffffff);  // keys that all rows see: [lo, hi)
+
+    const int tpb = a.lay.tpb, tsh = __builtin_ctz(static_cast<unsigned>(tpb));
+    const int32_t* tab = a.tables + it.table;
+    const size_t kbytes = static_cast<size_t>(a.layer) * 2 * a.lay.section + static_cast<size_t>(kh) * a.lay.head_bytes, vsec = a.lay.section;
+    int step = it.step + wave;
+    const int last = max(tokens - 1, 0) >> 4;  // 16 keys a table lookup; past the end the last again
+    // lane 2i + mt: the block of the wave's i-th step from here
+    auto lookup = [&](int from) { return tokens ? tab[min(2 * (from + (lane >> 1) * WK) + (lane & 1), last) << 4 >> tsh] : 0; };
+    int ids = lookup(step), more = lookup(step + 32 * WK), at = 0;
+    // bytes of key r16 (lane group g: 8 of each 32), of column pairs 2 r16 of keys 4g + i,
+    // and the scales of those keys
+    u32x2 kw[2][KC];
+    unsigned vw[2][4][KC];
+    struct alignas(8) Scales {
+        _Float16 d[4][KC];
+    } kd[2], vd[2];
+    auto block = [&](int mt, int stp, const char*& scales) __attribute__((always_inline)) {
+        const int id = __builtin_amdgcn_readlane(ids, 2 * at + mt), slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
+        const char* b = a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes;
+        scales = b + static_cast<size_t>(tpb) * D + static_cast<size_t>(slot) * KC * 2;
+        return b + static_cast<size_t>(slot) * D;
+    };
+    auto load_k = [&](int stp) __attribute__((always_inline)) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+            const char *sc, *b = block(mt, stp, sc);
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) kw[mt][kc] = *reinterpret_cast<const u32x2*>(b + r16 * D + 32 * kc + 8 * g);
+            kd[mt] = *reinterpret_cast<const Scales*>(sc + 4 * g * KC * 2);
+        }
+    };
+    auto load_v = [&](int stp) __attribute__((always_inline)) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+            const char *sc, *b = block(mt, stp, sc);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int kc = 0; kc < KC; ++kc)
+                    vw[mt][i][kc] = *reinterpret_cast<const uint16_t*>(b + vsec + (4 * g + i) * D + 32 * kc + 2 * r16);
+            vd[mt] = *reinterpret_cast<const Scales*>(sc + vsec + 4 * g * KC * 2);
+        }
+    };
+    bf16x8 q[KC][3];
+    {
+        const float* qp = a.q + (row * a.heads + head) * D + 8 * g;
+        f32x4 x[KC][2];
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                x[kc][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (live) x[kc][i] = *reinterpret_cast<const f32x4*>(qp + 32 * kc + 4 * i);
+            }
+        if (step < it.end) {
+            load_k(step);
+            load_v(step);
+        }
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) split3(x[kc][0] * a.qscale, x[kc][1] * a.qscale, q[kc]);
+    }
+    f32x4 acc[2 * KC];  // columns 32 kc + 2 m + e at 2 kc + e, m being the tile's row
+    float m = -INFINITY, l = 0.f, rounded = 0.f, nonfinite = 0.f;  // nonfinite: NaN once a score is not finite
+#pragma unroll
+    for (int dt = 0; dt < 2 * KC; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (; step < it.end; step += WK) {
+        const int next = step + WK, key0 = kFewStep * step;
+        f32x4 s[2];  // scores, then probabilities, of keys 16mt + 4g + i
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+            s[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) {
+                const unsigned w0 = kw[mt][kc][0], w1 = kw[mt][kc][1];
+                const bf16x8 k = eight(f32x4{sbyte_to_float<0>(w0), sbyte_to_float<1>(w0), sbyte_to_float<2>(w0), sbyte_to_float<3>(w0)},
+                                       f32x4{sbyte_to_float<0>(w1), sbyte_to_float<1>(w1), sbyte_to_float<2>(w1), sbyte_to_float<3>(w1)});
+                f32x4 part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[kc][2], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[kc][1], part, 0, 0, 0);
+                part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[kc][0], part, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[mt][i] = fmaf(part[i], static_cast<float>(kd[mt].d[i][kc]), s[mt][i]);
+            }
+        }
+        if (++at == 32) {
+            at = 0;
+            ids = more;
+            more = lookup(next + 32 * WK);
+        }
+        load_k(next);
+        const bool whole = key0 >= lo && key0 + kFewStep <= hi;  // every row sees every key
+        const int first = range.x - key0 - 4 * g, end = range.y - key0 - 4 * g;  // of the lane's keys 16mt + i
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (!whole) s[mt][i] = 16 * mt + i >= first && 16 * mt + i < end ? s[mt][i] : 0.f;
+                nonfinite = fmaf(s[mt][i], 0.f, nonfinite);
+            }
+        if (a.cap != 0.f) {
+            float most = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most = fmaxf(most, __builtin_fabsf(s[mt][i]));
+            const bool small = !__any(most > kSmallTanh);
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[mt][i] = a.cap * (small ? small_tanh(s[mt][i]) : any_tanh(s[mt][i]));
+        }
+        if (a.slopes) {
+            const int away = position - key0 - 4 * g;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[mt][i] = fmaf(-slope, static_cast<float>(abs(away - 16 * mt - i)), s[mt][i]);
+        }
+        if (!whole) {
+            // (a scale that is not finite does not reach the rows that do not see it)
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (16 * mt + i < first || 16 * mt + i >= end) {
+                        s[mt][i] = -INFINITY;
+#pragma unroll
+                        for (int kc = 0; kc < KC; ++kc) vd[mt].d[i][kc] = static_cast<_Float16>(0.f);
+                    }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[mt][i]);
+        if (__any(mx > m + kThreshold)) {
+            const float mn = fmaxf(m, cross_row_max(mx));
+            const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+            m = mn;
+            l *= alpha;
+            rounded *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < 2 * KC; ++dt) acc[dt] *= alpha;
+        }
+        const float base = m == -INFINITY ? 0.f : m;  // (no key seen yet: probabilities 0)
+        float sum = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[mt][i] = fast_exp2(s[mt][i] - base);
+                sum += s[mt][i];
+            }
+        add_to(l, rounded, sum);
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+            f32x4 d[2];
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[mt][i] = s[mt][i] * static_cast<float>(vd[mt].d[i][kc]);
+            bf16x8 p[3];
+            split3(d[0], d[1], p);
+            auto tile = [&](auto e) __attribute__((always_inline)) {
+                f32x4 x[2];
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[mt][i] = sbyte_to_float<e.value>(vw[mt][i][kc]);
+                const bf16x8 v = eight(x[0], x[1]);
+                f32x4 part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[2], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[1], part, 0, 0, 0);
+                acc[2 * kc + e.value] += __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[0], part, 0, 0, 0);
+            };
+            tile(std::integral_constant<int, 0>{});
+            tile(std::integral_constant<int, 1>{});
+        }
+        load_v(next);
+    }
+    if (__any(nonfinite != 0.f) && lane == 0) *a.err = 1;
+
+    // ---- the waves that shared these rows' keys, together
+    float total = cross_row_sum(l);
+    if (g == 0) stats[wave][r16] = make_float2(m, total);
+    __syncthreads();
+    {
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) top = fmaxf(top, stats[w][r16].x);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) sum = fmaf(fast_exp2(stats[w][r16].x - base), stats[w][r16].y, sum);
+        const float scale = fast_exp2(m - base);
+#pragma unroll
+        for (int dt = 0; dt < 2 * KC; ++dt) acc[dt] *= scale;
+        m = top;
+        total = sum;
+    }
+    // the n-th four columns of a lane, from 32 (n / 2) + 8 g + 4 (n % 2) on
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        if (h) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int kc = 2 * h + i / 2, o = 2 * (i % 2);
+            result(wave, i) = f32x4{acc[2 * kc][o], acc[2 * kc + 1][o], acc[2 * kc][o + 1], acc[2 * kc + 1][o + 1]};
+        }
+        __syncthreads();
+        f32x4 x = result(0, wave);
+#pragma unroll
+        for (int w = 1; w < WK; ++w) x += result(w, wave);
+        const int column = 32 * (2 * h + wave / 2) + 8 * g + 4 * (wave % 2);
+        if (!live) continue;
+        if (it.runs == 1) {
+            *reinterpret_cast<f32x4*>(a.out + (row * a.heads + head) * D + column) = x / (total != 0.f ? total : 1.f);
+        } else {
+            const size_t p = (static_cast<size_t>(it.slot) + static_cast<size_t>(index) * it.runs + it.run) * a.heads + head;
+            *reinterpret_cast<f32x4*>(a.part_acc + p * D + column) = x;
             if (h == 0 && wave == 0 && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m, total);
         }
     }
@@ -858,9 +1080,9 @@ void launch_score_tiles(const ScoreArgs& a, int block, int workgroups, hipStream
     if (block == kScoreFew) {
         const char* name = "score_attention_tiles";
         if (a.lay.head_dim == 128)
-            q8 ? go(name, score_tile_kernel<128, true>, kFewWaves) : go(name, score_tile_kernel<128, false>, kFewWaves);
+            q8 ? go(name, score_tile_q8_kernel<128>, kFewWaves) : go(name, score_tile_kernel<128>, kFewWaves);
         else
-            q8 ? go(name, score_tile_kernel<64, true>, kFewWaves) : go(name, score_tile_kernel<64, false>, kFewWaves);
+            q8 ? go(name, score_tile_q8_kernel<64>, kFewWaves) : go(name, score_tile_kernel<64>, kFewWaves);
     } else {
         const char* name = "score_attention_shared";
         if (a.lay.head_dim == 128)
