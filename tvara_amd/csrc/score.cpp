@@ -15,6 +15,10 @@ constexpr size_t kIntMax = static_cast<size_t>(std::numeric_limits<int32_t>::max
 constexpr size_t kMaxThreads = std::numeric_limits<uint32_t>::max(), kMaxWorkgroups = kMaxThreads / 512;
 // keys of a run of the row kernel, at least
 constexpr size_t kRowRun = 64;
+// rounds of workgroups that runs are cut for; what a run of few and of many rows costs
+// beside its steps, in steps (many: six prompts of 3 to 700 rows behind up to 2,500 keys, 32
+// heads of 64: 134 us at 2, whose runs are shorter and want merging, 130 at 8 and at 24)
+constexpr size_t kRounds = 4, kRunCost[2] = {12, 8};
 
 // A block of rows of a sequence that read the same keys: they share its runs.
 struct Block {
@@ -50,8 +54,8 @@ void ScorePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_
     group = static_cast<int>(h / g.kv_heads);
     rows = 0;
     for (size_t i = 0; i < n; ++i) {
-        // (the merge has a thread for two columns)
-        if (counts[i] > kIntMax || (rows += counts[i]) > std::min(kIntMax, kMaxThreads / g.head_dim) / h)
+        // (the merge has 256 threads a row in its grid's first dimension)
+        if (counts[i] > kIntMax || (rows += counts[i]) > std::min(kIntMax, kMaxThreads / g.head_dim) / h || rows > kMaxThreads / 256)
             throw std::invalid_argument("attention batch too large");
     }
 
@@ -84,8 +88,11 @@ void ScorePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_
         }
         seqs[i] = make_int4(offset[sequences[i]], static_cast<int>(t.length), static_cast<int>(counts[i]), static_cast<int>(row0));
         // Blocks of many rows share a key's parts among them and pay for padding and
-        // splitting with few (MI355X: see score_shared_kernel).
-        const int kind = tiles && counts[i] * per_block > 64 ? 1 : 0;
+        // splitting with few: eight contexts of 2,000, 32 heads on 8, attention rows a KV
+        // head, few against many (f32, us): head_dim 64 96 rows 51 and 57, 128 69 and 61;
+        // head_dim 128 64 rows 58 and 82, 96 90 and 85; (Q8_0) 64 128 rows 52 and 61, 256 78
+        // and 63; 128 128 rows 79 and 90, 256 123 and 93.
+        const int kind = tiles && counts[i] * per_block > (lay.format == kQ8 ? 160 : 96) ? 1 : 0;
         const size_t high = tiles ? (kind ? kScoreMany : kScoreFew) / per_block : 1;
         for (size_t j = 0; j < counts[i]; j += high) {
             Block b{static_cast<int>(i), static_cast<int>(row0 + j), static_cast<int>(std::min(high, counts[i] - j)),
@@ -114,8 +121,38 @@ void ScorePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_
             units = static_cast<size_t>(c->compute_units()) * score_units(lay, block);
             least = 4;
         }
-        for (const Block& b : blocks[kind]) total += static_cast<size_t>(b.end - b.step) * slices;
-        const size_t per = std::max(least, (total + units - 1) / units);
+        size_t longest_block = 0;
+        for (const Block& b : blocks[kind]) {
+            total += static_cast<size_t>(b.end - b.step) * slices;
+            longest_block = std::max(longest_block, static_cast<size_t>(b.end - b.step));
+        }
+        // Runs of the same length that the chip takes in as few whole rounds as possible: in
+        // one, two, … rounds the shortest that leave no workgroup for another, and of those the
+        // least time. (Cut by the average alone, the ragged lengths leave a few workgroups
+        // behind, for as long as all the others took.)
+        size_t per = std::max(least, (total + units - 1) / units), time = std::numeric_limits<size_t>::max();
+        auto cuts = [&](size_t length) {
+            size_t count = 0;
+            for (const Block& b : blocks[kind]) count += std::max<size_t>(1, (b.end - b.step + length - 1) / length) * slices;
+            return count;
+        };
+        bool at_once = false;
+        for (size_t rounds = 1; tiles && rounds <= kRounds; ++rounds) {
+            size_t low = std::max(least, (total + rounds * units - 1) / (rounds * units)), high = std::max(low, longest_block);
+            if (cuts(high) > rounds * units) continue;
+            while (low < high) {
+                const size_t mid = low + (high - low) / 2;
+                if (cuts(mid) <= rounds * units)
+                    high = mid;
+                else
+                    low = mid + 1;
+            }
+            if (rounds * (low + kRunCost[kind]) < time) {
+                time = rounds * (low + kRunCost[kind]);
+                per = low;
+                at_once = rounds == 1;
+            }
+        }
         std::vector<int4> list;
         std::vector<size_t> load;
         for (Block& b : blocks[kind]) {
@@ -139,7 +176,8 @@ void ScorePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_
         }
         if (!tiles) continue;
         // Workgroups that read the same keys one after the other, cut into the XCDs' equal
-        // shares (workgroup ids go to the XCDs round-robin), each from the longest down.
+        // shares (workgroup ids go to the XCDs round-robin), each from the longest down: shares
+        // of the work, or of the workgroups where all of them run at once.
         size_t sum = 0;
         for (size_t at = 0; at < blocks[kind].size();) {
             size_t to = at;
@@ -156,8 +194,8 @@ void ScorePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_
                             list.push_back(make_int4(seqs[b.seq].x, seqs[b.seq].y, b.rows, b.row));
                             list.push_back(make_int4(kh * group + h0, std::min(per_block, group - h0), s0, s1));
                             list.push_back(make_int4(r, b.runs, b.slot, b.position));
-                            load.push_back(s1 - s0 + 2);
-                            sum += load.back();
+                            load.push_back(s1 - s0 + kRunCost[kind]);
+                            sum += at_once ? 1 : load.back();
                             if (load.size() > kMaxWorkgroups / 2) throw std::invalid_argument("attention batch too large");
                         }
             at = to;
@@ -166,7 +204,7 @@ void ScorePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_
         size_t done = 0, longest = 0;
         for (size_t k = 0; k < load.size(); ++k) {
             lists[std::min<size_t>(xcds - 1, done * xcds / std::max<size_t>(sum, 1))].push_back(k);
-            done += load[k];
+            done += at_once ? 1 : load[k];
         }
         for (auto& l : lists) {
             std::stable_sort(l.begin(), l.end(), [&](size_t x, size_t y) { return load[x] > load[y]; });

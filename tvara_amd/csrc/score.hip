@@ -84,20 +84,27 @@ __global__ __launch_bounds__(64) void score_rows_kernel(const ScoreArgs a) {
     if (!whole && lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(m, l);
 }
 
-// A row's runs combined: a workgroup a (row, head), its waves take runs in turn, lanes
-// are columns, the maxima and sums of 64 runs in a wave's lanes at once.  The loads of
-// four runs are in flight.  What the additions round away is kept (add_to): beside one
-// run with all the weight the others' parts may each be less than half an ulp.
-template <int kColumns>
+// (rows, heads) up to which four waves take one
+constexpr size_t kMergeSpread = 8192;
+
+// A row's runs combined: waves take runs in turn, lanes are columns, the maxima and sums of
+// 64 runs in a wave's lanes at once.  The loads of four runs are in flight.  What the
+// additions round away is kept (add_to): beside one run with all the weight the others'
+// parts may each be less than half an ulp.  A workgroup takes a (row, head) with its four
+// waves where the chip has waves to spare, or one with each (2,200 rows
+// of 32 heads: 24 us, and 76 with four; a row of nine after 4,000 keys, with its attention,
+// 13.5, and 10.4 with four).
+template <int kColumns, int kWaves>
 __global__ __launch_bounds__(256) void score_merge_kernel(const ScoreArgs a) {
-    constexpr int kWaves = 4, kTogether = 4;
-    __shared__ float2 stats[kWaves];
-    __shared__ float sums[kWaves][64 * kColumns];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = a.lay.head_dim;
+    constexpr int kTogether = 4;
+    __shared__ float2 stats[4];
+    __shared__ float sums[4][64 * kColumns];
+    const int lane = threadIdx.x & 63, in_group = threadIdx.x >> 6, wave = in_group % kWaves, D = a.lay.head_dim;
     const size_t row = blockIdx.x;
-    const int h = blockIdx.y;
+    const int h = kWaves == 4 ? blockIdx.y : 4 * blockIdx.y + in_group;
     const int2 runs = a.runs[row];
     if (runs.y == 1) return;  // (written by the attention itself)
+    if (kWaves == 1 && h >= a.heads) return;
     float m = -INFINITY, l = 0.f, l_rest = 0.f, acc[kColumns], rest[kColumns];
 #pragma unroll
     for (int i = 0; i < kColumns; ++i) acc[i] = rest[i] = 0.f;
@@ -138,6 +145,13 @@ __global__ __launch_bounds__(256) void score_merge_kernel(const ScoreArgs a) {
                     for (int i = 0; i < kColumns; ++i) add_to(acc[i], rest[i], w[k] * x[k][i]);
         }
     }
+    if constexpr (kWaves == 1) {
+        const float div = l != 0.f ? l : 1.f;
+#pragma unroll
+        for (int i = 0; i < kColumns; ++i)
+            if (i * 64 + lane < D) a.out[(row * a.heads + h) * D + i * 64 + lane] = acc[i] / div;
+        return;
+    }
     if (lane == 0) stats[wave] = make_float2(m, l);
     __syncthreads();
     float top = -INFINITY, total = 0.f;
@@ -167,11 +181,20 @@ void launch_score_rows(const ScoreArgs& a, int items, hipStream_t s) {
 }
 
 void launch_score_merge(const ScoreArgs& a, hipStream_t s) {
-    auto go = [&](auto kernel) {
-        launch("score_attention_merge", kernel, dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>(a.heads)), dim3(256), 0, s, a);
+    auto go = [&](auto kernel, int groups) {
+        launch("score_attention_merge", kernel, dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>(groups)), dim3(256), 0, s, a);
     };
     const int columns = (a.lay.head_dim + 63) / 64;
-    columns == 1 ? go(score_merge_kernel<1>) : columns == 2 ? go(score_merge_kernel<2>) : go(score_merge_kernel<kMaxDim / 64>);
+    if (static_cast<size_t>(a.rows) * a.heads > kMergeSpread) {
+        const int groups = (a.heads + 3) / 4;
+        columns == 1   ? go(score_merge_kernel<1, 1>, groups)
+        : columns == 2 ? go(score_merge_kernel<2, 1>, groups)
+                       : go(score_merge_kernel<kMaxDim / 64, 1>, groups);
+    } else {
+        columns == 1   ? go(score_merge_kernel<1, 4>, a.heads)
+        : columns == 2 ? go(score_merge_kernel<2, 4>, a.heads)
+                       : go(score_merge_kernel<kMaxDim / 64, 4>, a.heads);
+    }
     TVARA_HIP(hipGetLastError());
 }
 

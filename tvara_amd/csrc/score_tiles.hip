@@ -256,7 +256,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_kernel(const Sco
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[mt][i] = a.cap * (small ? small_tanh(s[mt][i]) : any_tanh(s[mt][i]));
+                for (int i = 0; i < 4; ++i) s[mt][i] = a.cap * (small ? small_tanh(s[mt][i]) : both_tanh(s[mt][i]));
         }
         if (a.slopes) {
             const int away = position - key0 - 4 * g;
@@ -376,14 +376,29 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_kernel(const Sco
 // bf16, which holds a byte exactly, with queries and probabilities in three bf16 parts
 // (24 bits, f32's range).  A product over 32 columns is one group's: scores are multiplied
 // by the group's scale behind it, probabilities before, one column group after the other.
-// Bound: HBM (in f32 products it is the matrix pipe: eight contexts of 16,000 to 32,768
-// tokens, 32 heads on 8 of 128: 224 us, and TIME so).
+// A wave's bytes go straight into LDS, the next step's keys once the scores have read
+// these, its values behind the products; the queries' parts are there too, for registers
+// of three waves on a SIMD: eight contexts of 16,000 to 32,768 tokens, 32 heads on 8 of 128
+// (390 MB), take 95 us (4.1 TB/s), bound by the 850 vector instructions of a step, and 140 us
+// with the next step's bytes in registers and two waves.  (In f32 products the matrix
+// instructions bound it, at 224 us.)
 template <int D>
-__global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_q8_kernel(const ScoreArgs a) {
+__global__ __launch_bounds__(64 * kFewWaves, 3) void score_tile_q8_kernel(const ScoreArgs a) {
     constexpr int WK = kFewWaves, KC = D / 32, H = D / 64;
-    __shared__ f32x4 staged[WK][4 * 64];
-    auto result = [&](int w, int i) -> f32x4& { return staged[w][i * 64 + static_cast<int>(threadIdx.x & 63)]; };
+    // a wave's keys, values and scales of a step, straight from memory: the next step's keys are
+    // loaded once the scores have read them, its values behind the products.  At the end the
+    // wave's results, for the others.
+    struct alignas(16) Step {
+        char rows[2][kFewStep * D];     // keys, values; 16 bytes at p hold those at p ^ row % 8 (128 columns)
+        char scales[2][kFewStep * KC * 2];
+    };
+    __shared__ union {
+        Step step;
+        f32x4 result[4 * 64];
+    } staged[WK];
+    auto result = [&](int w, int i) -> f32x4& { return staged[w].result[i * 64 + static_cast<int>(threadIdx.x & 63)]; };
     __shared__ float2 stats[WK][16];
+    __shared__ u32x4 queries[KC][3][64];  // in three parts, the same for all waves
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, r16 = lane & 15;
     const Item it = item_of(a, blockIdx.x);
@@ -407,86 +422,125 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_q8_kernel(const 
     // lane 2i + mt: the block of the wave's i-th step from here
     auto lookup = [&](int from) { return tokens ? tab[min(2 * (from + (lane >> 1) * WK) + (lane & 1), last) << 4 >> tsh] : 0; };
     int ids = lookup(step), more = lookup(step + 32 * WK), at = 0;
-    // bytes of key r16 (lane group g: 8 of each 32), of column pairs 2 r16 of keys 4g + i,
-    // and the scales of those keys
-    u32x2 kw[2][KC];
-    unsigned vw[2][4][KC];
-    struct alignas(8) Scales {
-        _Float16 d[4][KC];
-    } kd[2], vd[2];
-    auto block = [&](int mt, int stp, const char*& scales) __attribute__((always_inline)) {
-        const int id = __builtin_amdgcn_readlane(ids, 2 * at + mt), slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
-        const char* b = a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes;
-        scales = b + static_cast<size_t>(tpb) * D + static_cast<size_t>(slot) * KC * 2;
-        return b + static_cast<size_t>(slot) * D;
-    };
-    auto load_k = [&](int stp) __attribute__((always_inline)) {
+    constexpr int P = D / 16;            // 16-byte parts of a row
+    constexpr int kLoads = 2 * D / 64 + 1;  // of a step's keys or values
+    const int swap = P - 1;                 // of a part's place, by row
+    unsigned part_at[D / 64];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-            const char *sc, *b = block(mt, stp, sc);
-#pragma unroll
-            for (int kc = 0; kc < KC; ++kc) kw[mt][kc] = *reinterpret_cast<const u32x2*>(b + r16 * D + 32 * kc + 8 * g);
-            kd[mt] = *reinterpret_cast<const Scales*>(sc + 4 * g * KC * 2);
-        }
-    };
-    auto load_v = [&](int stp) __attribute__((always_inline)) {
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-            const char *sc, *b = block(mt, stp, sc);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int kc = 0; kc < KC; ++kc)
-                    vw[mt][i][kc] = *reinterpret_cast<const uint16_t*>(b + vsec + (4 * g + i) * D + 32 * kc + 2 * r16);
-            vd[mt] = *reinterpret_cast<const Scales*>(sc + vsec + 4 * g * KC * 2);
-        }
-    };
-    bf16x8 q[KC][3];
-    {
-        const float* qp = a.q + (row * a.heads + head) * D + 8 * g;
-        f32x4 x[KC][2];
-#pragma unroll
-        for (int kc = 0; kc < KC; ++kc)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                x[kc][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (live) x[kc][i] = *reinterpret_cast<const f32x4*>(qp + 32 * kc + 4 * i);
-            }
-        if (step < it.end) {
-            load_k(step);
-            load_v(step);
-        }
-#pragma unroll
-        for (int kc = 0; kc < KC; ++kc) split3(x[kc][0] * a.qscale, x[kc][1] * a.qscale, q[kc]);
+    for (int n = 0; n < D / 64; ++n) {  // 64 / P keys a load
+        const int row = 64 / P * n + lane / P;
+        part_at[n] = row * D + ((lane % P) ^ (row & swap)) * 16;
     }
+    auto load = [&](int kind, int stp) __attribute__((always_inline)) {
+        typedef __attribute__((address_space(1))) const void* global;
+        typedef __attribute__((address_space(3))) void* shared;
+        const char* scales[2];
+        Step& to = staged[wave].step;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+            const int id = __builtin_amdgcn_readlane(ids, 2 * at + mt), slot = (min(2 * stp + mt, last) << 4) & (tpb - 1);
+            const char* b = a.pool + static_cast<size_t>(id) * a.lay.stride + kbytes + kind * vsec;
+            const char* from = b + static_cast<size_t>(slot) * D;
+            scales[mt] = b + static_cast<size_t>(tpb) * D + static_cast<size_t>(slot) * KC * 2;
+#pragma unroll
+            for (int n = 0; n < D / 64; ++n)
+                __builtin_amdgcn_global_load_lds((global)(from + part_at[n]), (shared)(to.rows[kind] + (16 * mt) * D + 1024 * n), 16, 0, 0);
+        }
+        // (of 64 columns half of the lanes are enough)
+        const char* x = (lane / (8 * KC) & 1 ? scales[1] : scales[0]) + lane % (8 * KC) * 4;
+        if (lane < 16 * KC) __builtin_amdgcn_global_load_lds((global)x, (shared)to.scales[kind], 4, 0, 0);
+    };
+    // bytes of key 16 mt + r16, columns 32 kc + 8 g on; of keys 16 mt + 4 g + i, columns 32 kc + 2 r16 on
+    auto key_bytes = [&](int mt, int kc) __attribute__((always_inline)) {
+        return *reinterpret_cast<const u32x2*>(staged[wave].step.rows[0] + (16 * mt + r16) * D + ((2 * kc + (g >> 1)) ^ (r16 & swap)) * 16 + 8 * (g & 1));
+    };
+    auto value_bytes = [&](int mt, int i, int kc) __attribute__((always_inline)) {
+        const int row = 4 * g + i;
+        return static_cast<unsigned>(*reinterpret_cast<const uint16_t*>(staged[wave].step.rows[1] + (16 * mt + row) * D +
+                                                                         ((2 * kc + (r16 >> 3)) ^ (row & swap)) * 16 + 2 * (r16 & 7)));
+    };
+    auto query = [&](int kc, int part) __attribute__((always_inline)) { return __builtin_bit_cast(bf16x8, queries[kc][part][lane]); };
+    struct Scales {
+        _Float16 d[4][KC];
+    };
+    // (read as vectors: a read of a struct waits for every load into LDS that is on its way)
+    auto scales_of = [&](int kind, int mt) __attribute__((always_inline)) {
+        const f32x4* x = reinterpret_cast<const f32x4*>(staged[wave].step.scales[kind] + (16 * mt + 4 * g) * KC * 2);
+        struct {
+            f32x4 v[KC / 2];
+        } all;
+#pragma unroll
+        for (int i = 0; i < KC / 2; ++i) all.v[i] = x[i];
+        return __builtin_bit_cast(Scales, all);
+    };
+    if (wave < KC) {
+        const float* qp = a.q + (row * a.heads + head) * D + 8 * g + 32 * wave;
+        f32x4 x[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (live) x[i] = *reinterpret_cast<const f32x4*>(qp + 4 * i);
+        }
+        bf16x8 q[3];
+        split3(x[0] * a.qscale, x[1] * a.qscale, q);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) queries[wave][i][lane] = __builtin_bit_cast(u32x4, q[i]);
+    }
+    static_assert(KC <= WK);
+    __syncthreads();
     f32x4 acc[2 * KC];  // columns 32 kc + 2 m + e at 2 kc + e, m being the tile's row
     float m = -INFINITY, l = 0.f, rounded = 0.f, nonfinite = 0.f;  // nonfinite: NaN once a score is not finite
 #pragma unroll
     for (int dt = 0; dt < 2 * KC; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto advance = [&](int next) {
+        if (++at == 32) {
+            at = 0;
+            ids = more;
+            more = lookup(next + 32 * WK);
+            wait_until_left<0>();
+            asm volatile("" : "+v"(more));  // (its load ends here, not at a use among loads into LDS)
+        }
+    };
+    if (step < it.end) {
+        wait_until_left<0>();
+        asm volatile("" : "+v"(ids), "+v"(more));
+        load(0, step);
+        load(1, step);
+    }
     for (; step < it.end; step += WK) {
-        const int next = step + WK, key0 = kFewStep * step;
+        const int key0 = kFewStep * step;
+        const bool another = step + WK < it.end;
+        wait_until_left<kLoads>();  // the values
+        Scales kd[2], vd[2];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) kd[mt] = scales_of(0, mt);
         f32x4 s[2];  // scores, then probabilities, of keys 16mt + 4g + i
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
             s[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc) {
-                const unsigned w0 = kw[mt][kc][0], w1 = kw[mt][kc][1];
+                const u32x2 w = key_bytes(mt, kc);
+                const unsigned w0 = w[0], w1 = w[1];
                 const bf16x8 k = eight(f32x4{sbyte_to_float<0>(w0), sbyte_to_float<1>(w0), sbyte_to_float<2>(w0), sbyte_to_float<3>(w0)},
                                        f32x4{sbyte_to_float<0>(w1), sbyte_to_float<1>(w1), sbyte_to_float<2>(w1), sbyte_to_float<3>(w1)});
-                f32x4 part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[kc][2], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[kc][1], part, 0, 0, 0);
-                part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[kc][0], part, 0, 0, 0);
+                f32x4 part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, query(kc, 2), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, query(kc, 1), part, 0, 0, 0);
+                part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, query(kc, 0), part, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[mt][i] = fmaf(part[i], static_cast<float>(kd[mt].d[i][kc]), s[mt][i]);
             }
         }
-        if (++at == 32) {
-            at = 0;
-            ids = more;
-            more = lookup(next + 32 * WK);
+        wait_for_lds();
+        advance(step + WK);
+        if (another) {
+            load(0, step + WK);
+            wait_until_left<kLoads>();  // the next keys
+        } else {
+            wait_until_left<0>();
         }
-        load_k(next);
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) vd[mt] = scales_of(1, mt);
         const bool whole = key0 >= lo && key0 + kFewStep <= hi;  // every row sees every key
         const int first = range.x - key0 - 4 * g, end = range.y - key0 - 4 * g;  // of the lane's keys 16mt + i
 #pragma unroll
@@ -506,7 +560,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_q8_kernel(const 
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[mt][i] = a.cap * (small ? small_tanh(s[mt][i]) : any_tanh(s[mt][i]));
+                for (int i = 0; i < 4; ++i) s[mt][i] = a.cap * (small ? small_tanh(s[mt][i]) : both_tanh(s[mt][i]));
         }
         if (a.slopes) {
             const int away = position - key0 - 4 * g;
@@ -560,12 +614,17 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_q8_kernel(const 
                 for (int i = 0; i < 4; ++i) d[mt][i] = s[mt][i] * static_cast<float>(vd[mt].d[i][kc]);
             bf16x8 p[3];
             split3(d[0], d[1], p);
+            unsigned w[2][4];
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[mt][i] = value_bytes(mt, i, kc);
             auto tile = [&](auto e) __attribute__((always_inline)) {
                 f32x4 x[2];
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[mt][i] = sbyte_to_float<e.value>(vw[mt][i][kc]);
+                    for (int i = 0; i < 4; ++i) x[mt][i] = sbyte_to_float<e.value>(w[mt][i]);
                 const bf16x8 v = eight(x[0], x[1]);
                 f32x4 part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[2], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
                 part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[1], part, 0, 0, 0);
@@ -574,8 +633,10 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_q8_kernel(const 
             tile(std::integral_constant<int, 0>{});
             tile(std::integral_constant<int, 1>{});
         }
-        load_v(next);
+        wait_for_lds();
+        if (another) load(1, step + WK);
     }
+    wait_until_left<0>();  // (LDS is used again)
     if (__any(nonfinite != 0.f) && lane == 0) *a.err = 1;
 
     // ---- the waves that shared these rows' keys, together
@@ -1070,8 +1131,10 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
 
 int score_step(const BlockLayout& lay, int block) { return block == kScoreFew ? kFewStep : 4096 / lay.head_dim; }
 
+// (us with 1, 2 and 3 for few rows, eight contexts of 4,000 to 9,000, 32 heads on 8: f32 of 64
+// 45, 47 and 50, of 128 92, 93 and 95; Q8_0 of 64 35, 27 and 25, of 128 48, 40 and 38)
 int score_units(const BlockLayout& lay, int block) {
-    return block == kScoreMany ? 1 : lay.head_dim == 64 ? 3 : lay.format == kQ8 ? 2 : 1;
+    return block == kScoreMany || lay.format != kQ8 ? 1 : 3;
 }
 
 void launch_score_tiles(const ScoreArgs& a, int block, int workgroups, hipStream_t s) {

@@ -40,5 +40,10 @@ constexpr float kSmallTanh = 0.625f;
 __device__ __forceinline__ float any_tanh(float x) {
     return __builtin_fabsf(x) <= kSmallTanh ? small_tanh(x) : large_tanh(x);
 }
+// the same without branches by lane, for more registers
+__device__ __forceinline__ float both_tanh(float x) {
+    const float small = small_tanh(x), large = large_tanh(x);
+    return __builtin_fabsf(x) <= kSmallTanh ? small : large;
+}
 
 }  // namespace tvara_amd
