@@ -503,7 +503,7 @@ TVARA_API int tvara_attn_tree(tvara_kv_cache* cache, const uint64_t* sequences, 
  * see it not finite.  The reference has causal attention alone (attention.hpp:57-89).
  *
  * Launching fails with TVARA_INVALID once the cache has changed.  rows * heads *
- * head_dim stays below 2^32 in all. */
+ * head_dim stays below 2^32 in all, the rows below 2^24. */
 TVARA_API tvara_score_plan* tvara_score_plan_create(tvara_kv_cache* cache, const uint64_t* sequences, size_t count,
                                                     size_t heads, size_t context, const size_t* start,
                                                     const size_t* rows, const size_t* first, const size_t* end,
@@ -535,8 +535,8 @@ TVARA_API int tvara_attn_score(tvara_kv_cache* cache, const uint64_t* sequences,
  * temperature 0 takes the lowest index of the largest.  -inf is never drawn, and
  * neither is a weight below 2^-45.  The same logits, numbers and parameters give the
  * same token whatever the batch: masses are summed as whole numbers of 64 bits. */
-/* Workspace for up to `rows` rows of `vocab` logits on the current device (rows * vocab
- * up to 2^33, vocab below 2^30). */
+/* Workspace for up to `rows` rows of `vocab` logits on the current device (at most 65,535
+ * rows, rows * vocab up to 2^33, vocab below 2^30). */
 TVARA_API tvara_sample_plan* tvara_sample_plan_create(size_t rows, size_t vocab);
 /* logits f32 [rows] rows of vocab, logits_stride floats apart (0: vocab); uniforms
  * [rows]; temperature, top_k, top_p, min_p [rows], or NULL for 1, 0, 1 and 0; tokens

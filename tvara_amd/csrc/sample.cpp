@@ -11,8 +11,8 @@ namespace tvara_amd {
 void SamplePlan::build(size_t n, size_t v) {
     constexpr size_t kIntMax = static_cast<size_t>(std::numeric_limits<int32_t>::max());
     if (!n || !v) throw std::invalid_argument("empty sample plan");
-    // (a workgroup a row, and a thread for every four logits)
-    if (v > kIntMax / 2 || n > kIntMax / 1024 || n > (size_t(1) << 33) / v) throw std::invalid_argument("sample plan too large");
+    // (rows are a grid's second dimension)
+    if (v > kIntMax / 2 || n > 65535 || n > (size_t(1) << 33) / v) throw std::invalid_argument("sample plan too large");
     TVARA_HIP(hipGetDevice(&device));
     rows = static_cast<int>(n);
     vocab = static_cast<int>(v);

@@ -63,14 +63,14 @@ def sample_batch(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
             raise InvalidArgument(f"one {what} for all rows or for each")
         if dtype is np.int32 and (values.dtype.kind not in "iu" or (values < 0).any() or (values > 2**31 - 1).any()):
             raise InvalidArgument(f"{what} is a whole number from 0")
-        return hip.DeviceArray.from_numpy(np.ascontiguousarray(np.broadcast_to(values.astype(dtype), (n,))))
+        return np.ascontiguousarray(np.broadcast_to(values.astype(dtype), (n,)))
 
     if np.shape(uniforms) != (n,):
         raise InvalidArgument("one random number for each row")
     given = [each(x, t, what) for x, t, what in ((uniforms, np.float32, "random number"), (temperature, np.float32, "temperature"),
                                                  (top_k, np.int32, "top_k"), (top_p, np.float32, "top_p"),
                                                  (min_p, np.float32, "min_p"))]
-    x = hip.DeviceArray.from_numpy(logits)
+    x, *given = (hip.DeviceArray.from_numpy(a) for a in (logits, *given))
     tokens, chances = hip.DeviceArray((n,), np.uint32), hip.DeviceArray((n,), np.float32)
     plan = SamplePlan(n, vocab)
     u, t, k, p, m = (d.ptr for d in given)
