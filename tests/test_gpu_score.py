@@ -384,3 +384,12 @@ def test_refusals(device, oracle):
     for x in (b.k, b.v):
         assert all(np.isfinite(y).all() for y in x)
     b.agree(cap=3.0)
+
+
+def test_more_rows_than_a_launch_holds(device, oracle):
+    say("score, too many rows")
+    b = Batch(device, oracle, 1, 1, 16, [20], [1])
+    for rows in (1 << 24, 1 << 40):
+        with pytest.raises(_capi.InvalidArgument, match="too large"):
+            attention.ScorePlan(b.cache, b.seqs, [0], [rows], 1, 1 << 20)
+    b.agree()
