@@ -592,7 +592,7 @@ TVARA_API int tvara_slot_plan_write(tvara_slot_plan* plan, const int64_t* slots,
  * q_out [n][heads * head_dim]; keys and values into slots[i] of `layer`, f32 as they are
  * or encoded as appends encode them (-1: nowhere; NULL: none is written); rotated keys
  * to k_out [n][kv_width] too, for rows that stay outside the cache (tree plans).
- * q_out and k_out may be NULL, or q_out q itself where q is packed.  A slot outside the
+ * q_out and k_out may be NULL, or q and keys themselves where those are packed.  A slot outside the
  * pool is skipped and reported by tvara_slot_plan_check; two entries of one slot leave
  * a mixture.  head_dim and rotary are even, head_dim up to 512.  Device pointers,
  * asynchronous.  The reference rotates on the host (model.hpp:67-76). */
@@ -604,8 +604,9 @@ TVARA_API int tvara_slot_plan_rotate(tvara_slot_plan* plan, const int64_t* slots
 /* K/V of layers layer .. layer + layers - 1 out of slots, as f32 (Q8_0 blocks: scale *
  * byte): entry t to element (t, layer, column) as tvara_slot_plan_write has them, the
  * first layer at 0; an entry with slot -1 leaves its rows as they are, a slot outside
- * the pool too and is reported by tvara_slot_plan_check.  Strides in multiples of 4 for
- * Q8_0 blocks.  Device pointers, asynchronous. */
+ * the pool too and is reported by tvara_slot_plan_check.  A row's layers lie before the
+ * next row, or a layer's rows before the next layer; strides in multiples of 4 for Q8_0
+ * blocks.  Device pointers, asynchronous. */
 TVARA_API int tvara_slot_plan_read(tvara_slot_plan* plan, const int64_t* slots, size_t n, size_t layer, size_t layers,
                                    float* keys, float* values, size_t row_stride, size_t layer_stride, void* stream);
 TVARA_API int tvara_slot_plan_check(tvara_slot_plan* plan);

@@ -298,3 +298,47 @@ def test_captured_and_on_another_stream(device, oracle):
     del graph
     hip.synchronize()
     b.cache.set_stream(None)
+
+
+@pytest.mark.parametrize("dim,interleaved,norm", [(64, False, True), (128, True, True), (10, False, True), (20, True, False)])
+def test_in_place(device, oracle, dim, interleaved, norm):
+    """Packed queries and keys onto themselves, in the kernel of eight columns a thread and in
+    the other; rows with something between them are refused."""
+    say("rotate, in place", dim, interleaved, norm)
+    b = Rows(device, 4, 2, dim, 9, fused=False)
+    up = hip.DeviceArray.from_numpy
+    pos, freqs, wq, wk = up(b.pos), up(b.freqs), up(b.wq), up(b.wk)
+    how = {"q_norm_ptr": wq.ptr, "k_norm_ptr": wk.ptr, "eps": 1e-5} if norm else {}
+    call = [b.ptrs[0], b.ptrs[1], None, pos.ptr, freqs.ptr, dim, 4, b.ptrs[0], b.ptrs[1]]
+    for strides in ({"q_stride": 4 * dim + 4}, {"kv_stride": 2 * dim + 4}):
+        with pytest.raises(_capi.InvalidArgument, match="overlap"):
+            b.plan.rotate(None, 9, 0, *call, interleaved=interleaved, **how, **strides)
+    b.plan.rotate(None, 9, 0, *call, interleaved=interleaved, **how)
+    b.plan.check()
+    for got, (want, bar) in zip(b.dev, b.want(dim, interleaved, norm)):
+        assert (abs(got.numpy() - want) <= bar).all()
+
+
+def test_rows_read_over_each_other_are_refused(device, oracle):
+    say("read, overlapping rows")
+    b = Rows(device, 4, 2, 64, 4, layers=3)
+    d, s, w = hip.DeviceArray((4 * 3 * 128 + 8,)), hip.DeviceArray.from_numpy(b.slots), 128
+    for row, layer in ((w, w), (2 * w, w), (3 * w - 4, w), (w, 4 * w - 4), (1 << 62, 1 << 61)):
+        with pytest.raises(_capi.InvalidArgument, match="overlap"):
+            b.plan.read(s.ptr, 4, 0, 3, d.ptr, d.ptr, row, layer)
+    for n, layers, row, layer in ((4, 3, 3 * w, w), (4, 3, w, 4 * w), (1, 3, w, w), (4, 1, w, 0)):
+        b.plan.read(s.ptr, n, 0, layers, d.ptr, d.ptr, row, layer)
+    b.plan.check()
+
+
+def test_rows_that_pass_the_address_space_are_refused(device, oracle):
+    say("rotate, strides without end")
+    b = Rows(device, 4, 2, 64, 4)
+    d, s = hip.DeviceArray.from_numpy(np.zeros(4096, np.float32)), hip.DeviceArray.from_numpy(b.slots)
+    for how in ({"q_stride": 1 << 62}, {"kv_stride": 1 << 62}, {"q_stride": 1 << 58}, {"kv_stride": (1 << 64) - 4}):
+        with pytest.raises(_capi.InvalidArgument, match="overlap"):
+            b.plan.rotate(s.ptr, 4, 0, d.ptr, d.ptr, d.ptr, d.ptr, d.ptr, 64, 4, None, **how)
+    for n, row, layer in ((4, 1 << 62, 0), (1, 128, 1 << 62), (4, (1 << 64) - 4, 128)):
+        with pytest.raises(_capi.InvalidArgument, match="overlap"):
+            b.plan.read(s.ptr, n, 0, 2, d.ptr, d.ptr, row, layer)
+    b.plan.check()

@@ -286,3 +286,12 @@ def test_refusals():
     with pytest.raises(bad):
         sample_batch(x[0], [0.1])
     assert sample_batch(np.zeros((0, 8)), [])[0].size == 0
+
+
+def test_rows_that_pass_the_address_space_are_refused():
+    say("sample, strides without end")
+    d, plan = hip.DeviceArray.from_numpy(np.zeros(64, np.float32)), SamplePlan(4, 8)
+    for stride in (1 << 62, 1 << 58, (1 << 64) - 4):
+        with pytest.raises(_capi.InvalidArgument, match="overlap"):
+            plan.launch(d.ptr, d.ptr, d.ptr, logits_stride=stride)
+    plan.check()

@@ -50,7 +50,7 @@ void SamplePlan::launch(size_t n, const float* logits, size_t stride, const floa
                         hipStream_t s) {
     if (n > static_cast<size_t>(rows)) throw std::invalid_argument("more rows than the sample plan has");
     if (!stride) stride = vocab;
-    if (stride < static_cast<size_t>(vocab)) throw std::invalid_argument("logit rows overlap");
+    if (stride < static_cast<size_t>(vocab) || (n && stride > (size_t(1) << 59) / n)) throw std::invalid_argument("logit rows overlap");
     if (!n) return;
     int dev = 0;
     TVARA_HIP(hipGetDevice(&dev));

@@ -510,6 +510,9 @@ void SlotPlan::write(const int64_t* slots, const int32_t* rows, size_t n, const 
     region.launched(s);
 }
 
+// whether `count` rows of floats this far apart may pass the end of the address space
+static bool wraps(size_t count, size_t stride) { return count && stride > (size_t(1) << 59) / count; }
+
 void SlotPlan::rotate(RotateArgs a, hipStream_t s) {
     if (cache->epoch() != epoch) throw std::invalid_argument("slot plan is stale: the cache changed");
     const Geometry& g = cache->geometry();
@@ -521,7 +524,11 @@ void SlotPlan::rotate(RotateArgs a, hipStream_t s) {
     const size_t hidden = a.heads * g.head_dim;
     if (!a.q_stride) a.q_stride = hidden;
     if (!a.kv_stride) a.kv_stride = g.kv_width();
-    if (a.q_stride < hidden || a.kv_stride < g.kv_width()) throw std::invalid_argument("token rows overlap");
+    if (a.q_stride < hidden || a.kv_stride < g.kv_width() || wraps(a.n, a.q_stride) || wraps(a.n, a.kv_stride))
+        throw std::invalid_argument("token rows overlap");
+    // (rows of other strides would be written while others are read)
+    if ((a.q_out && a.q_out == a.q && a.q_stride != hidden) || (a.k_out && a.k_out == a.keys && a.kv_stride != g.kv_width()))
+        throw std::invalid_argument("token rows overlap");
     if (a.n > kMaxWorkgroups || 2 * g.layers * g.kv_width() * g.tokens_per_block > kMaxThreads)
         throw std::invalid_argument("KV write too large");
     if (!a.n) return;
@@ -542,6 +549,13 @@ void SlotPlan::read(ReadArgs a, hipStream_t s) {
     if (a.layer < 0 || a.layers < 0 || static_cast<size_t>(a.layer) > g.layers || static_cast<size_t>(a.layers) > g.layers - a.layer)
         throw std::invalid_argument("layers outside the cache");
     if (a.row_stride < g.kv_width() || (a.layers > 1 && a.layer_stride < g.kv_width()))
+        throw std::invalid_argument("token rows overlap");
+    // one row's layers before the next row, or one layer's rows before the next layer, all
+    // of them without a turn round the address space
+    const size_t layers = std::max(a.layers, 1), rows = std::max<size_t>(a.n, 1);
+    if (wraps(rows, a.row_stride) || wraps(layers, a.layer_stride) ||
+        (rows > 1 && layers > 1 && a.row_stride < (layers - 1) * a.layer_stride + g.kv_width() &&
+         a.layer_stride < (rows - 1) * a.row_stride + g.kv_width()))
         throw std::invalid_argument("token rows overlap");
     if (a.n > kMaxWorkgroups || 2 * g.layers * g.kv_width() > size_t(65535) * 256 ||
         2 * g.layers * g.kv_width() * g.tokens_per_block > kMaxThreads)
