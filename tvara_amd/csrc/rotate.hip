@@ -99,7 +99,8 @@ __device__ __forceinline__ void put_eight(char* section, const BlockLayout& lay,
 }
 
 // Head sizes of eight columns times a power of two: a lane has eight columns, whole
-// pairs of them.  grid.x: token, grid.y: a share of its heads (of queries, then keys,
+// pairs of them.  Bound: HBM (4,000 tokens, 32 heads on 8 of 128, with norms: 41 us for 197 MB,
+// 4.8 TB/s); a launch where tokens are few (one: 3 us).  grid.x: token, grid.y: a share of its heads (of queries, then keys,
 // then values).
 template <bool kQ8>
 __global__ __launch_bounds__(kThreads) void rotate_kernel(const RotateArgs a, int turns) {
@@ -262,7 +263,8 @@ __global__ __launch_bounds__(64) void rotate_rows_kernel(const RotateArgs a) {
 }
 
 // Slots back to rows: grid.x: token, grid.y: a share of its rows of every (layer, kind),
-// kVec floats a thread.  Bound: HBM.
+// kVec floats a thread.  Bound: HBM (1,500 tokens, four layers, 8 heads of 128 out of Q8_0:
+// 14 to 16 us for 62 MB, 4.3 TB/s).
 template <bool kQ8, int kVec>
 __global__ __launch_bounds__(kThreads) void slot_read_kernel(const ReadArgs a) {
     int64_t block;

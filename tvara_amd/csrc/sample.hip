@@ -20,7 +20,9 @@
 //    go into the list, and the masses of what lies above are summed.
 //  finish: the borders exactly, from the list, and the draw.
 // Bound: the first by HBM and its f64 exponentials; the others by the steps of a
-// workgroup, and, where rows are many and flat, by their instructions.
+// workgroup, and, where rows are many and flat, by their instructions.  In us: a row of 32,000
+// logits 4, 7, 2 and 8; 32 rows of 128,256 with parameters of all kinds 8, 16, 20 and 22; 256 rows
+// of 128,256 with top-p (131 MB, 24 us to read) 45, 60, 92 and 24.
 #include <algorithm>
 
 #include "common.hpp"
