@@ -533,8 +533,9 @@ TVARA_API int tvara_attn_score(tvara_kv_cache* cache, const uint64_t* sequences,
  *   min-p  of those, w_i >= min_p
  * and then the first index up to which the kept mass exceeds u times all of it.
  * temperature 0 takes the lowest index of the largest.  -inf is never drawn, and
- * neither is a weight below 2^-45.  The same logits, numbers and parameters give the
- * same token whatever the batch: masses are summed as whole numbers of 64 bits. */
+ * neither is a weight below 2^-45 (of a vocabulary from 2^n logits, n >= 20, below
+ * 2^(n - 64)).  The same logits, numbers and parameters give the same token whatever
+ * the batch: masses are summed as whole numbers of 64 bits. */
 /* Workspace for up to `rows` rows of `vocab` logits on the current device (at most 65,535
  * rows, rows * vocab up to 2^33, vocab below 2^30). */
 TVARA_API tvara_sample_plan* tvara_sample_plan_create(size_t rows, size_t vocab);

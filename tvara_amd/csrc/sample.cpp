@@ -2,6 +2,8 @@
 #include "sample.hpp"
 
 #include <algorithm>
+#include <bit>
+#include <cmath>
 #include <limits>
 #include <stdexcept>
 #include <type_traits>
@@ -20,6 +22,9 @@ void SamplePlan::build(size_t n, size_t v) {
     while (v > static_cast<size_t>(chunk) * kSampleChunks) chunk *= 2;
     chunks = static_cast<int>((v + chunk - 1) / chunk);
     room = static_cast<int>(std::min<size_t>(v, kSampleList));
+    // A row's mass is at most v times the largest weight, and stays below 2^64 units: 2^44 of
+    // them to that weight up to 2^20 - 1 logits, half as many for each doubling from there.
+    one = std::ldexp(1.0, std::min(44, 64 - static_cast<int>(std::bit_width(v))));
     carve(nullptr, nullptr);
     space.ensure(bytes);
     auto* f = static_cast<volatile int*>(flag.acquire(2 * sizeof(int)));
@@ -62,6 +67,7 @@ void SamplePlan::launch(size_t n, const float* logits, size_t stride, const floa
     a.vocab = vocab;
     a.chunk = chunk;
     a.chunks = chunks;
+    a.one = one;
     a.uniforms = uniforms;
     a.temperature = temperature;
     a.top_k = top_k;

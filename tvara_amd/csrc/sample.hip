@@ -9,6 +9,8 @@
 // exponential in f64: sums are then exact and the same in any order, so that neither the
 // split of a row nor the order of atomics decides a token, and a border between two of
 // 100,000 tokens is missed by 1e-9 of a token's mass.  (Weights below 2^-45 are zero.)
+// From 2^20 logits on, whose sum may reach 2^64 of these, the unit is so much larger that
+// it does not (SamplePlan::build).
 //
 // Four launches.
 //  chunks: one read of the logits: of every 256 (a chunk) the maximum and, where the row
@@ -40,7 +42,6 @@ constexpr int kBins = kSampleBins;
 constexpr float kSpan = 32.f;  // of x / temperature that the bins cover: further down, weights are zero
 constexpr int kList = kSampleList;
 constexpr uint32_t kNone = 0xffffffffu;
-constexpr double kUnit = 17592186044416.0;  // 2^44
 
 // 2^a for a in [-1000, 0], 1e-14 of it: Taylor's series of 2^f, |f| <= 1/2, and a's whole
 // part (the low word of a + 1.5 * 2^52) into the exponent
@@ -68,10 +69,11 @@ __device__ __forceinline__ double weight_of(float x, float top, double c) {
     return x == top ? 1.0 : w;
 }
 
-// in whole units of 2^-44, rounded to nearest: the low bits of w * 2^44 + 2^52
-__device__ __forceinline__ u64 units_of(double w) {
+// in whole units, `one` to a weight of 1 (2^44 or less), rounded to nearest: the low bits of
+// w * one + 2^52
+__device__ __forceinline__ u64 units_of(double w, double one) {
     constexpr double kShift = 4503599627370496.0;
-    return __builtin_bit_cast(u64, fma(w, kUnit, kShift)) - __builtin_bit_cast(u64, kShift);
+    return __builtin_bit_cast(u64, fma(w, one, kShift)) - __builtin_bit_cast(u64, kShift);
 }
 
 // the order of floats as that of numbers (-0 as 0)
@@ -293,6 +295,7 @@ struct Row {
     float top, scale;  // scale: bins for two units of a logit
     double c;          // log2(e) / temperature
     double min_p;
+    double one;        // a mass of 1 (SampleArgs::one)
 
     __device__ __forceinline__ float distance(float v) const {
         return (v == top ? 0.f : 0.5f * top - 0.5f * v) * scale;  // (top - v may be beyond f32)
@@ -301,9 +304,9 @@ struct Row {
         return static_cast<int>(fminf(distance(v), static_cast<float>(kBins)));
     }
     __device__ __forceinline__ double weight(float v) const { return weight_of(v, top, c); }
-    __device__ __forceinline__ u64 units(float v) const { return units_of(weight(v)); }
+    __device__ __forceinline__ u64 units(float v) const { return units_of(weight(v), one); }
     __device__ __forceinline__ float share(float v, u64 sum) const {
-        return static_cast<float>(weight(v) / (static_cast<double>(sum) / kUnit));
+        return static_cast<float>(weight(v) / (static_cast<double>(sum) / one));
     }
 };
 
@@ -317,6 +320,7 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int row, const Asked&
     r.c = 1.4426950408889634 / static_cast<double>(ask.temperature);
     r.scale = fminf(2.f * kBins / kSpan / ask.temperature, 3e38f);
     r.min_p = ask.min_p;
+    r.one = a.one;
     return r;
 }
 
@@ -508,7 +512,7 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(const SampleArg
             float m = -INFINITY;
             for (int k = tid * kSampleGroup; k < min((tid + 1) * kSampleGroup, a.chunks); ++k) m = fmaxf(m, s.chunk_max[k]);
             if (m != -INFINITY)
-                units = static_cast<u64>(__builtin_rint(a.group_mass[static_cast<size_t>(row) * kSampleGroups + tid] * r.weight(m) * kUnit));
+                units = static_cast<u64>(__builtin_rint(a.group_mass[static_cast<size_t>(row) * kSampleGroups + tid] * r.weight(m) * a.one));
         }
         if (!ask.by_p && ask.min_p == 0.f) {  // every token: the draw
             if (!first) return;
@@ -551,7 +555,7 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(const SampleArg
     };
     if (!ask.by_k && ask.min_p > 0.f) down_to(ask.min_p);
     // weights below (1 - p) of the mean weigh less than 1 - p together
-    if (need) down_to(fmin((1.0 - ask.top_p) * static_cast<double>(total) / kUnit / a.vocab, 1.0));
+    if (need) down_to(fmin((1.0 - ask.top_p) * static_cast<double>(total) / a.one / a.vocab, 1.0));
     for (int i = tid; i < kBins; i += kThreads) {
         s.mass[i] = 0;
         s.count[i] = 0;
@@ -616,7 +620,7 @@ __device__ __forceinline__ Window window_of(const SampleArgs& a, Shared& s, int 
     if (ask.by_k && static_cast<u64>(state.size) > ask.top_k)
         w.k = find(s, kBins, ask.top_k, [&](int i) { return static_cast<u64>(count[i]); }, before);
     if (ask.by_p) {
-        double lo = static_cast<double>(state.total) * (2147483648.0 / kUnit), hi = lo;
+        double lo = static_cast<double>(state.total) * (2147483648.0 / a.one), hi = lo;
         if (ask.by_k) {  // of what top-k keeps: up to its bin, or with all of that
             u64 up = 0;
             for (int i = threadIdx.x; i < kBins; i += kThreads)
@@ -669,7 +673,7 @@ __global__ __launch_bounds__(kThreads) void sample_sweep_kernel(const SampleArgs
             u64 units = 0;
             each_packed(s, v, before, [&](float x) {
                 const double y = r.weight(x);
-                const u64 n = units_of(y);
+                const u64 n = units_of(y, r.one);
                 above += n;
                 if (y >= r.min_p) units += n;
             });
@@ -739,7 +743,7 @@ __device__ __forceinline__ void draw_listed(const SampleArgs& a, int row, Shared
     const uint32_t key = static_cast<uint32_t>(order >> 32), index = kNone - static_cast<uint32_t>(order);
     const bool in = t < size && static_cast<uint32_t>(t) < ask.top_k;
     const double w = in ? r.weight(unordered(key)) : 0.0;
-    const u64 units = in ? units_of(w) : 0;
+    const u64 units = in ? units_of(w, r.one) : 0;
     const u64 upto = scan_of(s, units, n);
     u64 need = 0;
     if (ask.by_p) {
@@ -917,7 +921,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(const SampleArg
             atomicAdd(&s.chunk_ties[i / a.chunk], 1u);
             return;
         }
-        const u64 n = units_of(y);
+        const u64 n = units_of(y, r.one);
         if (n) atomicAdd(&s.chunk_mass[i / a.chunk], n);
     });
     __syncthreads();
@@ -944,7 +948,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(const SampleArg
             const uint32_t key = ordered(v);
             const double y = r.weight(v);
             if (key < kept.key || y < r.min_p || r.bin(v) > st.last) return u64(0);
-            return key > kept.key ? units_of(y) : rank < kept.ties ? tie_units : u64(0);
+            return key > kept.key ? units_of(y, r.one) : rank < kept.ties ? tie_units : u64(0);
         },
         tie, x);
     if (lane == 0) answer(a, row, token, r.share(x, sum));

@@ -34,6 +34,7 @@ struct SampleArgs {
     size_t stride;
     int rows, vocab;
     int chunk, chunks;  // logits of a chunk (a multiple of 256), chunks of a row
+    double one;         // units of mass to the largest weight, a power of two
     const float* uniforms;     // [rows]
     const float* temperature;  // [rows] or null: 1
     const int32_t* top_k;      // [rows] or null: all
@@ -57,6 +58,7 @@ void launch_sample(const SampleArgs& a, hipStream_t s);
 
 struct SamplePlan {
     int rows = 0, vocab = 0, chunk = 0, chunks = 0, room = 0, device = 0;
+    double one = 0;
     DeviceBuffer space;
     PinnedBuffer flag;
     hipStream_t last = nullptr;
