@@ -153,6 +153,10 @@ void ScorePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_
                 at_once = rounds == 1;
             }
         }
+        if (tiles && !kind && per > 4 * kScoreChain) {
+            per = 4 * kScoreChain;
+            at_once = false;
+        }
         std::vector<int4> list;
         std::vector<size_t> load;
         for (Block& b : blocks[kind]) {

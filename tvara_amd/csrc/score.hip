@@ -44,11 +44,11 @@ __global__ __launch_bounds__(64) void score_rows_kernel(const ScoreArgs a) {
         if constexpr (kQ8) return scale_of(head, slot, d / 32) * static_cast<float>(reinterpret_cast<const int8_t*>(at)[d]);
         else return reinterpret_cast<const float*>(at)[d];
     };
-    // A batch of 64 keys is added up by itself and then joins the rest, the normaliser
-    // with what its additions have rounded away.
-    float m = -INFINITY, l = 0.f, rounded = 0.f, acc[kColumns];
+    // A batch of 64 keys is added up by itself and then joins the rest, with what the
+    // additions before have rounded away.
+    float m = -INFINITY, l = 0.f, rounded = 0.f, acc[kColumns], rest[kColumns];
 #pragma unroll
-    for (int i = 0; i < kColumns; ++i) acc[i] = 0.f;
+    for (int i = 0; i < kColumns; ++i) acc[i] = rest[i] = 0.f;
     bool bad = false;
     for (int base = part.z; base < part.w; base += 64) {
         const int key = base + lane;
@@ -119,7 +119,11 @@ __global__ __launch_bounds__(64) void score_rows_kernel(const ScoreArgs a) {
             }
         }
 #pragma unroll
-        for (int i = 0; i < kColumns; ++i) acc[i] = fmaf(acc[i], alpha, sum[i]);
+        for (int i = 0; i < kColumns; ++i) {
+            acc[i] *= alpha;
+            rest[i] *= alpha;
+            add_to(acc[i], rest[i], sum[i]);
+        }
     }
     if (__any(bad) && lane == 0) *a.err = 1;
     const bool whole = run.y == 1;

@@ -42,6 +42,12 @@ void launch_score_merge(const ScoreArgs& a, hipStream_t s);
 // score_tiles.hip (the layouts of tree_tiles_supported): blocks of up to 16
 // attention rows, or of up to kScoreMany
 constexpr int kScoreFew = 16, kScoreMany = 256;
+// Steps of a wave whose parts are added up in a row in f32.  Behind a large one each may be
+// lost, up to half an ulp, while the normaliser keeps them all: 64 are 3.8e-6 of a column at
+// the very worst, 128 7.6e-6, 4,096 2.4e-4.  Runs of few rows end there, of which four waves
+// share the steps, and join with what is rounded away; many rows' sums go to memory (2 x
+// 2,048 rows after 14,336, 32 heads on 8 of 128: 3,810 us, and 3,740 in one chain of 512).
+constexpr int kScoreChain = 64, kScoreManyChain = 128;
 int score_step(const BlockLayout& lay, int block);   // keys of a step
 int score_units(const BlockLayout& lay, int block);  // workgroups of a CU
 void launch_score_tiles(const ScoreArgs& a, int block, int workgroups, hipStream_t s);

@@ -748,6 +748,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
     // the queries' low parts, where registers do not hold them beside 128 columns of output
     constexpr bool kFar = D == 128;
     __shared__ u32x4 qlow[kFar ? kManyWaves : 1][kFar ? NT * KC : 1][64];
+    __shared__ float stored_max[NT][64 * kManyWaves];  // a lane's rows' maxima when their sums last went to memory
     __shared__ int odd_values;   // some value is not finite
     __shared__ int most_query;   // the exponent of the queries' largest element, scaled
     __shared__ int large_keys;   // some key may take a score out of f32
@@ -833,7 +834,10 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
     const size_t vsec = kQ8 ? a.lay.section : static_cast<size_t>(tpb) * kvw * sizeof(float);
     // (past the last key: its block again, whose slots are there whatever they hold)
     const int wkey = __builtin_amdgcn_readfirstlane(skey);  // the wave's first
-    auto lookup = [&](int stp) { return tab[min(KEYS * stp + wkey, tokens - 1) >> tsh]; };
+    // (constant to the compiler too: a scalar load, which waits for no other, though sums are
+    // stored between)
+    const auto ids = reinterpret_cast<__attribute__((address_space(4))) const int32_t*>(reinterpret_cast<uintptr_t>(tab));
+    auto lookup = [&](int stp) { return ids[min(KEYS * stp + wkey, tokens - 1) >> tsh]; };
     const unsigned in_row = kQ8 ? (skey - wkey) * D + col : ((skey - wkey) * kvw + col) * static_cast<unsigned>(sizeof(float));
     const unsigned in_scales = ((skey - wkey) * (D / 32) + col / 32) * 2;
     f32x4 kreg[2], vreg[2];
@@ -1078,14 +1082,51 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
         }
     };
 
-    if (it.step < it.end) {
-        load(it.step, lookup(it.step));
-        int id = lookup(it.step + 1);
+    // The sums to their rows' place (a result, a run's partial), onto those that are there
+    // already from kScoreManyChain steps before; `last`: divided.  A lane its own.
+    auto put = [&](bool again, bool last) __attribute__((always_inline)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const float total = last ? cross_row_sum(l[nt]) : 0.f;
+            int r = 32 * wave + 16 * nt + r16;
+            asm("" : "+v"(r));  // (worked out here, not kept through the loop)
+            const int row = r / it.heads, head = it.head + r - row * it.heads;
+            if (row >= it.rows) continue;
+            const bool whole = it.runs == 1;
+            const size_t at = (whole ? static_cast<size_t>(it.row0) + row
+                                     : static_cast<size_t>(it.slot) + static_cast<size_t>(row) * it.runs + it.run) * a.heads + head;
+            float* o = (whole ? a.out : a.part_acc) + at * D + 4 * g;
+            const float unit = power_of_two(asize[nt] - 2 * kHigh);
+            const float before = again ? fast_exp2(stored_max[nt][tid] - (m[nt] == -INFINITY ? 0.f : m[nt])) : 0.f;
+            float div = 1.f;
+            if (last) {
+                nonfinite = fmaf(total, 0.f, nonfinite);  // (a score that is NaN is in its row's sum)
+                if (whole && total != 0.f) div = total;
+                if (!whole && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(m[nt], total);
+            } else {
+                stored_max[nt][tid] = m[nt];
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                f32x4 x = acc[dt][nt] * unit;
+                if (again) x += *reinterpret_cast<const f32x4*>(o + 16 * dt) * before;
+                *reinterpret_cast<f32x4*>(o + 16 * dt) = last ? x / div : x;
+                acc[dt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+            asize[nt] = -97;
+        }
+    };
+
+    int step = it.step, buf = 0, id = 0;
+    if (step < it.end) {
+        load(step, lookup(step));
+        id = lookup(step + 1);
         __syncthreads();
         stage(0);
         __syncthreads();
-        int buf = 0;
-        for (int step = it.step; step < it.end; ++step, buf ^= 1) {
+    }
+    for (bool again = false;; again = true) {
+        for (const int until = min(it.end, step + kScoreManyChain); step < until; ++step, buf ^= 1) {
             scores(buf);
             load(step + 1, id);
             id = lookup(step + 2);
@@ -1093,23 +1134,8 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
             stage(buf ^ 1);
             __syncthreads();
         }
-    }
-    // (a score that is NaN is in its row's sum)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const float total = cross_row_sum(l[nt]);
-        int head;
-        const int row = row_of(nt, head);
-        if (row >= it.rows) continue;
-        nonfinite = fmaf(total, 0.f, nonfinite);
-        const bool whole = it.runs == 1;
-        const size_t at = (whole ? static_cast<size_t>(it.row0) + row
-                                 : static_cast<size_t>(it.slot) + static_cast<size_t>(row) * it.runs + it.run) * a.heads + head;
-        float* o = (whole ? a.out : a.part_acc) + at * D + 4 * g;
-        const float unit = power_of_two(asize[nt] - 2 * kHigh), div = whole && total != 0.f ? total : 1.f;
-        if (!whole && g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(m[nt], total);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(o + 16 * dt) = acc[dt][nt] * unit / div;
+        put(again, step >= it.end);
+        if (step >= it.end) break;
     }
     if (nonfinite != 0.f) *a.err = 1;
     if (it.step >= it.end || !odd_values) return;
