@@ -423,6 +423,10 @@ void DeviceModel::sample_many(const uint64_t* sequences, const uint32_t* tokens,
         sample_host_.release(s);
         sampler_->check();  // (waits for the stream)
     } catch (...) {
+        try {
+            sampler_->check();  // draws that are on their way end, and what they found with them
+        } catch (const std::exception&) {
+        }
         for (size_t i = 0; i < std::min(done + 1, n); ++i) cache_->truncate(sequences[i], positions[i]);
         throw;
     }
