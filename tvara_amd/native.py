@@ -18,6 +18,7 @@ from pathlib import Path
 import numpy as np
 
 from . import _capi
+from .sampling import f32_below_one
 
 
 class NativeModel:
@@ -180,7 +181,7 @@ class NativeModel:
         given = np.asarray(top_k)
         if given.dtype.kind not in "iu" or (given < 0).any() or (given > 2**31 - 1).any():
             raise ValueError("top_k is a whole number from 0")
-        u, t, p, m = (each(x, np.float32) for x in (uniforms, temperature, top_p, min_p))
+        u, t, p, m = (each(x, np.float32) for x in (f32_below_one(uniforms), temperature, top_p, min_p))
         k = each(given, np.int32)
         after, chances = np.zeros(seqs.size, np.uint32), np.zeros(seqs.size, np.float32)
 

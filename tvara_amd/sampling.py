@@ -14,6 +14,14 @@ from . import _capi
 from ._capi import InvalidArgument
 
 
+def f32_below_one(uniforms):
+    """Random numbers in f32: those below 1 in a wider type, the last 2^-25 before it
+    too, stay below 1."""
+    given = np.asarray(uniforms)
+    u = given.astype(np.float32)
+    return np.where((u == 1) & (given < 1), np.nextafter(np.float32(1), np.float32(0)), u)
+
+
 class SamplePlan:
     """Workspace for up to ``rows`` rows of ``vocab`` logits."""
 
@@ -67,9 +75,9 @@ def sample_batch(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
 
     if np.shape(uniforms) != (n,):
         raise InvalidArgument("one random number for each row")
-    given = [each(x, t, what) for x, t, what in ((uniforms, np.float32, "random number"), (temperature, np.float32, "temperature"),
-                                                 (top_k, np.int32, "top_k"), (top_p, np.float32, "top_p"),
-                                                 (min_p, np.float32, "min_p"))]
+    given = [each(x, t, what) for x, t, what in ((f32_below_one(uniforms), np.float32, "random number"),
+                                                 (temperature, np.float32, "temperature"), (top_k, np.int32, "top_k"),
+                                                 (top_p, np.float32, "top_p"), (min_p, np.float32, "min_p"))]
     x, *given = (hip.DeviceArray.from_numpy(a) for a in (logits, *given))
     tokens, chances = hip.DeviceArray((n,), np.uint32), hip.DeviceArray((n,), np.float32)
     plan = SamplePlan(n, vocab)
