@@ -496,11 +496,22 @@ TVARA_API int tvara_attn_tree(tvara_kv_cache* cache, const uint64_t* sequences, 
  * and zeros where a row sees no key.  The rows' own tokens are in the cache
  * (tvara_slot_plan_rotate, _write, or appends put them there).  first NULL: 0, end
  * NULL: p + 1; with both, windows, prefixes that see all of themselves, and packed
- * documents are ranges.  scale 0: 1 / sqrt(head_dim); slopes NULL: none.  f32
- * arithmetic, or products of as many bits; any layout (fast: head_dim 64 or 128,
- * blocks of a power of two from 16 tokens).  What a row does not see never reaches
- * it, whatever it holds; a value that is not finite makes its column of the rows that
- * see it not finite.  The reference has causal attention alone (attention.hpp:57-89).
+ * documents are ranges.  scale 0: 1 / sqrt(head_dim); slopes NULL: none.  Any layout
+ * (fast: head_dim 64 or 128, blocks of a power of two from 16 tokens).  What a row does
+ * not see never reaches it, whatever it holds; a value that is not finite makes its
+ * column of the rows that see it not finite.  The reference has causal attention alone
+ * (attention.hpp:57-89).
+ *
+ * Arithmetic is f32, products of Q8_0 bytes with 24 bits likewise.  Of the fast layouts
+ * the chunks of many rows (more than some 100 rows times query heads of a KV head) hold
+ * queries, keys, values, and weights times their values' largest element, as two fp16
+ * parts: each element to 2^-23 of itself or 2^-39 of its row's largest (a weight: of the
+ * largest one so far), whichever is more, and a product to 2^-21.  In rows of ordinary
+ * numbers that is as near as f32's sums are; beside an element 2^20 times the others
+ * these are off by 2^-19, and what is 2^39 times smaller is lost, where f32 has no such
+ * limit.  The calls whose names end in _f32 take f32 (24 bits) for every row and are
+ * slower over long chunks: 2 x 2,048 rows after 2,048, 32 heads on 8 of 128, 2,030 us in
+ * place of 790, over Q8_0 blocks 1,190 in place of 800.
  *
  * Launching fails with TVARA_INVALID once the cache has changed.  rows * heads *
  * head_dim stays below 2^32 in all, the rows below 2^24. */
@@ -508,6 +519,10 @@ TVARA_API tvara_score_plan* tvara_score_plan_create(tvara_kv_cache* cache, const
                                                     size_t heads, size_t context, const size_t* start,
                                                     const size_t* rows, const size_t* first, const size_t* end,
                                                     float scale, float cap, const float* slopes);
+TVARA_API tvara_score_plan* tvara_score_plan_create_f32(tvara_kv_cache* cache, const uint64_t* sequences, size_t count,
+                                                        size_t heads, size_t context, const size_t* start,
+                                                        const size_t* rows, const size_t* first, const size_t* end,
+                                                        float scale, float cap, const float* slopes);
 /* q and out f32 [sum rows][heads * head_dim], device pointers, asynchronous on
  * `stream` (NULL: the cache's).  Launches of one plan share its workspace: they run
  * one after the other, on one stream or in the caller's order, captured ones too (on
@@ -522,6 +537,10 @@ TVARA_API int tvara_attn_score(tvara_kv_cache* cache, const uint64_t* sequences,
                                size_t context, const size_t* start, const size_t* rows, const size_t* first,
                                const size_t* end, float scale, float cap, const float* slopes, const float* q, float* out,
                                int device_ptrs);
+TVARA_API int tvara_attn_score_f32(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, size_t layer,
+                                   size_t heads, size_t context, const size_t* start, const size_t* rows,
+                                   const size_t* first, const size_t* end, float scale, float cap, const float* slopes,
+                                   const float* q, float* out, int device_ptrs);
 
 /* ---------------------------------------------------------------- sampling
  *

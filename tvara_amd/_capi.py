@@ -128,11 +128,15 @@ SIGNATURES = {
     "tvara_sample_plan_destroy": (None, [_vp]),
     "tvara_score_plan_create": (_vp, [_vp, C.POINTER(_u64), _sz, _sz, _sz, C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz),
                                       C.POINTER(_sz), C.c_float, C.c_float, _fp]),
+    "tvara_score_plan_create_f32": (_vp, [_vp, C.POINTER(_u64), _sz, _sz, _sz, C.POINTER(_sz), C.POINTER(_sz),
+                                          C.POINTER(_sz), C.POINTER(_sz), C.c_float, C.c_float, _fp]),
     "tvara_score_plan_launch": (C.c_int, [_vp, _sz, _vp, _vp, _vp]),
     "tvara_score_plan_check": (C.c_int, [_vp]),
     "tvara_score_plan_destroy": (None, [_vp]),
     "tvara_attn_score": (C.c_int, [_vp, C.POINTER(_u64), _sz, _sz, _sz, _sz, C.POINTER(_sz), C.POINTER(_sz),
                                    C.POINTER(_sz), C.POINTER(_sz), C.c_float, C.c_float, _fp, _fp, _fp, C.c_int]),
+    "tvara_attn_score_f32": (C.c_int, [_vp, C.POINTER(_u64), _sz, _sz, _sz, _sz, C.POINTER(_sz), C.POINTER(_sz),
+                                       C.POINTER(_sz), C.POINTER(_sz), C.c_float, C.c_float, _fp, _fp, _fp, C.c_int]),
     "tvara_slot_plan_create": (_vp, [_vp, C.POINTER(_u64), _sz]),
     "tvara_slot_plan_build": (C.c_int, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _vp]),
     "tvara_slot_plan_write": (C.c_int, [_vp, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp]),

@@ -305,16 +305,24 @@ def _scored(seqs, starts, counts, heads, first, end, slopes):
                         _ptr(slopes))
 
 
+def _score_call(lib, name, precision):
+    """A call of scored attention: f32x3 (long chunks by fp16 parts) or f32 throughout."""
+    if precision not in ("f32", "f32x3"):
+        raise InvalidArgument("scored attention is f32x3 or f32")
+    return getattr(lib, name + ("_f32" if precision == "f32" else ""))
+
+
 def score_batch(cache, q, seqs, starts, counts, layer, heads, context, first=None, end=None, scale=None, cap=0.0,
-                slopes=None):
+                slopes=None, precision="f32x3"):
     """Scored attention (tvara_attn_score) of the cached rows starts[i] ..
     starts[i] + counts[i] - 1 of seqs[i], packed: q [rows, heads * head_dim]."""
+    call = _score_call(cache.lib, "tvara_attn_score", precision)
     rows, keep, (sp, st, ct, fp, ep, bp) = _scored(seqs, starts, counts, heads, first, end, slopes)
     hidden = heads * cache.head_dim
     q = _f32(q).reshape(rows, hidden)
     out = np.empty((max(rows, 1), hidden), np.float32)
-    _capi.check(cache.lib.tvara_attn_score(cache.h, sp, keep[0].size, layer, heads, context, st, ct, fp, ep, scale or 0.0,
-                                           cap, bp, _ptr(q), _ptr(out), 0))
+    _capi.check(call(cache.h, sp, keep[0].size, layer, heads, context, st, ct, fp, ep, scale or 0.0, cap, bp, _ptr(q),
+                     _ptr(out), 0))
     return out[:rows]
 
 
@@ -322,14 +330,17 @@ class ScorePlan:
     """Resident rows of scored attention over cached sequences
     (tvara_score_plan_*): scores are scale * q.k, capped as cap * tanh(s / cap)
     where cap is above 0, less slopes[head] times the distance of key and row;
-    row r sees the keys first[r] .. end[r] - 1 (None: from 0, to itself)."""
+    row r sees the keys first[r] .. end[r] - 1 (None: from 0, to itself).  precision
+    f32x3: chunks of many rows by fp16 parts, whose range tvara_capi.h states; f32:
+    f32 products for all rows."""
 
-    def __init__(self, cache, seqs, starts, counts, heads, context, first=None, end=None, scale=None, cap=0.0, slopes=None):
+    def __init__(self, cache, seqs, starts, counts, heads, context, first=None, end=None, scale=None, cap=0.0, slopes=None,
+                 precision="f32x3"):
+        create = _score_call(cache.lib, "tvara_score_plan_create", precision)
         self.cache = cache
         self.lib = cache.lib
         self.rows, keep, (sp, st, ct, fp, ep, bp) = _scored(seqs, starts, counts, heads, first, end, slopes)
-        self.h = self.lib.tvara_score_plan_create(cache.h, sp, keep[0].size, heads, context, st, ct, fp, ep, scale or 0.0, cap,
-                                                  bp)
+        self.h = create(cache.h, sp, keep[0].size, heads, context, st, ct, fp, ep, scale or 0.0, cap, bp)
         if not self.h:
             _capi.raise_last()
 

@@ -598,18 +598,31 @@ void tvara_slot_plan_destroy(tvara_slot_plan* plan) { delete plan; }
 
 // ------------------------------------------------------- scored attention
 
-tvara_score_plan* tvara_score_plan_create(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, size_t heads,
-                                          size_t context, const size_t* start, const size_t* rows, const size_t* first,
-                                          const size_t* end, float scale, float cap, const float* slopes) {
+static tvara_score_plan* score_plan(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, size_t heads,
+                                    size_t context, const size_t* start, const size_t* rows, const size_t* first,
+                                    const size_t* end, float scale, float cap, const float* slopes, bool parts) {
     tvara_score_plan* out = nullptr;
     guard([&] {
         auto& c = live(cache);
         tvara_amd::check_attention_config(c, heads, context);
         auto p = std::make_unique<tvara_score_plan>();
-        p->plan.build(&c, sequences, count, heads, context, start, rows, first, end, scale, cap, slopes);
+        p->plan.build(&c, sequences, count, heads, context, start, rows, first, end, scale, cap, slopes, parts);
         out = p.release();
     });
     return out;
+}
+
+tvara_score_plan* tvara_score_plan_create(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, size_t heads,
+                                          size_t context, const size_t* start, const size_t* rows, const size_t* first,
+                                          const size_t* end, float scale, float cap, const float* slopes) {
+    return score_plan(cache, sequences, count, heads, context, start, rows, first, end, scale, cap, slopes, true);
+}
+
+tvara_score_plan* tvara_score_plan_create_f32(tvara_kv_cache* cache, const uint64_t* sequences, size_t count,
+                                              size_t heads, size_t context, const size_t* start, const size_t* rows,
+                                              const size_t* first, const size_t* end, float scale, float cap,
+                                              const float* slopes) {
+    return score_plan(cache, sequences, count, heads, context, start, rows, first, end, scale, cap, slopes, false);
 }
 
 int tvara_score_plan_launch(tvara_score_plan* plan, size_t layer, const float* q, float* out, void* stream) {
@@ -633,16 +646,16 @@ int tvara_score_plan_check(tvara_score_plan* plan) {
 
 void tvara_score_plan_destroy(tvara_score_plan* plan) { delete plan; }
 
-int tvara_attn_score(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, size_t layer, size_t heads,
-                     size_t context, const size_t* start, const size_t* rows, const size_t* first, const size_t* end,
-                     float scale, float cap, const float* slopes, const float* q, float* out, int device_ptrs) {
+static int attn_score(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, size_t layer, size_t heads,
+                      size_t context, const size_t* start, const size_t* rows, const size_t* first, const size_t* end,
+                      float scale, float cap, const float* slopes, const float* q, float* out, int device_ptrs, bool parts) {
     return guard([&] {
         auto& c = live(cache);
         tvara_amd::check_attention_config(c, heads, context);
         if (!count) return;
         if (layer >= c.geometry().layers) throw std::invalid_argument("invalid fused attention shape");
         tvara_amd::ScorePlan plan;
-        plan.build(&c, sequences, count, heads, context, start, rows, first, end, scale, cap, slopes);
+        plan.build(&c, sequences, count, heads, context, start, rows, first, end, scale, cap, slopes, parts);
         if (!plan.rows) return;
         if (!q || !out) throw std::invalid_argument("invalid fused attention shape");
         hipStream_t s = c.stream();
@@ -666,6 +679,20 @@ int tvara_attn_score(tvara_kv_cache* cache, const uint64_t* sequences, size_t co
         plan.check();
         copier.parallel_copy(reinterpret_cast<char*>(out), reinterpret_cast<const char*>(back), n * sizeof(float));
     });
+}
+
+int tvara_attn_score(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, size_t layer, size_t heads,
+                     size_t context, const size_t* start, const size_t* rows, const size_t* first, const size_t* end,
+                     float scale, float cap, const float* slopes, const float* q, float* out, int device_ptrs) {
+    return attn_score(cache, sequences, count, layer, heads, context, start, rows, first, end, scale, cap, slopes, q, out,
+                      device_ptrs, true);
+}
+
+int tvara_attn_score_f32(tvara_kv_cache* cache, const uint64_t* sequences, size_t count, size_t layer, size_t heads,
+                         size_t context, const size_t* start, const size_t* rows, const size_t* first, const size_t* end,
+                         float scale, float cap, const float* slopes, const float* q, float* out, int device_ptrs) {
+    return attn_score(cache, sequences, count, layer, heads, context, start, rows, first, end, scale, cap, slopes, q, out,
+                      device_ptrs, false);
 }
 
 // --------------------------------------------------------------- sampling

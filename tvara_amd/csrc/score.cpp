@@ -32,7 +32,7 @@ struct Block {
 
 void ScorePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t h, size_t context, const size_t* start,
                       const size_t* counts, const size_t* first, const size_t* end, float scale, float limit,
-                      const float* slopes) {
+                      const float* slopes, bool parts_too) {
     cache = c;
     const Geometry& g = c->geometry();
     c->check_device();
@@ -87,12 +87,13 @@ void ScorePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_
             ranges[row0 + j] = lo < hi ? make_int2(static_cast<int>(lo), static_cast<int>(hi)) : make_int2(0, 0);
         }
         seqs[i] = make_int4(offset[sequences[i]], static_cast<int>(t.length), static_cast<int>(counts[i]), static_cast<int>(row0));
-        // Blocks of many rows share a key's parts among them and pay for padding and
+        // Blocks of many rows, whose products are of fp16 parts, are for plans that allow
+        // these.  They share a key's parts among them and pay for padding and
         // splitting with few: eight contexts of 2,000, 32 heads on 8, attention rows a KV
         // head, few against many (f32, us): head_dim 64 96 rows 51 and 57, 128 69 and 61;
         // head_dim 128 64 rows 58 and 82, 96 90 and 85; (Q8_0) 64 128 rows 52 and 61, 256 78
         // and 63; 128 128 rows 79 and 90, 256 123 and 93.
-        const int kind = tiles && counts[i] * per_block > (lay.format == kQ8 ? 160 : 96) ? 1 : 0;
+        const int kind = tiles && parts_too && counts[i] * per_block > (lay.format == kQ8 ? 160 : 96) ? 1 : 0;
         const size_t high = tiles ? (kind ? kScoreMany : kScoreFew) / per_block : 1;
         for (size_t j = 0; j < counts[i]; j += high) {
             Block b{static_cast<int>(i), static_cast<int>(row0 + j), static_cast<int>(std::min(high, counts[i] - j)),

@@ -64,7 +64,8 @@ struct ScorePlan {
     size_t tables_at = 0, ranges_at = 0, runs_at = 0, slopes_at = 0, few_at = 0, many_at = 0, acc_at = 0, ml_at = 0;
 
     void build(DeviceCache* c, const uint64_t* sequences, size_t n, size_t heads, size_t context, const size_t* start,
-               const size_t* rows, const size_t* first, const size_t* end, float scale, float cap, const float* slopes);
+               const size_t* rows, const size_t* first, const size_t* end, float scale, float cap, const float* slopes,
+               bool parts);  // whether long chunks' products may be of fp16 parts (score_tiles.hip)
     void launch(int layer, const float* q, float* out, hipStream_t s);
     void check();
 };
