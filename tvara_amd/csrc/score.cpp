@@ -15,6 +15,8 @@ constexpr size_t kIntMax = static_cast<size_t>(std::numeric_limits<int32_t>::max
 constexpr size_t kMaxThreads = std::numeric_limits<uint32_t>::max(), kMaxWorkgroups = kMaxThreads / 512;
 // keys of a run of the row kernel, at least
 constexpr size_t kRowRun = 64;
+// the largest bias of a score, in log2 units, with room for the score in f32
+constexpr float kMaxBias = 8.5e37f;
 // rounds of workgroups that runs are cut for; what a run of few and of many rows costs
 // beside its steps, in steps (many: six prompts of 3 to 700 rows behind up to 2,500 keys, 32
 // heads of 64: 134 us at 2, whose runs are shorter and want merging, 130 at 8 and at 24)
@@ -70,12 +72,13 @@ void ScorePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_
     std::vector<int4> seqs(n);
     std::vector<Block> blocks[2];  // of few rows (or the row kernel's), of many
     const int step[2] = {tiles ? score_step(lay, kScoreFew) : 1, tiles ? score_step(lay, kScoreMany) : 1};
-    size_t row0 = 0;
+    size_t row0 = 0, longest = 0;
     for (size_t i = 0; i < n; ++i) {
         const Table& t = c->sequence(sequences[i]);
         if (t.length > kIntMax / 2) throw std::invalid_argument("sequence too long for the device kernels");
         if (t.length > context || start[i] > t.length || counts[i] > t.length - start[i])
             throw std::invalid_argument("invalid fused attention shape");
+        longest = std::max(longest, t.length);
         if (!offset.count(sequences[i])) {
             offset[sequences[i]] = static_cast<int32_t>(tab.size());
             for (const Handle& b : t.blocks) tab.push_back(static_cast<int32_t>(b.id));
@@ -109,6 +112,9 @@ void ScorePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_
         row0 += counts[i];
     }
     epoch = c->epoch();
+    // (a bias that is infinite would take a key that a row sees from it, or be all that it has)
+    for (const float b : bias)
+        if (std::fabs(b) * static_cast<float>(longest) > kMaxBias) throw std::invalid_argument("invalid score slope");
 
     // Runs of steps, as many as give every CU its workgroups.
     slots = 0;

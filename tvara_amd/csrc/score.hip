@@ -125,6 +125,7 @@ __global__ __launch_bounds__(64) void score_rows_kernel(const ScoreArgs a) {
             add_to(acc[i], rest[i], sum[i]);
         }
     }
+    bad |= !__builtin_isfinite(l);  // (a score and its bias may be finite and their sum not)
     if (__any(bad) && lane == 0) *a.err = 1;
     const bool whole = run.y == 1;
     const size_t at = (whole ? row : static_cast<size_t>(run.z) + run.x) * a.heads + h;

@@ -334,10 +334,11 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void score_tile_kernel(const Sco
         load_v(next);
     }
     wait_until_left<0>();  // (LDS is used again)
-    if (__any(nonfinite != 0.f) && lane == 0) *a.err = 1;
 
     // ---- the waves that shared these rows' keys, together
     float total = cross_row_sum(l);
+    nonfinite = fmaf(total, 0.f, nonfinite);  // (a score and its bias may be finite and their sum not)
+    if (__any(nonfinite != 0.f) && lane == 0) *a.err = 1;
     if (g == 0) stats[wave][r16] = make_float2(m, total);
     __syncthreads();
     {
@@ -639,10 +640,11 @@ __global__ __launch_bounds__(64 * kFewWaves, 3) void score_tile_q8_kernel(const 
         if (another) load(1, step + WK);
     }
     wait_until_left<0>();  // (LDS is used again)
-    if (__any(nonfinite != 0.f) && lane == 0) *a.err = 1;
 
     // ---- the waves that shared these rows' keys, together
     float total = cross_row_sum(l);
+    nonfinite = fmaf(total, 0.f, nonfinite);  // (a score and its bias may be finite and their sum not)
+    if (__any(nonfinite != 0.f) && lane == 0) *a.err = 1;
     if (g == 0) stats[wave][r16] = make_float2(m, total);
     __syncthreads();
     {
