@@ -753,7 +753,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
     __shared__ float stored_max[NT][64 * kManyWaves];  // a lane's rows' maxima when their sums last went to memory
     __shared__ int odd_values;   // some value is not finite
     __shared__ int most_query;   // the exponent of the queries' largest element, scaled
-    __shared__ int large_keys;   // some key may take a score out of f32
+    __shared__ int large_keys;   // some score may be 2^17 or more, or leave f32
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, r16 = lane & 15;
     const Item it = item_of(a, blockIdx.x);
@@ -815,7 +815,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
         const int size = exponent_of(cross_row_max(most));
         const float up = power_of_two(kHigh - size);
         qsize[nt] = fmaxf(power_of_two(size - kHigh) * a.qscale, 1.17549435e-38f);
-        atomicMax(&most_query, size + exponent_of(a.qscale) + 1);
+        atomicMax(&most_query, size + exponent_of(fmaxf(a.qscale, a.qscale * a.cap)) + 1);  // (before a cap, and behind it)
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
             const Parts p = split8(x[kc][0] * up, x[kc][1] * up);
@@ -890,7 +890,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
         kmost = row_max<LPR>(kmost);
         vmost = row_max<LPR>(vmost);
         const int ksize = exponent_of(kmost), size = exponent_of(vmost);
-        if (ksize + most_query >= 110) large_keys = 1;
+        if (ksize + most_query >= 16) large_keys = 1;
         if (tid % LPR == 0) {
             kscale[buf][skey] = power_of_two(ksize - kHigh);
             vscale[buf][skey] = power_of_two(size);
@@ -958,6 +958,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
     auto output = [&](int buf, int stp) __attribute__((always_inline)) {
         const int key0 = KEYS * stp;
         const bool whole = key0 >= all_lo && key0 + KEYS <= all_hi;
+        const bool large = __builtin_amdgcn_readfirstlane(large_keys);
         float alpha[NT];
         Parts p[NT][MT / 2];
 #pragma unroll
@@ -967,7 +968,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
             float by = qsize[nt];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) s[mt][nt] *= *reinterpret_cast<const f32x4*>(&kscale[buf][16 * mt + 4 * g]);
-            if (large_keys) {
+            if (large) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -994,6 +995,13 @@ __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const Sco
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[mt][nt][i] = any_tanh(s[mt][nt][i]);
                 }
+            }
+            if (large) {
+                // (the maximum below is a rounded one: its product with `by` inside an
+                // exponential's argument would be off by half an ulp of the score)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s[mt][nt] *= by;
+                by = 1.f;
             }
             if (a.slopes) {
                 const int away = position[nt] - key0 - 4 * g;
