@@ -496,7 +496,8 @@ TVARA_API int tvara_attn_tree(tvara_kv_cache* cache, const uint64_t* sequences, 
  * and zeros where a row sees no key.  The rows' own tokens are in the cache
  * (tvara_slot_plan_rotate, _write, or appends put them there).  first NULL: 0, end
  * NULL: p + 1; with both, windows, prefixes that see all of themselves, and packed
- * documents are ranges.  scale 0: 1 / sqrt(head_dim); slopes NULL: none, of either sign
+ * documents are ranges.  scale 0: 1 / sqrt(head_dim); a cap of 2^64 or more is none (a
+ * score of up to 2^52 is the same to f32's last bit); slopes NULL: none, of either sign
  * up to 5.8e37 over the longest sequence's length.  Any layout
  * (fast: head_dim 64 or 128, blocks of a power of two from 16 tokens).  What a row does
  * not see never reaches it, whatever it holds; a value that is not finite makes its

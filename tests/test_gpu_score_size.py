@@ -37,3 +37,13 @@ def test_large_scores(device, oracle, dim, count, power, cap):
     # the others' weights are e^-(2^power / 12) of the largest, 5e-10 at 2^8 and nothing beyond, or
     # 1: values, weights and sums are off by 2^-21 and 2^-19 of what is added up at the most
     assert np.allclose(got, want, rtol=2.0 ** -21, atol=4e-6)
+
+
+@pytest.mark.parametrize("cap", [1e18, 1e20, 1e30, 1e35, 2e38])
+@pytest.mark.parametrize("fmt", ["f32", "q8_0"])
+@pytest.mark.parametrize("dim,count", [(64, 1), (128, 1), (64, 170), (128, 170), (96, 3)])
+def test_large_caps(device, oracle, dim, count, fmt, cap):
+    """Caps far above every score change none: the bars are those without a cap."""
+    ts.say("score, large caps", dim, count, fmt, cap)
+    b = ts.Batch(device, oracle, 2, 1, dim, [200], [count], q8=fmt == "q8_0")
+    b.agree(b.run(cap=cap))

@@ -15,6 +15,8 @@ constexpr size_t kIntMax = static_cast<size_t>(std::numeric_limits<int32_t>::max
 constexpr size_t kMaxThreads = std::numeric_limits<uint32_t>::max(), kMaxWorkgroups = kMaxThreads / 512;
 // keys of a run of the row kernel, at least
 constexpr size_t kRowRun = 64;
+// caps that are none
+constexpr float kNoCap = 18446744073709551616.f;  // 2^64
 // the largest bias of a score, in log2 units, with room for the score in f32
 constexpr float kMaxBias = 8.5e37f;
 // rounds of workgroups that runs are cut for; what a run of few and of many rows costs
@@ -42,6 +44,9 @@ void ScorePlan::build(DeviceCache* c, const uint64_t* sequences, size_t n, size_
     if (h > 65535) throw std::invalid_argument("invalid fused attention shape");  // (a grid's second dimension)
     if (!scale) scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(g.head_dim)));
     constexpr double kLog2e = 1.4426950408889634;
+    // (of scores up to 2^52 such a cap changes nothing that f32 holds, and scale / cap would
+    // leave the numbers that operands in parts hold: fp16's and bf16's)
+    if (limit >= kNoCap && std::isfinite(static_cast<float>(limit * kLog2e))) limit = 0;
     qscale = static_cast<float>(limit ? static_cast<double>(scale) / limit : scale * kLog2e);
     cap = static_cast<float>(limit * kLog2e);
     if (!(scale > 0) || !(limit >= 0) || !std::isfinite(qscale) || !(qscale > 0) || !std::isfinite(cap))
