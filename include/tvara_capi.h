@@ -508,7 +508,7 @@ TVARA_API int tvara_attn_tree(tvara_kv_cache* cache, const uint64_t* sequences, 
  * the chunks of many rows (more than some 100 rows times query heads of a KV head) hold
  * queries, keys, values, and weights times their values' largest element, as two fp16
  * parts: each element to 2^-23 of itself or 2^-39 of its row's largest (a weight: of the
- * largest one so far), whichever is more, and a product to 2^-21.  In rows of ordinary
+ * largest one so far; 2^-136 where that is less), whichever is more, and a product to 2^-21.  In rows of ordinary
  * numbers that is as near as f32's sums are; beside an element 2^20 times the others
  * these are off by 2^-19, and what is 2^39 times smaller is lost, where f32 has no such
  * limit.  The calls whose names end in _f32 take f32 (24 bits) for every row and are
@@ -608,7 +608,8 @@ TVARA_API int tvara_slot_plan_write(tvara_slot_plan* plan, const int64_t* slots,
  *   y = x * weight / sqrt(mean x^2 + eps)            where q_norm / k_norm are given
  *   (y_a, y_b) -> (y_a cos t - y_b sin t, y_a sin t + y_b cos t),  t = positions[i] * freqs[j]
  * for the pairs j of its first `rotary` columns: columns 2j and 2j + 1 where
- * interleaved, else j and j + rotary / 2; computed in f64, rounded once.  Token i's rows
+ * interleaved, else j and j + rotary / 2; computed in f64 (angles up to 2^52), rounded
+ * once.  Token i's rows
  * are at q + i * q_stride (heads * head_dim floats; 0: packed) and keys, values + i *
  * kv_stride (kv_width; 0: packed), such as the parts of a fused product.  Queries go to
  * q_out [n][heads * head_dim]; keys and values into slots[i] of `layer`, f32 as they are

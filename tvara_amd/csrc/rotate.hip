@@ -100,8 +100,9 @@ __device__ __forceinline__ void put_eight(char* section, const BlockLayout& lay,
 
 // Head sizes of eight columns times a power of two: a lane has eight columns, whole
 // pairs of them.  Bound: HBM (4,000 tokens, 32 heads on 8 of 128, with norms: 41 us for 197 MB,
-// 4.8 TB/s); a launch where tokens are few (one: 3 us).  grid.x: token, grid.y: a share of its heads (of queries, then keys,
-// then values).
+// 4.8 TB/s; 32 us over the same rows again and again, out of the last-level cache); a launch
+// where tokens are few (one: 3 us).  grid.x: token, grid.y: a share of its heads (of queries,
+// then keys, then values).
 template <bool kQ8>
 __global__ __launch_bounds__(kThreads) void rotate_kernel(const RotateArgs a, int turns) {
     __shared__ Turn angles[kMaxDim / 2];
@@ -301,8 +302,9 @@ void launch_rotate(const RotateArgs& a, hipStream_t s) {
     if (wide) {
         const int each = kThreads / (D / 8), shares = (units + each - 1) / each;
         // all of a token's heads in one workgroup, which takes their angles once, where
-        // tokens are many (32 heads on 8 of 128, us with all heads and with a share: 256 tokens
-        // 5.3 and 4.9, 1,024 9.3 and 10.1, 4,096 27.6 and 28.7)
+        // tokens are many (32 heads on 8 of 128, over the same rows again and again, which the
+        // last-level cache holds, us with all heads and with a share: 256 tokens 5.3 and 4.9,
+        // 1,024 9.3 and 10.1, 4,096 27.6 and 28.7)
         const int turns = a.n >= 1024 ? shares : 1;
         launch("rotate", q8 ? rotate_kernel<true> : rotate_kernel<false>,
                dim3(static_cast<unsigned>(a.n), static_cast<unsigned>((shares + turns - 1) / turns)), dim3(kThreads), 0, s, a, turns);

@@ -963,7 +963,9 @@ void launch_sample(const SampleArgs& a, hipStream_t s) {
     launch("sample_chunks", wide ? sample_chunks_kernel<true> : sample_chunks_kernel<false>, dim3((groups + 3) / 4, rows), dim3(256), 0, s, a);
     // as many workgroups a row as give every CU one, of a turn for each wave at the least
     // (128,256 logits, all launches, us, for 128, 256, 512 and 1,024 workgroups in all: 32 rows
-    // of all kinds 82, 66, 66 and 74; 256 rows with top-p 216, 216, 229 and 264)
+    // of all kinds 82, 66, 66 and 74; 256 rows with top-p 216, 216, 229 and 264; a CU holds one
+    // at a time, for its 90,272 bytes of LDS and 1,024 threads of 74 to 128 registers, so that
+    // more than 256 wait for each other)
     const unsigned shares = std::clamp(256 / rows, 1u, (static_cast<unsigned>(a.chunks) + kWaves - 1) / kWaves);
     launch("sample_gather", wide ? sample_gather_kernel<true> : sample_gather_kernel<false>, dim3(shares, rows), dim3(kThreads), 0, s, a);
     if (a.bin_mass)

@@ -734,9 +734,10 @@ constexpr int kHigh = 14;  // the exponent of a row's largest element in parts
 // staged), which the scores, and the probabilities before their own parts, are multiplied
 // by again.  All waves load and split a step's keys and values once, into the other of two
 // buffers in LDS; one barrier a step.  Bound: the vector instructions of the softmax and of
-// the probabilities' split beside the products, with two waves a SIMD (256 registers): 2 x
-// 2,048 rows after 2,048, 32 heads on 8 of 128, capped (206 GFLOP): 780 us, 264 TFLOP/s, 1.7
-// times what f32's products reach at their best, and 1,727 us with six products of bf16 parts.
+// the probabilities' split beside the products, with two waves a SIMD (256 registers, and of
+// 128 columns 10 to 16 more in scratch memory, of which a step reads one): 2 x 2,048 rows
+// after 2,048, 32 heads on 8 of 128, capped (206 GFLOP): 793 us, 260 TFLOP/s, 1.7 times what
+// f32's products reach at their best, and 1,727 us with six products of bf16 parts.
 template <int D, bool kQ8>
 __global__ __launch_bounds__(64 * kManyWaves) void score_shared_kernel(const ScoreArgs a) {
     constexpr int NT = 2, KC = D / 32, DT = D / 16;
