@@ -498,22 +498,22 @@ TVARA_API int tvara_attn_tree(tvara_kv_cache* cache, const uint64_t* sequences, 
  * NULL: p + 1; with both, windows, prefixes that see all of themselves, and packed
  * documents are ranges.  scale 0: 1 / sqrt(head_dim); a cap of 2^64 or more is none (a
  * score of up to 2^52 is the same to f32's last bit); slopes NULL: none, of either sign
- * up to 5.8e37 over the longest sequence's length.  Any layout
- * (fast: head_dim 64 or 128, blocks of a power of two from 16 tokens).  What a row does
- * not see never reaches it, whatever it holds; a value that is not finite makes its
- * column of the rows that see it not finite.  The reference has causal attention alone
- * (attention.hpp:57-89).
+ * up to 5.8e37 over the longest sequence's length.  Any layout (fast: head_dim 64 or 128,
+ * blocks of a power of two from 16 tokens).  What a row does not see never reaches it,
+ * whatever it holds; a value that is not finite makes its column of the rows that see it
+ * not finite, and so may values from 1e30 on, whose weighted sums leave f32 before they
+ * are divided.  The reference has causal attention alone (attention.hpp:57-89).
  *
  * Arithmetic is f32, products of Q8_0 bytes with 24 bits likewise.  Of the fast layouts
  * the chunks of many rows (more than some 100 rows times query heads of a KV head) hold
  * queries, keys, values, and weights times their values' largest element, as two fp16
  * parts: each element to 2^-23 of itself or 2^-39 of its row's largest (a weight: of the
- * largest one so far; 2^-136 where that is less), whichever is more, and a product to 2^-21.  In rows of ordinary
- * numbers that is as near as f32's sums are; beside an element 2^20 times the others
- * these are off by 2^-19, and what is 2^39 times smaller is lost, where f32 has no such
- * limit.  The calls whose names end in _f32 take f32 (24 bits) for every row and are
- * slower over long chunks: 2 x 2,048 rows after 2,048, 32 heads on 8 of 128, 2,030 us in
- * place of 790, over Q8_0 blocks 1,190 in place of 800.
+ * largest one so far; 2^-136 where that is less), whichever is more, and a product to
+ * 2^-21.  In rows of ordinary numbers that is as near as f32's sums are; beside an element
+ * 2^20 times the others these are off by 2^-19, and what is 2^39 times smaller is lost,
+ * where f32 has no such limit.  The calls whose names end in _f32 take f32 (24 bits) for
+ * every row and are slower over long chunks: 2 x 2,048 rows after 2,048, 32 heads on 8 of
+ * 128, 2,030 us in place of 790, over Q8_0 blocks 1,190 in place of 800.
  *
  * Launching fails with TVARA_INVALID once the cache has changed.  rows * heads *
  * head_dim stays below 2^32 in all, the rows below 2^24. */

@@ -720,8 +720,9 @@ __device__ __forceinline__ Parts split8(f32x4 x, f32x4 y) {
 
 // Rows go into parts multiplied by a power of two that brings their largest element to
 // 2^14 .. 2^15: then an element is off by 2^-23 of itself or 2^-39 of the row's largest,
-// whatever the row's size (plans in f32 keep such rows from here: ScorePlan::build).  The exponent (0 for 2^0 .. 2^1) of a magnitude, kept where
-// both that power and its inverse, times 2^15 more, are normal numbers.
+// whatever the row's size (plans in f32 keep all rows from here: ScorePlan::build).  The
+// exponent (0 for 2^0 .. 2^1) of a magnitude, kept where both that power and its inverse,
+// times 2^15 more, are normal numbers.
 __device__ __forceinline__ int exponent_of(float most) {
     return max(static_cast<int>(__builtin_bit_cast(unsigned, most) >> 23 & 255) - 127, -97);
 }
